@@ -244,6 +244,96 @@ int trk_gemv(const trk_mat *w, uint32_t item, uint32_t s0, uint32_t s1, uint32_t
              const float *scale, const int32_t *sum, uint32_t m, int pair, float *y, uint32_t ldy,
              const uint32_t *rows, int accumulate, void *stream);
 
+/* ---- routing by scores, and 8-bit products with a scale per token and per channel -------- */
+/* No counterpart in the reference, whose router knows trk_route's rules and whose weights and
+ * activations carry a scale per 16 or 32 values.  These serve layers whose experts or dense
+ * projections are int8 matrices with one scale per output channel, multiplied with activation rows
+ * quantised as a whole, and routers that choose by sigmoid scores, a balance bias or groups:
+ *
+ *   trk_route_scores -> trk_experts_plan -> trk_quantize_rows (x) -> trk_experts_up_i8
+ *                    -> trk_quantize_rows (h) -> trk_experts_down_i8
+ *
+ * Element types of the floating arrays: */
+enum { TRK_DT_F32 = 0, TRK_DT_BF16 = 1, TRK_DT_F16 = 2 };
+
+enum { TRK_SCORE_SOFTMAX = 0, TRK_SCORE_SIGMOID = 1 };
+
+/* How trk_route_scores chooses.  k experts per token (1..32, at most n_expert); score: softmax over
+ * the row's experts, or the sigmoid of each logit.  n_group (1..32) equal groups of neighbouring
+ * experts, of which the topk_group best may be chosen from (n_group = topk_group = 1: no groups);
+ * a group is worth the sum of its group_top (1 or 2) best experts' keys.  renorm: the chosen
+ * experts' scores are divided by their sum; factor: what every weight is multiplied with. */
+typedef struct {
+    uint32_t k, score;
+    uint32_t n_group, topk_group, group_top;
+    int32_t renorm;
+    float factor;
+} trk_score_policy;
+
+/* Per-row routing by scores.  Expert e's key is its score plus bias[e] (bias NULL: the order of the
+ * logits); the k largest keys of the kept groups are chosen, in descending order, the lower index
+ * first among equal ones, and weighted by their scores, without the bias.  Keys and group sums are
+ * compared as if in 64 bits.  An expert whose logit (or key) is NaN or -inf is never chosen, and
+ * adds nothing to the softmax's sum: a row chooses fewer than k, or none, where the others run out.
+ * ids / w: [m][32], n_sel: [m]; slots n_sel .. k - 1 get id 0xffffffff and weight 0, later ones stay
+ * as they were.  A softmax row with a logit of +inf has NaN scores: NaN weights, and with a bias no choice.  n_expert at most 1024. */
+int trk_route_scores(const float *logits, const float *bias, uint32_t m, uint32_t n_expert,
+                     const trk_score_policy *policy, uint32_t *ids, float *w, uint32_t *n_sel, void *stream);
+
+/* A stack of `count` int8 matrices [rows][k]: matrix i's row r is the k bytes at
+ * ptr + i * stride + r * ld, and stands for scale[i * rows + r] times them.  ptr, ld and (count > 1)
+ * stride are multiples of 16; rows are read in 16-byte pieces, so the bytes behind a row's k-th up
+ * to the next multiple of 16 have to be there (any value).  k at most 131071: every product
+ * of two rows then fits its 32-bit sum. */
+typedef struct {
+    const int8_t *ptr;
+    const float *scale;
+    uint32_t rows, k, count;
+    uint64_t ld, stride; /* bytes */
+} trk_i8_mat;
+
+/* Rows quantised as a whole: scale[i] = max |x[i]| / 127, q[i][j] = 127 x[i][j] / max |x[i]| rounded
+ * to the nearest integer, ties to even, as if computed exactly.  x: [m][k] of type `dtype`, rows ldx
+ * elements apart; q: rows ldq bytes apart, only the k bytes of each written.  A row whose largest
+ * magnitude is under 127 * 2^-126 (its scale would be no normal number) gets scale 0 and zeros; one
+ * with a NaN or an infinity gets scale NaN and zeros, which makes every product of it NaN. */
+int trk_quantize_rows(const void *x, uint32_t dtype, uint64_t ldx, uint32_t m, uint32_t k, int8_t *q, uint64_t ldq,
+                      float *scale, void *stream);
+
+/* y[i][r] = scale[i] * w.scale[r] * sum_j q[i][j] w[r][j] (+ bias[r]) (+ y[i][r] with accumulate),
+ * for every row r of matrix `item`: the sum is an exact integer, the scaling in 32 bits, rounded to
+ * y's type once.  q: rows ldq bytes apart, laid out as a trk_i8_mat's; y: rows ldy elements apart;
+ * bias: [rows] or NULL. */
+int trk_gemm_i8(const trk_i8_mat *w, uint32_t item, const int8_t *q, uint64_t ldq, const float *scale, uint32_t m,
+                const float *bias, void *y, uint32_t dtype, uint64_t ldy, int accumulate, void *stream);
+
+/* The products of each token with the experts it was routed to.  ids / w [m][32] and n_sel [m] as
+ * trk_route, trk_route_scores or the caller leaves them; `slots` (1..32) of each row are looked at.
+ * Slot j of token t is an entry where j < n_sel[t] and ids[t][j] is below the stack's count (an
+ * expert that lives elsewhere is passed over); its row of h is t * slots + j.
+ *
+ * plan: the entries sorted by expert, of trk_experts_plan_words words, made by trk_experts_plan for
+ * the same ids, n_sel, m, slots and n_expert (= the stacks' count).  0 words: the products of that few entries
+ * take none (NULL). */
+int trk_experts_plan_words(uint32_t m, uint32_t slots, uint32_t n_expert, uint64_t *words);
+int trk_experts_plan(const uint32_t *ids, const uint32_t *n_sel, uint32_t m, uint32_t slots, uint32_t n_expert,
+                     uint32_t *plan, void *stream);
+
+/* h[t * slots + j][F] = silu(g) * u of every entry, g and u the products of row t of q with its expert's gate and
+ * up rows (as trk_gemm_i8, in 32 bits), rounded once to `dtype`; rows of h that are no entry's stay as they were. */
+int trk_experts_up_i8(const trk_i8_mat *gate, const trk_i8_mat *up, const int8_t *q, uint64_t ldq, const float *scale,
+                      uint32_t m, const uint32_t *ids, const uint32_t *n_sel, uint32_t slots, const uint32_t *plan,
+                      void *h, uint32_t dtype, uint64_t ldh, void *stream);
+
+/* y[t] (+)= sum_j w[t][j] * (product of h row t * slots + j, quantised to q / scale, with its
+ * expert's down rows) over the token's entries, in slot order, in 32 bits; a token without entries
+ * gets zeros.  work: trk_experts_down_work_bytes of device memory, 16-byte aligned (NULL where that is 0). */
+int trk_experts_down_work_bytes(uint32_t m, uint32_t slots, uint32_t n_expert, uint32_t rows, uint64_t *bytes);
+int trk_experts_down_i8(const trk_i8_mat *down, const int8_t *q, uint64_t ldq, const float *scale, uint32_t m,
+                        const uint32_t *ids, const float *w, const uint32_t *n_sel, uint32_t slots,
+                        const uint32_t *plan, void *work, void *y, uint32_t dtype, uint64_t ldy, int accumulate,
+                        void *stream);
+
 /* y = silu(g) * u (elem::swiglu_vec, elem.rs:173-175) over n floats. */
 int trk_swiglu(const float *g, const float *u, float *y, size_t n, void *stream);
 

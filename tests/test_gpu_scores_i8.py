@@ -1,0 +1,495 @@
+"""Routing by scores and the int8 products on the GPU against their plain 64-bit forms (tests/i8ref.py).
+
+Routing ids, quantised values and entry selection are equal; weights and products are within the roundings that their
+definitions name (i8ref.gemm_tol, swiglu_tol, and the bounds written at each test)."""
+from __future__ import annotations
+
+import sys
+
+import i8ref as R
+import numpy as np
+import pytest
+
+import trmoe
+
+pytestmark = pytest.mark.gpu
+DTYPES = ["f32", "bf16", "f16"]
+
+
+def say(msg):
+    print(f"[gpu] {msg}", flush=True)
+    sys.stdout.flush()
+
+
+def dev(a):
+    import torch
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def host(t):
+    return t.detach().float().cpu().numpy() if t.is_floating_point() else t.detach().cpu().numpy()
+
+
+def padded(a, fill=77, spare=0):
+    """int8 [..][k] on the GPU with rows a multiple of 16 bytes (+ 16 spare) apart, `fill` behind each row."""
+    import torch
+    k = a.shape[-1]
+    t = torch.full((*a.shape[:-1], (k + 15) // 16 * 16 + 16 * spare), fill, dtype=torch.int8, device="cuda")
+    t[..., :k] = dev(a)
+    return t[..., :k]
+
+
+def i8(rng, *shape):
+    return np.clip(np.rint(rng.standard_normal(shape) * 40), -128, 127).astype(np.int8)
+
+
+def scales(rng, *shape, around=0.03):
+    return (rng.uniform(0.5, 1.5, shape) * around).astype(np.float32)
+
+
+# ---- routing by scores ------------------------------------------------------------------------------
+
+# 64-bit scores differ by a few ulp between libraries; a choice that hangs on them is no test
+def settled(logits, bias, score, **kw):
+    """Rows whose choice stays when every key moves by 1e-12 of itself: all of them, with these inputs."""
+    a = R.route(logits, bias=bias, score=score, **kw)[0]
+    moved = np.where(np.isfinite(logits), logits.astype(np.float64) * (1 + 1e-12), logits)
+    b = R.route(moved, bias=bias, score=score, **kw)[0]
+    return np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("m,E,k,score,bias,groups,keep,top,renorm,factor", [
+    (1, 1, 1, "sigmoid", False, 1, 1, 1, True, 1.0), (3, 5, 5, "softmax", True, 1, 1, 2, False, 1.0),
+    (5, 64, 8, "sigmoid", True, 8, 4, 2, True, 2.5), (130, 256, 8, "sigmoid", True, 8, 4, 2, True, 2.5),
+    (9, 160, 6, "softmax", False, 8, 3, 1, False, 16.0), (7, 257, 32, "softmax", True, 1, 1, 2, True, 1.0),
+    (33, 512, 10, "softmax", False, 1, 1, 2, True, 1.0), (6, 1024, 32, "sigmoid", True, 32, 5, 2, True, 1.0),
+    (4, 1020, 17, "softmax", True, 17, 6, 2, True, 1.0), (4, 96, 4, "sigmoid", False, 3, 2, 2, True, 1.0),
+    (4, 32, 3, "sigmoid", True, 32, 3, 2, True, 1.0), (257, 128, 1, "sigmoid", True, 4, 1, 1, True, 1.0)])
+def test_route_scores(m, E, k, score, bias, groups, keep, top, renorm, factor):
+    say(f"route_scores m={m} E={E} k={k} {score} groups={groups}/{keep}")
+    rng = np.random.default_rng(m * 1000 + E + k)
+    lg = (rng.standard_normal((m, E)) * 1.5).astype(np.float32)
+    lg[rng.random((m, E)) < 0.1] = -np.inf
+    lg[rng.random((m, E)) < 0.02] = np.nan
+    if m > 3:
+        lg[1] = -np.inf                  # nothing to choose
+        lg[2, 1:] = -np.inf              # one expert
+        lg[3, :] = lg[3, 0] if np.isfinite(lg[3, 0]) else 0.5  # all alike: the lowest indices
+    b = (rng.standard_normal(E) * 0.1).astype(np.float32) if bias else None
+    if bias and E > 8:
+        b[5] = -np.inf                   # never chosen
+    kw = dict(k=k, n_group=groups, topk_group=keep, group_top=top, renorm=renorm, factor=factor)
+    assert settled(lg, b, score, **kw)
+    ids, w, n = trmoe.route_scores(dev(lg), bias=None if b is None else dev(b), score=score, **kw)
+    rid, rw, rn = R.route(lg, bias=b, score=score, **kw)
+    assert np.array_equal(host(n), rn)
+    assert np.array_equal(host(ids)[:, :k], rid)
+    # one rounding to 32 bits; a softmax that stays unnormalised also has its sum of at most 1024 exponentials, each within
+    # 2^-22, and 22 roundings of a tree of them
+    rtol = 2.0 ** -22 if renorm or score == "sigmoid" else 2.0 ** -18
+    np.testing.assert_allclose(host(w)[:, :k], rw, rtol=rtol, atol=2.0 ** -149)
+
+
+def test_route_scores_ties_and_near_ties():
+    """Equal keys go to the lower index; keys that 32 bits cannot tell apart go by their 64-bit values."""
+    say("route_scores ties")
+    E = 64
+    lg = np.zeros((4, E), np.float32)
+    lg[1, 40] = np.nextafter(np.float32(0), np.float32(1))  # a denormal above the others, behind them
+    lg[2] = 2.0
+    lg[2, 63] = np.nextafter(np.float32(2), np.float32(3))  # sigmoid moves by a fraction of a 32-bit step
+    lg[3] = 30.0
+    lg[3, 50] = 31.0                                        # both sigmoids are 1 in 32 bits
+    b = np.full(E, 0.25, np.float32)
+    for bias in (None, b):
+        kw = dict(k=4, n_group=1, topk_group=1, group_top=2, renorm=True, factor=1.0)
+        ids, w, n = trmoe.route_scores(dev(lg), bias=None if bias is None else dev(bias), score="sigmoid", **kw)
+        rid, rw, rn = R.route(lg, bias=bias, score="sigmoid", **kw)
+        assert np.array_equal(host(ids)[:, :4], rid)
+        np.testing.assert_allclose(host(w)[:, :4], rw, rtol=2.0 ** -22)
+    # groups told apart only by their sums' last bits
+    lg = np.full((1, E), -1.0, np.float32)
+    lg[0, 0:2] = (1.0, 0.5)
+    lg[0, 32:34] = (1.0, np.nextafter(np.float32(0.5), np.float32(1)))
+    kw = dict(k=2, n_group=2, topk_group=1, group_top=2, renorm=True, factor=1.0)
+    ids, _, _ = trmoe.route_scores(dev(lg), score="sigmoid", **kw)
+    assert host(ids)[0, :2].tolist() == [32, 33]
+
+
+def test_route_scores_extremes():
+    """Scores that underflow in 32 bits still make weights; where all vanish the weights are zeros."""
+    say("route_scores extremes")
+    lg = np.array([[-100.0, -101.0, -200.0, -300.0], [-800.0, -900.0, -801.0, -1000.0], [88.0, 1000.0, -5.0, 0.0]], np.float32)
+    kw = dict(k=3, n_group=1, topk_group=1, group_top=2, renorm=True, factor=2.0)
+    for score in ("sigmoid", "softmax"):
+        ids, w, n = trmoe.route_scores(dev(lg), score=score, **kw)
+        rid, rw, rn = R.route(lg, bias=None, score=score, **kw)
+        assert np.array_equal(host(ids)[:, :3], rid)
+        np.testing.assert_allclose(host(w)[:, :3], rw, rtol=2.0 ** -22, atol=2.0 ** -149)
+
+
+def test_route_scores_leaves_the_rest():
+    import torch
+    say("route_scores leaves slots past k")
+    ids = torch.full((3, 32), 7, dtype=torch.int32, device="cuda")
+    w = torch.full((3, 32), 7.0, device="cuda")
+    n = torch.full((3,), 7, dtype=torch.int32, device="cuda")
+    lg = torch.randn((2, 40), device="cuda")
+    trmoe.route_scores(lg, 5, out=(ids[:2], w[:2], n[:2]))
+    assert (ids[:, 5:] == 7).all() and (w[:, 5:] == 7).all() and (ids[2] == 7).all() and n[2] == 7
+    assert trmoe.route_scores(lg[:0], 5)[0].shape == (0, 32)
+
+
+# ---- rows to int8 -----------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,k,lead,spare", [(1, 1, 0, 0), (2, 16, 0, 0), (3, 17, 1, 2), (5, 2048, 0, 0), (2, 4099, 3, 8),
+                                            (300, 333, 0, 0), (7, 1024, 8, 8), (1, 131071, 0, 0), (9, 8192, 0, 0)])
+def test_quantize_rows(dtype, m, k, lead, spare):
+    import torch
+    say(f"quantize_rows {dtype} m={m} k={k} lead={lead} spare={spare}")
+    rng = np.random.default_rng(m + k)
+    x = rng.standard_normal((m, k)) * np.exp(rng.uniform(-6, 6, (m, 1)))
+    if m > 2:
+        x[1] = 0
+        x[2, :] = np.resize(np.arange(-126, 127) + 0.5, k)  # halves: ties to even
+        x[2, 0] = 127
+    if m > 4:
+        x[3] *= 1e-41 if dtype != "f16" else 0   # a scale that is no normal number
+        x[4] = 6e4 * np.sign(x[4])
+    wide = torch.zeros((m, lead + k + spare), dtype=R.torch_dtype(dtype), device="cuda")
+    wide[:, lead:lead + k] = dev(x).to(wide.dtype)
+    xs = wide[:, lead:lead + k]
+    ref_q, ref_s = R.quantize(xs.double().cpu().numpy())
+    q, s = trmoe.quantize_rows(xs)
+    assert np.array_equal(host(q), ref_q)
+    assert np.array_equal(host(s).view(np.uint32), ref_s.view(np.uint32))
+    # into a place of the caller's, any stride: the bytes around it stay
+    out = torch.full((m + 1, k + 5), 99, dtype=torch.int8, device="cuda")
+    sc = torch.empty(m, device="cuda")
+    trmoe.quantize_rows(xs, out=(out[:m, 3:3 + k], sc))
+    assert np.array_equal(host(out)[:m, 3:3 + k], ref_q)
+    assert (out[:, :3] == 99).all() and (out[:, 3 + k:] == 99).all() and (out[m] == 99).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_rows_poison(dtype):
+    say(f"quantize_rows poison {dtype}")
+    x = np.ones((4, 100), np.float32)
+    x[1, 70], x[2, 99], x[3, 0] = np.nan, np.inf, -np.inf
+    q, s = trmoe.quantize_rows(dev(x).to(R.torch_dtype(dtype)))
+    q, s = host(q), host(s)
+    assert (q[0] == 127).all() and np.isfinite(s[0])
+    assert (q[1:] == 0).all() and np.isnan(s[1:]).all()
+
+
+def test_quantize_rows_largest_and_smallest():
+    say("quantize_rows f32 range ends")
+    top = np.finfo(np.float32).max
+    least = np.float32(127 * 2.0 ** -126)
+    x = np.array([[top, -top, top / 2, 1.0], [least, -least, least / 2, 0], [np.nextafter(least, np.float32(0)), 0, 0, 0]],
+                 np.float32)
+    rq, rs = R.quantize(x)
+    q, s = trmoe.quantize_rows(dev(x))
+    assert np.array_equal(host(q), rq) and np.array_equal(host(s).view(np.uint32), rs.view(np.uint32))
+
+
+# ---- the dense product ------------------------------------------------------------------------------
+
+def run_gemm(rng, m, rows, k, dtype, bias, spare=0, q=None, w=None):
+    import torch
+    q = i8(rng, m, k) if q is None else q
+    w = i8(rng, rows, k) if w is None else w
+    s, ws = scales(rng, m), scales(rng, rows, around=0.01)
+    b = (rng.standard_normal(rows) * 0.3).astype(np.float32) if bias else None
+    W = trmoe.I8Weights(padded(w, spare=spare), dev(ws))
+    wide = torch.full((m + 1, rows + 3), 9.0, dtype=R.torch_dtype(dtype), device="cuda")
+    y = trmoe.gemm_i8(W, padded(q, fill=-77, spare=spare), dev(s), bias=None if b is None else dev(b), out=wide[:m, :rows])
+    assert (wide[m] == 9).all() and (wide[:, rows:] == 9).all()
+    ref = R.gemm(q, s, w, ws)
+    tol = R.gemm_tol(ref, dtype, bias=b)
+    got = host(y).astype(np.float64)
+    ref = ref + (0 if b is None else b)
+    bad = np.abs(got - ref) > tol
+    assert not bad.any(), (np.argwhere(bad)[:4], got[bad][:4], ref[bad][:4])
+    return W, q, s, ref
+
+
+@pytest.mark.parametrize("m,rows,k", [(1, 1, 1), (1, 16, 64), (2, 17, 15), (16, 33, 16), (17, 100, 129), (65, 5, 1000),
+                                      (130, 130, 257), (300, 260, 640), (1, 4099, 2560), (5, 4099, 2561), (33, 1030, 511),
+                                      (64, 2048, 2048), (129, 384, 4096), (256, 256, 127), (1000, 513, 128),
+                                      (513, 1537, 1055)])
+@pytest.mark.parametrize("dtype,bias", [("f32", False), ("bf16", True), ("f16", False)])
+def test_gemm_i8(m, rows, k, dtype, bias):
+    say(f"gemm_i8 m={m} rows={rows} k={k} {dtype} bias={bias}")
+    run_gemm(np.random.default_rng(m * 7 + rows + k), m, rows, k, dtype, bias, spare=m % 2)
+
+
+@pytest.mark.parametrize("m,rows", [(2, 3), (40, 70), (300, 300)])
+def test_gemm_i8_largest_sum(m, rows):
+    """k at its limit, every value -128: 2^14 * 131071, the largest sum that fits."""
+    say(f"gemm_i8 largest sum m={m} rows={rows}")
+    k = 131071
+    run_gemm(np.random.default_rng(1), m, rows, k, "f32", False, q=np.full((m, k), -128, np.int8),
+             w=np.full((rows, k), -128, np.int8))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m", [3, 50, 400])
+def test_gemm_i8_accumulates_and_takes_an_item(dtype, m):
+    import torch
+    say(f"gemm_i8 accumulate {dtype} m={m}")
+    rng = np.random.default_rng(m)
+    rows, k = 200, 300
+    w, ws = i8(rng, 3, rows, k), scales(rng, 3, rows, around=0.01)
+    q, s = i8(rng, m, k), scales(rng, m)
+    W = trmoe.I8Weights(padded(w), dev(ws))
+    y = torch.randn((m, rows), device="cuda").to(R.torch_dtype(dtype))
+    old = y.double().cpu().numpy()
+    b = rng.standard_normal(rows).astype(np.float32)
+    trmoe.gemm_i8(W, padded(q), dev(s), bias=dev(b), out=y, accumulate=True, item=2)
+    ref = R.gemm(q, s, w[2], ws[2])
+    assert (np.abs(host(y) - (ref + b + old)) <= R.gemm_tol(ref, dtype, bias=b, old=old)).all()
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_gemm_i8_poison_stays_in_its_row(m):
+    say(f"gemm_i8 poison m={m}")
+    rng = np.random.default_rng(3)
+    q, w = i8(rng, m, 96), i8(rng, 64, 96)
+    s, ws = scales(rng, m), scales(rng, 64)
+    q[0], s[0] = 0, np.nan
+    y = host(trmoe.gemm_i8(trmoe.I8Weights(padded(w), dev(ws)), padded(q), dev(s)))
+    assert np.isnan(y[0]).all() and np.isfinite(y[1:]).all()
+
+
+def test_gemm_i8_empty_and_refused():
+    import torch
+    say("gemm_i8 empty, refused")
+    W = trmoe.quantize_weights(torch.randn((8, 40), device="cuda"))
+    assert trmoe.gemm_i8(W, torch.empty((0, 48), dtype=torch.int8, device="cuda")[:, :40],
+                         torch.empty(0, device="cuda")).shape == (0, 8)
+    q, s = trmoe.quantize_rows(torch.randn((3, 40), device="cuda"))
+    for bad in (dict(q=q[:, :39]), dict(scale=s[:2]), dict(out=torch.empty((3, 9), device="cuda")), dict(item=1),
+                dict(accumulate=True), dict(dtype=torch.float64), dict(bias=torch.zeros(7, device="cuda")),
+                dict(q=torch.zeros((3, 40), dtype=torch.int8, device="cuda"))):
+        with pytest.raises(trmoe.TrkError):
+            trmoe.gemm_i8(**{**dict(w=W, q=q, scale=s), **bad})
+
+
+# ---- the experts' products --------------------------------------------------------------------------
+
+def routing(rng, m, E, slots, kind):
+    """ids [m][32] (garbage past the slots), weights, n_sel."""
+    ids = rng.integers(0, 1 << 31, (m, 32)).astype(np.int32)
+    w = np.full((m, 32), np.nan, np.float32)
+    w[:, :slots] = rng.standard_normal((m, slots))
+    n = np.full(m, slots, np.int32)
+    for t in range(m):
+        ids[t, :slots] = rng.permutation(E)[:slots] if E >= slots else rng.integers(0, E, slots)
+    if kind == "one":            # every token to the same expert
+        ids[:, :slots] = E - 1
+    if kind in ("ragged", "elsewhere"):
+        n = rng.integers(0, slots + 1, m).astype(np.int32)
+        n[0] = 0
+    if kind == "elsewhere":      # experts of other machines, no expert, and counts past the slots
+        ids[:, :slots] = np.where(rng.random((m, slots)) < 0.4, rng.choice([E, E + 5, -1]), ids[:, :slots])
+        n[-1] = 99
+        ids[m // 2, :slots] = -1
+    w = np.where(np.arange(32)[None, :] < np.minimum(n, slots)[:, None], w, np.nan).astype(np.float32)
+    return ids, w, n
+
+
+CASES = [(1, 1, 1, 64, 32, "plain"), (1, 512, 10, 256, 48, "plain"), (3, 64, 8, 300, 100, "ragged"),
+         (8, 8, 2, 129, 17, "elsewhere"), (9, 8, 2, 129, 17, "elsewhere"), (40, 16, 4, 512, 130, "plain"),
+         (64, 5, 32, 96, 65, "ragged"), (150, 512, 10, 256, 64, "plain"), (300, 3, 1, 640, 200, "one"),
+         (700, 40, 6, 272, 96, "elsewhere"), (33, 1024, 32, 64, 16, "plain"), (2000, 7, 3, 160, 129, "ragged")]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,E,slots,H,F,kind", CASES)
+def test_experts_up(m, E, slots, H, F, kind, dtype):
+    import torch
+    say(f"experts_up m={m} E={E} slots={slots} H={H} F={F} {kind} {dtype}")
+    rng = np.random.default_rng(m + E + H)
+    ids, _, n = routing(rng, m, E, slots, kind)
+    q, s = i8(rng, m, H), scales(rng, m)
+    gw, uw = i8(rng, E, F, H), i8(rng, E, F, H)
+    gs, us = (scales(rng, E, F, around=0.03 / np.sqrt(H)) for _ in range(2))
+    dq, ds, di, dn = padded(q, fill=-77), dev(s), dev(ids), dev(n)
+    plan = trmoe.experts_plan(di, dn, slots, E)
+    wide = torch.full((m * slots + 1, F + 5), 9.0, dtype=R.torch_dtype(dtype), device="cuda")
+    trmoe.experts_up_i8(trmoe.I8Weights(padded(gw), dev(gs)), trmoe.I8Weights(padded(uw, fill=-1), dev(us)), dq, ds, di, dn,
+                        slots, plan=plan, out=wide[:m * slots, :F])
+    got = host(wide).astype(np.float64)
+    live = R.entries(ids, n, slots, E).reshape(-1)
+    assert (got[:-1][~live] == 9).all() and (got[-1] == 9).all() and (got[:, F:] == 9).all()
+    for e in range(E):
+        rows = np.nonzero(live & (ids[:, :slots].reshape(-1) == e))[0]
+        if rows.size:
+            g, u = (R.gemm(q[rows // slots], s[rows // slots], a[e], b[e]) for a, b in ((gw, gs), (uw, us)))
+            assert np.abs(g).max() < 80
+            assert (np.abs(got[rows, :F] - R.swiglu(g, u)) <= R.swiglu_tol(g, u, dtype)).all(), e
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,E,slots,F,H,kind", CASES)
+def test_experts_down(m, E, slots, F, H, kind, dtype):
+    import torch
+    say(f"experts_down m={m} E={E} slots={slots} F={F} H={H} {kind} {dtype}")
+    rng = np.random.default_rng(m + E + H)
+    ids, w, n = routing(rng, m, E, slots, kind)
+    live = R.entries(ids, n, slots, E)
+    q, s = i8(rng, m * slots, F), scales(rng, m * slots)
+    s[~live.reshape(-1)] = np.nan  # rows that are no entry's are never read
+    dw, dws = i8(rng, E, H, F), scales(rng, E, H, around=0.01)
+    di, dn, dwt = dev(ids), dev(n), dev(w)
+    W = trmoe.I8Weights(padded(dw), dev(dws))
+    plan = trmoe.experts_plan(di, dn, slots, E)
+    terms = np.zeros((m, slots, H))
+    for e in range(E):
+        t, j = np.nonzero(live & (ids[:, :slots] == e))
+        if t.size:
+            terms[t, j] = R.gemm(q[t * slots + j], s[t * slots + j], dw[e], dws[e]) * w[t, j][:, None].astype(np.float64)
+    ref, size = terms.sum(1), np.abs(terms).sum(1)
+    # a term: three roundings of its product, one of the weight; the sum: one a slot
+    err = (4 + slots) * 1.01 * R.EPS["f32"] * size
+    for acc in (False, True):
+        wide = torch.full((m + 1, H + 5), 9.0, dtype=R.torch_dtype(dtype), device="cuda")
+        trmoe.experts_down_i8(W, padded(q, fill=-77), dev(s), di, dwt, dn, slots, plan=plan, out=wide[:m, :H], accumulate=acc)
+        got = host(wide).astype(np.float64)
+        assert (got[m] == 9).all() and (got[:, H:] == 9).all()
+        want = ref + (9 if acc else 0)
+        tol = err + (1.01 * R.EPS["f32"] * (size + 9) if acc else 0) + 1.01 * R.round_rel(np.abs(want) + err, dtype)
+        assert (np.abs(got[:m, :H] - want) <= tol).all()
+
+
+def test_experts_refuse():
+    import torch
+    say("experts refusals")
+    W = trmoe.quantize_weights(torch.randn((4, 24, 40), device="cuda"))
+    q, s = trmoe.quantize_rows(torch.randn((64, 40), device="cuda"))
+    ids, w, n = trmoe.route_scores(torch.randn((64, 4), device="cuda"), 2)
+    with pytest.raises(trmoe.TrkError, match="plan"):
+        trmoe.experts_up_i8(W, W, q, s, ids, n, 2)
+    plan = trmoe.experts_plan(ids, n, 2, 4)
+    with pytest.raises(trmoe.TrkError, match="plan"):
+        trmoe.experts_up_i8(W, W, q, s, ids, n, 2, plan=plan[:-1])
+    h = trmoe.experts_up_i8(W, W, q, s, ids, n, 2, plan=plan)
+    D = trmoe.quantize_weights(torch.randn((4, 40, 24), device="cuda"))
+    hq, hs = trmoe.quantize_rows(h)
+    with pytest.raises(trmoe.TrkError, match="work"):
+        trmoe.experts_down_i8(D, hq, hs, ids, w, n, 2, plan=plan, work=torch.empty(8, device="cuda"))
+    with pytest.raises(trmoe.TrkError, match="q"):
+        trmoe.experts_down_i8(D, hq[:-1], hs[:-1], ids, w, n, 2, plan=plan)
+
+
+# ---- together ---------------------------------------------------------------------------------------
+
+def block(x, router, bias, gate, up, down, k, **out):
+    """A MoE block with int8 weights."""
+    rlog, _ = trmoe.router_logits(router, x)
+    ids, w, n = trmoe.route_scores(rlog, k, bias=bias, n_group=4, topk_group=2, factor=1.5)
+    plan = trmoe.experts_plan(ids, n, k, gate.count)
+    q, s = trmoe.quantize_rows(x)
+    h = trmoe.experts_up_i8(gate, up, q, s, ids, n, k, plan=plan)
+    hq, hs = trmoe.quantize_rows(h)
+    return trmoe.experts_down_i8(down, hq, hs, ids, w, n, k, plan=plan, **out)
+
+
+def a_block(seed, E=32, H=256, F=128):
+    import torch
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+
+    def normal(*shape, by=1.0):
+        return torch.randn(shape, device="cuda", generator=g) * by
+
+    W = [trmoe.quantize_weights(normal(E, r, c, by=c ** -0.5)) for r, c in ((F, H), (F, H), (H, F))]
+    return normal(E, H, by=H ** -0.5), normal(E, by=0.05), *W
+
+
+@pytest.mark.parametrize("m", [1, 5, 64, 300])
+def test_a_block_of_them(m):
+    import torch
+    say(f"block m={m}")
+    k = 4
+    router, bias, gate, up, down = a_block(m)
+    x = torch.randn((m, 256), device="cuda")
+    y = host(block(x, router, bias, gate, up, down, k)).astype(np.float64)
+    rlog, _ = trmoe.router_logits(router, x)
+    kw = dict(k=k, n_group=4, topk_group=2, group_top=2, renorm=True, factor=1.5)
+    ids, w, _ = R.route(host(rlog), bias=host(bias), score="sigmoid", **kw)
+    G, U, D = ((host(a.q).astype(np.float64), host(a.scale).astype(np.float64)) for a in (gate, up, down))
+    q, s = R.quantize(host(x))
+    ref, size, loose = np.zeros_like(y), np.zeros_like(y), np.zeros_like(y)
+    for t in range(m):
+        for j in range(k):
+            e = ids[t, j]
+            g, u = (R.gemm(q[t:t + 1], s[t:t + 1], a[0][e], a[1][e]) for a in (G, U))
+            h = R.swiglu(g, u)
+            top = np.abs(h).max()
+            hq, hs = R.quantize(h)
+            # values so near a border that h's own error (its tolerance, and the peak's) may move them one step
+            off = (R.swiglu_tol(g, u, "f32") + np.abs(h) * R.swiglu_tol(g, u, "f32").max() / top) * 127 / top + 1e-9
+            near = np.abs(np.abs(127 * h / top - np.rint(127 * h / top)) - 0.5) <= off
+            term = R.gemm(hq, hs, D[0][e], D[1][e])[0] * w[t, j]
+            ref[t] += term
+            size[t] += np.abs(term)
+            loose[t] += np.abs(w[t, j]) * float(hs[0]) * (np.abs(D[0][e])[:, near[0]].sum(1) * D[1][e])
+    # the scales of h carry its peak's error (swiglu_tol: under 40 half steps here, |g| < 6), the sum k + 4 roundings
+    tol = (50 + k) * R.EPS["f32"] * size + loose * 1.001 + 1e-30
+    assert (np.abs(y - ref) <= tol).all()
+
+
+@pytest.mark.parametrize("m", [2, 100])
+def test_captured_and_replayed(m):
+    """The block in a graph, replayed with the program's own work between, on new inputs each time."""
+    import torch
+    say(f"block captured m={m}")
+    router, bias, gate, up, down = a_block(9)
+    x = torch.randn((m, 256), device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        block(x, router, bias, gate, up, down, 4)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = block(x, router, bias, gate, up, down, 4)
+    for i in range(5):
+        x.copy_(torch.randn((m, 256), device="cuda"))
+        g.replay()
+        torch.cuda.synchronize()
+        got = y.clone()
+        assert torch.equal(got, block(x, router, bias, gate, up, down, 4)), i
+
+
+def test_on_two_streams_at_once():
+    import torch
+    say("block on two streams")
+    router, bias, gate, up, down = a_block(11)
+    xs = [torch.randn((n, 256), device="cuda") for n in (200, 3, 77, 200)]
+    want = [block(x, router, bias, gate, up, down, 4) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = []
+    for x, st in zip(xs, streams):
+        with torch.cuda.stream(st):
+            for _ in range(3):
+                y = block(x, router, bias, gate, up, down, 4)
+            got.append(y)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_the_same_bits_every_time():
+    import torch
+    say("block twice")
+    router, bias, gate, up, down = a_block(12, E=8)
+    x = torch.randn((500, 256), device="cuda")
+    a = block(x, router, bias, gate, up, down, 4)
+    assert all(torch.equal(a, block(x, router, bias, gate, up, down, 4)) for _ in range(4))
+    # a token's result does not depend on its batch
+    one = block(x[:1], router, bias, gate, up, down, 4)
+    assert torch.equal(one, a[:1])

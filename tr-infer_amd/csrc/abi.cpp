@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -874,6 +875,180 @@ extern "C" int trk_gemv(const trk_mat* w, uint32_t item, uint32_t s0, uint32_t s
     if (m == 0 || s0 == s1) return TRK_OK;
     Mat M{(const uint8_t*)w->ptr, w->count > 1 ? w->stride : mbytes, w->rows, w->k, w->fmt, (uint32_t)pitch};
     HIP_TRY(launch_gemv(M, item, s0, s1, kb, q, scale, sum, m, pair, y, ldy, rows, accumulate, (hipStream_t)stream));
+    return TRK_OK;
+}
+
+// ---- routing by scores, 8-bit products with a scale per token and per channel ------------------------
+
+extern "C" int trk_route_scores(const float* logits, const float* bias, uint32_t m, uint32_t n_expert,
+                                const trk_score_policy* p, uint32_t* ids, float* w, uint32_t* n_sel, void* stream) {
+    if (!p) return fail(TRK_E_INVALID, "null argument");
+    if (n_expert == 0 || n_expert > 1024) return fail(TRK_E_INVALID, "n_expert (%u) must be in 1..1024", n_expert);
+    if (p->k < 1 || p->k > TRK_MOE_K_MAX || p->k > n_expert)
+        return fail(TRK_E_POLICY, "score policy: k (%u) must be in 1..min(32, n_expert)", p->k);
+    if (p->score != TRK_SCORE_SOFTMAX && p->score != TRK_SCORE_SIGMOID)
+        return fail(TRK_E_POLICY, "score policy: unknown score %u", p->score);
+    if (p->n_group < 1 || p->n_group > 32 || n_expert % p->n_group)
+        return fail(TRK_E_POLICY, "score policy: n_group (%u) must be in 1..32 and divide n_expert (%u)", p->n_group,
+                    n_expert);
+    if (p->topk_group < 1 || p->topk_group > p->n_group)
+        return fail(TRK_E_POLICY, "score policy: topk_group (%u) must be in 1..n_group (%u)", p->topk_group, p->n_group);
+    if (p->group_top != 1 && p->group_top != 2)
+        return fail(TRK_E_POLICY, "score policy: group_top (%u) must be 1 or 2", p->group_top);
+    if (!std::isfinite(p->factor)) return fail(TRK_E_POLICY, "score policy: factor (%g) must be finite", (double)p->factor);
+    if (m == 0) return TRK_OK;
+    if (!logits || !ids || !w || !n_sel) return fail(TRK_E_INVALID, "null argument");
+    const ScorePolicy sp{p->k, p->score, p->n_group, p->topk_group, p->group_top, p->renorm, p->factor};
+    HIP_TRY(launch_route_scores(logits, bias, m, n_expert, sp, ids, w, n_sel, (hipStream_t)stream));
+    return TRK_OK;
+}
+
+static int check_dtype(uint32_t dt) {
+    if (dt != TRK_DT_F32 && dt != TRK_DT_BF16 && dt != TRK_DT_F16) return fail(TRK_E_INVALID, "unknown element type %u", dt);
+    return TRK_OK;
+}
+
+static int check_elem_ptr(const void* p, uint32_t dt, const char* what) {
+    if ((uintptr_t)p % (dt == TRK_DT_F32 ? 4 : 2)) return fail(TRK_E_INVALID, "%s is not aligned to its elements", what);
+    return TRK_OK;
+}
+
+constexpr uint32_t I8_K_MAX = 131071;  // 2^14 k < 2^31: the sums of a row's products fit 32 bits
+
+static int check_i8_rows(const void* q, uint64_t ldq, uint32_t k, const char* what) {
+    if ((uintptr_t)q % 16 || ldq % 16) return fail(TRK_E_INVALID, "%s: pointer and row stride must be multiples of 16", what);
+    if (ldq < k) return fail(TRK_E_INVALID, "%s: row stride %llu below k (%u)", what, (unsigned long long)ldq, k);
+    return TRK_OK;
+}
+
+static int check_i8_mat(const trk_i8_mat* w, const char* what) {
+    if (!w || !w->ptr || !w->scale) return fail(TRK_E_INVALID, "%s: null argument", what);
+    if (w->rows == 0 || w->k == 0 || w->count == 0) return fail(TRK_E_INVALID, "%s: empty matrix", what);
+    if (w->k > I8_K_MAX) return fail(TRK_E_INVALID, "%s: k (%u) above %u", what, w->k, I8_K_MAX);
+    if (int rc = check_i8_rows(w->ptr, w->ld, w->k, what)) return rc;
+    if (w->ld >> 40) return fail(TRK_E_INVALID, "%s: row stride %llu too large", what, (unsigned long long)w->ld);
+    if (w->count > 1 && (w->stride % 16 || w->stride < (w->rows - 1ull) * w->ld + w->k))
+        return fail(TRK_E_INVALID, "%s: stride %llu is no multiple of 16 that holds a matrix", what,
+                    (unsigned long long)w->stride);
+    return TRK_OK;
+}
+
+static I8Mat i8_mat(const trk_i8_mat& w) {
+    return I8Mat{w.ptr, w.scale, w.rows, w.k, w.count, w.ld, w.count > 1 ? w.stride : 0};
+}
+
+extern "C" int trk_quantize_rows(const void* x, uint32_t dtype, uint64_t ldx, uint32_t m, uint32_t k, int8_t* q,
+                                 uint64_t ldq, float* scale, void* stream) {
+    int rc = check_dtype(dtype);
+    if (rc || (rc = check_elem_ptr(x, dtype, "x"))) return rc;
+    if (k == 0) return fail(TRK_E_INVALID, "k must be positive");
+    if (m > 1 && (ldx < k || ldq < k)) return fail(TRK_E_INVALID, "row stride below k (%u)", k);
+    if (m == 0) return TRK_OK;
+    if (!x || !q || !scale) return fail(TRK_E_INVALID, "null argument");
+    HIP_TRY(launch_quantize_rows(x, dtype, ldx, m, k, q, ldq, scale, (hipStream_t)stream));
+    return TRK_OK;
+}
+
+extern "C" int trk_gemm_i8(const trk_i8_mat* w, uint32_t item, const int8_t* q, uint64_t ldq, const float* scale,
+                           uint32_t m, const float* bias, void* y, uint32_t dtype, uint64_t ldy, int accumulate,
+                           void* stream) {
+    int rc = check_i8_mat(w, "w");
+    if (rc) return rc;
+    if (item >= w->count) return fail(TRK_E_INVALID, "item %u out of range", item);
+    if ((rc = check_dtype(dtype)) || (rc = check_elem_ptr(y, dtype, "y"))) return rc;
+    if ((rc = check_i8_rows(q, ldq, w->k, "q"))) return rc;
+    if (m > 1 && ldy < w->rows) return fail(TRK_E_INVALID, "ldy %llu below rows (%u)", (unsigned long long)ldy, w->rows);
+    if (m == 0) return TRK_OK;
+    if (!q || !scale || !y) return fail(TRK_E_INVALID, "null argument");
+    const I8Mat M = i8_mat(*w);
+    const I8Gemm a{M.ptr + item * M.stride, M.scale + (uint64_t)item * M.rows, M.rows, M.k, M.ld, q, ldq, scale, m, bias,
+                   y, dtype, ldy, accumulate};
+    HIP_TRY(launch_gemm_i8(a, (hipStream_t)stream));
+    return TRK_OK;
+}
+
+// What the experts' calls have in common: a plan or work area is sized in 32-bit entries.
+static int check_entries(uint32_t m, uint32_t slots, uint32_t n_expert) {
+    if (slots < 1 || slots > TRK_MOE_K_MAX) return fail(TRK_E_INVALID, "slots (%u) must be in 1..32", slots);
+    if (n_expert < 1 || n_expert > 1024) return fail(TRK_E_INVALID, "n_expert (%u) must be in 1..1024", n_expert);
+    if ((uint64_t)m * slots > 0x7fffffffull) return fail(TRK_E_INVALID, "m * slots (%u * %u) too large", m, slots);
+    return TRK_OK;
+}
+
+extern "C" int trk_experts_plan_words(uint32_t m, uint32_t slots, uint32_t n_expert, uint64_t* words) {
+    if (!words) return fail(TRK_E_INVALID, "null argument");
+    if (int rc = check_entries(m, slots, n_expert)) return rc;
+    *words = geo::plan_used(m, slots, n_expert) ? geo::plan_words(m, slots, n_expert) : 0;
+    return TRK_OK;
+}
+
+extern "C" int trk_experts_plan(const uint32_t* ids, const uint32_t* n_sel, uint32_t m, uint32_t slots,
+                                uint32_t n_expert, uint32_t* plan, void* stream) {
+    if (int rc = check_entries(m, slots, n_expert)) return rc;
+    if (!geo::plan_used(m, slots, n_expert)) return TRK_OK;
+    if (!ids || !n_sel || !plan) return fail(TRK_E_INVALID, "null argument");
+    if ((uintptr_t)plan % 16) return fail(TRK_E_INVALID, "plan must be 16-byte aligned");
+    HIP_TRY(launch_experts_plan(ids, n_sel, m, slots, n_expert, plan, (hipStream_t)stream));
+    return TRK_OK;
+}
+
+// The plan of a call: NULL where the call takes none.
+static int check_plan(const uint32_t*& plan, uint32_t m, uint32_t slots, uint32_t n_expert) {
+    if (!geo::plan_used(m, slots, n_expert)) {
+        plan = nullptr;
+        return TRK_OK;
+    }
+    if (!plan) return fail(TRK_E_INVALID, "%u tokens of %u slots need a plan (trk_experts_plan)", m, slots);
+    if ((uintptr_t)plan % 16) return fail(TRK_E_INVALID, "plan must be 16-byte aligned");
+    return TRK_OK;
+}
+
+extern "C" int trk_experts_up_i8(const trk_i8_mat* gate, const trk_i8_mat* up, const int8_t* q, uint64_t ldq,
+                                 const float* scale, uint32_t m, const uint32_t* ids, const uint32_t* n_sel,
+                                 uint32_t slots, const uint32_t* plan, void* h, uint32_t dtype, uint64_t ldh,
+                                 void* stream) {
+    int rc = check_i8_mat(gate, "gate");
+    if (rc || (rc = check_i8_mat(up, "up"))) return rc;
+    if (gate->rows != up->rows || gate->k != up->k || gate->count != up->count)
+        return fail(TRK_E_INVALID, "gate [%u][%u][%u] and up [%u][%u][%u] differ in shape", gate->count, gate->rows, gate->k,
+                    up->count, up->rows, up->k);
+    if ((rc = check_entries(m, slots, gate->count))) return rc;
+    if ((rc = check_dtype(dtype)) || (rc = check_elem_ptr(h, dtype, "h"))) return rc;
+    if ((rc = check_i8_rows(q, ldq, gate->k, "q"))) return rc;
+    if (ldh < gate->rows) return fail(TRK_E_INVALID, "ldh %llu below rows (%u)", (unsigned long long)ldh, gate->rows);
+    if (m == 0) return TRK_OK;
+    if (!q || !scale || !ids || !n_sel || !h) return fail(TRK_E_INVALID, "null argument");
+    if ((rc = check_plan(plan, m, slots, gate->count))) return rc;
+    const I8Up a{i8_mat(*gate), i8_mat(*up), q, ldq, scale, m, slots, ids, n_sel, h, dtype, ldh};
+    HIP_TRY(launch_experts_up(a, plan, (hipStream_t)stream));
+    return TRK_OK;
+}
+
+extern "C" int trk_experts_down_work_bytes(uint32_t m, uint32_t slots, uint32_t n_expert, uint32_t rows,
+                                           uint64_t* bytes) {
+    if (!bytes) return fail(TRK_E_INVALID, "null argument");
+    if (int rc = check_entries(m, slots, n_expert)) return rc;
+    *bytes = geo::plan_used(m, slots, n_expert) ? 4ull * m * slots * rows : 0;
+    return TRK_OK;
+}
+
+extern "C" int trk_experts_down_i8(const trk_i8_mat* down, const int8_t* q, uint64_t ldq, const float* scale, uint32_t m,
+                                   const uint32_t* ids, const float* w, const uint32_t* n_sel, uint32_t slots,
+                                   const uint32_t* plan, void* work, void* y, uint32_t dtype, uint64_t ldy,
+                                   int accumulate, void* stream) {
+    int rc = check_i8_mat(down, "down");
+    if (rc) return rc;
+    if ((rc = check_entries(m, slots, down->count))) return rc;
+    if ((rc = check_dtype(dtype)) || (rc = check_elem_ptr(y, dtype, "y"))) return rc;
+    if ((rc = check_i8_rows(q, ldq, down->k, "q"))) return rc;
+    if (m > 1 && ldy < down->rows) return fail(TRK_E_INVALID, "ldy %llu below rows (%u)", (unsigned long long)ldy, down->rows);
+    if (m == 0) return TRK_OK;
+    if (!q || !scale || !ids || !w || !n_sel || !y) return fail(TRK_E_INVALID, "null argument");
+    if ((rc = check_plan(plan, m, slots, down->count))) return rc;
+    if (plan && (!work || (uintptr_t)work % 16))
+        return fail(TRK_E_INVALID, "work must be 16-byte aligned memory of trk_experts_down_work_bytes");
+    const I8Down a{i8_mat(*down), q, ldq, scale, m, slots, ids, n_sel, w, (float*)work, y, dtype, ldy, accumulate};
+    HIP_TRY(launch_experts_down(a, plan, (hipStream_t)stream));
     return TRK_OK;
 }
 

@@ -177,6 +177,25 @@ inline bool gemv_tiles(uint64_t workgroups, uint32_t tq, uint32_t k) {  // tq: 0
     return workgroups > (bits == 8 && k > 3072 ? 2303u : 2048u);
 }
 
+// The int8 experts' plan (k_i8x.hip): entries sorted by expert and cut into tiles of at most plan_rows entries of one
+// expert.  Words: {tiles, 3 unused}, ent [m * slots], then (16-byte aligned) four words per tile.
+inline bool plan_used(uint32_t m, uint32_t slots, uint32_t E) {
+    (void)slots, (void)E;
+    return m > 8;
+}
+inline uint32_t plan_rows(uint32_t m, uint32_t slots, uint32_t E) {
+    (void)m, (void)slots, (void)E;
+    return 16;
+}
+inline uint64_t plan_tiles(uint32_t m, uint32_t slots, uint32_t E, uint32_t rows) {  // no call has more
+    const uint64_t n = (uint64_t)m * slots;
+    return (n < E ? n : E) + n / rows;
+}
+inline uint64_t plan_tile_at(uint32_t m, uint32_t slots) { return 4 + ((uint64_t)m * slots + 3) / 4 * 4; }
+inline uint64_t plan_words(uint32_t m, uint32_t slots, uint32_t E) {
+    return plan_tile_at(m, slots) + 4 * plan_tiles(m, slots, E, plan_rows(m, slots, E));
+}
+
 // Every invariant a call of m rows with kcap selections per token relies on; returns nullptr when
 // they hold, else what failed.  tq: the experts are TQ strips (k_tq.hip), not GGUF superblocks.
 inline const char* check_call(const Caps& c, uint32_t m, uint32_t kcap, bool tq = false) {

@@ -220,6 +220,78 @@ inline bool tqm_fits(uint32_t H, uint32_t F) {
 inline size_t hc_image_bytes(uint32_t m, uint32_t lr) { return (size_t)(m + 15) / 16 * 22 * lr; }
 hipError_t launch_hc_mix(const Mat& up, uint32_t hc, uint32_t hh, uint32_t lr, const float* xn, const float* lo,
                          uint32_t m, int pair, const Workspace& ws, float* mixed, hipStream_t st);
+// routing by scores (k_score.hip)
+struct ScorePolicy {
+    uint32_t k, score, n_group, topk_group, group_top;
+    int renorm;
+    float factor;
+};
+hipError_t launch_route_scores(const float* logits, const float* bias, uint32_t m, uint32_t E, const ScorePolicy& p,
+                               uint32_t* ids, float* w, uint32_t* n_sel, hipStream_t st);
+// 8-bit products with a scale per token and per channel (k_i8.hip; the experts' k_i8x.hip)
+struct I8Mat {
+    const int8_t* ptr;
+    const float* scale;
+    uint32_t rows, k, count;
+    uint64_t ld, stride;
+};
+struct I8Gemm {
+    const int8_t* w;
+    const float* sw;
+    uint32_t rows, k;
+    uint64_t ldw;
+    const int8_t* q;
+    uint64_t ldq;
+    const float* sx;
+    uint32_t m;
+    const float* bias;
+    void* y;
+    uint32_t dt;
+    uint64_t ldy;
+    int accumulate;
+};
+struct I8Up {
+    I8Mat gate, up;
+    const int8_t* q;
+    uint64_t ldq;
+    const float* sx;
+    uint32_t m, slots;
+    const uint32_t *ids, *n_sel;
+    void* h;
+    uint32_t dt;
+    uint64_t ldh;
+};
+struct I8Down {
+    I8Mat down;
+    const int8_t* q;
+    uint64_t ldq;
+    const float* sx;
+    uint32_t m, slots;
+    const uint32_t *ids, *n_sel;
+    const float* w;
+    float* work;
+    void* y;
+    uint32_t dt;
+    uint64_t ldy;
+    int accumulate;
+};
+struct PlanTile {
+    uint32_t expert, row0, rows, pad;  // entries ent[row0 .. row0 + rows)
+};
+struct Plan {
+    uint32_t *n_tiles, *ent;
+    PlanTile* tile;
+};
+__host__ __device__ inline Plan plan_at(uint32_t* p, uint32_t m, uint32_t slots) {
+    return Plan{p, p + 4, reinterpret_cast<PlanTile*>(p + 4 + ((uint64_t)m * slots + 3) / 4 * 4)};  // geo::plan_tile_at
+}
+hipError_t launch_quantize_rows(const void* x, uint32_t dt, uint64_t ldx, uint32_t m, uint32_t k, int8_t* q,
+                                uint64_t ldq, float* scale, hipStream_t st);
+hipError_t launch_gemm_i8(const I8Gemm& a, hipStream_t st);
+hipError_t launch_experts_plan(const uint32_t* ids, const uint32_t* n_sel, uint32_t m, uint32_t slots, uint32_t E,
+                               uint32_t* plan, hipStream_t st);
+hipError_t launch_experts_up(const I8Up& a, const uint32_t* plan, hipStream_t st);
+hipError_t launch_experts_down(const I8Down& a, const uint32_t* plan, hipStream_t st);
 hipError_t launch_swiglu(const float* g, const float* u, float* y, size_t n, hipStream_t st);
 hipError_t launch_rmsnorm(const float* x, const float* w, float eps, uint32_t m, uint32_t n, float* y,
                           hipStream_t st);

@@ -20,6 +20,8 @@ FMT_Q4_K, FMT_Q6_K, FMT_Q8_0, FMT_Q5_1 = 12, 14, 8, 7
 FMT_TQ4_16, FMT_TQ4_32, FMT_TQ5_16, FMT_TQ5_32, FMT_TQ8_16, FMT_TQ8_32 = 0x410, 0x420, 0x510, 0x520, 0x810, 0x820
 TQ_FMTS = (FMT_TQ4_16, FMT_TQ4_32, FMT_TQ5_16, FMT_TQ5_32, FMT_TQ8_16, FMT_TQ8_32)
 BASIS_ALL, BASIS_TOP = 0, 1
+DT_F32, DT_BF16, DT_F16 = 0, 1, 2
+SCORES = {"softmax": 0, "sigmoid": 1}
 K_MAX = 32
 (WS_RLOG, WS_IDS, WS_W, WS_NSEL, WS_ENT_TOK, WS_ENT_W, WS_ENT_EXP, WS_GRP_START, WS_GRP_EXP, WS_NGROUPS, WS_XQ,
  WS_XS, WS_ACTQ, WS_ACTS, WS_SHLOGIT, WS_BARRIER_ERR, WS_MIXED) = range(1, 18)
@@ -46,6 +48,18 @@ class MoeW(C.Structure):
 
 class Policy(C.Structure):
     _fields_ = [("min", C.c_uint32), ("max", C.c_uint32), ("mass", C.c_float), ("basis", C.c_uint32)]
+
+
+class ScorePolicy(C.Structure):
+    """trk_score_policy: how trk_route_scores chooses."""
+    _fields_ = [("k", C.c_uint32), ("score", C.c_uint32), ("n_group", C.c_uint32), ("topk_group", C.c_uint32),
+                ("group_top", C.c_uint32), ("renorm", C.c_int32), ("factor", C.c_float)]
+
+
+class I8Mat(C.Structure):
+    """trk_i8_mat: a stack of int8 matrices with a scale per row."""
+    _fields_ = [("ptr", C.c_void_p), ("scale", C.c_void_p), ("rows", C.c_uint32), ("k", C.c_uint32),
+                ("count", C.c_uint32), ("ld", C.c_uint64), ("stride", C.c_uint64)]
 
 
 class Cfg(C.Structure):
@@ -87,6 +101,16 @@ def lib() -> C.CDLL:
         L.trk_route.argtypes = [vp, u32, u32, u32, C.POINTER(Policy), vp, vp, vp, vp]
         L.trk_quantize.argtypes = [vp, u32, u32, u32, i, vp, vp, vp, vp]
         L.trk_gemv.argtypes = [C.POINTER(Mat), u32, u32, u32, u32, vp, vp, vp, u32, i, vp, u32, vp, i, vp]
+        L.trk_route_scores.argtypes = [vp, vp, u32, u32, C.POINTER(ScorePolicy), vp, vp, vp, vp]
+        L.trk_quantize_rows.argtypes = [vp, u32, u64, u32, u32, vp, u64, vp, vp]
+        L.trk_gemm_i8.argtypes = [C.POINTER(I8Mat), u32, vp, u64, vp, u32, vp, vp, u32, u64, i, vp]
+        L.trk_experts_plan_words.argtypes = [u32, u32, u32, C.POINTER(u64)]
+        L.trk_experts_plan.argtypes = [vp, vp, u32, u32, u32, vp, vp]
+        L.trk_experts_up_i8.argtypes = [C.POINTER(I8Mat), C.POINTER(I8Mat), vp, u64, vp, u32, vp, vp, u32, vp, vp, u32,
+                                        u64, vp]
+        L.trk_experts_down_work_bytes.argtypes = [u32, u32, u32, u32, C.POINTER(u64)]
+        L.trk_experts_down_i8.argtypes = [C.POINTER(I8Mat), vp, u64, vp, u32, vp, vp, vp, u32, vp, vp, vp, u32, u64, i,
+                                          vp]
         L.trk_swiglu.argtypes = [vp, vp, vp, sz, vp]
         L.trk_rmsnorm.argtypes = [vp, vp, f, u32, u32, vp, vp]
         L.trk_add_inplace.argtypes = [vp, vp, sz, vp]
@@ -513,6 +537,267 @@ def gemv(wt, rows, k, fmt, item, count, kb, q, s, su, pair=False, y=None, ldy=No
     check(lib().trk_gemv(C.byref(mat), item, s0, s1, kb, _ptr(q), _ptr(s), _ptr(su), m, int(pair), _ptr(y),
                          ldy if ldy is not None else width, _ptr(rowmap), int(accumulate), _stream(stream)))
     return y
+
+
+# ---- routing by scores, 8-bit products with a scale per token and per channel --------------------
+#
+# The kernels run on torch's current stream (or `stream`) of the current device; tensors elsewhere are
+# refused.  Outputs are allocated where none is given.
+
+_dt = None
+_device = None
+
+
+def _dtype(t):
+    """TRK_DT_* of a torch dtype."""
+    global _dt
+    if _dt is None:
+        import torch
+        _dt = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
+    try:
+        return _dt[t]
+    except KeyError:
+        raise TrkError(f"element type {t}: float32, bfloat16 or float16 is needed") from None
+
+
+def _here(*tensors):
+    """Every tensor given is on the current device."""
+    global _device
+    if _device is None:
+        import torch
+        _device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+    at = [t.get_device() for t in tensors if t is not None]
+    if min(at) < 0:
+        raise TrkError("tensors have to be on the GPU")
+    dev = _device()
+    if at.count(dev) != len(at):
+        raise TrkError(f"tensors on devices {sorted(set(at))}: all have to be on the current device, {dev}")
+
+
+def _rows(t, what, m=None, k=None):
+    """The stride between the rows of a matrix with contiguous rows, [m][k] where they are given."""
+    if t.dim() != 2 or (m is not None and t.shape[0] != m) or (k is not None and t.shape[1] != k):
+        raise TrkError(f"{what}: shape {tuple(t.shape)}, [{'m' if m is None else m}][{'k' if k is None else k}] is needed")
+    s = t.stride()
+    if s[1] != 1 and t.shape[1] > 1:
+        raise TrkError(f"{what}: the values of a row have to be contiguous")
+    if t.shape[0] > 1:
+        return s[0]
+    return max(s[0], (t.shape[1] + 15) // 16 * 16)  # of one row: any that the checks take
+
+
+def _vector(t, what, dtype, *shape):
+    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+        raise TrkError(f"{what}: a contiguous {dtype} tensor of shape {shape} is needed, not {t.dtype} {tuple(t.shape)}")
+
+
+def _i8_empty(rows, k, device):
+    """int8 [rows][k], rows a multiple of 16 bytes apart."""
+    import torch
+    ld = (k + 15) // 16 * 16
+    q = torch.empty((rows, ld), dtype=torch.int8, device=device)
+    return q if ld == k else q[:, :k]
+
+
+class I8Weights:
+    """A stack of int8 matrices with a scale per row (trk_i8_mat): q int8 [count][rows][k] or [rows][k], its rows and
+    matrices a multiple of 16 bytes apart (`quantize_weights` makes them so), scale float32 [count][rows] or [rows].
+    Keeps the tensors; copies nothing."""
+
+    def __init__(self, q, scale):
+        import torch
+        if q.dtype != torch.int8 or q.dim() not in (2, 3):
+            raise TrkError(f"weights: int8 [count][rows][k] or [rows][k] is needed, not {q.dtype} {tuple(q.shape)}")
+        _vector(scale, "weight scales", torch.float32, *q.shape[:-1])
+        if min(q.shape) == 0:
+            raise TrkError(f"weights: empty shape {tuple(q.shape)}")
+        if q.shape[-1] > 1 and q.stride(-1) != 1:
+            raise TrkError("weights: the values of a row have to be contiguous")
+        _here(q, scale)
+        self.q, self.scale = q, scale
+        self.count = q.shape[0] if q.dim() == 3 else 1
+        self.rows, self.k = q.shape[-2:]
+        ld = q.stride(-2) if self.rows > 1 else max(q.stride(-2), (self.k + 15) // 16 * 16)
+        if self.k % 16:
+            _whole_pieces(q, 1, 0, (q.stride(0) * (self.count - 1) if self.count > 1 else 0) + ld * (self.rows - 1) + self.k,
+                          "weights")
+        self.mat = I8Mat(q.data_ptr(), scale.data_ptr(), self.rows, self.k, self.count, ld,
+                         q.stride(0) if self.count > 1 else 0)
+        self.ref = C.byref(self.mat)
+        self.device = q.get_device()
+
+
+def quantize_weights(w, stream=None):
+    """float [count][rows][k] or [rows][k] -> I8Weights: each row quantised as `quantize_rows` does."""
+    flat = w.reshape(-1, w.shape[-1])
+    q, s = quantize_rows(flat, stream=stream)
+    q = q.as_strided((*w.shape[:-1], w.shape[-1]), (*[q.stride(0) * w.shape[-2]] * (w.dim() - 2), q.stride(0), 1))
+    return I8Weights(q, s.view(w.shape[:-1]))
+
+
+def route_scores(logits, k, bias=None, score="sigmoid", n_group=1, topk_group=1, group_top=2, renorm=True, factor=1.0,
+                 out=None, stream=None):
+    """trk_route_scores: logits [m][E] -> (ids [m][32], w [m][32], n_sel [m]); slots k .. 31 are not written."""
+    import torch
+    if logits.dim() != 2 or logits.dtype != torch.float32 or not logits.is_contiguous():
+        raise TrkError(f"logits: contiguous float32 [m][E] is needed, not {logits.dtype} {tuple(logits.shape)}")
+    m, E = logits.shape
+    if bias is not None:
+        _vector(bias, "bias", torch.float32, E)
+    if score not in SCORES:
+        raise TrkError(f"score {score!r}: softmax or sigmoid")
+    dev = logits.device
+    if out is None:
+        ids = torch.empty((m, K_MAX), dtype=torch.int32, device=dev)
+        w = torch.empty((m, K_MAX), dtype=torch.float32, device=dev)
+        n = torch.empty(m, dtype=torch.int32, device=dev)
+    else:
+        ids, w, n = out
+        _routing(ids, n, m, w)
+    _here(logits, bias, ids, w, n)
+    p = ScorePolicy(k, SCORES[score], n_group, topk_group, group_top, int(renorm), factor)
+    check(lib().trk_route_scores(logits.data_ptr(), _ptr(bias), m, E, C.byref(p), ids.data_ptr(), w.data_ptr(),
+                                 n.data_ptr(), _stream(stream)))
+    return ids, w, n
+
+
+def _routing(ids, n_sel, m, w=None):
+    import torch
+    _vector(ids, "ids", torch.int32, m, K_MAX)
+    _vector(n_sel, "n_sel", torch.int32, m)
+    if w is not None:
+        _vector(w, "w", torch.float32, m, K_MAX)
+
+
+def quantize_rows(x, out=None, stream=None):
+    """trk_quantize_rows: x [m][k] -> (q int8 [m][k], scale [m]); the rows of a new q are a multiple of 16 bytes apart."""
+    import torch
+    ldx = _rows(x, "x")
+    m, k = x.shape
+    if out is None:
+        q, scale = _i8_empty(m, k, x.device), torch.empty(m, dtype=torch.float32, device=x.device)
+        ldq = (k + 15) // 16 * 16
+    else:
+        q, scale = out
+        ldq = _i8_rows(q, scale, m, k, read=False)
+    _here(x, q, scale)
+    check(lib().trk_quantize_rows(x.data_ptr(), _dtype(x.dtype), ldx, m, k, q.data_ptr(), ldq, scale.data_ptr(),
+                                  _stream(stream)))
+    return q, scale
+
+
+def _i8_rows(q, scale, m, k, read=True):
+    import torch
+    if q.dtype != torch.int8:
+        raise TrkError(f"q: int8 is needed, not {q.dtype}")
+    ld = _rows(q, "q", m, k)
+    _vector(scale, "scale", torch.float32, m)
+    if read and k % 16:
+        _whole_pieces(q, m, ld, k, "q")
+    return ld
+
+
+def _whole_pieces(q, rows, ld, k, what):
+    """The last row's last 16-byte piece lies inside the tensor's storage."""
+    if rows and q.storage_offset() + (rows - 1) * ld + (k + 15) // 16 * 16 > q.untyped_storage().nbytes():
+        raise TrkError(f"{what}: rows are read in 16-byte pieces, and the storage ends inside the last one")
+
+
+def gemm_i8(w: I8Weights, q, scale, bias=None, dtype=None, out=None, accumulate=False, item=0, stream=None):
+    """trk_gemm_i8: q int8 [m][k] with a scale per row, times matrix `item` of w -> [m][rows] (float32 unless `dtype` or
+    `out` says otherwise)."""
+    import torch
+    m = q.shape[0]
+    ldq = _i8_rows(q, scale, m, w.k)
+    if bias is not None:
+        _vector(bias, "bias", torch.float32, w.rows)
+    if out is None:
+        if accumulate:
+            raise TrkError("accumulate needs the output that is added to")
+        out = torch.empty((m, w.rows), dtype=dtype or torch.float32, device=q.device)
+        ldy = w.rows
+    else:
+        ldy = _rows(out, "out", m, w.rows)
+    _here(q, scale, bias, out, w.q)
+    check(lib().trk_gemm_i8(w.ref, item, q.data_ptr(), ldq, scale.data_ptr(), m, _ptr(bias), out.data_ptr(),
+                            _dtype(out.dtype), ldy, int(accumulate), _stream(stream)))
+    return out
+
+
+def experts_plan(ids, n_sel, slots, n_expert, stream=None):
+    """trk_experts_plan: the entries sorted by expert, for `experts_up_i8` and `experts_down_i8` of the same routing; None
+    where the entries are so few that the products take none."""
+    import torch
+    m = ids.shape[0]
+    _routing(ids, n_sel, m)
+    words = C.c_uint64()
+    check(lib().trk_experts_plan_words(m, slots, n_expert, C.byref(words)))
+    if not words.value:
+        return None
+    _here(ids, n_sel)
+    plan = torch.empty(words.value, dtype=torch.int32, device=ids.device)
+    check(lib().trk_experts_plan(ids.data_ptr(), n_sel.data_ptr(), m, slots, n_expert, plan.data_ptr(), _stream(stream)))
+    return plan
+
+
+def _check_plan(plan, m, slots, count):
+    import torch
+    words = C.c_uint64()
+    check(lib().trk_experts_plan_words(m, slots, count, C.byref(words)))
+    if words.value:
+        if plan is None:
+            raise TrkError(f"{m} tokens of {slots} slots need a plan (experts_plan)")
+        _vector(plan, "plan", torch.int32, words.value)
+
+
+def experts_up_i8(gate: I8Weights, up: I8Weights, q, scale, ids, n_sel, slots, plan=None, dtype=None, out=None,
+                  stream=None):
+    """trk_experts_up_i8: q int8 [m][H] through each token's experts -> h [m * slots][F]; rows that are no entry's are not
+    written."""
+    import torch
+    m = q.shape[0]
+    ldq = _i8_rows(q, scale, m, gate.k)
+    _routing(ids, n_sel, m)
+    _check_plan(plan, m, slots, gate.count)
+    if out is None:
+        out = torch.empty((m * slots, gate.rows), dtype=dtype or torch.float32, device=q.device)
+        ldh = gate.rows
+    else:
+        ldh = _rows(out, "out", m * slots, gate.rows)
+    _here(q, scale, ids, n_sel, plan, out, gate.q, up.q)
+    check(lib().trk_experts_up_i8(gate.ref, up.ref, q.data_ptr(), ldq, scale.data_ptr(), m, ids.data_ptr(),
+                                  n_sel.data_ptr(), slots, _ptr(plan), out.data_ptr(), _dtype(out.dtype), ldh,
+                                  _stream(stream)))
+    return out
+
+
+def experts_down_i8(down: I8Weights, q, scale, ids, w, n_sel, slots, plan=None, dtype=None, out=None, work=None,
+                    accumulate=False, stream=None):
+    """trk_experts_down_i8: q int8 [m * slots][F] through the experts' down rows, weighted with w and summed per token ->
+    [m][H].  work: at least trk_experts_down_work_bytes as a float32 tensor, allocated where it is not given."""
+    import torch
+    m = ids.shape[0]
+    ldq = _i8_rows(q, scale, m * slots, down.k)
+    _routing(ids, n_sel, m, w)
+    _check_plan(plan, m, slots, down.count)
+    if out is None:
+        if accumulate:
+            raise TrkError("accumulate needs the output that is added to")
+        out = torch.empty((m, down.rows), dtype=dtype or torch.float32, device=q.device)
+        ldy = down.rows
+    else:
+        ldy = _rows(out, "out", m, down.rows)
+    need = C.c_uint64()
+    check(lib().trk_experts_down_work_bytes(m, slots, down.count, down.rows, C.byref(need)))
+    if work is None:
+        work = torch.empty(need.value // 4, dtype=torch.float32, device=q.device) if need.value else None
+    elif work.dtype != torch.float32 or not work.is_contiguous() or work.numel() * 4 < need.value:
+        raise TrkError(f"work: {need.value // 4} contiguous float32 values are needed")
+    _here(q, scale, ids, w, n_sel, plan, work, out, down.q)
+    check(lib().trk_experts_down_i8(down.ref, q.data_ptr(), ldq, scale.data_ptr(), m, ids.data_ptr(), w.data_ptr(),
+                                    n_sel.data_ptr(), slots, _ptr(plan), _ptr(work), out.data_ptr(), _dtype(out.dtype),
+                                    ldy, int(accumulate), _stream(stream)))
+    return out
 
 
 def swiglu(g, u, stream=None):
