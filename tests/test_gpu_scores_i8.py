@@ -218,7 +218,7 @@ def run_gemm(rng, m, rows, k, dtype, bias, spare=0, q=None, w=None):
 @pytest.mark.parametrize("m,rows,k", [(1, 1, 1), (1, 16, 64), (2, 17, 15), (16, 33, 16), (17, 100, 129), (65, 5, 1000),
                                       (130, 130, 257), (300, 260, 640), (1, 4099, 2560), (5, 4099, 2561), (33, 1030, 511),
                                       (64, 2048, 2048), (129, 384, 4096), (256, 256, 127), (1000, 513, 128),
-                                      (513, 1537, 1055)])
+                                      (513, 1537, 1055), (4001, 4093, 200)])  # the largest tiles, ragged everywhere
 @pytest.mark.parametrize("dtype,bias", [("f32", False), ("bf16", True), ("f16", False)])
 def test_gemm_i8(m, rows, k, dtype, bias):
     say(f"gemm_i8 m={m} rows={rows} k={k} {dtype} bias={bias}")
@@ -235,12 +235,11 @@ def test_gemm_i8_largest_sum(m, rows):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("m", [3, 50, 400])
-def test_gemm_i8_accumulates_and_takes_an_item(dtype, m):
+@pytest.mark.parametrize("m,rows,k", [(3, 200, 300), (50, 200, 300), (400, 200, 300), (1000, 2050, 300), (4001, 4093, 200)])
+def test_gemm_i8_accumulates_and_takes_an_item(dtype, m, rows, k):
     import torch
-    say(f"gemm_i8 accumulate {dtype} m={m}")
+    say(f"gemm_i8 accumulate {dtype} m={m} rows={rows}")
     rng = np.random.default_rng(m)
-    rows, k = 200, 300
     w, ws = i8(rng, 3, rows, k), scales(rng, 3, rows, around=0.01)
     q, s = i8(rng, m, k), scales(rng, m)
     W = trmoe.I8Weights(padded(w), dev(ws))

@@ -8,6 +8,8 @@
 
 #include <stdint.h>
 
+#include <initializer_list>
+
 namespace trk {
 namespace geo {
 
@@ -175,6 +177,45 @@ inline bool gemv_tiles(uint64_t workgroups, uint32_t tq, uint32_t k) {  // tq: 0
     if (tq == 0 || k <= (bits == 4 ? 1024u : tq == 0x810 ? 512u : 768u)) return workgroups >= 1792;
     if (bits == 4 && k <= 3072) return workgroups >= 1920;
     return workgroups > (bits == 8 && k > 3072 ? 2303u : 2048u);
+}
+
+// trk_gemm_i8 (k_i8.hip): 16-row strips whose waves share K, or tiles of weight rows x tokens through LDS (256 x 256,
+// 128 x 128, 64 x 64, 64 x 32).
+enum I8Form { I8_STRIP, I8_TILE_32, I8_TILE_64, I8_TILE_128, I8_TILE_256 };
+inline uint64_t i8_tiles(uint64_t rows, uint64_t m, uint32_t bn, uint32_t bm) {
+    return (rows + bn - 1) / bn * ((m + bm - 1) / bm);
+}
+// Strips have every wave's share of K in flight at once and win while each has a CU of its own; beyond it the weights come
+// faster through LDS.  us, strips / 64 x 32 tiles, k = 512 and 2560: [1024] x 16 rows (64 strips) 2.6 / 3.1 and 4.2 / 6.2,
+// [2560] x 16 (160) 2.7 / 3.1 and 4.8 / 6.4, [5000] x 1 (313) 2.6 / 3.0 and 5.4 / 6.5, x 16 3.1 / 3.1 and 7.1 / 6.5,
+// [12288] x 1 (768) 3.5 / 3.6 and 7.2 / 7.0, x 16 4.0 / 3.8 and 9.3 / 7.1.
+inline bool i8_strips(uint32_t m, uint32_t rows) {
+    const uint64_t wgs = i8_tiles(rows, m, 16, 16);
+    return wgs <= 256 || (m <= 4 && wgs <= 512);
+}
+// A tile's time in ns: what it takes to begin and end, and each of its stages (128 bytes of k); n tiles of a CU share it.
+// Fitted to, us at 256 x 256 / 128 x 128 / 64 x 64 / 64 x 32: [512] x 48, k = 512 9.0 / 5.9 / 3.9 / 3.4 and k = 4096
+// 42 / 23 / 10.4 / 8.7; [2560] x 400, k = 4096 49 / 27 / 13.7 / 17.5; [12288] x 512, k = 2560 41 / 26 / 33 / 43; [6000] x
+// 1600, k = 512 15.9 / 15.7 / 18.4 / 26 and k = 4096 49 / 57 / 65 / 89; [12288] x 1024, k = 2560 42 / 47 / 59 / 83,
+// x 4096 125 / 148 / 219 / 315; 8192 cubed 423 / 506 / 824 / 1162.
+inline uint64_t i8_tile_ns(I8Form f, uint32_t m, uint32_t rows, uint32_t k) {
+    const uint64_t S = (k + 127) / 128;
+    auto per_cu = [&](uint32_t bn, uint32_t bm) { return (i8_tiles(rows, m, bn, bm) + 255) / 256; };
+    if (f == I8_TILE_256) return per_cu(256, 256) * (10000 + 1450 * S);
+    if (f == I8_TILE_128) {  // two resident on a CU
+        const uint64_t n = per_cu(128, 128);
+        return 1500 + n / 2 * (5500 + 850 * S) + n % 2 * (2500 + 660 * S);
+    }
+    if (f == I8_TILE_64) return 2000 + per_cu(64, 64) * (900 + 190 * S);
+    return 2000 + per_cu(64, 32) * (500 + 155 * S);
+}
+inline I8Form gemm_i8_form(uint32_t m, uint32_t rows, uint32_t k, uint64_t ldw, uint64_t ldq) {
+    // the tiles address their rows by 32-bit offsets from the first
+    if (ldw >= 1u << 23 || ldq >= 1u << 23 || i8_strips(m, rows)) return I8_STRIP;
+    I8Form best = I8_TILE_32;
+    for (I8Form f : {I8_TILE_64, I8_TILE_128, I8_TILE_256})
+        if (i8_tile_ns(f, m, rows, k) < i8_tile_ns(best, m, rows, k)) best = f;
+    return best;
 }
 
 // The int8 experts' plan (k_i8x.hip): entries sorted by expert and cut into tiles of at most plan_rows entries of one

@@ -1,5 +1,5 @@
 // Rows quantised as a whole (trk_quantize_rows) and the dense int8 product (trk_gemm_i8).
-#include "i8.hpp"
+#include "i8tile.hpp"
 
 namespace trk {
 
@@ -52,40 +52,137 @@ __global__ __launch_bounds__(QUANT_T) void quantize_whole_rows_kernel(const type
 // the dense product
 // ============================================================================================
 
-// A workgroup takes 16 weight rows and up to 16 tokens: its waves share K, 64 bytes at a time, and add their sums in
-// LDS.
-constexpr uint32_t ST_WAVES = 4;
+constexpr uint32_t ST_WAVES = 4;  // 8 or 16 waves are as fast from one row of 2560 values to 16 of 10240
 
+// A workgroup takes 16 weight rows and up to 16 tokens: its waves share K and add their sums in LDS.
 template <uint32_t DT>
-__global__ __launch_bounds__(ST_WAVES * WAVE) void gemm_i8_strip_kernel(I8Gemm g) {
+__global__ __launch_bounds__(ST_WAVES* WAVE) void gemm_i8_strip_kernel(I8Gemm g) {
     __shared__ int32_t part[ST_WAVES][16][16];  // [wave][token][weight row]
     const uint32_t strips = (g.rows + 15) / 16, id = run_id();
     const uint32_t r0 = id % strips * 16, t0 = id / strips * 16;
     if (t0 >= g.m) return;  // the whole workgroup
-    const uint32_t wv = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, c = lane % 16, kg = lane / 16 * 16;
+    const uint32_t wv = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, c = lane % 16;
     const int8_t* wr = g.w + (r0 + c < g.rows ? r0 + c : g.rows - 1) * g.ldw;
     const int8_t* xr = g.q + (uint64_t)(t0 + c < g.m ? t0 + c : g.m - 1) * g.ldq;
-    i32x4 acc = {0, 0, 0, 0};
-    for (uint32_t at = wv * 64; at < g.k; at += ST_WAVES * 64) {
-        const uint32_t o = at + kg, n = o < g.k ? (g.k - o < 16 ? g.k - o : 16) : 0, oc = n ? o : 0;
-        acc = mfma_i8(*reinterpret_cast<const i32x4*>(wr + oc),
-                      first_bytes(*reinterpret_cast<const i32x4*>(xr + oc), n), acc);
-    }
-    *reinterpret_cast<i32x4*>(&part[wv][c][lane / 16 * 4]) = acc;
-    __syncthreads();
     const uint32_t t = t0 + threadIdx.x / 16, r = r0 + threadIdx.x % 16;
-    if (t >= g.m || r >= g.rows) return;
+    const bool out = threadIdx.x < 256 && t < g.m && r < g.rows;
+    float sx = 0.0f, sw = 0.0f, b = 0.0f;
+    if (out) sx = g.sx[t], sw = g.sw[r], b = g.bias ? g.bias[r] : 0.0f;
+    *reinterpret_cast<i32x4*>(&part[wv][c][lane / 16 * 4]) = strip_sum(wr, xr, g.k, wv, ST_WAVES, lane);
+    __syncthreads();
+    if (!out) return;
     int32_t sum = 0;
 #pragma unroll
     for (uint32_t i = 0; i < ST_WAVES; i++) sum += part[i][threadIdx.x / 16][threadIdx.x % 16];
     typedef Elem<DT> O;
     typename O::T* y = reinterpret_cast<typename O::T*>(g.y) + t * g.ldy + r;
-    float v = i8_scaled(sum, g.sx[t], g.sw[r]);
-    if (g.bias) v += g.bias[r];
+    float v = i8_scaled(sum, sx, sw);
+    if (g.bias) v += b;
     if (g.accumulate) v += O::get(*y);
     *y = O::put(v);
 }
 
+void launch_strip(const I8Gemm& a, hipStream_t st) {
+    const uint64_t wgs = (uint64_t)((a.rows + 15) / 16) * (((uint64_t)a.m + 15) / 16);
+    const geo::Grid2 g = geo::grid_run(wgs, ST_WAVES * WAVE);
+    const dim3 grid(g.x, g.y);
+    if (a.dt == TRK_DT_F32)
+        gemm_i8_strip_kernel<TRK_DT_F32><<<grid, ST_WAVES * WAVE, 0, st>>>(a);
+    else if (a.dt == TRK_DT_BF16)
+        gemm_i8_strip_kernel<TRK_DT_BF16><<<grid, ST_WAVES * WAVE, 0, st>>>(a);
+    else
+        gemm_i8_strip_kernel<TRK_DT_F16><<<grid, ST_WAVES * WAVE, 0, st>>>(a);
+}
+
+// The tiles' place in the launch: panels of eight weight tiles, activation tiles after one another inside each, so that
+// the tiles that run at once on an XCD (a contiguous run of them) share rows of both in its L2.
+__device__ __forceinline__ void tile_place(uint32_t idx, uint32_t tn, uint32_t tm, uint32_t& n, uint32_t& m) {
+    const uint32_t panel = idx / (8 * tm), left = tn - panel * 8, w = left < 8 ? left : 8, rem = idx - panel * 8 * tm;
+    n = panel * 8 + rem % w, m = rem / w;
+}
+
+template <typename Tile, uint32_t DT>
+__global__ __launch_bounds__(Tile::T) void gemm_i8_tile_kernel(I8Gemm g) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[Tile::LDS];
+    const uint32_t tn = (g.rows + Tile::BN - 1) / Tile::BN, tm = (g.m + Tile::BM - 1) / Tile::BM;
+    uint32_t idx, n, m;
+    if (!xcd_order_1d(tn * tm, idx, run_id())) return;  // the whole workgroup
+    tile_place(idx, tn, tm, n, m);
+    const uint32_t r0 = n * Tile::BN, t0 = m * Tile::BM, rl = g.rows - r0 - 1, tl = g.m - t0 - 1;  // the last rows there are
+    Tile t;
+    i32x4 rw[Tile::NA];
+    uint32_t wo[Tile::NA], xo[Tile::NB];
+#pragma unroll
+    for (int i = 0; i < Tile::NA; i++) {
+        const uint32_t r = t.load_row(i);
+        rw[i] = buffer_at(g.w + r0 * g.ldw), wo[i] = (r < rl ? r : rl) * (uint32_t)g.ldw;
+    }
+#pragma unroll
+    for (int i = 0; i < Tile::NB; i++) {
+        const uint32_t r = t.load_row(i);
+        xo[i] = (r < tl ? r : tl) * (uint32_t)g.ldq;
+    }
+    t.run(lds, rw, wo, buffer_at(g.q + t0 * g.ldq), xo, g.k, [&](int i) { return t.wn + 16 * i; });
+    // every scale first (rows past the end: the last one's), so that the stores wait for memory once
+    typedef Elem<DT> O;
+    float sw[Tile::FN][4], bias[Tile::FN][4], sx[Tile::FM];
+    auto col = [&](int i, int c) {
+        const uint32_t r = t.wn + 16 * i + t.lane / 16 * 4 + c;
+        return r0 + (r < rl ? r : rl);
+    };
+#pragma unroll
+    for (int i = 0; i < Tile::FN; i++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) sw[i][c] = g.sw[col(i, c)], bias[i][c] = g.bias ? g.bias[col(i, c)] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < Tile::FM; j++) {
+        const uint32_t row = t.wm + 16 * j + t.lane % 16;
+        sx[j] = g.sx[t0 + (row < tl ? row : tl)];
+    }
+#pragma unroll
+    for (int j = 0; j < Tile::FM; j++) {
+        const uint32_t row = t0 + t.wm + 16 * j + t.lane % 16;
+        if (row >= g.m) continue;
+        typename O::T* y = reinterpret_cast<typename O::T*>(g.y) + row * g.ldy;
+        float v[Tile::FN][4];
+#pragma unroll
+        for (int i = 0; i < Tile::FN; i++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                v[i][c] = i8_scaled(t.acc[i][j][c], sx[j], sw[i][c]);
+                if (g.bias) v[i][c] += bias[i][c];
+            }
+        if (g.accumulate) {
+            typename O::T old[Tile::FN][4];
+#pragma unroll
+            for (int i = 0; i < Tile::FN; i++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) old[i][c] = y[col(i, c)];
+#pragma unroll
+            for (int i = 0; i < Tile::FN; i++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) v[i][c] += O::get(old[i][c]);
+        }
+#pragma unroll
+        for (int i = 0; i < Tile::FN; i++) {
+            const uint32_t r = r0 + t.wn + 16 * i + t.lane / 16 * 4;
+            store4<DT>(y + r, v[i], r < g.rows ? g.rows - r : 0, g.vec);
+        }
+    }
+}
+
+template <typename Tile>
+void launch_tile(const I8Gemm& a, hipStream_t st) {
+    const uint64_t wgs = (uint64_t)((a.rows + Tile::BN - 1) / Tile::BN) * (((uint64_t)a.m + Tile::BM - 1) / Tile::BM);
+    const geo::Grid2 g = geo::grid_run(wgs, Tile::T);
+    const dim3 grid(g.x, g.y);
+    if (a.dt == TRK_DT_F32)
+        gemm_i8_tile_kernel<Tile, TRK_DT_F32><<<grid, Tile::T, 0, st>>>(a);
+    else if (a.dt == TRK_DT_BF16)
+        gemm_i8_tile_kernel<Tile, TRK_DT_BF16><<<grid, Tile::T, 0, st>>>(a);
+    else
+        gemm_i8_tile_kernel<Tile, TRK_DT_F16><<<grid, Tile::T, 0, st>>>(a);
+}
 }  // namespace
 
 hipError_t launch_quantize_rows(const void* x, uint32_t dt, uint64_t ldx, uint32_t m, uint32_t k, int8_t* q,
@@ -102,15 +199,13 @@ hipError_t launch_quantize_rows(const void* x, uint32_t dt, uint64_t ldx, uint32
 }
 
 hipError_t launch_gemm_i8(const I8Gemm& a, hipStream_t st) {
-    const uint64_t wgs = (uint64_t)((a.rows + 15) / 16) * (((uint64_t)a.m + 15) / 16);
-    const geo::Grid2 g = geo::grid_run(wgs, ST_WAVES * WAVE);
-    const dim3 grid(g.x, g.y);
-    if (a.dt == TRK_DT_F32)
-        gemm_i8_strip_kernel<TRK_DT_F32><<<grid, ST_WAVES * WAVE, 0, st>>>(a);
-    else if (a.dt == TRK_DT_BF16)
-        gemm_i8_strip_kernel<TRK_DT_BF16><<<grid, ST_WAVES * WAVE, 0, st>>>(a);
-    else
-        gemm_i8_strip_kernel<TRK_DT_F16><<<grid, ST_WAVES * WAVE, 0, st>>>(a);
+    switch (geo::gemm_i8_form(a.m, a.rows, a.k, a.ldw, a.ldq)) {
+    case geo::I8_TILE_256: launch_tile<I8Tile<256, 256, 64, 128, 2>>(a, st); break;
+    case geo::I8_TILE_128: launch_tile<I8Tile<128, 128, 64, 64, 2>>(a, st); break;
+    case geo::I8_TILE_64: launch_tile<I8Tile<64, 64, 32, 32, 4>>(a, st); break;
+    case geo::I8_TILE_32: launch_tile<I8Tile<64, 32, 16, 32, 4>>(a, st); break;
+    default: launch_strip(a, st);
+    }
     return hipGetLastError();
 }
 

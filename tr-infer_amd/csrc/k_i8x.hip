@@ -56,19 +56,10 @@ __global__ __launch_bounds__(PLAN_T) void experts_plan_kernel(const uint32_t* __
 
 constexpr uint32_t ST_WAVES = 4;
 
-// The exact sums of 16 weight rows (r0 ..) with up to 16 activation rows (xr: this lane's, row lane % 16), this wave's
-// share of K.
-__device__ __forceinline__ i32x4 strip_sum(const I8Mat& w, uint32_t e, uint32_t r0, const int8_t* xr, uint32_t first,
-                                           uint32_t step, uint32_t lane) {
-    const uint32_t r = r0 + lane % 16, kg = lane / 16 * 16;
-    const int8_t* wr = w.ptr + e * w.stride + (r < w.rows ? r : w.rows - 1) * w.ld;
-    i32x4 acc = {0, 0, 0, 0};
-    for (uint32_t at = first * 64; at < w.k; at += step * 64) {
-        const uint32_t o = at + kg, n = o < w.k ? (w.k - o < 16 ? w.k - o : 16) : 0, oc = n ? o : 0;
-        acc = mfma_i8(*reinterpret_cast<const i32x4*>(wr + oc),
-                      first_bytes(*reinterpret_cast<const i32x4*>(xr + oc), n), acc);
-    }
-    return acc;
+// This lane's row of the 16 from r0 on
+__device__ __forceinline__ const int8_t* strip_row(const I8Mat& w, uint32_t e, uint32_t r0, uint32_t lane) {
+    const uint32_t r = r0 + lane % 16;
+    return w.ptr + e * w.stride + (r < w.rows ? r : w.rows - 1) * w.ld;
 }
 
 // A workgroup takes 16 rows of gate and up and a tile's (or, without a plan, one) entries; its waves share K.
@@ -92,8 +83,8 @@ __global__ __launch_bounds__(ST_WAVES * WAVE) void experts_up_strip_kernel(I8Up 
     __syncthreads();
     const uint32_t wv = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, c = lane % 16;
     const int8_t* xr = a.q + (uint64_t)(ent[c] / a.slots) * a.ldq;
-    *reinterpret_cast<i32x4*>(&part[0][wv][c][lane / 16 * 4]) = strip_sum(a.gate, e, r0, xr, wv, ST_WAVES, lane);
-    *reinterpret_cast<i32x4*>(&part[1][wv][c][lane / 16 * 4]) = strip_sum(a.up, e, r0, xr, wv, ST_WAVES, lane);
+    *reinterpret_cast<i32x4*>(&part[0][wv][c][lane / 16 * 4]) = strip_sum(strip_row(a.gate, e, r0, lane), xr, a.gate.k, wv, ST_WAVES, lane);
+    *reinterpret_cast<i32x4*>(&part[1][wv][c][lane / 16 * 4]) = strip_sum(strip_row(a.up, e, r0, lane), xr, a.gate.k, wv, ST_WAVES, lane);
     __syncthreads();
     const uint32_t ei = threadIdx.x / 16, ri = threadIdx.x % 16, r = r0 + ri;
     if (ei >= n || r >= a.gate.rows) return;
@@ -119,7 +110,7 @@ __global__ __launch_bounds__(ST_WAVES * WAVE) void experts_down_strip_kernel(I8D
         const uint32_t e = a.ids[(size_t)t * K_MAX + j];
         if (e >= a.down.count) continue;
         const uint64_t row = (uint64_t)t * a.slots + j;
-        const i32x4 s = strip_sum(a.down, e, r0, a.q + row * a.ldq, 0, 1, lane);
+        const i32x4 s = strip_sum(strip_row(a.down, e, r0, lane), a.q + row * a.ldq, a.down.k, 0, 1, lane);
         if (lane % 16 == 0)
 #pragma unroll
             for (uint32_t i = 0; i < 4; i++) {
@@ -154,7 +145,7 @@ __global__ __launch_bounds__(ST_WAVES * WAVE) void experts_down_tile_kernel(I8Do
     __syncthreads();
     const uint32_t wv = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, c = lane % 16;
     *reinterpret_cast<i32x4*>(&part[wv][c][lane / 16 * 4]) =
-            strip_sum(a.down, t.expert, r0, a.q + (uint64_t)ent[c] * a.ldq, wv, ST_WAVES, lane);
+            strip_sum(strip_row(a.down, t.expert, r0, lane), a.q + (uint64_t)ent[c] * a.ldq, a.down.k, wv, ST_WAVES, lane);
     __syncthreads();
     const uint32_t ei = threadIdx.x / 16, ri = threadIdx.x % 16, r = r0 + ri;
     if (ei >= t.rows || r >= a.down.rows) return;
