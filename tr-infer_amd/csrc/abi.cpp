@@ -979,14 +979,14 @@ static int check_entries(uint32_t m, uint32_t slots, uint32_t n_expert) {
 extern "C" int trk_experts_plan_words(uint32_t m, uint32_t slots, uint32_t n_expert, uint64_t* words) {
     if (!words) return fail(TRK_E_INVALID, "null argument");
     if (int rc = check_entries(m, slots, n_expert)) return rc;
-    *words = geo::plan_used(m, slots, n_expert) ? geo::plan_words(m, slots, n_expert) : 0;
+    *words = geo::plan_used(m) ? geo::plan_words(m, slots, n_expert) : 0;
     return TRK_OK;
 }
 
 extern "C" int trk_experts_plan(const uint32_t* ids, const uint32_t* n_sel, uint32_t m, uint32_t slots,
                                 uint32_t n_expert, uint32_t* plan, void* stream) {
     if (int rc = check_entries(m, slots, n_expert)) return rc;
-    if (!geo::plan_used(m, slots, n_expert)) return TRK_OK;
+    if (!geo::plan_used(m)) return TRK_OK;
     if (!ids || !n_sel || !plan) return fail(TRK_E_INVALID, "null argument");
     if ((uintptr_t)plan % 16) return fail(TRK_E_INVALID, "plan must be 16-byte aligned");
     HIP_TRY(launch_experts_plan(ids, n_sel, m, slots, n_expert, plan, (hipStream_t)stream));
@@ -995,7 +995,7 @@ extern "C" int trk_experts_plan(const uint32_t* ids, const uint32_t* n_sel, uint
 
 // The plan of a call: NULL where the call takes none.
 static int check_plan(const uint32_t*& plan, uint32_t m, uint32_t slots, uint32_t n_expert) {
-    if (!geo::plan_used(m, slots, n_expert)) {
+    if (!geo::plan_used(m)) {
         plan = nullptr;
         return TRK_OK;
     }
@@ -1020,7 +1020,8 @@ extern "C" int trk_experts_up_i8(const trk_i8_mat* gate, const trk_i8_mat* up, c
     if (m == 0) return TRK_OK;
     if (!q || !scale || !ids || !n_sel || !h) return fail(TRK_E_INVALID, "null argument");
     if ((rc = check_plan(plan, m, slots, gate->count))) return rc;
-    const I8Up a{i8_mat(*gate), i8_mat(*up), q, ldq, scale, m, slots, ids, n_sel, h, dtype, ldh};
+    const int vec = (uintptr_t)h % (dtype == TRK_DT_F32 ? 16 : 8) == 0 && ldh % 4 == 0;
+    const I8Up a{i8_mat(*gate), i8_mat(*up), q, ldq, scale, m, slots, ids, n_sel, h, dtype, ldh, vec};
     HIP_TRY(launch_experts_up(a, plan, (hipStream_t)stream));
     return TRK_OK;
 }
@@ -1029,7 +1030,7 @@ extern "C" int trk_experts_down_work_bytes(uint32_t m, uint32_t slots, uint32_t 
                                            uint64_t* bytes) {
     if (!bytes) return fail(TRK_E_INVALID, "null argument");
     if (int rc = check_entries(m, slots, n_expert)) return rc;
-    *bytes = geo::plan_used(m, slots, n_expert) ? 4ull * m * slots * rows : 0;
+    *bytes = geo::plan_used(m) ? 4ull * m * slots * rows : 0;
     return TRK_OK;
 }
 
@@ -1048,7 +1049,8 @@ extern "C" int trk_experts_down_i8(const trk_i8_mat* down, const int8_t* q, uint
     if ((rc = check_plan(plan, m, slots, down->count))) return rc;
     if (plan && (!work || (uintptr_t)work % 16))
         return fail(TRK_E_INVALID, "work must be 16-byte aligned memory of trk_experts_down_work_bytes");
-    const I8Down a{i8_mat(*down), q, ldq, scale, m, slots, ids, n_sel, w, (float*)work, y, dtype, ldy, accumulate};
+    const int vec = (uintptr_t)y % (dtype == TRK_DT_F32 ? 16 : 8) == 0 && (m == 1 || ldy % 4 == 0);
+    const I8Down a{i8_mat(*down), q, ldq, scale, m, slots, ids, n_sel, w, (float*)work, y, dtype, ldy, accumulate, vec};
     HIP_TRY(launch_experts_down(a, plan, (hipStream_t)stream));
     return TRK_OK;
 }

@@ -218,23 +218,42 @@ inline I8Form gemm_i8_form(uint32_t m, uint32_t rows, uint32_t k, uint64_t ldw, 
     return best;
 }
 
-// The int8 experts' plan (k_i8x.hip): entries sorted by expert and cut into tiles of at most plan_rows entries of one
-// expert.  Words: {tiles, 3 unused}, ent [m * slots], then (16-byte aligned) four words per tile.
-inline bool plan_used(uint32_t m, uint32_t slots, uint32_t E) {
-    (void)slots, (void)E;
-    return m > 8;
-}
+// The int8 experts' products (k_i8x.hip): up to eight tokens each entry by itself, beyond it by a plan: entries sorted
+// by expert and cut into tiles of at most plan_rows entries of one expert.
+// us, up and down by themselves / planned (the plan included; H = 2048): 8 tokens of 10 in 512 experts of F = 512 52 / 58, of 8
+// in 128 of 768 60 / 67, of 2 in 8 of 1024 22 / 24; 16 tokens 90 / 89, 105 / 91 and 36 / 24.
+inline bool plan_used(uint32_t m) { return m > 8; }
+// us, up at 32 / 64 / 128 rows: 2 entries an expert (4 of 16 x 100 tokens: 25) 7.1 / 7.3 / 8.1, 62 (8 of 128 x 1000) 110 / 94
+// / 91, 80 (10 of 512 x 4096) 309 / 270 / 245; down at 10 entries (10 of 512 x 512) 134 / 139 / 154, at 62 93 / 88 / 89.
 inline uint32_t plan_rows(uint32_t m, uint32_t slots, uint32_t E) {
-    (void)m, (void)slots, (void)E;
-    return 16;
+    const uint64_t avg = (uint64_t)m * slots / E;
+    return avg <= 24 ? 32 : avg <= 48 ? 64 : 128;
 }
+// The tiles address weight rows from their block's first, activation rows from the first of all, by 32 bits.
+inline bool i8_tile_addresses(uint64_t ldw, uint64_t ldq, uint64_t rows) {
+    return ldw < 1u << 23 && ldq <= 0xffffffffull / rows;
+}
+// Up tiles of 128 entries: 256 weight rows from three workgroups per CU on, else 128 (two resident).  us, 256 / 128 rows:
+// 4096 tokens of 10 in 512 experts of F = 512 245 / 256, 1000 of 8 in 128 of 768 91 / 94; 3000 of 2 in 8 of 768 28 / 24.
+inline bool up_wide(uint32_t rows, uint64_t tiles) { return (rows + 127) / 128 * tiles >= 768; }
+// The plan's words: {tiles, 3 unused}, ent [m * slots], (16-byte aligned) four words per tile, then the counts of each of
+// plan_workgroups' entries [workgroups][E].
 inline uint64_t plan_tiles(uint32_t m, uint32_t slots, uint32_t E, uint32_t rows) {  // no call has more
     const uint64_t n = (uint64_t)m * slots;
     return (n < E ? n : E) + n / rows;
 }
 inline uint64_t plan_tile_at(uint32_t m, uint32_t slots) { return 4 + ((uint64_t)m * slots + 3) / 4 * 4; }
-inline uint64_t plan_words(uint32_t m, uint32_t slots, uint32_t E) {
+inline uint64_t plan_counts_at(uint32_t m, uint32_t slots, uint32_t E) {
     return plan_tile_at(m, slots) + 4 * plan_tiles(m, slots, E, plan_rows(m, slots, E));
+}
+// One workgroup sorts up to 4096 entries by itself (us, 1 / several: 3000 entries 6.1 / 7.5, 5120 8.2 / 7.1, 40960 42 / 9.3).
+inline uint32_t plan_workgroups(uint32_t m, uint32_t slots) {
+    const uint64_t n = (uint64_t)m * slots;
+    return n <= 4096 ? 1u : n > 65536 ? 64u : (uint32_t)((n + 1023) / 1024);
+}
+inline uint64_t plan_words(uint32_t m, uint32_t slots, uint32_t E) {
+    const uint32_t wgs = plan_workgroups(m, slots);
+    return plan_counts_at(m, slots, E) + (wgs > 1 ? (uint64_t)wgs * E : 0);
 }
 
 // Every invariant a call of m rows with kcap selections per token relies on; returns nullptr when

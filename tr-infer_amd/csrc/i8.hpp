@@ -28,38 +28,43 @@ __device__ __forceinline__ i32x4 first_bytes(i32x4 v, uint32_t n) {
     return v;
 }
 
-// U pieces of 64 bytes of both rows, all requested before the first is needed.
-template <uint32_t U>
-__device__ __forceinline__ i32x4 strip_pieces(const int8_t* __restrict__ wr, const int8_t* __restrict__ xr, uint32_t step,
-                                              i32x4 acc) {
-    i32x4 w[U], x[U];
+// U pieces of 64 bytes of an activation row and of NM matrices' rows, all requested before the first is needed.
+template <uint32_t U, uint32_t NM>
+__device__ __forceinline__ void strip_pieces(const int8_t* const (&wr)[NM], const int8_t* __restrict__ xr, uint32_t at,
+                                             uint32_t step, i32x4 (&acc)[NM]) {
+    i32x4 w[NM][U], x[U];
 #pragma unroll
     for (uint32_t u = 0; u < U; u++) {
-        w[u] = *reinterpret_cast<const i32x4*>(wr + u * step * 64);
-        x[u] = *reinterpret_cast<const i32x4*>(xr + u * step * 64);
-    }
+        x[u] = *reinterpret_cast<const i32x4*>(xr + at + u * step * 64);
 #pragma unroll
-    for (uint32_t u = 0; u < U; u++) acc = mfma_i8(w[u], x[u], acc);
-    return acc;
+        for (uint32_t i = 0; i < NM; i++) w[i][u] = *reinterpret_cast<const i32x4*>(wr[i] + at + u * step * 64);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // else some wait for others' registers
+#pragma unroll
+    for (uint32_t u = 0; u < U; u++)
+#pragma unroll
+        for (uint32_t i = 0; i < NM; i++) acc[i] = mfma_i8(w[i][u], x[u], acc[i]);
 }
 
-// The exact sums of 16 weight rows and 16 activation rows over this wave's share of K: every `step`-th 64 bytes from the
-// first-th on.  wr, xr: this lane's row of each (row lane % 16).
-__device__ __forceinline__ i32x4 strip_sum(const int8_t* __restrict__ wr, const int8_t* __restrict__ xr, uint32_t k,
-                                           uint32_t first, uint32_t step, uint32_t lane) {
-    i32x4 acc = {0, 0, 0, 0};
+// The exact sums of 16 weight rows of NM matrices and 16 activation rows over this wave's share of K: every `step`-th 64
+// bytes from the first-th on.  wr, xr: this lane's row of each (row lane % 16).
+template <uint32_t NM>
+__device__ __forceinline__ void strip_sums(const int8_t* const (&wr)[NM], const int8_t* __restrict__ xr, uint32_t k,
+                                           uint32_t first, uint32_t step, uint32_t lane, i32x4 (&acc)[NM]) {
+#pragma unroll
+    for (uint32_t i = 0; i < NM; i++) acc[i] = i32x4{0, 0, 0, 0};
     const uint32_t kg = lane / 16 * 16, whole = k / 64;
     uint32_t n = first < whole ? (whole - first + step - 1) / step : 0, at = first * 64 + kg;  // whole pieces of this wave
-    for (; n >= 8; n -= 8, at += 8 * step * 64) acc = strip_pieces<8>(wr + at, xr + at, step, acc);
-    if (n & 4) acc = strip_pieces<4>(wr + at, xr + at, step, acc), at += 4 * step * 64;
-    if (n & 2) acc = strip_pieces<2>(wr + at, xr + at, step, acc), at += 2 * step * 64;
-    if (n & 1) acc = strip_pieces<1>(wr + at, xr + at, step, acc);
+    for (; n >= 8; n -= 8, at += 8 * step * 64) strip_pieces<8, NM>(wr, xr, at, step, acc);
+    if (n & 4) strip_pieces<4, NM>(wr, xr, at, step, acc), at += 4 * step * 64;
+    if (n & 2) strip_pieces<2, NM>(wr, xr, at, step, acc), at += 2 * step * 64;
+    if (n & 1) strip_pieces<1, NM>(wr, xr, at, step, acc);
     if (k % 64 && whole % step == first) {  // the row's end
         const uint32_t o = whole * 64 + kg, oc = o < k ? o : 0;
-        acc = mfma_i8(*reinterpret_cast<const i32x4*>(wr + oc),
-                      first_bytes(*reinterpret_cast<const i32x4*>(xr + oc), o < k ? (k - o < 16 ? k - o : 16) : 0), acc);
+        const i32x4 x = first_bytes(*reinterpret_cast<const i32x4*>(xr + oc), o < k ? (k - o < 16 ? k - o : 16) : 0);
+#pragma unroll
+        for (uint32_t i = 0; i < NM; i++) acc[i] = mfma_i8(*reinterpret_cast<const i32x4*>(wr[i] + oc), x, acc[i]);
     }
-    return acc;
 }
 
 __device__ __forceinline__ float i8_scaled(int32_t acc, float sx, float sw) { return ((float)acc * sx) * sw; }

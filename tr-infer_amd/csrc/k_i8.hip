@@ -68,7 +68,9 @@ __global__ __launch_bounds__(ST_WAVES* WAVE) void gemm_i8_strip_kernel(I8Gemm g)
     const bool out = threadIdx.x < 256 && t < g.m && r < g.rows;
     float sx = 0.0f, sw = 0.0f, b = 0.0f;
     if (out) sx = g.sx[t], sw = g.sw[r], b = g.bias ? g.bias[r] : 0.0f;
-    *reinterpret_cast<i32x4*>(&part[wv][c][lane / 16 * 4]) = strip_sum(wr, xr, g.k, wv, ST_WAVES, lane);
+    i32x4 acc[1];
+    strip_sums<1>({wr}, xr, g.k, wv, ST_WAVES, lane, acc);
+    *reinterpret_cast<i32x4*>(&part[wv][c][lane / 16 * 4]) = acc[0];
     __syncthreads();
     if (!out) return;
     int32_t sum = 0;

@@ -1,5 +1,5 @@
 // The int8 products of each token with its experts (trk_experts_plan, trk_experts_up_i8, trk_experts_down_i8).
-#include "i8.hpp"
+#include "i8tile.hpp"
 
 namespace trk {
 
@@ -9,45 +9,86 @@ namespace {
 // the plan: entries sorted by expert
 // ============================================================================================
 
-constexpr uint32_t PLAN_T = 1024;
+constexpr uint32_t PLAN_T = 1024;  // threads, and the most experts
 
-// One workgroup: the entries of each expert counted in LDS, the counts summed to offsets, the entries put to their
-// places and every expert's run cut into tiles.  The order of an expert's entries is that of the atomics and may change;
-// nothing that the products write depends on it (an entry's row is computed by itself and kept at its own place).
-__global__ __launch_bounds__(PLAN_T) void experts_plan_kernel(const uint32_t* __restrict__ ids,
-                                                              const uint32_t* __restrict__ n_sel, uint32_t m,
-                                                              uint32_t slots, uint32_t E, uint32_t rows,
-                                                              uint32_t* __restrict__ plan) {
-    __shared__ uint32_t cnt[PLAN_T], tcnt[PLAN_T], wsum[2][PLAN_T / WAVE];
-    const uint32_t tid = threadIdx.x, lane = tid % WAVE, wv = tid / WAVE, n = m * slots;
-    cnt[tid] = 0;
+// The expert of entry i, ~0 for a slot that is none.
+__device__ __forceinline__ uint32_t entry_expert(const uint32_t* __restrict__ ids, const uint32_t* __restrict__ n_sel,
+                                                 uint32_t slots, uint32_t E, uint32_t i, uint32_t n) {
+    const uint32_t ic = i < n ? i : n - 1, t = ic / slots, j = ic % slots;
+    const uint32_t e = ids[(size_t)t * K_MAX + j], c = n_sel[t];  // both requested before either is looked at
+    return i < n && j < c && e < E ? e : 0xffffffffu;
+}
+
+// The counts of `per` * PLAN_T entries from i0 on, into cnt[] of LDS (zeroed here).
+__device__ __forceinline__ void plan_count(const uint32_t* __restrict__ ids, const uint32_t* __restrict__ n_sel, uint32_t slots,
+                                           uint32_t E, uint32_t n, uint32_t i0, uint32_t per, uint32_t* cnt) {
+    cnt[threadIdx.x] = 0;
     __syncthreads();
-    auto expert = [&](uint32_t i) {
-        const uint32_t t = i / slots, j = i % slots;
-        const uint32_t e = j < n_sel[t] ? ids[(size_t)t * K_MAX + j] : 0xffffffffu;
-        return e < E ? e : 0xffffffffu;
-    };
-    for (uint32_t i = tid; i < n; i += PLAN_T) {
-        const uint32_t e = expert(i);
-        if (e != 0xffffffffu) atomicAdd(&cnt[e], 1u);
+    for (uint32_t p = 0; p < per; p += 4) {
+        uint32_t e[4];
+#pragma unroll
+        for (uint32_t u = 0; u < 4; u++)
+            e[u] = p + u < per ? entry_expert(ids, n_sel, slots, E, i0 + (p + u) * PLAN_T + threadIdx.x, n) : 0xffffffffu;
+#pragma unroll
+        for (uint32_t u = 0; u < 4; u++)
+            if (e[u] != 0xffffffffu) atomicAdd(&cnt[e[u]], 1u);
     }
     __syncthreads();
-    const uint32_t c = cnt[tid], tc = (c + rows - 1) / rows;
+}
+
+// The counts of each workgroup's share of the entries, for the next kernel's offsets.
+__global__ __launch_bounds__(PLAN_T) void experts_count_kernel(const uint32_t* __restrict__ ids,
+                                                               const uint32_t* __restrict__ n_sel, uint32_t m,
+                                                               uint32_t slots, uint32_t E, uint32_t per,
+                                                               uint32_t* __restrict__ counts) {
+    __shared__ uint32_t cnt[PLAN_T];
+    plan_count(ids, n_sel, slots, E, m * slots, blockIdx.x * per * PLAN_T, per, cnt);
+    if (threadIdx.x < E) counts[blockIdx.x * E + threadIdx.x] = cnt[threadIdx.x];
+}
+
+// Counts summed to offsets (every workgroup for itself: `counts` [gridDim.x][E], or its own where it is the only one),
+// this workgroup's entries put to their places, and (the first) every expert's run cut into tiles.  The order of an
+// expert's entries is that of the LDS atomics and may change; nothing that the products write depends on it (an entry's
+// row is computed by itself and kept at its own place).
+__global__ __launch_bounds__(PLAN_T) void experts_plan_kernel(const uint32_t* __restrict__ ids,
+                                                              const uint32_t* __restrict__ n_sel, uint32_t m,
+                                                              uint32_t slots, uint32_t E, uint32_t rows, uint32_t per,
+                                                              const uint32_t* __restrict__ counts, Plan P) {
+    __shared__ uint32_t cnt[PLAN_T], wsum[2][PLAN_T / WAVE];
+    const uint32_t tid = threadIdx.x, lane = tid % WAVE, wv = tid / WAVE, n = m * slots, i0 = blockIdx.x * per * PLAN_T;
+    uint32_t c = 0, before = 0;  // expert tid's entries, and those of the workgroups before this one
+    if (gridDim.x == 1) {
+        plan_count(ids, n_sel, slots, E, n, 0, per, cnt);
+        c = cnt[tid];
+    } else if (tid < E) {
+#pragma unroll 8
+        for (uint32_t b = 0; b < gridDim.x; b++) {
+            const uint32_t v = counts[b * E + tid];
+            c += v;
+            before += b < blockIdx.x ? v : 0;
+        }
+    }
+    const uint32_t tc = (c + rows - 1) / rows;
     const uint32_t si = wave_incl_scan_u32(c), ti = wave_incl_scan_u32(tc);
     if (lane == WAVE - 1) wsum[0][wv] = si, wsum[1][wv] = ti;
     __syncthreads();
     uint32_t so = si - c, to = ti - tc;
     for (uint32_t i = 0; i < wv; i++) so += wsum[0][i], to += wsum[1][i];
-    const Plan P = plan_at(plan, m, slots);
+    cnt[tid] = so + before;
+    __syncthreads();
+    for (uint32_t p = 0; p < per; p += 4) {
+        uint32_t e[4];
+#pragma unroll
+        for (uint32_t u = 0; u < 4; u++)
+            e[u] = p + u < per ? entry_expert(ids, n_sel, slots, E, i0 + (p + u) * PLAN_T + tid, n) : 0xffffffffu;
+#pragma unroll
+        for (uint32_t u = 0; u < 4; u++)
+            if (e[u] != 0xffffffffu) P.ent[atomicAdd(&cnt[e[u]], 1u)] = i0 + (p + u) * PLAN_T + tid;
+    }
+    if (blockIdx.x) return;
     for (uint32_t i = 0; i < tc; i++)
         P.tile[to + i] = PlanTile{tid, so + i * rows, c - i * rows < rows ? c - i * rows : rows, 0};
     if (tid == PLAN_T - 1) *P.n_tiles = to + tc;
-    cnt[tid] = so;
-    __syncthreads();
-    for (uint32_t i = tid; i < n; i += PLAN_T) {
-        const uint32_t e = expert(i);
-        if (e != 0xffffffffu) P.ent[atomicAdd(&cnt[e], 1u)] = i;
-    }
 }
 
 // ============================================================================================
@@ -62,69 +103,77 @@ __device__ __forceinline__ const int8_t* strip_row(const I8Mat& w, uint32_t e, u
     return w.ptr + e * w.stride + (r < w.rows ? r : w.rows - 1) * w.ld;
 }
 
-// A workgroup takes 16 rows of gate and up and a tile's (or, without a plan, one) entries; its waves share K.
+// A workgroup takes 16 rows of gate and up and one entry; its waves share K.
 template <uint32_t DT>
-__global__ __launch_bounds__(ST_WAVES * WAVE) void experts_up_strip_kernel(I8Up a, Plan P) {
-    __shared__ int32_t part[2][ST_WAVES][16][16];  // [gate, up][wave][entry][weight row]
-    __shared__ uint32_t ent[16];
-    const uint32_t strips = (a.gate.rows + 15) / 16, id = run_id(), r0 = id % strips * 16, it = id / strips;
-    uint32_t e, n;
-    if (P.ent) {
-        if (it >= *P.n_tiles) return;
-        const PlanTile t = P.tile[it];
-        e = t.expert, n = t.rows;
-        if (threadIdx.x < 16) ent[threadIdx.x] = P.ent[t.row0 + (threadIdx.x < n ? threadIdx.x : 0)];
-    } else {
-        if (it >= a.m * a.slots || it % a.slots >= a.n_sel[it / a.slots]) return;
-        e = a.ids[(size_t)(it / a.slots) * K_MAX + it % a.slots], n = 1;
-        if (e >= a.gate.count) return;
-        if (threadIdx.x < 16) ent[threadIdx.x] = it;
+__global__ __launch_bounds__(ST_WAVES * WAVE) void experts_up_strip_kernel(I8Up a) {
+    __shared__ int32_t part[2][ST_WAVES][16];  // [gate, up][wave][weight row]
+    const uint32_t strips = (a.gate.rows + 15) / 16, id = run_id(), r0 = id % strips * 16, en = id / strips;
+    const uint32_t t = en / a.slots, j = en % a.slots;
+    if (t >= a.m) return;  // the whole workgroup, here and below
+    const uint32_t e = a.ids[(size_t)t * K_MAX + j], n = a.n_sel[t];
+    if (j >= n || e >= a.gate.count) return;
+    const uint32_t wv = threadIdx.x / WAVE, lane = threadIdx.x % WAVE;
+    const uint32_t r = r0 + threadIdx.x;
+    const bool out = threadIdx.x < 16 && r < a.gate.rows;
+    float sx = 0.0f, sg = 0.0f, su = 0.0f;
+    if (out) sx = a.sx[t], sg = a.gate.scale[(uint64_t)e * a.gate.rows + r], su = a.up.scale[(uint64_t)e * a.gate.rows + r];
+    i32x4 acc[2];
+    // every column of the matrix instruction is this token's row
+    strip_sums<2>({strip_row(a.gate, e, r0, lane), strip_row(a.up, e, r0, lane)}, a.q + (uint64_t)t * a.ldq, a.gate.k, wv,
+                  ST_WAVES, lane, acc);
+    if (lane % 16 == 0) {
+        *reinterpret_cast<i32x4*>(&part[0][wv][lane / 16 * 4]) = acc[0];
+        *reinterpret_cast<i32x4*>(&part[1][wv][lane / 16 * 4]) = acc[1];
     }
     __syncthreads();
-    const uint32_t wv = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, c = lane % 16;
-    const int8_t* xr = a.q + (uint64_t)(ent[c] / a.slots) * a.ldq;
-    *reinterpret_cast<i32x4*>(&part[0][wv][c][lane / 16 * 4]) = strip_sum(strip_row(a.gate, e, r0, lane), xr, a.gate.k, wv, ST_WAVES, lane);
-    *reinterpret_cast<i32x4*>(&part[1][wv][c][lane / 16 * 4]) = strip_sum(strip_row(a.up, e, r0, lane), xr, a.gate.k, wv, ST_WAVES, lane);
-    __syncthreads();
-    const uint32_t ei = threadIdx.x / 16, ri = threadIdx.x % 16, r = r0 + ri;
-    if (ei >= n || r >= a.gate.rows) return;
-    int32_t sg = 0, su = 0;
+    if (!out) return;
+    int32_t g = 0, u = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < ST_WAVES; i++) sg += part[0][i][ei][ri], su += part[1][i][ei][ri];
-    const float sx = a.sx[ent[ei] / a.slots];
-    const uint64_t ws = (uint64_t)e * a.gate.rows + r;
+    for (uint32_t i = 0; i < ST_WAVES; i++) g += part[0][i][threadIdx.x], u += part[1][i][threadIdx.x];
     typedef Elem<DT> O;
-    reinterpret_cast<typename O::T*>(a.h)[ent[ei] * a.ldh + r] =
-            O::put(swiglu(i8_scaled(sg, sx, a.gate.scale[ws]), i8_scaled(su, sx, a.up.scale[ws])));
+    reinterpret_cast<typename O::T*>(a.h)[en * a.ldh + r] = O::put(swiglu(i8_scaled(g, sx, sg), i8_scaled(u, sx, su)));
 }
 
-// A workgroup takes 16 down rows and one token: a wave per slot in turn, the slots' rows added in order.
+// A workgroup takes 16 down rows and one token: a wave per slot (several where there are fewer slots than waves, sharing
+// K; in turn where there are more), then a thread per (slot, row) scales and weights, and a thread per row adds in slot
+// order.
+constexpr uint32_t DOWN_WAVES = 8;  // 12 and 16 are slower: four tokens of ten slots 11.3, 13.1 and 13.2 us
+
 template <uint32_t DT>
-__global__ __launch_bounds__(ST_WAVES * WAVE) void experts_down_strip_kernel(I8Down a) {
-    __shared__ float part[K_MAX][16];
+__global__ __launch_bounds__(DOWN_WAVES* WAVE) void experts_down_strip_kernel(I8Down a) {
+    __shared__ int32_t part[K_MAX * 4][16];  // [slot * share of K][weight row]
+    __shared__ float term[K_MAX][16];
     const uint32_t strips = (a.down.rows + 15) / 16, id = run_id(), r0 = id % strips * 16, t = id / strips;
     if (t >= a.m) return;
     const uint32_t wv = threadIdx.x / WAVE, lane = threadIdx.x % WAVE;
-    const uint32_t n = a.n_sel[t] < a.slots ? a.n_sel[t] : a.slots;
-    for (uint32_t j = wv; j < n; j += ST_WAVES) {
-        const uint32_t e = a.ids[(size_t)t * K_MAX + j];
-        if (e >= a.down.count) continue;
-        const uint64_t row = (uint64_t)t * a.slots + j;
-        const i32x4 s = strip_sum(strip_row(a.down, e, r0, lane), a.q + row * a.ldq, a.down.k, 0, 1, lane);
-        if (lane % 16 == 0)
-#pragma unroll
-            for (uint32_t i = 0; i < 4; i++) {
-                const uint32_t r = r0 + lane / 16 * 4 + i, rc = r < a.down.rows ? r : a.down.rows - 1;
-                part[j][lane / 16 * 4 + i] =
-                        i8_scaled(s[i], a.sx[row], a.down.scale[(uint64_t)e * a.down.rows + rc]) * a.w[(size_t)t * K_MAX + j];
-            }
+    const uint32_t ks = DOWN_WAVES / a.slots >= 4 ? 4 : DOWN_WAVES / a.slots >= 2 ? 2 : 1;  // waves that share a slot
+    const uint32_t* ids = a.ids + (size_t)t * K_MAX;
+    const uint32_t ns = a.n_sel[t], n = ns < a.slots ? ns : a.slots;
+    static_assert(DOWN_WAVES * WAVE >= K_MAX * 16, "a thread per (slot, row)");
+    const uint32_t ri = threadIdx.x % 16, r = r0 + ri, rc = r < a.down.rows ? r : a.down.rows - 1;
+    const uint32_t j = threadIdx.x / 16, jc = j < a.slots ? j : 0, e = ids[jc];
+    const bool there = j < n && e < a.down.count;
+    const float sx = a.sx[(uint64_t)t * a.slots + jc], wt = a.w[(size_t)t * K_MAX + jc];
+    const float sw = a.down.scale[(uint64_t)(there ? e : 0) * a.down.rows + rc];
+    for (uint32_t w = wv; w < a.slots * ks; w += DOWN_WAVES) {
+        const uint32_t ew = ids[w / ks];
+        if (w / ks >= n || ew >= a.down.count) continue;
+        i32x4 acc[1];
+        strip_sums<1>({strip_row(a.down, ew, r0, lane)}, a.q + ((uint64_t)t * a.slots + w / ks) * a.ldq, a.down.k, w % ks, ks,
+                      lane, acc);
+        if (lane % 16 == 0) *reinterpret_cast<i32x4*>(&part[w][lane / 16 * 4]) = acc[0];
     }
     __syncthreads();
-    const uint32_t r = r0 + threadIdx.x;
+    if (j < n) {
+        int32_t s = part[j * ks][ri];
+        for (uint32_t c = 1; c < ks; c++) s += part[j * ks + c][ri];
+        term[j][ri] = there ? i8_scaled(s, sx, sw) * wt : 0.0f;
+    }
+    __syncthreads();
     if (threadIdx.x >= 16 || r >= a.down.rows) return;
     float v = 0.0f;
-    for (uint32_t j = 0; j < n; j++)
-        if (a.ids[(size_t)t * K_MAX + j] < a.down.count) v += part[j][threadIdx.x];
+#pragma unroll 8
+    for (uint32_t i = 0; i < n; i++) v += term[i][ri];
     typedef Elem<DT> O;
     typename O::T* y = reinterpret_cast<typename O::T*>(a.y) + t * a.ldy + r;
     *y = O::put(a.accumulate ? O::get(*y) + v : v);
@@ -134,42 +183,164 @@ __global__ __launch_bounds__(ST_WAVES * WAVE) void experts_down_strip_kernel(I8D
 // many entries: tiles of one expert's
 // ============================================================================================
 
-// 16 down rows of a tile's entries into work [m * slots][rows], weighted
-__global__ __launch_bounds__(ST_WAVES * WAVE) void experts_down_tile_kernel(I8Down a, Plan P) {
-    __shared__ int32_t part[ST_WAVES][16][16];
-    __shared__ uint32_t ent[16];
-    const uint32_t strips = (a.down.rows + 15) / 16, id = run_id(), r0 = id % strips * 16, it = id / strips;
-    if (it >= *P.n_tiles) return;
-    const PlanTile t = P.tile[it];
-    if (threadIdx.x < 16) ent[threadIdx.x] = P.ent[t.row0 + (threadIdx.x < t.rows ? threadIdx.x : 0)];
-    __syncthreads();
-    const uint32_t wv = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, c = lane % 16;
-    *reinterpret_cast<i32x4*>(&part[wv][c][lane / 16 * 4]) =
-            strip_sum(strip_row(a.down, t.expert, r0, lane), a.q + (uint64_t)ent[c] * a.ldq, a.down.k, wv, ST_WAVES, lane);
-    __syncthreads();
-    const uint32_t ei = threadIdx.x / 16, ri = threadIdx.x % 16, r = r0 + ri;
-    if (ei >= t.rows || r >= a.down.rows) return;
-    int32_t s = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < ST_WAVES; i++) s += part[i][ei][ri];
-    const uint32_t en = ent[ei];
-    a.work[(uint64_t)en * a.down.rows + r] =
-            i8_scaled(s, a.sx[en], a.down.scale[(uint64_t)t.expert * a.down.rows + r]) *
-            a.w[(size_t)(en / a.slots) * K_MAX + en % a.slots];
+// A tile's place: entries of one expert (the plan's tile) x a block of weight rows, the blocks of a tile next to one
+// another and each expert's tiles in turn on one XCD, whose L2 then holds the entries' rows and the expert's weights.
+template <typename Tile>
+__device__ __forceinline__ bool expert_tile(const Plan& P, uint32_t blocks, PlanTile& t, uint32_t& block) {
+    uint32_t idx;
+    if (!xcd_order_1d(*P.n_tiles * blocks, idx, run_id())) return false;
+    t = P.tile[idx / blocks], block = idx % blocks;
+    return true;
 }
 
-// y[t] (+)= the rows of its entries, in slot order
+// gate and up: a tile's weight rows are BN / 2 rows of gate, then the same rows of up, and a wave has both of each
+template <typename Tile, uint32_t DT>
+__global__ __launch_bounds__(Tile::T) void experts_up_tile_kernel(I8Up a, Plan P) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[Tile::LDS];
+    constexpr uint32_t BR = Tile::BN / 2, FR = Tile::FN / 2;
+    static_assert(BR % (8 * Tile::NW) == 0 && Tile::WN % 32 == 0, "a load takes rows of one matrix");
+    PlanTile pt;
+    uint32_t block;
+    if (!expert_tile<Tile>(P, (a.gate.rows + BR - 1) / BR, pt, block)) return;  // the whole workgroup
+    const uint32_t r0 = block * BR, rl = a.gate.rows - r0 - 1;                  // the last row there is
+    Tile t;
+    auto entry = [&](uint32_t i) { return P.ent[pt.row0 + (i < pt.rows ? i : pt.rows - 1)]; };
+    const i32x4 bg = buffer_at(a.gate.ptr + pt.expert * a.gate.stride + r0 * a.gate.ld);
+    const i32x4 bu = buffer_at(a.up.ptr + pt.expert * a.up.stride + r0 * a.up.ld);
+    i32x4 rw[Tile::NA];
+    uint32_t wo[Tile::NA], xo[Tile::NB];
+#pragma unroll
+    for (int i = 0; i < Tile::NB; i++) xo[i] = entry(t.load_row(i)) / a.slots * (uint32_t)a.ldq;
+#pragma unroll
+    for (int i = 0; i < Tile::NA; i++) {
+        const bool up = i * Tile::NW * 8 >= BR;
+        const uint32_t r = t.load_row(i) - (up ? BR : 0), rc = r < rl ? r : rl;
+        rw[i] = up ? bu : bg, wo[i] = rc * (uint32_t)(up ? a.up.ld : a.gate.ld);
+    }
+    const uint32_t wr = t.wn / 2;  // this wave's first row of both
+    t.run(lds, rw, wo, buffer_at(a.q), xo, a.gate.k, [&](int i) { return i < FR ? wr + 16 * i : BR + wr + 16 * (i - FR); });
+    typedef Elem<DT> O;
+    float sg[FR][4], su[FR][4], sx[Tile::FM];
+    uint32_t en[Tile::FM];
+#pragma unroll
+    for (int j = 0; j < Tile::FM; j++) en[j] = entry(t.wm + 16 * j + t.lane % 16);
+#pragma unroll
+    for (uint32_t i = 0; i < FR; i++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const uint32_t r = wr + 16 * i + t.lane / 16 * 4 + c;
+            const uint64_t at = (uint64_t)pt.expert * a.gate.rows + r0 + (r < rl ? r : rl);
+            sg[i][c] = a.gate.scale[at], su[i][c] = a.up.scale[at];
+        }
+#pragma unroll
+    for (int j = 0; j < Tile::FM; j++) sx[j] = a.sx[en[j] / a.slots];
+#pragma unroll
+    for (int j = 0; j < Tile::FM; j++) {
+        if (t.wm + 16 * j + t.lane % 16 >= pt.rows) continue;
+        typename O::T* h = reinterpret_cast<typename O::T*>(a.h) + en[j] * a.ldh;
+#pragma unroll
+        for (uint32_t i = 0; i < FR; i++) {
+            const uint32_t r = r0 + wr + 16 * i + t.lane / 16 * 4;
+            float v[4];
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                v[c] = swiglu(i8_scaled(t.acc[i][j][c], sx[j], sg[i][c]), i8_scaled(t.acc[FR + i][j][c], sx[j], su[i][c]));
+            store4<DT>(h + r, v, r < a.gate.rows ? a.gate.rows - r : 0, a.vec);
+        }
+    }
+}
+
+// down: the entries' weighted rows into work [m * slots][rows]
+template <typename Tile>
+__global__ __launch_bounds__(Tile::T) void experts_down_tile_kernel(I8Down a, Plan P) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[Tile::LDS];
+    PlanTile pt;
+    uint32_t block;
+    if (!expert_tile<Tile>(P, (a.down.rows + Tile::BN - 1) / Tile::BN, pt, block)) return;  // the whole workgroup
+    const uint32_t r0 = block * Tile::BN, rl = a.down.rows - r0 - 1;
+    Tile t;
+    auto entry = [&](uint32_t i) { return P.ent[pt.row0 + (i < pt.rows ? i : pt.rows - 1)]; };
+    const i32x4 bw = buffer_at(a.down.ptr + pt.expert * a.down.stride + r0 * a.down.ld);
+    i32x4 rw[Tile::NA];
+    uint32_t wo[Tile::NA], xo[Tile::NB];
+#pragma unroll
+    for (int i = 0; i < Tile::NB; i++) xo[i] = entry(t.load_row(i)) * (uint32_t)a.ldq;
+#pragma unroll
+    for (int i = 0; i < Tile::NA; i++) {
+        const uint32_t r = t.load_row(i);
+        rw[i] = bw, wo[i] = (r < rl ? r : rl) * (uint32_t)a.down.ld;
+    }
+    t.run(lds, rw, wo, buffer_at(a.q), xo, a.down.k, [&](int i) { return t.wn + 16 * i; });
+    float sw[Tile::FN][4], sx[Tile::FM], w[Tile::FM];
+    uint32_t en[Tile::FM];
+#pragma unroll
+    for (int j = 0; j < Tile::FM; j++) en[j] = entry(t.wm + 16 * j + t.lane % 16);
+#pragma unroll
+    for (int i = 0; i < Tile::FN; i++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const uint32_t r = t.wn + 16 * i + t.lane / 16 * 4 + c;
+            sw[i][c] = a.down.scale[(uint64_t)pt.expert * a.down.rows + r0 + (r < rl ? r : rl)];
+        }
+#pragma unroll
+    for (int j = 0; j < Tile::FM; j++)
+        sx[j] = a.sx[en[j]], w[j] = a.w[(size_t)(en[j] / a.slots) * K_MAX + en[j] % a.slots];
+#pragma unroll
+    for (int j = 0; j < Tile::FM; j++) {
+        if (t.wm + 16 * j + t.lane % 16 >= pt.rows) continue;
+        float* y = a.work + (uint64_t)en[j] * a.down.rows;
+#pragma unroll
+        for (int i = 0; i < Tile::FN; i++) {
+            const uint32_t r = r0 + t.wn + 16 * i + t.lane / 16 * 4;
+            float v[4];
+#pragma unroll
+            for (int c = 0; c < 4; c++) v[c] = i8_scaled(t.acc[i][j][c], sx[j], sw[i][c]) * w[j];
+            store4<TRK_DT_F32>(y + r, v, r < a.down.rows ? a.down.rows - r : 0, a.down.rows % 4 == 0);
+        }
+    }
+}
+
+// y[t] (+)= the rows of its entries, in slot order: a thread per four columns, several tokens a workgroup where a row is
+// short.  Four slots' rows are requested before the first is added.
 template <uint32_t DT>
 __global__ __launch_bounds__(256) void experts_combine_kernel(I8Down a) {
-    const uint32_t cols = (a.down.rows + 255) / 256, id = run_id(), t = id / cols, r = id % cols * 256 + threadIdx.x;
-    if (t >= a.m || r >= a.down.rows) return;
-    float v = 0.0f;
+    const uint32_t w = a.down.rows, q = (w + 3) / 4, per = q < 256 ? 256 / q : 1, cols = (q + 255) / 256, id = run_id();
+    const uint32_t sub = q < 256 ? threadIdx.x / q : 0, t = id / cols * per + sub;
+    const uint32_t r = 4 * (q < 256 ? threadIdx.x % q : id % cols * 256 + threadIdx.x);
+    if (t >= a.m || r >= w || sub >= per) return;
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     const uint32_t n = a.n_sel[t] < a.slots ? a.n_sel[t] : a.slots;
-    for (uint32_t j = 0; j < n; j++)
-        if (a.ids[(size_t)t * K_MAX + j] < a.down.count) v += a.work[((uint64_t)t * a.slots + j) * a.down.rows + r];
+    const float* s = a.work + (uint64_t)t * a.slots * w + r;
+    for (uint32_t j0 = 0; j0 < n; j0 += 4) {
+        float p[4][4];
+        bool on[4];
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
+            const uint32_t jc = j0 + j < n ? j0 + j : n - 1;
+            on[j] = j0 + j < n && a.ids[(size_t)t * K_MAX + jc] < a.down.count;
+            if (!on[j]) continue;
+            const float* f = s + (uint64_t)jc * w;
+            if (w % 4 == 0) {
+                const float4 x = *reinterpret_cast<const float4*>(f);
+                p[j][0] = x.x, p[j][1] = x.y, p[j][2] = x.z, p[j][3] = x.w;
+            } else {
+#pragma unroll
+                for (uint32_t c = 0; c < 4; c++) p[j][c] = f[r + c < w ? c : 0];
+            }
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++)
+            if (on[j])
+#pragma unroll
+                for (uint32_t c = 0; c < 4; c++) v[c] += p[j][c];
+    }
     typedef Elem<DT> O;
     typename O::T* y = reinterpret_cast<typename O::T*>(a.y) + t * a.ldy + r;
-    *y = O::put(a.accumulate ? O::get(*y) + v : v);
+    if (a.accumulate)
+#pragma unroll
+        for (uint32_t c = 0; c < 4; c++)
+            if (r + c < w) v[c] += O::get(y[c]);
+    store4<DT>(y, v, w - r, a.vec);
 }
 
 dim3 run_of(uint64_t wgs, uint32_t threads) {
@@ -181,48 +352,90 @@ dim3 run_of(uint64_t wgs, uint32_t threads) {
 
 hipError_t launch_experts_plan(const uint32_t* ids, const uint32_t* n_sel, uint32_t m, uint32_t slots, uint32_t E,
                                uint32_t* plan, hipStream_t st) {
-    experts_plan_kernel<<<1, PLAN_T, 0, st>>>(ids, n_sel, m, slots, E, geo::plan_rows(m, slots, E), plan);
+    const Plan P = plan_at(plan, m, slots);
+    const uint32_t wgs = geo::plan_workgroups(m, slots), n = m * slots, per = (n + wgs * PLAN_T - 1) / (wgs * PLAN_T);
+    uint32_t* counts = plan + geo::plan_counts_at(m, slots, E);
+    if (wgs > 1) {
+        experts_count_kernel<<<wgs, PLAN_T, 0, st>>>(ids, n_sel, m, slots, E, per, counts);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    experts_plan_kernel<<<wgs, PLAN_T, 0, st>>>(ids, n_sel, m, slots, E, geo::plan_rows(m, slots, E), per, counts, P);
     return hipGetLastError();
+}
+
+template <typename Tile>
+static void launch_up_tile(const I8Up& a, const Plan& P, uint64_t tiles, hipStream_t st) {
+    const dim3 g = run_of((a.gate.rows + Tile::BN / 2 - 1) / (Tile::BN / 2) * tiles, Tile::T);
+    if (a.dt == TRK_DT_F32)
+        experts_up_tile_kernel<Tile, TRK_DT_F32><<<g, Tile::T, 0, st>>>(a, P);
+    else if (a.dt == TRK_DT_BF16)
+        experts_up_tile_kernel<Tile, TRK_DT_BF16><<<g, Tile::T, 0, st>>>(a, P);
+    else
+        experts_up_tile_kernel<Tile, TRK_DT_F16><<<g, Tile::T, 0, st>>>(a, P);
 }
 
 hipError_t launch_experts_up(const I8Up& a, const uint32_t* plan, hipStream_t st) {
     const uint32_t E = a.gate.count;
-    Plan P{};
-    uint64_t items = (uint64_t)a.m * a.slots;
-    if (plan) {
-        const uint32_t rows = geo::plan_rows(a.m, a.slots, E);
-        P = plan_at(const_cast<uint32_t*>(plan), a.m, a.slots);
-        items = geo::plan_tiles(a.m, a.slots, E, rows);
-    }
-    const dim3 g = run_of((a.gate.rows + 15) / 16 * items, ST_WAVES * WAVE);
-    if (a.dt == TRK_DT_F32)
-        experts_up_strip_kernel<TRK_DT_F32><<<g, ST_WAVES * WAVE, 0, st>>>(a, P);
-    else if (a.dt == TRK_DT_BF16)
-        experts_up_strip_kernel<TRK_DT_BF16><<<g, ST_WAVES * WAVE, 0, st>>>(a, P);
-    else
-        experts_up_strip_kernel<TRK_DT_F16><<<g, ST_WAVES * WAVE, 0, st>>>(a, P);
-    return hipGetLastError();
-}
-
-hipError_t launch_experts_down(const I8Down& a, const uint32_t* plan, hipStream_t st) {
-    const uint32_t E = a.down.count;
-    if (!plan) {
-        const dim3 g = run_of((uint64_t)((a.down.rows + 15) / 16) * a.m, ST_WAVES * WAVE);
+    if (!plan || !geo::i8_tile_addresses(a.gate.ld, a.ldq, a.m) || !geo::i8_tile_addresses(a.up.ld, a.ldq, a.m)) {
+        const dim3 g = run_of((uint64_t)((a.gate.rows + 15) / 16) * a.m * a.slots, ST_WAVES * WAVE);
         if (a.dt == TRK_DT_F32)
-            experts_down_strip_kernel<TRK_DT_F32><<<g, ST_WAVES * WAVE, 0, st>>>(a);
+            experts_up_strip_kernel<TRK_DT_F32><<<g, ST_WAVES * WAVE, 0, st>>>(a);
         else if (a.dt == TRK_DT_BF16)
-            experts_down_strip_kernel<TRK_DT_BF16><<<g, ST_WAVES * WAVE, 0, st>>>(a);
+            experts_up_strip_kernel<TRK_DT_BF16><<<g, ST_WAVES * WAVE, 0, st>>>(a);
         else
-            experts_down_strip_kernel<TRK_DT_F16><<<g, ST_WAVES * WAVE, 0, st>>>(a);
+            experts_up_strip_kernel<TRK_DT_F16><<<g, ST_WAVES * WAVE, 0, st>>>(a);
         return hipGetLastError();
     }
     const uint32_t rows = geo::plan_rows(a.m, a.slots, E);
     const Plan P = plan_at(const_cast<uint32_t*>(plan), a.m, a.slots);
-    experts_down_tile_kernel<<<run_of((a.down.rows + 15) / 16 * geo::plan_tiles(a.m, a.slots, E, rows),
-                                      ST_WAVES * WAVE), ST_WAVES * WAVE, 0, st>>>(a, P);
-    hipError_t e = hipGetLastError();
+    const uint64_t tiles = geo::plan_tiles(a.m, a.slots, E, rows);
+    if (rows == 32)
+        launch_up_tile<I8Tile<128, 32, 32, 32, 3>>(a, P, tiles, st);
+    else if (rows == 64)
+        launch_up_tile<I8Tile<128, 64, 64, 32, 2>>(a, P, tiles, st);
+    else if (geo::up_wide(a.gate.rows, tiles))
+        launch_up_tile<I8Tile<256, 128, 64, 64, 3>>(a, P, tiles, st);
+    else
+        launch_up_tile<I8Tile<128, 128, 64, 64, 2>>(a, P, tiles, st);
+    return hipGetLastError();
+}
+
+static void launch_down_strip(const I8Down& a, hipStream_t st) {
+    const dim3 g = run_of((uint64_t)((a.down.rows + 15) / 16) * a.m, DOWN_WAVES * WAVE);
+    if (a.dt == TRK_DT_F32)
+        experts_down_strip_kernel<TRK_DT_F32><<<g, DOWN_WAVES * WAVE, 0, st>>>(a);
+    else if (a.dt == TRK_DT_BF16)
+        experts_down_strip_kernel<TRK_DT_BF16><<<g, DOWN_WAVES * WAVE, 0, st>>>(a);
+    else
+        experts_down_strip_kernel<TRK_DT_F16><<<g, DOWN_WAVES * WAVE, 0, st>>>(a);
+}
+
+template <typename Tile>
+static void launch_down_tile(const I8Down& a, const Plan& P, uint64_t tiles, hipStream_t st) {
+    const dim3 g = run_of((a.down.rows + Tile::BN - 1) / Tile::BN * tiles, Tile::T);
+    experts_down_tile_kernel<Tile><<<g, Tile::T, 0, st>>>(a, P);
+}
+
+hipError_t launch_experts_down(const I8Down& a, const uint32_t* plan, hipStream_t st) {
+    const uint32_t E = a.down.count;
+    if (!plan || !geo::i8_tile_addresses(a.down.ld, a.ldq, (uint64_t)a.m * a.slots)) {
+        launch_down_strip(a, st);
+        return hipGetLastError();
+    }
+    const uint32_t rows = geo::plan_rows(a.m, a.slots, E);
+    const Plan P = plan_at(const_cast<uint32_t*>(plan), a.m, a.slots);
+    const uint64_t tiles = geo::plan_tiles(a.m, a.slots, E, rows);
+    if (rows == 32)
+        launch_down_tile<I8Tile<128, 32, 32, 32, 3>>(a, P, tiles, st);
+    else if (rows == 64)
+        launch_down_tile<I8Tile<128, 64, 64, 32, 3>>(a, P, tiles, st);
+    else
+        launch_down_tile<I8Tile<128, 128, 64, 64, 2>>(a, P, tiles, st);
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const dim3 g = run_of((uint64_t)((a.down.rows + 255) / 256) * a.m, 256);
+    const uint32_t q = (a.down.rows + 3) / 4, per = q < 256 ? 256 / q : 1;
+    const dim3 g = run_of((uint64_t)((q + 255) / 256) * ((a.m + per - 1) / per), 256);
     if (a.dt == TRK_DT_F32)
         experts_combine_kernel<TRK_DT_F32><<<g, 256, 0, st>>>(a);
     else if (a.dt == TRK_DT_BF16)

@@ -261,6 +261,7 @@ struct I8Up {
     void* h;
     uint32_t dt;
     uint64_t ldh;
+    int vec;  // four neighbouring values of h lie on a boundary of four
 };
 struct I8Down {
     I8Mat down;
@@ -274,7 +275,7 @@ struct I8Down {
     void* y;
     uint32_t dt;
     uint64_t ldy;
-    int accumulate;
+    int accumulate, vec;  // vec: as I8Gemm's
 };
 struct PlanTile {
     uint32_t expert, row0, rows, pad;  // entries ent[row0 .. row0 + rows)
