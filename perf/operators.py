@@ -30,11 +30,11 @@ TILE = 64   # entries of one expert that the plain form multiplies together
 
 
 def _package():
-    at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "tr-infer_amd")
-    if at not in sys.path:
-        sys.path.insert(0, at)
-    import trmoe
-    return trmoe
+    """This repository's package, as a program has it imported once."""
+    if "trmoe" not in sys.modules:
+        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "tr-infer_amd"))
+        import trmoe  # noqa: F401
+    return sys.modules["trmoe"]
 
 
 # ---- the cases -------------------------------------------------------------------------------------
