@@ -90,6 +90,7 @@ def test_experts_entry_counts_are_checked():
     assert L.trk_experts_plan_words(1, 1, 8, None) == -1
     assert words(0, 4, 8) == 0 and words(1, 8, 256) == 0  # one token takes no plan
     assert words(4096, 10, 512) >= 4 + 40960
+    assert words(trmoe.EXPERTS_DIRECT_M, 10, 512) == 0 and words(trmoe.EXPERTS_DIRECT_M + 1, 10, 512) > 0
 
 
 def up(gate=None, up_=None, q=P, ldq=112, m=4096, ids=P, slots=2, plan=P, h=P, dtype=0, ldh=64):

@@ -222,7 +222,8 @@ inline I8Form gemm_i8_form(uint32_t m, uint32_t rows, uint32_t k, uint64_t ldw, 
 // by expert and cut into tiles of at most plan_rows entries of one expert.
 // us, up and down by themselves / planned (the plan included; H = 2048): 8 tokens of 10 in 512 experts of F = 512 52 / 58, of 8
 // in 128 of 768 60 / 67, of 2 in 8 of 1024 22 / 24; 16 tokens 90 / 89, 105 / 91 and 36 / 24.
-inline bool plan_used(uint32_t m) { return m > 8; }
+constexpr uint32_t DIRECT_M = 8;  // TRK_EXPERTS_DIRECT_M
+inline bool plan_used(uint32_t m) { return m > DIRECT_M; }
 // us, up at 32 / 64 / 128 rows: 2 entries an expert (4 of 16 x 100 tokens: 25) 7.1 / 7.3 / 8.1, 62 (8 of 128 x 1000) 110 / 94
 // / 91, 80 (10 of 512 x 4096) 309 / 270 / 245; down at 10 entries (10 of 512 x 512) 134 / 139 / 154, at 62 93 / 88 / 89.
 inline uint32_t plan_rows(uint32_t m, uint32_t slots, uint32_t E) {

@@ -9,28 +9,34 @@ namespace {
 // rows to int8
 // ============================================================================================
 
-// 127 x / top rounded to nearest, ties to even, as exact arithmetic would.  In 32 bits the quotient is off by
-// at most 2 ulp of 128 (2^-15); within 2^-12 of a border (a half) it is taken again in 64 bits, where it is right: 127 x
-// is exact, and a quotient of a 31-bit and a 24-bit integer that is no tie is further than 2^-32 from one.
-__device__ __forceinline__ int32_t quant_one(float x, float top, float inv) {
-    const float t = x * inv, r = __builtin_rintf(t);
-    if (__builtin_fabsf(__builtin_fabsf(t - r) - 0.5f) > 0x1p-12f) return (int32_t)r;
-    return (int32_t)::rint((double)x * 127.0 / (double)top);
-}
+// 127 x / top rounded to nearest, ties to even, as exact arithmetic would.  In 32 bits the quotient carries three
+// roundings, under 2^-15 in all; one that near to a border (a half) is taken again in 64 bits, where it is right: 127 x is
+// exact, and a quotient of a 31-bit and a 24-bit integer that is no tie is further than 2^-32 from one.
+__device__ __forceinline__ float quant_exact(float x, float top) { return (float)::rint((double)x * 127.0 / (double)top); }
+constexpr float QUANT_BORDER = 0.5f - 0x1p-15f;  // |t - rint(t)| above it: near a border
 
 constexpr float QUANT_LEAST = 127.0f * 0x1p-126f;  // the least magnitude whose scale is a normal number
 constexpr uint32_t QUANT_T = 256;
 
+struct QuantScale {
+    float top, inv, scale;
+};
+__device__ __forceinline__ QuantScale quant_scale(uint32_t top) {  // a magnitude's bits: NaN above infinity above every number
+    const float t = __uint_as_float(top);
+    const bool poison = top >= 0x7f800000u, zero = poison || t < QUANT_LEAST;
+    return QuantScale{t, zero ? 0.0f : 127.0f / t, poison ? __builtin_nanf("") : zero ? 0.0f : t / 127.0f};
+}
+
+// Rows too long to be held: a workgroup each, every row read twice.
 template <uint32_t DT>
-__global__ __launch_bounds__(QUANT_T) void quantize_whole_rows_kernel(const typename Elem<DT>::T* __restrict__ x,
-                                                                      uint64_t ldx, uint32_t m, uint32_t k,
-                                                                      int8_t* __restrict__ q, uint64_t ldq,
-                                                                      float* __restrict__ scale) {
+__global__ __launch_bounds__(QUANT_T) void quantize_long_rows_kernel(const typename Elem<DT>::T* __restrict__ x, uint64_t ldx,
+                                                                    uint32_t m, uint32_t k, int8_t* __restrict__ q,
+                                                                    uint64_t ldq, float* __restrict__ scale) {
     __shared__ uint32_t part[QUANT_T / WAVE];
     const uint32_t row = run_id(), tid = threadIdx.x;
     if (row >= m) return;  // the whole workgroup
     const auto* xr = x + row * ldx;
-    uint32_t top = 0;  // magnitudes as bit patterns: NaN above infinity above every number
+    uint32_t top = 0;
     for (uint32_t i = tid; i < k; i += QUANT_T) {
         const uint32_t b = __float_as_uint(Elem<DT>::get(xr[i])) & 0x7fffffffu;
         top = b > top ? b : top;
@@ -40,12 +46,161 @@ __global__ __launch_bounds__(QUANT_T) void quantize_whole_rows_kernel(const type
     __syncthreads();
 #pragma unroll
     for (uint32_t i = 0; i < QUANT_T / WAVE; i++) top = part[i] > top ? part[i] : top;
-    const float t = __uint_as_float(top);
-    const bool poison = top >= 0x7f800000u, zero = poison || t < QUANT_LEAST;
-    const float inv = zero ? 0.0f : 127.0f / t;
-    if (tid == 0) scale[row] = poison ? __builtin_nanf("") : zero ? 0.0f : t / 127.0f;
+    const QuantScale s = quant_scale(top);
+    if (tid == 0) scale[row] = s.scale;
     int8_t* qr = q + row * ldq;
-    for (uint32_t i = tid; i < k; i += QUANT_T) qr[i] = zero ? 0 : (int8_t)quant_one(Elem<DT>::get(xr[i]), t, inv);
+    for (uint32_t i = tid; i < k; i += QUANT_T) {
+        const float v = Elem<DT>::get(xr[i]), t = v * s.inv;
+        float r = __builtin_rintf(t);
+        if (__builtin_fabsf(t - r) > QUANT_BORDER) r = quant_exact(v, s.top);
+        qr[i] = s.inv == 0.0f ? 0 : (int8_t)(int)r;
+    }
+}
+
+// Rows that TPR threads hold in registers, PC pieces of 8 values a thread: read once, written once.  Pieces may lie at any
+// address (a slice of a wider tensor).  Rounding: t + 1.5 2^23 has rint(t), as an 8-bit integer, in its low byte.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x4_f32 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+constexpr float QUANT_MAGIC = 12582912.0f;
+
+// 8 values of a row as they lie in memory, n of them there
+template <uint32_t DT>
+struct QuantPiece {
+    static constexpr int W = DT == TRK_DT_F32 ? 8 : 4;
+    uint32_t w[W];
+    __device__ __forceinline__ void load(const typename Elem<DT>::T* p, uint32_t n) {
+        if (n >= 8) {
+            if constexpr (DT == TRK_DT_F32) {
+                const u32x4_f32 a = *reinterpret_cast<const u32x4_f32*>(p), b = *reinterpret_cast<const u32x4_f32*>(p + 4);
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] = a[i], w[4 + i] = b[i];
+            } else {
+                const u32x4_any a = *reinterpret_cast<const u32x4_any*>(p);
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] = a[i];
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < W; i++) w[i] = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            if (i >= n) continue;
+            if constexpr (DT == TRK_DT_F32)
+                w[i] = __float_as_uint(p[i]);
+            else
+                w[i / 2] |= (uint32_t)p[i] << (16 * (i % 2));
+        }
+    }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (DT == TRK_DT_F32) return __uint_as_float(w[i]);
+        return Elem<DT>::get((typename Elem<DT>::T)(w[i / 2] >> (16 * (i % 2))));
+    }
+    // the largest magnitude so far, as bits of the type: two 16-bit ones side by side
+    __device__ __forceinline__ uint32_t most(uint32_t top) const {
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int i = 0; i < W; i++) {
+            if constexpr (DT == TRK_DT_F32) {
+                const uint32_t b = w[i] & 0x7fffffffu;
+                top = b > top ? b : top;
+            } else {
+                const u16x2 b = __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu);
+                top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top), b));
+            }
+        }
+        return top;
+    }
+    static __device__ __forceinline__ uint32_t most32(uint32_t top) {  // as bits of a float
+        if constexpr (DT == TRK_DT_F32) return top;
+        const uint32_t lo = top & 0xffffu, hi = top >> 16;
+        return __float_as_uint(Elem<DT>::get((typename Elem<DT>::T)(lo > hi ? lo : hi)));
+    }
+};
+
+template <uint32_t DT, uint32_t TPR, uint32_t PC>
+__global__ __launch_bounds__(QUANT_T) void quantize_held_rows_kernel(const typename Elem<DT>::T* __restrict__ x, uint64_t ldx,
+                                                                     uint32_t m, uint32_t k, int8_t* __restrict__ q,
+                                                                     uint64_t ldq, float* __restrict__ scale) {
+    __shared__ uint32_t part[QUANT_T / WAVE];
+    const uint32_t row = run_id() * (QUANT_T / TPR) + threadIdx.x / TPR, tid = threadIdx.x % TPR;
+    if (row >= m) return;  // a whole wave, or the whole workgroup
+    const auto* xr = x + row * ldx;
+    QuantPiece<DT> v[PC];
+#pragma unroll
+    for (uint32_t p = 0; p < PC; p++) {
+        const uint32_t at = (p * TPR + tid) * 8;
+        v[p].load(xr + (at < k ? at : 0), at < k ? k - at : 0);
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (uint32_t p = 0; p < PC; p++) top = v[p].most(top);
+    top = wave_max_u32(QuantPiece<DT>::most32(top));
+    if constexpr (TPR > WAVE) {
+        if (tid % WAVE == 0) part[tid / WAVE] = top;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < QUANT_T / WAVE; i++) top = part[i] > top ? part[i] : top;
+    }
+    const QuantScale s = quant_scale(top);
+    if (tid == 0) scale[row] = s.scale;
+    int8_t* qr = q + row * ldq;
+#pragma unroll
+    for (uint32_t p = 0; p < PC; p++) {
+        const uint32_t at = (p * TPR + tid) * 8;
+        if (at >= k) continue;
+        uint32_t r[8];
+        float far = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float t = v[p].get(i) * s.inv, u = t + QUANT_MAGIC;
+            r[i] = __float_as_uint(u);
+            far = __builtin_fmaxf(far, __builtin_fabsf(t - (u - QUANT_MAGIC)));
+        }
+        if (far > QUANT_BORDER)
+#pragma unroll
+            for (int i = 0; i < 8; i++) r[i] = (uint32_t)(int)quant_exact(v[p].get(i), s.top);
+        uint32_t w[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {  // the low bytes of four words
+            const uint32_t lo = __builtin_amdgcn_perm(r[4 * i + 1], r[4 * i], 0x0c0c0400u);
+            const uint32_t hi = __builtin_amdgcn_perm(r[4 * i + 3], r[4 * i + 2], 0x04000c0cu);
+            w[i] = s.inv == 0.0f ? 0 : lo | hi;
+        }
+        if (at + 8 <= k) {
+            *reinterpret_cast<u32x2_any*>(qr + at) = u32x2_any{w[0], w[1]};
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++)
+                if (at + i < k) qr[at + i] = (int8_t)(w[i / 4] >> (8 * (i % 4)));
+        }
+    }
+}
+
+template <uint32_t DT>
+void launch_quantize(const void* x, uint64_t ldx, uint32_t m, uint32_t k, int8_t* q, uint64_t ldq, float* scale,
+                     hipStream_t st) {
+    typedef typename Elem<DT>::T T;
+    const uint32_t per = k <= 2048 ? QUANT_T / WAVE : 1;  // rows of a workgroup: a wave each while they fit its registers
+    const geo::Grid2 g = geo::grid_run(((uint64_t)m + per - 1) / per, QUANT_T);
+    const dim3 grid(g.x, g.y);
+#define GO(TPR, PC) quantize_held_rows_kernel<DT, TPR, PC><<<grid, QUANT_T, 0, st>>>((const T*)x, ldx, m, k, q, ldq, scale)
+    if (k <= 512)
+        GO(WAVE, 1);
+    else if (k <= 1024)
+        GO(WAVE, 2);
+    else if (k <= 2048)
+        GO(WAVE, 4);
+    else if (k <= 4096)
+        GO(QUANT_T, 2);
+    else if (k <= 8192)
+        GO(QUANT_T, 4);
+    else if (k <= 16384)
+        GO(QUANT_T, 8);
+    else
+        quantize_long_rows_kernel<DT><<<grid, QUANT_T, 0, st>>>((const T*)x, ldx, m, k, q, ldq, scale);
+#undef GO
 }
 
 // ============================================================================================
@@ -189,14 +344,12 @@ void launch_tile(const I8Gemm& a, hipStream_t st) {
 
 hipError_t launch_quantize_rows(const void* x, uint32_t dt, uint64_t ldx, uint32_t m, uint32_t k, int8_t* q,
                                 uint64_t ldq, float* scale, hipStream_t st) {
-    const geo::Grid2 g = geo::grid_run(m, QUANT_T);
-    const dim3 grid(g.x, g.y);
     if (dt == TRK_DT_F32)
-        quantize_whole_rows_kernel<TRK_DT_F32><<<grid, QUANT_T, 0, st>>>((const float*)x, ldx, m, k, q, ldq, scale);
+        launch_quantize<TRK_DT_F32>(x, ldx, m, k, q, ldq, scale, st);
     else if (dt == TRK_DT_BF16)
-        quantize_whole_rows_kernel<TRK_DT_BF16><<<grid, QUANT_T, 0, st>>>((const uint16_t*)x, ldx, m, k, q, ldq, scale);
+        launch_quantize<TRK_DT_BF16>(x, ldx, m, k, q, ldq, scale, st);
     else
-        quantize_whole_rows_kernel<TRK_DT_F16><<<grid, QUANT_T, 0, st>>>((const uint16_t*)x, ldx, m, k, q, ldq, scale);
+        launch_quantize<TRK_DT_F16>(x, ldx, m, k, q, ldq, scale, st);
     return hipGetLastError();
 }
 

@@ -1,6 +1,11 @@
 // Routing by scores (trk_route_scores): sigmoid or softmax scores, a bias that moves the choice but not the
 // weights, groups, top-k, renormalised weights.  One wave per token.
-#include "common.hpp"
+//
+// A row is 4 E bytes and some ten operations a logit; what bounds the kernel is the chain of steps of a row (scores,
+// groups, selection) with few waves, and their instructions with many.  So keys are compared in 32 bits with a bound
+// on what 32 bits get wrong: a row in which two keys (or group sums) that decide something are nearer than that, or in
+// which more than 64 keys are in question, is done again in 64 bits.  Some rows in a thousand are.
+#include "route.hpp"
 
 namespace trk {
 
@@ -106,17 +111,190 @@ __device__ void score_row(const float* __restrict__ lg, const float* __restrict_
     if (lane == 0) *n_sel = n;
 }
 
+// ---- 32 bits, and what they may be off by ----------------------------------------------------------
+
+template <int CTRL>
+__device__ __forceinline__ float dpp_or(float v, float none) {  // lanes without a source get `none`
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float wave_sum32(float v) {
+    v += dpp_or<0x111>(v, 0.0f);  // row_shr:1, 2, 4, 8: lane 15 of each row has its sum
+    v += dpp_or<0x112>(v, 0.0f);
+    v += dpp_or<0x114>(v, 0.0f);
+    v += dpp_or<0x118>(v, 0.0f);
+    return rdl(v, 15) + rdl(v, 31) + (rdl(v, 47) + rdl(v, 63));
+}
+
+// The two largest of a and b's two each
+__device__ __forceinline__ void merge2(float& a1, float& a2, float b1, float b2) {
+    a2 = __builtin_fmaxf(__builtin_fminf(a1, b1), __builtin_fmaxf(a2, b2));
+    a1 = __builtin_fmaxf(a1, b1);
+}
+
+constexpr float LOG2E = 1.44269504f;
+constexpr uint32_t SC_CAND = 64 + 34;  // LDS entries a wave: candidates, then the best in order
+
+// One row; false where 64 bits have to decide.  NJ: logits a lane holds.  Lanes are split evenly over the groups.
+template <int NJ>
+__device__ bool score_row32(const float* __restrict__ lg, const float* __restrict__ bias, uint32_t E, const ScorePolicy& p,
+                            uint32_t lane, uint2* cand, uint32_t* __restrict__ ids, float* __restrict__ w,
+                            uint32_t* __restrict__ n_sel) {
+    const float NONE = -__builtin_inff();
+    const uint32_t gs = E / p.n_group, L = p.group_lanes, g = lane / L, r0 = lane % L;
+    float v[NJ], key[NJ];
+    uint32_t idx[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+        const uint32_t r = r0 + L * j;
+        const bool in = g < p.n_group && r < gs;
+        idx[j] = in ? g * gs + r : 0;
+        v[j] = lg[idx[j]];
+        key[j] = bias ? bias[idx[j]] : 0.0f;
+        if (!in || !(v[j] > NONE)) v[j] = NONE;  // NaN compares false
+    }
+    float mx = 0.0f, denom = 1.0f, tol = 0.0f, scale = 1.0f;
+    const bool sums = p.n_group > 1 && p.group_top == 2, scored = bias || sums;
+    if (p.score == TRK_SCORE_SOFTMAX) {
+        uint32_t mk = 0;
+#pragma unroll
+        for (int j = 0; j < NJ; j++) mk = mk > fkey(v[j]) ? mk : fkey(v[j]);
+        mk = wave_max_u32(mk);
+        if (mk == 0 || mk == fkey(__builtin_inff())) return false;  // nothing to choose, or scores that are NaN
+        mx = fkey_inv(mk);
+        float s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NJ; j++) s += __builtin_amdgcn_exp2f((v[j] - mx) * LOG2E);
+        denom = wave_sum32(s);
+        scale = 1.0f / denom;  // the largest score
+        // (l - mx) log2 e and its power are off by d 3 2^-24 + 2^-23 at distance d, where d e^-d <= 0.37; the sum by 38
+        // roundings and its terms': a score by less than 2^-18 of the largest
+        tol = scale * 0x1p-16f;
+    } else {
+        // s (1 - s) |l| <= 0.23: the argument's two roundings, the power's, the sum's and the reciprocal's make less
+        // than 2^-22
+        tol = 0x1p-20f;
+    }
+    float a1 = NONE, a2 = NONE;  // of this lane's keys
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+        if (scored) {
+            const float s = p.score == TRK_SCORE_SOFTMAX
+                                    ? __builtin_amdgcn_exp2f((v[j] - mx) * LOG2E) * scale
+                                    : __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-v[j] * LOG2E));
+            const float k = s + key[j];
+            key[j] = v[j] > NONE && k > NONE ? k : NONE;
+        } else {
+            key[j] = v[j];
+        }
+        merge2(a1, a2, key[j], NONE);
+    }
+    bool near = false;
+    if (p.n_group > 1) {
+        if (L > 1) merge2(a1, a2, dpp_f<0xB1>(a1), dpp_f<0xB1>(a2));    // lane ^ 1
+        if (L > 2) merge2(a1, a2, dpp_f<0x4E>(a1), dpp_f<0x4E>(a2));    // ^ 2
+        if (L > 4) merge2(a1, a2, dpp_f<0x141>(a1), dpp_f<0x141>(a2));  // mirrored in 8: the other quad
+        if (L > 8) merge2(a1, a2, dpp_f<0x140>(a1), dpp_f<0x140>(a2));  // mirrored in 16: the other 8
+        if (L > 16) merge2(a1, a2, __shfl_xor(a1, 16), __shfl_xor(a2, 16));
+        const float worth = g >= p.n_group ? NONE : sums && a2 > NONE ? a1 + a2 : a1;
+        uint32_t rank = 0;
+        for (uint32_t i = 0; i < p.n_group; i++) {
+            const float o = rdl(worth, i * L);
+            rank += o > worth || (o == worth && i < g) ? 1u : 0u;
+        }
+        const bool kept = rank < p.topk_group && worth > NONE;
+        // the worst group kept and the best one dropped; a sum of two keys is off by twice a key
+        const uint32_t lo = ~wave_max_u32(kept ? ~fkey(worth) : 0u), hi = wave_max_u32(kept ? 0u : fkey(worth));
+        if (scored && hi && lo != 0xffffffffu) {
+            const float fl = fkey_inv(lo), fh = fkey_inv(hi);
+            near = !(fl - fh > 2.0f * tol + 0x1p-20f * __builtin_fmaxf(__builtin_fabsf(fl), __builtin_fabsf(fh)));
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+            if (!bias && sums) key[j] = v[j];  // the choice itself goes by the logits
+            if (!kept) key[j] = NONE;
+        }
+    }
+    // Selection as route_select's: the kk-th largest of the lanes' maxima, cut to 16 bits, bounds the kk-th largest key
+    // from below; the keys that reach it are ranked.  kk = k + 1 where the next key has to be told from the k-th.
+    const uint32_t kk = p.k + (bias ? 1u : 0u);
+    uint32_t fk[NJ], lmax = 0;
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+        fk[j] = fkey(key[j]);
+        lmax = lmax > fk[j] ? lmax : fk[j];
+    }
+    uint32_t T = 0;
+#pragma unroll
+    for (int b = 30; b >= 16; b -= 2) {
+        const uint32_t t1 = T | (1u << b), t2 = T | (2u << b), t3 = T | (3u << b);
+        const uint32_t c1 = (uint32_t)__popcll(__ballot(lmax >= t1));
+        const uint32_t c2 = (uint32_t)__popcll(__ballot(lmax >= t2));
+        const uint32_t c3 = (uint32_t)__popcll(__ballot(lmax >= t3));
+        T = c3 >= kk ? t3 : (c2 >= kk ? t2 : (c1 >= kk ? t1 : T));
+    }
+    T = T > 1u ? T : 1u;
+    uint32_t C = 0;
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+        const bool c = fk[j] >= T;
+        const uint64_t m = __ballot(c);
+        const uint32_t at = C + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
+        if (c && at < 64u) cand[at] = make_uint2(fk[j], idx[j]);
+        C += (uint32_t)__popcll(m);
+    }
+    if (near || C > 64u) return false;
+    wave_sync();
+    const uint2 me = lane < C ? cand[lane] : make_uint2(0u, 0xffffffffu);
+    uint32_t rank = 0;
+    for (uint32_t t = 0; t < C; t++) {
+        const uint32_t kt = (uint32_t)__builtin_amdgcn_readlane((int)me.x, (int)t);
+        const uint32_t it = (uint32_t)__builtin_amdgcn_readlane((int)me.y, (int)t);
+        rank += kt > me.x || (kt == me.x && it < me.y) ? 1u : 0u;
+    }
+    if (lane < C && rank < kk) cand[64 + rank] = me;
+    wave_sync();
+    const uint32_t have = C < kk ? C : kk, n = have < p.k ? have : p.k;
+    const uint2 best = lane < have ? cand[64 + lane] : make_uint2(0u, 0xffffffffu);
+    if (bias) {
+        const uint32_t next = (uint32_t)__shfl_down((int)best.x, 1);
+        const float k0 = fkey_inv(best.x), k1 = fkey_inv(next);
+        const bool close = !(k0 - k1 > 2.0f * tol + 0x1p-21f * __builtin_fmaxf(__builtin_fabsf(k0), __builtin_fabsf(k1)));
+        if (__ballot(lane + 1 < have && close)) return false;
+    }
+    // the weights in 64 bits, a lane each: sigmoids that 32 bits lose below their sum still have their ratios
+    double s = 0.0;
+    if (lane < n) {
+        const double l = (double)lg[best.y];
+        s = p.score == TRK_SCORE_SOFTMAX ? ::exp(l - (double)mx) / (double)denom : 1.0 / (1.0 + ::exp(-l));
+    }
+    if (p.renorm) {
+        double sum = s;
+        for (int d = n > 32 ? 32 : n > 16 ? 16 : n > 8 ? 8 : n > 4 ? 4 : n > 2 ? 2 : 1; d; d >>= 1) sum += __shfl_xor(sum, d);
+        s = sum > 0.0 ? s / sum : sum;
+    }
+    if (lane < p.k) {
+        ids[lane] = lane < n ? best.y : 0xffffffffu;
+        w[lane] = lane < n ? (float)(s * (double)p.factor) : 0.0f;
+    }
+    if (lane == 0) *n_sel = n;
+    return true;
+}
+
+template <int NJ>
 __global__ __launch_bounds__(SC_WAVES * WAVE) void route_scores_kernel(const float* __restrict__ logits,
                                                                        const float* __restrict__ bias, uint32_t m,
                                                                        uint32_t E, ScorePolicy p,
                                                                        uint32_t* __restrict__ ids, float* __restrict__ w,
                                                                        uint32_t* __restrict__ n_sel) {
     extern __shared__ double keys[];  // [SC_WAVES][E]
+    __shared__ uint2 cand[SC_WAVES][SC_CAND];
     const uint32_t wv = threadIdx.x / WAVE, lane = threadIdx.x % WAVE;
     const uint32_t row = run_id() * SC_WAVES + wv;
     if (row >= m) return;
-    score_row(logits + (size_t)row * E, bias, E, p, lane, keys + (size_t)wv * E, ids + (size_t)row * K_MAX,
-              w + (size_t)row * K_MAX, n_sel + row);
+    const float* lg = logits + (size_t)row * E;
+    if (!score_row32<NJ>(lg, bias, E, p, lane, cand[wv], ids + (size_t)row * K_MAX, w + (size_t)row * K_MAX, n_sel + row))
+        score_row(lg, bias, E, p, lane, keys + (size_t)wv * E, ids + (size_t)row * K_MAX, w + (size_t)row * K_MAX,
+                  n_sel + row);
 }
 
 }  // namespace
@@ -124,8 +302,26 @@ __global__ __launch_bounds__(SC_WAVES * WAVE) void route_scores_kernel(const flo
 hipError_t launch_route_scores(const float* logits, const float* bias, uint32_t m, uint32_t E, const ScorePolicy& p,
                                uint32_t* ids, float* w, uint32_t* n_sel, hipStream_t st) {
     const geo::Grid2 g = geo::grid_run(((uint64_t)m + SC_WAVES - 1) / SC_WAVES, SC_WAVES * WAVE);
-    route_scores_kernel<<<dim3(g.x, g.y), SC_WAVES * WAVE, (size_t)SC_WAVES * E * sizeof(double), st>>>(
-            logits, bias, m, E, p, ids, w, n_sel);
+    const size_t lds = (size_t)SC_WAVES * E * sizeof(double);
+    ScorePolicy q = p;
+    q.group_lanes = WAVE;
+    while (q.group_lanes * p.n_group > WAVE) q.group_lanes /= 2;
+    const uint32_t nj = (E / p.n_group + q.group_lanes - 1) / q.group_lanes;
+    const dim3 grid(g.x, g.y);
+#define GO(N) route_scores_kernel<N><<<grid, SC_WAVES * WAVE, lds, st>>>(logits, bias, m, E, q, ids, w, n_sel)
+    if (nj <= 1)
+        GO(1);
+    else if (nj <= 2)
+        GO(2);
+    else if (nj <= 4)
+        GO(4);
+    else if (nj <= 8)
+        GO(8);
+    else if (nj <= 16)
+        GO(16);
+    else
+        GO(32);
+#undef GO
     return hipGetLastError();
 }
 

@@ -11,6 +11,7 @@
 namespace trk {
 
 constexpr int K_MAX = TRK_MOE_K_MAX;
+static_assert(geo::DIRECT_M == TRK_EXPERTS_DIRECT_M, "one rule");
 
 // Routing policy as the kernels take it (enabled == 0: fixed top-k).  packed: n_expert_packed of a
 // subset pack, the routed ids are folded onto experts 0 .. packed - 1 (fold_ids); 0: no folding.
@@ -225,6 +226,7 @@ struct ScorePolicy {
     uint32_t k, score, n_group, topk_group, group_top;
     int renorm;
     float factor;
+    uint32_t group_lanes = 0;  // lanes of a wave per group (the launcher's)
 };
 hipError_t launch_route_scores(const float* logits, const float* bias, uint32_t m, uint32_t E, const ScorePolicy& p,
                                uint32_t* ids, float* w, uint32_t* n_sel, hipStream_t st);

@@ -544,56 +544,64 @@ def gemv(wt, rows, k, fmt, item, count, kb, q, s, su, pair=False, y=None, ldy=No
 # The kernels run on torch's current stream (or `stream`) of the current device; tensors elsewhere are
 # refused.  Outputs are allocated where none is given.
 
+_torch = None  # the module, its dtypes and its device lookup once a call has needed them
 _dt = None
 _device = None
+EXPERTS_DIRECT_M = 8  # TRK_EXPERTS_DIRECT_M
+
+
+def _late():
+    """torch, imported at the first call that needs it (an import statement in each call costs half a microsecond)."""
+    global _torch, _dt, _device
+    import torch
+    _dt = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
+    _device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+    _torch = torch
+    return torch
 
 
 def _dtype(t):
     """TRK_DT_* of a torch dtype."""
-    global _dt
-    if _dt is None:
-        import torch
-        _dt = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
-    try:
-        return _dt[t]
-    except KeyError:
-        raise TrkError(f"element type {t}: float32, bfloat16 or float16 is needed") from None
+    d = _dt.get(t)
+    if d is None:
+        raise TrkError(f"element type {t}: float32, bfloat16 or float16 is needed")
+    return d
 
 
 def _here(*tensors):
     """Every tensor given is on the current device."""
-    global _device
-    if _device is None:
-        import torch
-        _device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
-    at = [t.get_device() for t in tensors if t is not None]
-    if min(at) < 0:
-        raise TrkError("tensors have to be on the GPU")
-    dev = _device()
-    if at.count(dev) != len(at):
-        raise TrkError(f"tensors on devices {sorted(set(at))}: all have to be on the current device, {dev}")
+    dev = -1
+    for t in tensors:
+        if t is not None:
+            at = t.get_device()
+            if at < 0:
+                raise TrkError("tensors have to be on the GPU")
+            if dev < 0:
+                dev = _device()
+            if at != dev:
+                raise TrkError(f"a tensor on device {at}: all have to be on the current device, {dev}")
 
 
 def _rows(t, what, m=None, k=None):
     """The stride between the rows of a matrix with contiguous rows, [m][k] where they are given."""
-    if t.dim() != 2 or (m is not None and t.shape[0] != m) or (k is not None and t.shape[1] != k):
-        raise TrkError(f"{what}: shape {tuple(t.shape)}, [{'m' if m is None else m}][{'k' if k is None else k}] is needed")
+    shape = t.shape
+    if len(shape) != 2 or (m is not None and shape[0] != m) or (k is not None and shape[1] != k):
+        raise TrkError(f"{what}: shape {tuple(shape)}, [{'m' if m is None else m}][{'k' if k is None else k}] is needed")
     s = t.stride()
-    if s[1] != 1 and t.shape[1] > 1:
+    if s[1] != 1 and shape[1] > 1:
         raise TrkError(f"{what}: the values of a row have to be contiguous")
-    if t.shape[0] > 1:
+    if shape[0] > 1:
         return s[0]
-    return max(s[0], (t.shape[1] + 15) // 16 * 16)  # of one row: any that the checks take
+    return max(s[0], (shape[1] + 15) // 16 * 16)  # of one row: any that the checks take
 
 
 def _vector(t, what, dtype, *shape):
-    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
         raise TrkError(f"{what}: a contiguous {dtype} tensor of shape {shape} is needed, not {t.dtype} {tuple(t.shape)}")
 
 
-def _i8_empty(rows, k, device):
+def _i8_empty(torch, rows, k, device):
     """int8 [rows][k], rows a multiple of 16 bytes apart."""
-    import torch
     ld = (k + 15) // 16 * 16
     q = torch.empty((rows, ld), dtype=torch.int8, device=device)
     return q if ld == k else q[:, :k]
@@ -605,7 +613,7 @@ class I8Weights:
     Keeps the tensors; copies nothing."""
 
     def __init__(self, q, scale):
-        import torch
+        torch = _torch or _late()
         if q.dtype != torch.int8 or q.dim() not in (2, 3):
             raise TrkError(f"weights: int8 [count][rows][k] or [rows][k] is needed, not {q.dtype} {tuple(q.shape)}")
         _vector(scale, "weight scales", torch.float32, *q.shape[:-1])
@@ -638,7 +646,7 @@ def quantize_weights(w, stream=None):
 def route_scores(logits, k, bias=None, score="sigmoid", n_group=1, topk_group=1, group_top=2, renorm=True, factor=1.0,
                  out=None, stream=None):
     """trk_route_scores: logits [m][E] -> (ids [m][32], w [m][32], n_sel [m]); slots k .. 31 are not written."""
-    import torch
+    torch = _torch or _late()
     if logits.dim() != 2 or logits.dtype != torch.float32 or not logits.is_contiguous():
         raise TrkError(f"logits: contiguous float32 [m][E] is needed, not {logits.dtype} {tuple(logits.shape)}")
     m, E = logits.shape
@@ -662,7 +670,7 @@ def route_scores(logits, k, bias=None, score="sigmoid", n_group=1, topk_group=1,
 
 
 def _routing(ids, n_sel, m, w=None):
-    import torch
+    torch = _torch or _late()
     _vector(ids, "ids", torch.int32, m, K_MAX)
     _vector(n_sel, "n_sel", torch.int32, m)
     if w is not None:
@@ -671,11 +679,11 @@ def _routing(ids, n_sel, m, w=None):
 
 def quantize_rows(x, out=None, stream=None):
     """trk_quantize_rows: x [m][k] -> (q int8 [m][k], scale [m]); the rows of a new q are a multiple of 16 bytes apart."""
-    import torch
+    torch = _torch or _late()
     ldx = _rows(x, "x")
     m, k = x.shape
     if out is None:
-        q, scale = _i8_empty(m, k, x.device), torch.empty(m, dtype=torch.float32, device=x.device)
+        q, scale = _i8_empty(torch, m, k, x.device), torch.empty(m, dtype=torch.float32, device=x.device)
         ldq = (k + 15) // 16 * 16
     else:
         q, scale = out
@@ -687,7 +695,7 @@ def quantize_rows(x, out=None, stream=None):
 
 
 def _i8_rows(q, scale, m, k, read=True):
-    import torch
+    torch = _torch or _late()
     if q.dtype != torch.int8:
         raise TrkError(f"q: int8 is needed, not {q.dtype}")
     ld = _rows(q, "q", m, k)
@@ -706,7 +714,7 @@ def _whole_pieces(q, rows, ld, k, what):
 def gemm_i8(w: I8Weights, q, scale, bias=None, dtype=None, out=None, accumulate=False, item=0, stream=None):
     """trk_gemm_i8: q int8 [m][k] with a scale per row, times matrix `item` of w -> [m][rows] (float32 unless `dtype` or
     `out` says otherwise)."""
-    import torch
+    torch = _torch or _late()
     m = q.shape[0]
     ldq = _i8_rows(q, scale, m, w.k)
     if bias is not None:
@@ -727,13 +735,13 @@ def gemm_i8(w: I8Weights, q, scale, bias=None, dtype=None, out=None, accumulate=
 def experts_plan(ids, n_sel, slots, n_expert, stream=None):
     """trk_experts_plan: the entries sorted by expert, for `experts_up_i8` and `experts_down_i8` of the same routing; None
     where the entries are so few that the products take none."""
-    import torch
+    torch = _torch or _late()
     m = ids.shape[0]
     _routing(ids, n_sel, m)
+    if m <= EXPERTS_DIRECT_M:
+        return None
     words = C.c_uint64()
     check(lib().trk_experts_plan_words(m, slots, n_expert, C.byref(words)))
-    if not words.value:
-        return None
     _here(ids, n_sel)
     plan = torch.empty(words.value, dtype=torch.int32, device=ids.device)
     check(lib().trk_experts_plan(ids.data_ptr(), n_sel.data_ptr(), m, slots, n_expert, plan.data_ptr(), _stream(stream)))
@@ -741,20 +749,20 @@ def experts_plan(ids, n_sel, slots, n_expert, stream=None):
 
 
 def _check_plan(plan, m, slots, count):
-    import torch
+    if m <= EXPERTS_DIRECT_M:
+        return
     words = C.c_uint64()
     check(lib().trk_experts_plan_words(m, slots, count, C.byref(words)))
-    if words.value:
-        if plan is None:
-            raise TrkError(f"{m} tokens of {slots} slots need a plan (experts_plan)")
-        _vector(plan, "plan", torch.int32, words.value)
+    if plan is None:
+        raise TrkError(f"{m} tokens of {slots} slots need a plan (experts_plan)")
+    _vector(plan, "plan", _torch.int32, words.value)
 
 
 def experts_up_i8(gate: I8Weights, up: I8Weights, q, scale, ids, n_sel, slots, plan=None, dtype=None, out=None,
                   stream=None):
     """trk_experts_up_i8: q int8 [m][H] through each token's experts -> h [m * slots][F]; rows that are no entry's are not
     written."""
-    import torch
+    torch = _torch or _late()
     m = q.shape[0]
     ldq = _i8_rows(q, scale, m, gate.k)
     _routing(ids, n_sel, m)
@@ -775,7 +783,7 @@ def experts_down_i8(down: I8Weights, q, scale, ids, w, n_sel, slots, plan=None, 
                     accumulate=False, stream=None):
     """trk_experts_down_i8: q int8 [m * slots][F] through the experts' down rows, weighted with w and summed per token ->
     [m][H].  work: at least trk_experts_down_work_bytes as a float32 tensor, allocated where it is not given."""
-    import torch
+    torch = _torch or _late()
     m = ids.shape[0]
     ldq = _i8_rows(q, scale, m * slots, down.k)
     _routing(ids, n_sel, m, w)
@@ -788,7 +796,8 @@ def experts_down_i8(down: I8Weights, q, scale, ids, w, n_sel, slots, plan=None, 
     else:
         ldy = _rows(out, "out", m, down.rows)
     need = C.c_uint64()
-    check(lib().trk_experts_down_work_bytes(m, slots, down.count, down.rows, C.byref(need)))
+    if m > EXPERTS_DIRECT_M:
+        check(lib().trk_experts_down_work_bytes(m, slots, down.count, down.rows, C.byref(need)))
     if work is None:
         work = torch.empty(need.value // 4, dtype=torch.float32, device=q.device) if need.value else None
     elif work.dtype != torch.float32 or not work.is_contiguous() or work.numel() * 4 < need.value:
