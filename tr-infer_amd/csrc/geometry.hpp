@@ -234,9 +234,15 @@ inline uint32_t plan_rows(uint32_t m, uint32_t slots, uint32_t E) {
 inline bool i8_tile_addresses(uint64_t ldw, uint64_t ldq, uint64_t rows) {
     return ldw < 1u << 23 && ldq <= 0xffffffffull / rows;
 }
-// Up tiles of 128 entries: 256 weight rows from three workgroups per CU on, else 128 (two resident).  us, 256 / 128 rows:
-// 4096 tokens of 10 in 512 experts of F = 512 245 / 256, 1000 of 8 in 128 of 768 91 / 94; 3000 of 2 in 8 of 768 28 / 24.
-inline bool up_wide(uint32_t rows, uint64_t tiles) { return (rows + 127) / 128 * tiles >= 768; }
+// Weight rows of an experts' tile (up: of gate and up together): 128, 64 where those leave CUs without a second tile, and
+// (up, of 128 entries) 256 from three tiles per CU on.  us: up, 64 / 128 rows, 100 tokens of 4 in 16 experts (H = 1024, F
+// = 512) at 32 / 64 / 128 entries a tile 7.1 / 7.5, 7.3 / 10.0, 8.1 / 11.2; down 9.5 / 9.6, 9.2 / 10.1, 9.7 / 11.2; 2000 tokens
+// of 8 in 128 (2048, 768) 138 / 124.  Up, 128 / 256: 4096 of 10 in 512 256 / 245, 1000 of 8 in 128 94 / 91, 3000 of 2 in 8 24 / 28.
+enum ExpertsWidth { X_NARROW, X_128, X_WIDE };
+inline ExpertsWidth experts_width(uint32_t rows, uint64_t tiles, bool wide) {
+    const uint64_t wgs = (rows + 127) / 128 * tiles;
+    return wgs < 512 ? X_NARROW : wide && wgs >= 1536 ? X_WIDE : X_128;
+}
 // The plan's words: {tiles, 3 unused}, ent [m * slots], (16-byte aligned) four words per tile, then the counts of each of
 // plan_workgroups' entries [workgroups][E].
 inline uint64_t plan_tiles(uint32_t m, uint32_t slots, uint32_t E, uint32_t rows) {  // no call has more

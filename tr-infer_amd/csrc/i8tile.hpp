@@ -59,9 +59,10 @@ struct I8Tile {
 
     // rw[i], wo[i]: buffer and this lane's row offset for its i-th eight weight rows; rx, xo: the activations'.
     // lrow(i): the LDS row of the wave's i-th 16 weight rows.
-    template <typename Frag>
+    // live: this wave's 16-row groups of activations that hold any (PART: the others' products are left out).
+    template <bool PART, typename Frag>
     __device__ __forceinline__ void run(uint8_t* lds, const i32x4 (&rw)[NA], const uint32_t (&wo)[NA], i32x4 rx,
-                                        const uint32_t (&xo)[NB], uint32_t k, Frag&& lrow) {
+                                        const uint32_t (&xo)[NB], uint32_t k, uint32_t live, Frag&& lrow) {
         const uint32_t l0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
         const uint32_t S = (k + BK - 1) / BK;
         const uint32_t piece = 16 * (lane % 8 ^ lane / 8);  // where in a row this lane loads
@@ -87,21 +88,36 @@ struct I8Tile {
         auto read_b = [&](uint32_t at, int kk, int h, int to) {
 #pragma unroll
             for (int j = 0; j < FH; j++)
-                b[to][j] = *reinterpret_cast<const i32x4*>(lds + at + (BN + wm + (h * FH + j) * 16) * BK + (la ^ (64 * kk)));
+                if (!PART || h * FH + j < (int)live) b[to][j] = *reinterpret_cast<const i32x4*>(lds + at + (BN + wm + (h * FH + j) * 16) * BK + (la ^ (64 * kk)));
         };
         // a phase's products, with the loads of a stage between them: all at once they would hold up every wave for as
         // long as the memory pipe takes to accept them
         auto mul = [&](int kk, int h, int from, bool loads, uint32_t o, uint32_t at) {
+            if constexpr (PART) {
 #pragma unroll
-            for (int i = 0; i < FN; i++) {
+                for (int j = 0; j < FH; j++) {
+                    if (h * FH + j < (int)live) {
 #pragma unroll
-                for (int j = 0; j < FH; j++) acc[i][h * FH + j] = mfma_i8(a[kk][i], b[from][j], acc[i][h * FH + j]);
-                // the products stay where they are, on their side of the barrier
+                        for (int i = 0; i < FN; i++) acc[i][h * FH + j] = mfma_i8(a[kk][i], b[from][j], acc[i][h * FH + j]);
 #pragma unroll
-                for (int j = 0; j < FH; j++) asm volatile("" : "+v"(acc[i][h * FH + j]));
-                if (loads)
+                        for (int i = 0; i < FN; i++) asm volatile("" : "+v"(acc[i][h * FH + j]));
+                    }
+                    if (loads)
 #pragma unroll
-                    for (int n = i * (NA + NB) / FN; n < (i + 1) * (NA + NB) / FN; n++) load1(o, at, n);
+                        for (int n = j * (NA + NB) / FH; n < (j + 1) * (NA + NB) / FH; n++) load1(o, at, n);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < FN; i++) {
+#pragma unroll
+                    for (int j = 0; j < FH; j++) acc[i][h * FH + j] = mfma_i8(a[kk][i], b[from][j], acc[i][h * FH + j]);
+                    // the products stay where they are, on their side of the barrier
+#pragma unroll
+                    for (int j = 0; j < FH; j++) asm volatile("" : "+v"(acc[i][h * FH + j]));
+                    if (loads)
+#pragma unroll
+                        for (int n = i * (NA + NB) / FN; n < (i + 1) * (NA + NB) / FN; n++) load1(o, at, n);
+                }
             }
             __builtin_amdgcn_sched_barrier(0);
         };

@@ -218,8 +218,7 @@ __global__ __launch_bounds__(Tile::T) void experts_up_tile_kernel(I8Up a, Plan P
         rw[i] = up ? bu : bg, wo[i] = rc * (uint32_t)(up ? a.up.ld : a.gate.ld);
     }
     const uint32_t wr = t.wn / 2;  // this wave's first row of both
-    t.run(lds, rw, wo, buffer_at(a.q), xo, a.gate.k, [&](int i) { return i < FR ? wr + 16 * i : BR + wr + 16 * (i - FR); });
-    typedef Elem<DT> O;
+    // what the entries and rows are scaled with, before the loads that the products wait for
     float sg[FR][4], su[FR][4], sx[Tile::FM];
     uint32_t en[Tile::FM];
 #pragma unroll
@@ -234,6 +233,9 @@ __global__ __launch_bounds__(Tile::T) void experts_up_tile_kernel(I8Up a, Plan P
         }
 #pragma unroll
     for (int j = 0; j < Tile::FM; j++) sx[j] = a.sx[en[j] / a.slots];
+    const uint32_t live = t.wm < pt.rows ? (pt.rows - t.wm + 15) / 16 : 0;
+    t.template run<true>(lds, rw, wo, buffer_at(a.q), xo, a.gate.k, live, [&](int i) { return i < FR ? wr + 16 * i : BR + wr + 16 * (i - FR); });
+    typedef Elem<DT> O;
 #pragma unroll
     for (int j = 0; j < Tile::FM; j++) {
         if (t.wm + 16 * j + t.lane % 16 >= pt.rows) continue;
@@ -270,7 +272,6 @@ __global__ __launch_bounds__(Tile::T) void experts_down_tile_kernel(I8Down a, Pl
         const uint32_t r = t.load_row(i);
         rw[i] = bw, wo[i] = (r < rl ? r : rl) * (uint32_t)a.down.ld;
     }
-    t.run(lds, rw, wo, buffer_at(a.q), xo, a.down.k, [&](int i) { return t.wn + 16 * i; });
     float sw[Tile::FN][4], sx[Tile::FM], w[Tile::FM];
     uint32_t en[Tile::FM];
 #pragma unroll
@@ -285,6 +286,8 @@ __global__ __launch_bounds__(Tile::T) void experts_down_tile_kernel(I8Down a, Pl
 #pragma unroll
     for (int j = 0; j < Tile::FM; j++)
         sx[j] = a.sx[en[j]], w[j] = a.w[(size_t)(en[j] / a.slots) * K_MAX + en[j] % a.slots];
+    const uint32_t live = t.wm < pt.rows ? (pt.rows - t.wm + 15) / 16 : 0;
+    t.template run<true>(lds, rw, wo, buffer_at(a.q), xo, a.down.k, live, [&](int i) { return t.wn + 16 * i; });
 #pragma unroll
     for (int j = 0; j < Tile::FM; j++) {
         if (t.wm + 16 * j + t.lane % 16 >= pt.rows) continue;
@@ -318,7 +321,7 @@ __global__ __launch_bounds__(256) void experts_combine_kernel(I8Down a) {
         for (uint32_t j = 0; j < 4; j++) {
             const uint32_t jc = j0 + j < n ? j0 + j : n - 1;
             on[j] = j0 + j < n && a.ids[(size_t)t * K_MAX + jc] < a.down.count;
-            if (!on[j]) continue;
+            if (j0 + j >= n) continue;  // a row of no entry is read (anything) and not added: no load waits for another
             const float* f = s + (uint64_t)jc * w;
             if (w % 4 == 0) {
                 const float4 x = *reinterpret_cast<const float4*>(f);
@@ -390,14 +393,18 @@ hipError_t launch_experts_up(const I8Up& a, const uint32_t* plan, hipStream_t st
     const uint32_t rows = geo::plan_rows(a.m, a.slots, E);
     const Plan P = plan_at(const_cast<uint32_t*>(plan), a.m, a.slots);
     const uint64_t tiles = geo::plan_tiles(a.m, a.slots, E, rows);
+    const geo::ExpertsWidth w = geo::experts_width(2 * a.gate.rows, tiles, rows == 128);
     if (rows == 32)
-        launch_up_tile<I8Tile<128, 32, 32, 32, 3>>(a, P, tiles, st);
+        w == geo::X_NARROW ? launch_up_tile<I8Tile<64, 32, 32, 16, 4>>(a, P, tiles, st)
+                           : launch_up_tile<I8Tile<128, 32, 32, 32, 3>>(a, P, tiles, st);
     else if (rows == 64)
-        launch_up_tile<I8Tile<128, 64, 64, 32, 2>>(a, P, tiles, st);
-    else if (geo::up_wide(a.gate.rows, tiles))
-        launch_up_tile<I8Tile<256, 128, 64, 64, 3>>(a, P, tiles, st);
+        w == geo::X_NARROW ? launch_up_tile<I8Tile<64, 64, 32, 32, 4>>(a, P, tiles, st)
+                           : launch_up_tile<I8Tile<128, 64, 64, 32, 2>>(a, P, tiles, st);
+    else if (w == geo::X_NARROW)
+        launch_up_tile<I8Tile<64, 128, 32, 64, 3>>(a, P, tiles, st);
     else
-        launch_up_tile<I8Tile<128, 128, 64, 64, 2>>(a, P, tiles, st);
+        w == geo::X_WIDE ? launch_up_tile<I8Tile<256, 128, 64, 64, 3>>(a, P, tiles, st)
+                         : launch_up_tile<I8Tile<128, 128, 64, 64, 2>>(a, P, tiles, st);
     return hipGetLastError();
 }
 
@@ -426,12 +433,16 @@ hipError_t launch_experts_down(const I8Down& a, const uint32_t* plan, hipStream_
     const uint32_t rows = geo::plan_rows(a.m, a.slots, E);
     const Plan P = plan_at(const_cast<uint32_t*>(plan), a.m, a.slots);
     const uint64_t tiles = geo::plan_tiles(a.m, a.slots, E, rows);
+    const bool narrow = geo::experts_width(a.down.rows, tiles, false) == geo::X_NARROW;
     if (rows == 32)
-        launch_down_tile<I8Tile<128, 32, 32, 32, 3>>(a, P, tiles, st);
+        narrow ? launch_down_tile<I8Tile<64, 32, 16, 32, 4>>(a, P, tiles, st)
+               : launch_down_tile<I8Tile<128, 32, 32, 32, 3>>(a, P, tiles, st);
     else if (rows == 64)
-        launch_down_tile<I8Tile<128, 64, 64, 32, 3>>(a, P, tiles, st);
+        narrow ? launch_down_tile<I8Tile<64, 64, 32, 32, 4>>(a, P, tiles, st)
+               : launch_down_tile<I8Tile<128, 64, 64, 32, 3>>(a, P, tiles, st);
     else
-        launch_down_tile<I8Tile<128, 128, 64, 64, 2>>(a, P, tiles, st);
+        narrow ? launch_down_tile<I8Tile<64, 128, 32, 64, 3>>(a, P, tiles, st)
+               : launch_down_tile<I8Tile<128, 128, 64, 64, 2>>(a, P, tiles, st);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const uint32_t q = (a.down.rows + 3) / 4, per = q < 256 ? 256 / q : 1;
