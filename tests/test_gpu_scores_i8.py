@@ -302,7 +302,10 @@ def routing(rng, m, E, slots, kind):
 CASES = [(1, 1, 1, 64, 32, "plain"), (1, 512, 10, 256, 48, "plain"), (3, 64, 8, 300, 100, "ragged"),
          (8, 8, 2, 129, 17, "elsewhere"), (9, 8, 2, 129, 17, "elsewhere"), (40, 16, 4, 512, 130, "plain"),
          (64, 5, 32, 96, 65, "ragged"), (150, 512, 10, 256, 64, "plain"), (300, 3, 1, 640, 200, "one"),
-         (700, 40, 6, 272, 96, "elsewhere"), (33, 1024, 32, 64, 16, "plain"), (2000, 7, 3, 160, 129, "ragged")]
+         (700, 40, 6, 272, 96, "elsewhere"), (33, 1024, 32, 64, 16, "plain"), (2000, 7, 3, 160, 129, "ragged"),
+         # enough tiles for the wider ones: 32, 64 and 128 entries, and up's of 256 weight rows
+         (250, 64, 4, 80, 1030, "plain"), (500, 64, 4, 80, 1030, "ragged"), (700, 40, 6, 64, 1100, "elsewhere"),
+         (1600, 50, 4, 48, 1024, "plain")]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -361,6 +364,42 @@ def test_experts_down(m, E, slots, F, H, kind, dtype):
         want = ref + (9 if acc else 0)
         tol = err + (1.01 * R.EPS["f32"] * (size + 9) if acc else 0) + 1.01 * R.round_rel(np.abs(want) + err, dtype)
         assert (np.abs(got[:m, :H] - want) <= tol).all()
+
+
+@pytest.mark.parametrize("far", ["weights", "rows"])
+def test_rows_far_apart(far):
+    """Rows so far apart that 32-bit offsets do not reach them (4 GB of activations, 8 MB between weight rows)."""
+    import torch
+    say(f"rows far apart: {far}")
+    rng = np.random.default_rng(8)
+    ld = 1 << 23
+    m, E, slots, F, H, k = (520, 2, 1, 17, 70, 70) if far == "rows" else (40, 2, 2, 17, 70, 70)
+
+    def apart(a, on):
+        if not on:
+            return padded(a)
+        rows = a.reshape(-1, a.shape[-1])
+        t = torch.empty((rows.shape[0], ld), dtype=torch.int8, device="cuda")
+        t[:, :a.shape[-1]] = dev(rows)
+        return t.view(*a.shape[:-1], ld)[..., :a.shape[-1]]
+
+    q, s = i8(rng, m, k), scales(rng, m)
+    w, ws = i8(rng, E, F, k), scales(rng, E, F, around=0.005)
+    W, Q = trmoe.I8Weights(apart(w, far == "weights"), dev(ws)), apart(q, far == "rows")
+    ref = R.gemm(q, s, w[1], ws[1])
+    assert (np.abs(host(trmoe.gemm_i8(W, Q, dev(s), item=1)) - ref) <= R.gemm_tol(ref, "f32")).all()
+    ids, wt, n = routing(rng, m, E, slots, "plain")
+    di, dn = dev(ids), dev(n)
+    plan = trmoe.experts_plan(di, dn, slots, E)
+    h = host(trmoe.experts_up_i8(W, W, Q, dev(s), di, dn, slots, plan=plan)).astype(np.float64)
+    e = ids[:, :slots].reshape(-1)
+    t = np.arange(m * slots) // slots
+    g = np.concatenate([R.gemm(q[t[i]:t[i] + 1], s[t[i]:t[i] + 1], w[e[i]], ws[e[i]]) for i in range(m * slots)])
+    assert (np.abs(h - R.swiglu(g, g)) <= R.swiglu_tol(g, g, "f32")).all()
+    if far == "rows":  # one slot: row t is entry t
+        y = host(trmoe.experts_down_i8(W, Q, dev(s), di, dev(wt), dn, slots, plan=plan)).astype(np.float64)
+        ref = g * wt[:, :1].astype(np.float64)
+        assert (np.abs(y - ref) <= 5.05 * R.EPS["f32"] * np.abs(ref) + 1.01 * R.round_rel(ref, "f32")).all()
 
 
 def test_experts_refuse():
@@ -480,6 +519,35 @@ def test_on_two_streams_at_once():
             got.append(y)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_stream_given():
+    """Every call on a stream of the caller's, after work queued there, while the current stream goes on."""
+    import torch
+    say("a stream given")
+    _, bias, gate, up, down = a_block(21)
+    lg, x = torch.randn((60, 32), device="cuda"), torch.randn((60, 256), device="cuda")
+    st = torch.cuda.Stream()
+
+    def run(**kw):
+        ids, w, n = trmoe.route_scores(lg, 4, bias=bias, **kw)
+        plan = trmoe.experts_plan(ids, n, 4, gate.count, **kw)
+        q, s = trmoe.quantize_rows(x, **kw)
+        h = trmoe.experts_up_i8(gate, up, q, s, ids, n, 4, plan=plan, **kw)
+        hq, hs = trmoe.quantize_rows(h, **kw)
+        y = trmoe.experts_down_i8(down, hq, hs, ids, w, n, 4, plan=plan, **kw)
+        W = trmoe.I8Weights(gate.q[3], gate.scale[3])
+        return y, trmoe.gemm_i8(W, q, s, **kw), (ids, w, n, plan, q, s, h, hq, hs)  # kept until the stream is done
+
+    want = run()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        st.wait_stream(torch.cuda.current_stream())
+        got = run(stream=st)
+        junk = [torch.full((60 * 4 * 256,), float("nan"), device="cuda") for _ in range(4)]  # over what was freed
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        del junk
 
 
 def test_the_same_bits_every_time():

@@ -148,3 +148,15 @@ def test_python_calls_refuse_tensors_elsewhere_and_of_wrong_shape():
         trmoe.route_scores(torch.zeros((2, 8)), 2, bias=torch.zeros(7))
     with pytest.raises(trmoe.TrkError, match="ids"):
         trmoe.experts_plan(torch.zeros((2, 8), dtype=torch.int32), torch.zeros(2, dtype=torch.int32), 2, 8)
+
+
+def test_forms_and_plan_extents_on_the_host(tmp_path):
+    """The rules that choose a form, at sizes where the forms were timed, and the plan's sizes under any load."""
+    import os
+    import subprocess
+    here = os.path.dirname(os.path.abspath(__file__))
+    exe = str(tmp_path / "i8_rules_check")
+    subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-Werror", os.path.join(here, "i8_rules_check.cpp"), "-o", exe],
+                   check=True)
+    r = subprocess.run([exe], capture_output=True, text=True)
+    assert r.returncode == 0 and r.stdout.startswith("ok"), r.stdout

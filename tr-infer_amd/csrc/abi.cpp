@@ -962,7 +962,7 @@ extern "C" int trk_gemm_i8(const trk_i8_mat* w, uint32_t item, const int8_t* q, 
     if (!q || !scale || !y) return fail(TRK_E_INVALID, "null argument");
     const I8Mat M = i8_mat(*w);
     const float* ws = M.scale + (uint64_t)item * M.rows;
-    const int vec = (uintptr_t)ws % 16 == 0 && (uintptr_t)y % (dtype == TRK_DT_F32 ? 16 : 8) == 0 && (m == 1 || ldy % 4 == 0);
+    const int vec = (uintptr_t)y % (dtype == TRK_DT_F32 ? 16 : 8) == 0 && (m == 1 || ldy % 4 == 0);
     const I8Gemm a{M.ptr + item * M.stride, ws, M.rows, M.k, M.ld, q, ldq, scale, m, bias, y, dtype, ldy, accumulate, vec};
     HIP_TRY(launch_gemm_i8(a, (hipStream_t)stream));
     return TRK_OK;

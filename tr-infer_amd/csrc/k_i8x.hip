@@ -378,9 +378,17 @@ static void launch_up_tile(const I8Up& a, const Plan& P, uint64_t tiles, hipStre
         experts_up_tile_kernel<Tile, TRK_DT_F16><<<g, Tile::T, 0, st>>>(a, P);
 }
 
-hipError_t launch_experts_up(const I8Up& a, const uint32_t* plan, hipStream_t st) {
-    const uint32_t E = a.gate.count;
-    if (!plan || !geo::i8_tile_addresses(a.gate.ld, a.ldq, a.m) || !geo::i8_tile_addresses(a.up.ld, a.ldq, a.m)) {
+// The kernels number their workgroups by 32 bits: of entries beyond, so many tokens a launch.
+static uint32_t strip_tokens(uint32_t rows, uint32_t per_token) {
+    const uint64_t t = 0x7fffffffull / ((rows + 15) / 16) / per_token;
+    return t < 1 ? 1 : t > 0x7fffffffull ? 0x7fffffffu : (uint32_t)t;
+}
+
+static void launch_up_strip(I8Up a, hipStream_t st) {
+    const uint32_t m = a.m, step = strip_tokens(a.gate.rows, a.slots);
+    const uint64_t size = a.dt == TRK_DT_F32 ? 4 : 2;
+    for (uint64_t t = 0; t < m; t += step) {
+        a.m = m - t < step ? m - (uint32_t)t : step;
         const dim3 g = run_of((uint64_t)((a.gate.rows + 15) / 16) * a.m * a.slots, ST_WAVES * WAVE);
         if (a.dt == TRK_DT_F32)
             experts_up_strip_kernel<TRK_DT_F32><<<g, ST_WAVES * WAVE, 0, st>>>(a);
@@ -388,6 +396,15 @@ hipError_t launch_experts_up(const I8Up& a, const uint32_t* plan, hipStream_t st
             experts_up_strip_kernel<TRK_DT_BF16><<<g, ST_WAVES * WAVE, 0, st>>>(a);
         else
             experts_up_strip_kernel<TRK_DT_F16><<<g, ST_WAVES * WAVE, 0, st>>>(a);
+        a.q += step * a.ldq, a.sx += step, a.ids += (uint64_t)step * K_MAX, a.n_sel += step;
+        a.h = (char*)a.h + (uint64_t)step * a.slots * a.ldh * size;
+    }
+}
+
+hipError_t launch_experts_up(const I8Up& a, const uint32_t* plan, hipStream_t st) {
+    const uint32_t E = a.gate.count;
+    if (!plan || !geo::i8_tile_addresses(a.gate.ld, a.ldq, a.m) || !geo::i8_tile_addresses(a.up.ld, a.ldq, a.m)) {
+        launch_up_strip(a, st);
         return hipGetLastError();
     }
     const uint32_t rows = geo::plan_rows(a.m, a.slots, E);
@@ -408,14 +425,22 @@ hipError_t launch_experts_up(const I8Up& a, const uint32_t* plan, hipStream_t st
     return hipGetLastError();
 }
 
-static void launch_down_strip(const I8Down& a, hipStream_t st) {
-    const dim3 g = run_of((uint64_t)((a.down.rows + 15) / 16) * a.m, DOWN_WAVES * WAVE);
-    if (a.dt == TRK_DT_F32)
-        experts_down_strip_kernel<TRK_DT_F32><<<g, DOWN_WAVES * WAVE, 0, st>>>(a);
-    else if (a.dt == TRK_DT_BF16)
-        experts_down_strip_kernel<TRK_DT_BF16><<<g, DOWN_WAVES * WAVE, 0, st>>>(a);
-    else
-        experts_down_strip_kernel<TRK_DT_F16><<<g, DOWN_WAVES * WAVE, 0, st>>>(a);
+static void launch_down_strip(I8Down a, hipStream_t st) {
+    const uint32_t m = a.m, step = strip_tokens(a.down.rows, 1);
+    const uint64_t size = a.dt == TRK_DT_F32 ? 4 : 2;
+    for (uint64_t t = 0; t < m; t += step) {
+        a.m = m - t < step ? m - (uint32_t)t : step;
+        const dim3 g = run_of((uint64_t)((a.down.rows + 15) / 16) * a.m, DOWN_WAVES * WAVE);
+        if (a.dt == TRK_DT_F32)
+            experts_down_strip_kernel<TRK_DT_F32><<<g, DOWN_WAVES * WAVE, 0, st>>>(a);
+        else if (a.dt == TRK_DT_BF16)
+            experts_down_strip_kernel<TRK_DT_BF16><<<g, DOWN_WAVES * WAVE, 0, st>>>(a);
+        else
+            experts_down_strip_kernel<TRK_DT_F16><<<g, DOWN_WAVES * WAVE, 0, st>>>(a);
+        const uint64_t rows = (uint64_t)step * a.slots;
+        a.q += rows * a.ldq, a.sx += rows, a.ids += (uint64_t)step * K_MAX, a.w += (uint64_t)step * K_MAX, a.n_sel += step;
+        a.y = (char*)a.y + step * a.ldy * size;
+    }
 }
 
 template <typename Tile>

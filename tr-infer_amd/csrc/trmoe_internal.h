@@ -251,7 +251,7 @@ struct I8Gemm {
     uint32_t dt;
     uint64_t ldy;
     int accumulate;
-    int vec;  // four neighbouring outputs, and their scales, lie on a boundary of four
+    int vec;  // four neighbouring outputs lie on a boundary of four
 };
 struct I8Up {
     I8Mat gate, up;

@@ -8,6 +8,7 @@ There is no CPU fallback: without the built HIP library every entry point raises
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -643,6 +644,12 @@ def quantize_weights(w, stream=None):
     return I8Weights(q, s.view(w.shape[:-1]))
 
 
+@functools.lru_cache(maxsize=64)
+def _score_policy(*fields):
+    """A trk_score_policy by reference: a program has few, and making one takes as long as a launch."""
+    return C.byref(ScorePolicy(*fields))
+
+
 def route_scores(logits, k, bias=None, score="sigmoid", n_group=1, topk_group=1, group_top=2, renorm=True, factor=1.0,
                  out=None, stream=None):
     """trk_route_scores: logits [m][E] -> (ids [m][32], w [m][32], n_sel [m]); slots k .. 31 are not written."""
@@ -663,8 +670,8 @@ def route_scores(logits, k, bias=None, score="sigmoid", n_group=1, topk_group=1,
         ids, w, n = out
         _routing(ids, n, m, w)
     _here(logits, bias, ids, w, n)
-    p = ScorePolicy(k, SCORES[score], n_group, topk_group, group_top, int(renorm), factor)
-    check(lib().trk_route_scores(logits.data_ptr(), _ptr(bias), m, E, C.byref(p), ids.data_ptr(), w.data_ptr(),
+    p = _score_policy(k, SCORES[score], n_group, topk_group, group_top, int(renorm), factor)
+    check(lib().trk_route_scores(logits.data_ptr(), _ptr(bias), m, E, p, ids.data_ptr(), w.data_ptr(),
                                  n.data_ptr(), _stream(stream)))
     return ids, w, n
 
@@ -799,7 +806,10 @@ def experts_down_i8(down: I8Weights, q, scale, ids, w, n_sel, slots, plan=None, 
     if m > EXPERTS_DIRECT_M:
         check(lib().trk_experts_down_work_bytes(m, slots, down.count, down.rows, C.byref(need)))
     if work is None:
-        work = torch.empty(need.value // 4, dtype=torch.float32, device=q.device) if need.value else None
+        if need.value:
+            work = torch.empty(need.value // 4, dtype=torch.float32, device=q.device)
+            if stream is not None:
+                work.record_stream(stream)  # given back on return, while that stream still works on it
     elif work.dtype != torch.float32 or not work.is_contiguous() or work.numel() * 4 < need.value:
         raise TrkError(f"work: {need.value // 4} contiguous float32 values are needed")
     _here(q, scale, ids, w, n_sel, plan, work, out, down.q)
