@@ -116,6 +116,27 @@ def test_route_scores_ties_and_near_ties():
     assert host(ids)[0, :2].tolist() == [32, 33]
 
 
+@pytest.mark.parametrize("score,groups,keep", [("sigmoid", 1, 1), ("softmax", 1, 1), ("sigmoid", 8, 4), ("softmax", 4, 2)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_route_scores_crowded(score, groups, keep, bias):
+    """Keys so near that 32 bits do not order them, and grids of values with many ties."""
+    say(f"route_scores crowded {score} {groups}/{keep} bias={bias}")
+    rng = np.random.default_rng(groups + bias)
+    E, m, k = 256, 40, 8
+    near = (rng.standard_normal((m, E)) * 1e-4).astype(np.float32)
+    ties = (np.rint(rng.standard_normal((m, E)) * 8) / 8).astype(np.float32)
+    b = (rng.standard_normal(E) * 0.05).astype(np.float32)
+    for lg, bb in ((near, b * 1e-4), (near + 3, b * 0), (ties, np.rint(b * 16).astype(np.float32) / 16), (ties, b * 1e3)):
+        bb = bb.astype(np.float32) if bias else None
+        lg = lg.astype(np.float32)
+        for top in (1, 2):
+            kw = dict(k=k, n_group=groups, topk_group=keep, group_top=top, renorm=True, factor=1.0)
+            ids, w, n = trmoe.route_scores(dev(lg), bias=None if bb is None else dev(bb), score=score, **kw)
+            rid, rw, rn = R.route(lg, bias=bb, score=score, **kw)
+            assert np.array_equal(host(ids)[:, :k], rid) and np.array_equal(host(n), rn)
+            np.testing.assert_allclose(host(w)[:, :k], rw, rtol=2.0 ** -22)
+
+
 def test_route_scores_extremes():
     """Scores that underflow in 32 bits still make weights; where all vanish the weights are zeros."""
     say("route_scores extremes")

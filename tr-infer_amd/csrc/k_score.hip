@@ -3,8 +3,9 @@
 //
 // A row is 4 E bytes and some ten operations a logit; what bounds the kernel is the chain of steps of a row (scores,
 // groups, selection) with few waves, and their instructions with many.  So keys are compared in 32 bits with a bound
-// on what 32 bits get wrong: a row in which two keys (or group sums) that decide something are nearer than that, or in
-// which more than 64 keys are in question, is done again in 64 bits.  Some rows in a thousand are.
+// on what 32 bits get wrong.  Where two group sums or keys that decide something are nearer than that (some rows in a
+// thousand), the sums, or the few keys in question, are taken in 64 bits; a row with more than 64 keys in question (many
+// equal ones) is done in 64 bits from the start.
 #include "route.hpp"
 
 namespace trk {
@@ -134,9 +135,10 @@ __device__ __forceinline__ void merge2(float& a1, float& a2, float b1, float b2)
 constexpr float LOG2E = 1.44269504f;
 constexpr uint32_t SC_CAND = 64 + 34;  // LDS entries a wave: candidates, then the best in order
 
-// One row; false where 64 bits have to decide.  NJ: logits a lane holds.  Lanes are split evenly over the groups.
-template <int NJ>
-__device__ bool score_row32(const float* __restrict__ lg, const float* __restrict__ bias, uint32_t E, const ScorePolicy& p,
+// One row; false where 64 bits have to decide.  NJ: logits a lane holds.  Lanes are split evenly over the groups.  What the
+// policy asks for is in the template: with branches on it between a row's loads they wait for one another.
+template <int NJ, bool SOFT, bool BIAS, bool GROUPED>
+__device__ __forceinline__ bool score_row32(const float* __restrict__ lg, const float* __restrict__ bias, uint32_t E, const ScorePolicy& p,
                             uint32_t lane, uint2* cand, uint32_t* __restrict__ ids, float* __restrict__ w,
                             uint32_t* __restrict__ n_sel) {
     const float NONE = -__builtin_inff();
@@ -149,17 +151,22 @@ __device__ bool score_row32(const float* __restrict__ lg, const float* __restric
         const bool in = g < p.n_group && r < gs;
         idx[j] = in ? g * gs + r : 0;
         v[j] = lg[idx[j]];
-        key[j] = bias ? bias[idx[j]] : 0.0f;
-        if (!in || !(v[j] > NONE)) v[j] = NONE;  // NaN compares false
+        key[j] = BIAS ? bias[idx[j]] : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+        const bool in = g < p.n_group && r0 + L * j < gs;
+        v[j] = in && v[j] > NONE ? v[j] : NONE;  // NaN compares false
     }
     float mx = 0.0f, denom = 1.0f, tol = 0.0f, scale = 1.0f;
-    const bool sums = p.n_group > 1 && p.group_top == 2, scored = bias || sums;
-    if (p.score == TRK_SCORE_SOFTMAX) {
+    const bool sums = GROUPED && p.group_top == 2;
+    const bool scored = BIAS || sums;  // else keys are logits
+    if constexpr (SOFT) {
         uint32_t mk = 0;
 #pragma unroll
         for (int j = 0; j < NJ; j++) mk = mk > fkey(v[j]) ? mk : fkey(v[j]);
         mk = wave_max_u32(mk);
-        if (mk == 0 || mk == fkey(__builtin_inff())) return false;  // nothing to choose, or scores that are NaN
+        if (mk == fkey(__builtin_inff())) return false;  // scores that are NaN
         mx = fkey_inv(mk);
         float s = 0.0f;
 #pragma unroll
@@ -168,28 +175,39 @@ __device__ bool score_row32(const float* __restrict__ lg, const float* __restric
         scale = 1.0f / denom;  // the largest score
         // (l - mx) log2 e and its power are off by d 3 2^-24 + 2^-23 at distance d, where d e^-d <= 0.37; the sum by 38
         // roundings and its terms': a score by less than 2^-18 of the largest
-        tol = scale * 0x1p-16f;
+        tol = scale * 0x1p-18f;
     } else {
         // s (1 - s) |l| <= 0.23: the argument's two roundings, the power's, the sum's and the reciprocal's make less
         // than 2^-22
-        tol = 0x1p-20f;
+        tol = 0x1p-22f;
     }
     float a1 = NONE, a2 = NONE;  // of this lane's keys
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
-        if (scored) {
-            const float s = p.score == TRK_SCORE_SOFTMAX
-                                    ? __builtin_amdgcn_exp2f((v[j] - mx) * LOG2E) * scale
-                                    : __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-v[j] * LOG2E));
+        if (BIAS || GROUPED) {  // (groups by their best logit alone: the logits again, below)
+            const float s = SOFT ? __builtin_amdgcn_exp2f((v[j] - mx) * LOG2E) * scale
+                                 : __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-v[j] * LOG2E));
             const float k = s + key[j];
-            key[j] = v[j] > NONE && k > NONE ? k : NONE;
+            key[j] = v[j] > NONE && k > NONE ? (scored ? k : v[j]) : NONE;
         } else {
             key[j] = v[j];
         }
         merge2(a1, a2, key[j], NONE);
     }
-    bool near = false;
-    if (p.n_group > 1) {
+    // score and key in 64 bits; the softmax's sum too, once one of them is asked for
+    double denom64 = 0.0;
+    auto sum64 = [&] {
+        if (!SOFT || denom64 != 0.0) return;
+        double s = 0.0;
+#pragma unroll
+        for (int j = 0; j < NJ; j++) s += v[j] > NONE ? ::exp((double)v[j] - (double)mx) : 0.0;
+        denom64 = wave_sum(s);
+    };
+    auto key64 = [&](float l, float b) {
+        const double s = SOFT ? ::exp((double)l - (double)mx) / denom64 : 1.0 / (1.0 + ::exp(-(double)l));
+        return s + (BIAS ? (double)b : 0.0);
+    };
+    if constexpr (GROUPED) {
         if (L > 1) merge2(a1, a2, dpp_f<0xB1>(a1), dpp_f<0xB1>(a2));    // lane ^ 1
         if (L > 2) merge2(a1, a2, dpp_f<0x4E>(a1), dpp_f<0x4E>(a2));    // ^ 2
         if (L > 4) merge2(a1, a2, dpp_f<0x141>(a1), dpp_f<0x141>(a2));  // mirrored in 8: the other quad
@@ -201,22 +219,43 @@ __device__ bool score_row32(const float* __restrict__ lg, const float* __restric
             const float o = rdl(worth, i * L);
             rank += o > worth || (o == worth && i < g) ? 1u : 0u;
         }
-        const bool kept = rank < p.topk_group && worth > NONE;
-        // the worst group kept and the best one dropped; a sum of two keys is off by twice a key
+        bool kept = rank < p.topk_group && worth > NONE;
+        // the worst group kept and the best one dropped; a sum of two keys is off by twice a key and a rounding
         const uint32_t lo = ~wave_max_u32(kept ? ~fkey(worth) : 0u), hi = wave_max_u32(kept ? 0u : fkey(worth));
         if (scored && hi && lo != 0xffffffffu) {
             const float fl = fkey_inv(lo), fh = fkey_inv(hi);
-            near = !(fl - fh > 2.0f * tol + 0x1p-20f * __builtin_fmaxf(__builtin_fabsf(fl), __builtin_fabsf(fh)));
+            // of a sum: its keys' errors, their roundings and its own
+            const float both = __builtin_fabsf(a1) + (a2 > NONE ? __builtin_fabsf(a2) : 0.0f);
+            const float big = __uint_as_float(wave_max_u32(g < p.n_group && a1 > NONE ? __float_as_uint(both) : 0u));
+            if (!(fl - fh > 4.0f * tol + 0x1p-22f * big)) {
+                sum64();
+                double d1 = (double)NONE, d2 = (double)NONE;
+#pragma unroll
+                for (int j = 0; j < NJ; j++) {
+                    const double k = key[j] > NONE ? key64(v[j], BIAS ? bias[idx[j]] : 0.0f) : (double)NONE;
+                    d2 = ::fmax(d2, ::fmin(d1, k)), d1 = ::fmax(d1, k);
+                }
+                for (uint32_t d = 1; d < L; d *= 2) {
+                    const double o1 = __shfl_xor(d1, d), o2 = __shfl_xor(d2, d);
+                    d2 = ::fmax(::fmin(d1, o1), ::fmax(d2, o2)), d1 = ::fmax(d1, o1);
+                }
+                const double w64 = g >= p.n_group ? (double)NONE : sums && d2 > (double)NONE ? d1 + d2 : d1;
+                rank = 0;
+                for (uint32_t i = 0; i < p.n_group; i++) {
+                    const double o = __shfl(w64, i * L);
+                    rank += o > w64 || (o == w64 && i < g) ? 1u : 0u;
+                }
+                kept = rank < p.topk_group && w64 > (double)NONE;
+            }
         }
 #pragma unroll
         for (int j = 0; j < NJ; j++) {
-            if (!bias && sums) key[j] = v[j];  // the choice itself goes by the logits
-            if (!kept) key[j] = NONE;
+            key[j] = !kept ? NONE : BIAS ? key[j] : v[j];  // without a bias the choice goes by the logits
         }
     }
     // Selection as route_select's: the kk-th largest of the lanes' maxima, cut to 16 bits, bounds the kk-th largest key
     // from below; the keys that reach it are ranked.  kk = k + 1 where the next key has to be told from the k-th.
-    const uint32_t kk = p.k + (bias ? 1u : 0u);
+    const uint32_t kk = p.k + (BIAS ? 1u : 0u);
     uint32_t fk[NJ], lmax = 0;
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
@@ -232,6 +271,10 @@ __device__ bool score_row32(const float* __restrict__ lg, const float* __restric
         const uint32_t c3 = (uint32_t)__popcll(__ballot(lmax >= t3));
         T = c3 >= kk ? t3 : (c2 >= kk ? t2 : (c1 >= kk ? t1 : T));
     }
+    if (BIAS && T > 1u) {  // and what 32 bits may have put below it
+        const float f = fkey_inv(T);
+        T = fkey(f - 2.0f * tol - 0x1p-22f * __builtin_fabsf(f));
+    }
     T = T > 1u ? T : 1u;
     uint32_t C = 0;
 #pragma unroll
@@ -242,7 +285,7 @@ __device__ bool score_row32(const float* __restrict__ lg, const float* __restric
         if (c && at < 64u) cand[at] = make_uint2(fk[j], idx[j]);
         C += (uint32_t)__popcll(m);
     }
-    if (near || C > 64u) return false;
+    if (C > 64u) return false;
     wave_sync();
     const uint2 me = lane < C ? cand[lane] : make_uint2(0u, 0xffffffffu);
     uint32_t rank = 0;
@@ -255,17 +298,31 @@ __device__ bool score_row32(const float* __restrict__ lg, const float* __restric
     wave_sync();
     const uint32_t have = C < kk ? C : kk, n = have < p.k ? have : p.k;
     const uint2 best = lane < have ? cand[64 + lane] : make_uint2(0u, 0xffffffffu);
-    if (bias) {
+    uint32_t mine = best.y;
+    if constexpr (BIAS) {
         const uint32_t next = (uint32_t)__shfl_down((int)best.x, 1);
         const float k0 = fkey_inv(best.x), k1 = fkey_inv(next);
-        const bool close = !(k0 - k1 > 2.0f * tol + 0x1p-21f * __builtin_fmaxf(__builtin_fabsf(k0), __builtin_fabsf(k1)));
-        if (__ballot(lane + 1 < have && close)) return false;
+        const bool close = !(k0 - k1 > 2.0f * tol + 0x1p-22f * __builtin_fmaxf(__builtin_fabsf(k0), __builtin_fabsf(k1)));
+        if (__ballot(lane + 1 < have && close)) {  // the candidates once more, by their keys in 64 bits
+            sum64();
+            const double k = lane < C ? key64(lg[me.y], bias[me.y]) : -__builtin_inf();
+            rank = 0;
+            for (uint32_t t = 0; t < C; t++) {
+                const double kt = __shfl(k, t);
+                const uint32_t it = (uint32_t)__builtin_amdgcn_readlane((int)me.y, (int)t);
+                rank += kt > k || (kt == k && it < me.y) ? 1u : 0u;
+            }
+            wave_sync();
+            if (lane < C && rank < kk) cand[64 + rank] = me;
+            wave_sync();
+            mine = lane < have ? cand[64 + lane].y : 0xffffffffu;
+        }
     }
     // the weights in 64 bits, a lane each: sigmoids that 32 bits lose below their sum still have their ratios
     double s = 0.0;
     if (lane < n) {
-        const double l = (double)lg[best.y];
-        s = p.score == TRK_SCORE_SOFTMAX ? ::exp(l - (double)mx) / (double)denom : 1.0 / (1.0 + ::exp(-l));
+        const double l = (double)lg[mine];
+        s = SOFT ? ::exp(l - (double)mx) / (p.renorm ? 1.0 : (double)denom) : 1.0 / (1.0 + ::exp(-l));
     }
     if (p.renorm) {
         double sum = s;
@@ -273,14 +330,14 @@ __device__ bool score_row32(const float* __restrict__ lg, const float* __restric
         s = sum > 0.0 ? s / sum : sum;
     }
     if (lane < p.k) {
-        ids[lane] = lane < n ? best.y : 0xffffffffu;
+        ids[lane] = lane < n ? mine : 0xffffffffu;
         w[lane] = lane < n ? (float)(s * (double)p.factor) : 0.0f;
     }
     if (lane == 0) *n_sel = n;
     return true;
 }
 
-template <int NJ>
+template <int NJ, bool SOFT, bool BIAS, bool GROUPED>
 __global__ __launch_bounds__(SC_WAVES * WAVE) void route_scores_kernel(const float* __restrict__ logits,
                                                                        const float* __restrict__ bias, uint32_t m,
                                                                        uint32_t E, ScorePolicy p,
@@ -292,9 +349,22 @@ __global__ __launch_bounds__(SC_WAVES * WAVE) void route_scores_kernel(const flo
     const uint32_t row = run_id() * SC_WAVES + wv;
     if (row >= m) return;
     const float* lg = logits + (size_t)row * E;
-    if (!score_row32<NJ>(lg, bias, E, p, lane, cand[wv], ids + (size_t)row * K_MAX, w + (size_t)row * K_MAX, n_sel + row))
+    if (!score_row32<NJ, SOFT, BIAS, GROUPED>(lg, bias, E, p, lane, cand[wv], ids + (size_t)row * K_MAX,
+                                              w + (size_t)row * K_MAX, n_sel + row))
         score_row(lg, bias, E, p, lane, keys + (size_t)wv * E, ids + (size_t)row * K_MAX, w + (size_t)row * K_MAX,
                   n_sel + row);
+}
+
+template <int NJ>
+void launch_scores(dim3 grid, size_t lds, hipStream_t st, const float* logits, const float* bias, uint32_t m, uint32_t E,
+                   const ScorePolicy& p, uint32_t* ids, float* w, uint32_t* n_sel) {
+#define GO(S, B, G) route_scores_kernel<NJ, S, B, G><<<grid, SC_WAVES * WAVE, lds, st>>>(logits, bias, m, E, p, ids, w, n_sel)
+    const bool b = bias, g = p.n_group > 1;
+    if (p.score == TRK_SCORE_SOFTMAX)
+        b ? (g ? GO(true, true, true) : GO(true, true, false)) : (g ? GO(true, false, true) : GO(true, false, false));
+    else
+        b ? (g ? GO(false, true, true) : GO(false, true, false)) : (g ? GO(false, false, true) : GO(false, false, false));
+#undef GO
 }
 
 }  // namespace
@@ -308,10 +378,8 @@ hipError_t launch_route_scores(const float* logits, const float* bias, uint32_t 
     while (q.group_lanes * p.n_group > WAVE) q.group_lanes /= 2;
     const uint32_t nj = (E / p.n_group + q.group_lanes - 1) / q.group_lanes;
     const dim3 grid(g.x, g.y);
-#define GO(N) route_scores_kernel<N><<<grid, SC_WAVES * WAVE, lds, st>>>(logits, bias, m, E, q, ids, w, n_sel)
-    if (nj <= 1)
-        GO(1);
-    else if (nj <= 2)
+#define GO(N) launch_scores<N>(grid, lds, st, logits, bias, m, E, q, ids, w, n_sel)
+    if (nj <= 2)
         GO(2);
     else if (nj <= 4)
         GO(4);
