@@ -140,7 +140,9 @@ def test_route_scores_crowded(score, groups, keep, bias):
 def test_route_scores_extremes():
     """Scores that underflow in 32 bits still make weights; where all vanish the weights are zeros."""
     say("route_scores extremes")
-    lg = np.array([[-100.0, -101.0, -200.0, -300.0], [-800.0, -900.0, -801.0, -1000.0], [88.0, 1000.0, -5.0, 0.0]], np.float32)
+    low = np.finfo(np.float32).min  # the lowest number is a low logit, not a mask
+    lg = np.array([[-100.0, -101.0, -200.0, -300.0], [-800.0, -900.0, -801.0, -1000.0], [88.0, 1000.0, -5.0, 0.0],
+                   [low, low, 1.0, low], [low, low, low, low], [low, -np.inf, -low, low]], np.float32)
     kw = dict(k=3, n_group=1, topk_group=1, group_top=2, renorm=True, factor=2.0)
     for score in ("sigmoid", "softmax"):
         ids, w, n = trmoe.route_scores(dev(lg), score=score, **kw)
@@ -281,6 +283,20 @@ def test_gemm_i8_poison_stays_in_its_row(m):
     q[0], s[0] = 0, np.nan
     y = host(trmoe.gemm_i8(trmoe.I8Weights(padded(w), dev(ws)), padded(q), dev(s)))
     assert np.isnan(y[0]).all() and np.isfinite(y[1:]).all()
+
+
+def test_gemm_i8_one_row_of_a_wider_tensor():
+    """One row, and one weight row, whose strides no check needs."""
+    import torch
+    say("gemm_i8 one row")
+    rng = np.random.default_rng(2)
+    q, w = i8(rng, 1, 50), i8(rng, 1, 50)
+    Q, Wt = torch.zeros((1, 1001), dtype=torch.int8, device="cuda"), torch.zeros((1, 333), dtype=torch.int8, device="cuda")
+    Q[:, 16:66], Wt[:, :50] = dev(q), dev(w)
+    s, ws = scales(rng, 1), scales(rng, 1)
+    ref = R.gemm(q, s, w, ws)
+    y = host(trmoe.gemm_i8(trmoe.I8Weights(Wt[:, :50], dev(ws)), Q[:, 16:66], dev(s)))
+    assert (np.abs(y - ref) <= R.gemm_tol(ref, "f32")).all()
 
 
 def test_gemm_i8_empty_and_refused():

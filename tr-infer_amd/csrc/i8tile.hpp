@@ -13,7 +13,7 @@
 namespace trk {
 
 // 16 bytes a lane from base + off (per lane) to the 1024 bytes of LDS at `lds`; vmcnt counts it.  In asm, because the
-// compiler would hold every later LDS read until it has arrived.
+// compiler would hold every later LDS read until it has arrived; m0 is a register that it keeps nothing in.
 __device__ __forceinline__ void lds_dma(i32x4 rsrc, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc)
                  : "memory");

@@ -593,7 +593,7 @@ def _rows(t, what, m=None, k=None):
         raise TrkError(f"{what}: the values of a row have to be contiguous")
     if shape[0] > 1:
         return s[0]
-    return max(s[0], (shape[1] + 15) // 16 * 16)  # of one row: any that the checks take
+    return (shape[1] + 15) // 16 * 16  # of one row: any that the checks take
 
 
 def _vector(t, what, dtype, *shape):
@@ -626,7 +626,7 @@ class I8Weights:
         self.q, self.scale = q, scale
         self.count = q.shape[0] if q.dim() == 3 else 1
         self.rows, self.k = q.shape[-2:]
-        ld = q.stride(-2) if self.rows > 1 else max(q.stride(-2), (self.k + 15) // 16 * 16)
+        ld = q.stride(-2) if self.rows > 1 else (self.k + 15) // 16 * 16
         if self.k % 16:
             _whole_pieces(q, 1, 0, (q.stride(0) * (self.count - 1) if self.count > 1 else 0) + ld * (self.rows - 1) + self.k,
                           "weights")
@@ -739,6 +739,21 @@ def gemm_i8(w: I8Weights, q, scale, bias=None, dtype=None, out=None, accumulate=
     return out
 
 
+@functools.lru_cache(maxsize=256)
+def _plan_words(m, slots, n_expert):
+    n = C.c_uint64()
+    check(lib().trk_experts_plan_words(m, slots, n_expert, C.byref(n)))
+    return n.value
+
+
+@functools.lru_cache(maxsize=256)
+def _down_work(m, slots, n_expert, rows):
+    """float32 values of trk_experts_down_i8's work."""
+    n = C.c_uint64()
+    check(lib().trk_experts_down_work_bytes(m, slots, n_expert, rows, C.byref(n)))
+    return n.value // 4
+
+
 def experts_plan(ids, n_sel, slots, n_expert, stream=None):
     """trk_experts_plan: the entries sorted by expert, for `experts_up_i8` and `experts_down_i8` of the same routing; None
     where the entries are so few that the products take none."""
@@ -747,10 +762,8 @@ def experts_plan(ids, n_sel, slots, n_expert, stream=None):
     _routing(ids, n_sel, m)
     if m <= EXPERTS_DIRECT_M:
         return None
-    words = C.c_uint64()
-    check(lib().trk_experts_plan_words(m, slots, n_expert, C.byref(words)))
     _here(ids, n_sel)
-    plan = torch.empty(words.value, dtype=torch.int32, device=ids.device)
+    plan = torch.empty(_plan_words(m, slots, n_expert), dtype=torch.int32, device=ids.device)
     check(lib().trk_experts_plan(ids.data_ptr(), n_sel.data_ptr(), m, slots, n_expert, plan.data_ptr(), _stream(stream)))
     return plan
 
@@ -758,11 +771,9 @@ def experts_plan(ids, n_sel, slots, n_expert, stream=None):
 def _check_plan(plan, m, slots, count):
     if m <= EXPERTS_DIRECT_M:
         return
-    words = C.c_uint64()
-    check(lib().trk_experts_plan_words(m, slots, count, C.byref(words)))
     if plan is None:
         raise TrkError(f"{m} tokens of {slots} slots need a plan (experts_plan)")
-    _vector(plan, "plan", _torch.int32, words.value)
+    _vector(plan, "plan", _torch.int32, _plan_words(m, slots, count))
 
 
 def experts_up_i8(gate: I8Weights, up: I8Weights, q, scale, ids, n_sel, slots, plan=None, dtype=None, out=None,
@@ -802,16 +813,14 @@ def experts_down_i8(down: I8Weights, q, scale, ids, w, n_sel, slots, plan=None, 
         ldy = down.rows
     else:
         ldy = _rows(out, "out", m, down.rows)
-    need = C.c_uint64()
-    if m > EXPERTS_DIRECT_M:
-        check(lib().trk_experts_down_work_bytes(m, slots, down.count, down.rows, C.byref(need)))
+    need = _down_work(m, slots, down.count, down.rows) if m > EXPERTS_DIRECT_M else 0
     if work is None:
-        if need.value:
-            work = torch.empty(need.value // 4, dtype=torch.float32, device=q.device)
+        if need:
+            work = torch.empty(need, dtype=torch.float32, device=q.device)
             if stream is not None:
                 work.record_stream(stream)  # given back on return, while that stream still works on it
-    elif work.dtype != torch.float32 or not work.is_contiguous() or work.numel() * 4 < need.value:
-        raise TrkError(f"work: {need.value // 4} contiguous float32 values are needed")
+    elif work.dtype != torch.float32 or not work.is_contiguous() or work.numel() < need:
+        raise TrkError(f"work: {need} contiguous float32 values are needed")
     _here(q, scale, ids, w, n_sel, plan, work, out, down.q)
     check(lib().trk_experts_down_i8(down.ref, q.data_ptr(), ldq, scale.data_ptr(), m, ids.data_ptr(), w.data_ptr(),
                                     n_sel.data_ptr(), slots, _ptr(plan), _ptr(work), out.data_ptr(), _dtype(out.dtype),
