@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define TRK_ABI_VERSION 3
+#define TRK_ABI_VERSION 4
 #define TRK_MOE_K_MAX 32 /* router.rs:6 MOE_K_MAX */
 
 typedef enum {

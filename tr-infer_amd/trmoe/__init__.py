@@ -661,11 +661,10 @@ def route_scores(logits, k, bias=None, score="sigmoid", n_group=1, topk_group=1,
         _vector(bias, "bias", torch.float32, E)
     if score not in SCORES:
         raise TrkError(f"score {score!r}: softmax or sigmoid")
-    dev = logits.device
     if out is None:
-        ids = torch.empty((m, K_MAX), dtype=torch.int32, device=dev)
-        w = torch.empty((m, K_MAX), dtype=torch.float32, device=dev)
-        n = torch.empty(m, dtype=torch.int32, device=dev)
+        ids = torch.empty((m, K_MAX), dtype=torch.int32, device=logits.device)
+        w = logits.new_empty((m, K_MAX))
+        n = ids.new_empty(m)
     else:
         ids, w, n = out
         _routing(ids, n, m, w)
