@@ -11,6 +11,7 @@
 namespace trk {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // C += A B: lane l holds 16 bytes of A's row l % 16 and of B's column l % 16 (the same k of both), and rows 4 (l / 16) ..
 // + 3 of C's column l % 16.
