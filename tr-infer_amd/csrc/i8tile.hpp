@@ -14,9 +14,15 @@ namespace trk {
 
 // 16 bytes a lane from base + off (per lane) to the 1024 bytes of LDS at `lds`; vmcnt counts it.  In asm, because the
 // compiler would hold every later LDS read until it has arrived; m0 is a register that it keeps nothing in.
+// ONCE: nobody reads these bytes again, and they are the first that the caches drop.
+template <bool ONCE>
 __device__ __forceinline__ void lds_dma(i32x4 rsrc, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc)
-                 : "memory");
+    if constexpr (ONCE)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds" ::"s"(lds), "v"(off), "s"(rsrc)
+                     : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc)
+                     : "memory");
 }
 template <int N>
 __device__ __forceinline__ void wait_dma() {  // all but the last N, and this wave's LDS reads
@@ -60,7 +66,8 @@ struct I8Tile {
     // rw[i], wo[i]: buffer and this lane's row offset for its i-th eight weight rows; rx, xo: the activations'.
     // lrow(i): the LDS row of the wave's i-th 16 weight rows.
     // live: this wave's 16-row groups of activations that hold any (PART: the others' products are left out).
-    template <bool PART, typename Frag>
+    // ONCE: the weight rows are this workgroup's alone.
+    template <bool PART, bool ONCE, typename Frag>
     __device__ __forceinline__ void run(uint8_t* lds, const i32x4 (&rw)[NA], const uint32_t (&wo)[NA], i32x4 rx,
                                         const uint32_t (&xo)[NB], uint32_t k, uint32_t live, Frag&& lrow) {
         const uint32_t l0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
@@ -69,9 +76,9 @@ struct I8Tile {
         // the n-th of a wave's loads of stage s
         auto load1 = [&](uint32_t o, uint32_t at, int n) {
             if (n < NA)
-                lds_dma(rw[n < NA ? n : 0], wo[n < NA ? n : 0] + o, at + n * NW * 1024);
+                lds_dma<ONCE>(rw[n < NA ? n : 0], wo[n < NA ? n : 0] + o, at + n * NW * 1024);
             else
-                lds_dma(rx, xo[n < NA ? 0 : n - NA] + o, at + n * NW * 1024);  // the activations' rows follow the weights'
+                lds_dma<false>(rx, xo[n < NA ? 0 : n - NA] + o, at + n * NW * 1024);  // the activations' rows follow the weights'
         };
         auto load_off = [&](uint32_t s) {
             const uint32_t o = s * BK + piece;

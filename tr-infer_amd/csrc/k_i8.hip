@@ -279,7 +279,7 @@ __global__ __launch_bounds__(Tile::T) void gemm_i8_tile_kernel(I8Gemm g) {
         const uint32_t r = t.load_row(i);
         xo[i] = (r < tl ? r : tl) * (uint32_t)g.ldq;
     }
-    t.template run<false>(lds, rw, wo, buffer_at(g.q + t0 * g.ldq), xo, g.k, 0, [&](int i) { return t.wn + 16 * i; });
+    t.template run<false, false>(lds, rw, wo, buffer_at(g.q + t0 * g.ldq), xo, g.k, 0, [&](int i) { return t.wn + 16 * i; });
     // every scale first (rows past the end: the last one's), so that the stores wait for memory once
     typedef Elem<DT> O;
     float sw[Tile::FN][4], bias[Tile::FN][4], sx[Tile::FM];

@@ -234,7 +234,7 @@ __global__ __launch_bounds__(Tile::T) void experts_up_tile_kernel(I8Up a, Plan P
 #pragma unroll
     for (int j = 0; j < Tile::FM; j++) sx[j] = a.sx[en[j] / a.slots];
     const uint32_t live = t.wm < pt.rows ? (pt.rows - t.wm + 15) / 16 : 0;
-    t.template run<true>(lds, rw, wo, buffer_at(a.q), xo, a.gate.k, live, [&](int i) { return i < FR ? wr + 16 * i : BR + wr + 16 * (i - FR); });
+    t.template run<true, false>(lds, rw, wo, buffer_at(a.q), xo, a.gate.k, live, [&](int i) { return i < FR ? wr + 16 * i : BR + wr + 16 * (i - FR); });
     typedef Elem<DT> O;
 #pragma unroll
     for (int j = 0; j < Tile::FM; j++) {
@@ -252,8 +252,8 @@ __global__ __launch_bounds__(Tile::T) void experts_up_tile_kernel(I8Up a, Plan P
     }
 }
 
-// down: the entries' weighted rows into work [m * slots][rows]
-template <typename Tile>
+// down: the entries' weighted rows into work [m * slots][rows].  ONCE: geo::experts_once.
+template <typename Tile, bool ONCE>
 __global__ __launch_bounds__(Tile::T) void experts_down_tile_kernel(I8Down a, Plan P) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[Tile::LDS];
     PlanTile pt;
@@ -287,7 +287,7 @@ __global__ __launch_bounds__(Tile::T) void experts_down_tile_kernel(I8Down a, Pl
     for (int j = 0; j < Tile::FM; j++)
         sx[j] = a.sx[en[j]], w[j] = a.w[(size_t)(en[j] / a.slots) * K_MAX + en[j] % a.slots];
     const uint32_t live = t.wm < pt.rows ? (pt.rows - t.wm + 15) / 16 : 0;
-    t.template run<true>(lds, rw, wo, buffer_at(a.q), xo, a.down.k, live, [&](int i) { return t.wn + 16 * i; });
+    t.template run<true, ONCE>(lds, rw, wo, buffer_at(a.q), xo, a.down.k, live, [&](int i) { return t.wn + 16 * i; });
 #pragma unroll
     for (int j = 0; j < Tile::FM; j++) {
         if (t.wm + 16 * j + t.lane % 16 >= pt.rows) continue;
@@ -446,10 +446,10 @@ static void launch_down_strip(I8Down a, hipStream_t st) {
     }
 }
 
-template <typename Tile>
+template <typename Tile, bool ONCE = true>
 static void launch_down_tile(const I8Down& a, const Plan& P, uint64_t tiles, hipStream_t st) {
     const dim3 g = run_of((a.down.rows + Tile::BN - 1) / Tile::BN * tiles, Tile::T);
-    experts_down_tile_kernel<Tile><<<g, Tile::T, 0, st>>>(a, P);
+    experts_down_tile_kernel<Tile, ONCE><<<g, Tile::T, 0, st>>>(a, P);
 }
 
 hipError_t launch_experts_down(const I8Down& a, const uint32_t* plan, hipStream_t st) {
@@ -468,9 +468,12 @@ hipError_t launch_experts_down(const I8Down& a, const uint32_t* plan, hipStream_
     else if (rows == 64)
         narrow ? launch_down_tile<I8Tile<64, 64, 32, 32, 4>>(a, P, tiles, st)
                : launch_down_tile<I8Tile<128, 64, 64, 32, 3>>(a, P, tiles, st);
-    else
+    else if (geo::experts_once(a.m, a.slots, E))
         narrow ? launch_down_tile<I8Tile<64, 128, 32, 64, 3>>(a, P, tiles, st)
                : launch_down_tile<I8Tile<128, 128, 64, 64, 2>>(a, P, tiles, st);
+    else
+        narrow ? launch_down_tile<I8Tile<64, 128, 32, 64, 3>, false>(a, P, tiles, st)
+               : launch_down_tile<I8Tile<128, 128, 64, 64, 2>, false>(a, P, tiles, st);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const uint32_t q = (a.down.rows + 3) / 4, per = q < 256 ? 256 / q : 1;
