@@ -403,6 +403,18 @@ def test_experts_down(m, E, slots, F, H, kind, dtype):
         assert (np.abs(got[:m, :H] - want) <= tol).all()
 
 
+# experts of some 60 and of 160 entries: the weights read past the caches' order or not, at each width of a 128-entry tile
+CROWDS = [(240, 16, 4, 80, 100, "ragged"), (1200, 80, 4, 48, 640, "plain"), (1200, 80, 4, 48, 1024, "elsewhere"),
+          (1600, 40, 4, 48, 1024, "plain"), (320, 8, 4, 64, 72, "plain")]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,E,slots,k,rows,kind", CROWDS)
+def test_experts_of_many_entries(m, E, slots, k, rows, kind, dtype):
+    test_experts_up(m, E, slots, k, rows, kind, dtype)
+    test_experts_down(m, E, slots, k, rows, kind, dtype)
+
+
 @pytest.mark.parametrize("far", ["weights", "rows"])
 def test_rows_far_apart(far):
     """Rows so far apart that 32-bit offsets do not reach them (4 GB of activations, 8 MB between weight rows)."""

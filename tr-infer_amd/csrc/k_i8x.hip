@@ -193,8 +193,9 @@ __device__ __forceinline__ bool expert_tile(const Plan& P, uint32_t blocks, Plan
     return true;
 }
 
-// gate and up: a tile's weight rows are BN / 2 rows of gate, then the same rows of up, and a wave has both of each
-template <typename Tile, uint32_t DT>
+// gate and up: a tile's weight rows are BN / 2 rows of gate, then the same rows of up, and a wave has both of each.  ONCE:
+// geo::experts_once.
+template <typename Tile, uint32_t DT, bool ONCE>
 __global__ __launch_bounds__(Tile::T) void experts_up_tile_kernel(I8Up a, Plan P) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[Tile::LDS];
     constexpr uint32_t BR = Tile::BN / 2, FR = Tile::FN / 2;
@@ -234,7 +235,7 @@ __global__ __launch_bounds__(Tile::T) void experts_up_tile_kernel(I8Up a, Plan P
 #pragma unroll
     for (int j = 0; j < Tile::FM; j++) sx[j] = a.sx[en[j] / a.slots];
     const uint32_t live = t.wm < pt.rows ? (pt.rows - t.wm + 15) / 16 : 0;
-    t.template run<true, false>(lds, rw, wo, buffer_at(a.q), xo, a.gate.k, live, [&](int i) { return i < FR ? wr + 16 * i : BR + wr + 16 * (i - FR); });
+    t.template run<true, ONCE>(lds, rw, wo, buffer_at(a.q), xo, a.gate.k, live, [&](int i) { return i < FR ? wr + 16 * i : BR + wr + 16 * (i - FR); });
     typedef Elem<DT> O;
 #pragma unroll
     for (int j = 0; j < Tile::FM; j++) {
@@ -370,15 +371,15 @@ hipError_t launch_experts_plan(const uint32_t* ids, const uint32_t* n_sel, uint3
     return hipGetLastError();
 }
 
-template <typename Tile>
+template <typename Tile, bool ONCE = true>
 static void launch_up_tile(const I8Up& a, const Plan& P, uint64_t tiles, hipStream_t st) {
     const dim3 g = run_of((a.gate.rows + Tile::BN / 2 - 1) / (Tile::BN / 2) * tiles, Tile::T);
     if (a.dt == TRK_DT_F32)
-        experts_up_tile_kernel<Tile, TRK_DT_F32><<<g, Tile::T, 0, st>>>(a, P);
+        experts_up_tile_kernel<Tile, TRK_DT_F32, ONCE><<<g, Tile::T, 0, st>>>(a, P);
     else if (a.dt == TRK_DT_BF16)
-        experts_up_tile_kernel<Tile, TRK_DT_BF16><<<g, Tile::T, 0, st>>>(a, P);
+        experts_up_tile_kernel<Tile, TRK_DT_BF16, ONCE><<<g, Tile::T, 0, st>>>(a, P);
     else
-        experts_up_tile_kernel<Tile, TRK_DT_F16><<<g, Tile::T, 0, st>>>(a, P);
+        experts_up_tile_kernel<Tile, TRK_DT_F16, ONCE><<<g, Tile::T, 0, st>>>(a, P);
 }
 
 // The kernels number their workgroups by 32 bits: of entries beyond, so many tokens a launch.
@@ -404,6 +405,15 @@ static void launch_up_strip(I8Up a, hipStream_t st) {
     }
 }
 
+template <bool ONCE>
+static void launch_up_128(const I8Up& a, const Plan& P, uint64_t tiles, geo::ExpertsWidth w, hipStream_t st) {
+    if (w == geo::X_NARROW)
+        launch_up_tile<I8Tile<64, 128, 32, 64, 3>, ONCE>(a, P, tiles, st);
+    else
+        w == geo::X_WIDE ? launch_up_tile<I8Tile<256, 128, 64, 64, 3>, ONCE>(a, P, tiles, st)
+                         : launch_up_tile<I8Tile<128, 128, 64, 64, 2>, ONCE>(a, P, tiles, st);
+}
+
 hipError_t launch_experts_up(const I8Up& a, const uint32_t* plan, hipStream_t st) {
     const uint32_t E = a.gate.count;
     if (!plan || !geo::i8_tile_addresses(a.gate.ld, a.ldq, a.m) || !geo::i8_tile_addresses(a.up.ld, a.ldq, a.m)) {
@@ -420,11 +430,10 @@ hipError_t launch_experts_up(const I8Up& a, const uint32_t* plan, hipStream_t st
     else if (rows == 64)
         w == geo::X_NARROW ? launch_up_tile<I8Tile<64, 64, 32, 32, 4>>(a, P, tiles, st)
                            : launch_up_tile<I8Tile<128, 64, 64, 32, 2>>(a, P, tiles, st);
-    else if (w == geo::X_NARROW)
-        launch_up_tile<I8Tile<64, 128, 32, 64, 3>>(a, P, tiles, st);
+    else if (geo::experts_once(a.m, a.slots, E, 64))
+        launch_up_128<true>(a, P, tiles, w, st);
     else
-        w == geo::X_WIDE ? launch_up_tile<I8Tile<256, 128, 64, 64, 3>>(a, P, tiles, st)
-                         : launch_up_tile<I8Tile<128, 128, 64, 64, 2>>(a, P, tiles, st);
+        launch_up_128<false>(a, P, tiles, w, st);
     return hipGetLastError();
 }
 
@@ -468,7 +477,7 @@ hipError_t launch_experts_down(const I8Down& a, const uint32_t* plan, hipStream_
     else if (rows == 64)
         narrow ? launch_down_tile<I8Tile<64, 64, 32, 32, 4>>(a, P, tiles, st)
                : launch_down_tile<I8Tile<128, 64, 64, 32, 3>>(a, P, tiles, st);
-    else if (geo::experts_once(a.m, a.slots, E))
+    else if (geo::experts_once(a.m, a.slots, E, 128))
         narrow ? launch_down_tile<I8Tile<64, 128, 32, 64, 3>>(a, P, tiles, st)
                : launch_down_tile<I8Tile<128, 128, 64, 64, 2>>(a, P, tiles, st);
     else
