@@ -196,6 +196,24 @@ def test_quantize_rows(dtype, m, k, lead, spare):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k,lead,spare", [(16385, 0, 0), (20001, 1, 3), (32768, 0, 0), (32769, 0, 7), (70003, 3, 0)])
+def test_quantize_long_rows(dtype, k, lead, spare):
+    test_quantize_rows(dtype, 5, k, lead, spare)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k", [20000, 40000])
+def test_quantize_long_rows_poison(dtype, k):
+    say(f"quantize_rows poison {dtype} k={k}")
+    x = np.ones((4, k), np.float32)
+    x[1, k - 1], x[2, k // 2], x[3, 0] = np.nan, np.inf, -np.inf
+    q, s = trmoe.quantize_rows(dev(x).to(R.torch_dtype(dtype)))
+    q, s = host(q), host(s)
+    assert (q[0] == 127).all() and np.isfinite(s[0])
+    assert (q[1:] == 0).all() and np.isnan(s[1:]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_quantize_rows_poison(dtype):
     say(f"quantize_rows poison {dtype}")
     x = np.ones((4, 100), np.float32)

@@ -16,7 +16,7 @@ __device__ __forceinline__ float quant_exact(float x, float top) { return (float
 constexpr float QUANT_BORDER = 0.5f - 0x1p-15f;  // |t - rint(t)| above it: near a border
 
 constexpr float QUANT_LEAST = 127.0f * 0x1p-126f;  // the least magnitude whose scale is a normal number
-constexpr uint32_t QUANT_T = 256;
+constexpr uint32_t QUANT_T = 256, QUANT_LONG_T = 1024;
 
 struct QuantScale {
     float top, inv, scale;
@@ -27,38 +27,7 @@ __device__ __forceinline__ QuantScale quant_scale(uint32_t top) {  // a magnitud
     return QuantScale{t, zero ? 0.0f : 127.0f / t, poison ? __builtin_nanf("") : zero ? 0.0f : t / 127.0f};
 }
 
-// Rows too long to be held: a workgroup each, every row read twice.
-template <uint32_t DT>
-__global__ __launch_bounds__(QUANT_T) void quantize_long_rows_kernel(const typename Elem<DT>::T* __restrict__ x, uint64_t ldx,
-                                                                    uint32_t m, uint32_t k, int8_t* __restrict__ q,
-                                                                    uint64_t ldq, float* __restrict__ scale) {
-    __shared__ uint32_t part[QUANT_T / WAVE];
-    const uint32_t row = run_id(), tid = threadIdx.x;
-    if (row >= m) return;  // the whole workgroup
-    const auto* xr = x + row * ldx;
-    uint32_t top = 0;
-    for (uint32_t i = tid; i < k; i += QUANT_T) {
-        const uint32_t b = __float_as_uint(Elem<DT>::get(xr[i])) & 0x7fffffffu;
-        top = b > top ? b : top;
-    }
-    top = wave_max_u32(top);
-    if (tid % WAVE == 0) part[tid / WAVE] = top;
-    __syncthreads();
-#pragma unroll
-    for (uint32_t i = 0; i < QUANT_T / WAVE; i++) top = part[i] > top ? part[i] : top;
-    const QuantScale s = quant_scale(top);
-    if (tid == 0) scale[row] = s.scale;
-    int8_t* qr = q + row * ldq;
-    for (uint32_t i = tid; i < k; i += QUANT_T) {
-        const float v = Elem<DT>::get(xr[i]), t = v * s.inv;
-        float r = __builtin_rintf(t);
-        if (__builtin_fabsf(t - r) > QUANT_BORDER) r = quant_exact(v, s.top);
-        qr[i] = s.inv == 0.0f ? 0 : (int8_t)(int)r;
-    }
-}
-
-// Rows that TPR threads hold in registers, PC pieces of 8 values a thread: read once, written once.  Pieces may lie at any
-// address (a slice of a wider tensor).  Rounding: t + 1.5 2^23 has rint(t), as an 8-bit integer, in its low byte.
+// Rows go by in pieces of 8 values, which may lie at any address (a slice of a wider tensor).
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u32x4_f32 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
@@ -119,12 +88,62 @@ struct QuantPiece {
     }
 };
 
+// The largest of the workgroup's values (of a row's WAVES waves), or of the wave's where those are one.
+template <uint32_t WAVES>
+__device__ __forceinline__ uint32_t quant_top(uint32_t top, uint32_t* part) {
+    top = wave_max_u32(top);
+    if constexpr (WAVES > 1) {
+        if (threadIdx.x % WAVE == 0) part[threadIdx.x / WAVE] = top;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < WAVES; i++) top = part[i] > top ? part[i] : top;
+    }
+    return top;
+}
+// A piece of a row scaled, rounded and written, n of its values there: t + 1.5 2^23 has rint(t), as an 8-bit integer, in its
+// low byte.
+template <uint32_t DT>
+__device__ __forceinline__ void quant_write(const QuantPiece<DT>& v, const QuantScale& s, int8_t* q, uint32_t n) {
+    uint32_t r[8];
+    float far = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float t = v.get(i) * s.inv, u = t + QUANT_MAGIC;
+        r[i] = __float_as_uint(u);
+        far = __builtin_fmaxf(far, __builtin_fabsf(t - (u - QUANT_MAGIC)));
+    }
+    if (far > QUANT_BORDER) {
+        asm volatile("");  // else the compiler takes the 64-bit quotients of every value and selects: 40960 x 512 18 -> 23 us
+#pragma unroll
+        for (int i = 0; i < 8; i++) r[i] = (uint32_t)(int)quant_exact(v.get(i), s.top);
+    }
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {  // the low bytes of four words
+        const uint32_t lo = __builtin_amdgcn_perm(r[4 * i + 1], r[4 * i], 0x0c0c0400u);
+        const uint32_t hi = __builtin_amdgcn_perm(r[4 * i + 3], r[4 * i + 2], 0x04000c0cu);
+        w[i] = s.inv == 0.0f ? 0 : lo | hi;
+    }
+    if (n >= 8) {
+        *reinterpret_cast<u32x2_any*>(q) = u32x2_any{w[0], w[1]};
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++)
+            if (i < n) q[i] = (int8_t)(w[i / 4] >> (8 * (i % 4)));
+    }
+}
+
+// Rows that TPR threads hold in registers, PC pieces a thread: read once, written once, for memory is what bounds it (8192 x
+// 4096: bf16 24 us, 4.2 TB/s, f32 31 us, 5.4 TB/s; read twice, value by value, 57 in bf16).  Beside it stand 8 instructions a
+// value.  Few rows take the time of one row's chain (4 x 2048: 2.4 us).  Rows over 16384 by 1024 threads: 1024 x 28672 in bf16 24
+// us (held) against 69 by 256 threads that read them twice, value by value.
 template <uint32_t DT, uint32_t TPR, uint32_t PC>
-__global__ __launch_bounds__(QUANT_T) void quantize_held_rows_kernel(const typename Elem<DT>::T* __restrict__ x, uint64_t ldx,
-                                                                     uint32_t m, uint32_t k, int8_t* __restrict__ q,
-                                                                     uint64_t ldq, float* __restrict__ scale) {
-    __shared__ uint32_t part[QUANT_T / WAVE];
-    const uint32_t row = run_id() * (QUANT_T / TPR) + threadIdx.x / TPR, tid = threadIdx.x % TPR;
+__global__ __launch_bounds__(TPR > QUANT_T ? TPR : QUANT_T) void quantize_held_rows_kernel(
+    const typename Elem<DT>::T* __restrict__ x, uint64_t ldx, uint32_t m, uint32_t k, int8_t* __restrict__ q, uint64_t ldq,
+    float* __restrict__ scale) {
+    constexpr uint32_t T = TPR > QUANT_T ? TPR : QUANT_T;
+    __shared__ uint32_t part[T / WAVE];
+    const uint32_t row = run_id() * (T / TPR) + threadIdx.x / TPR, tid = threadIdx.x % TPR;
     if (row >= m) return;  // a whole wave, or the whole workgroup
     const auto* xr = x + row * ldx;
     QuantPiece<DT> v[PC];
@@ -136,44 +155,49 @@ __global__ __launch_bounds__(QUANT_T) void quantize_held_rows_kernel(const typen
     uint32_t top = 0;
 #pragma unroll
     for (uint32_t p = 0; p < PC; p++) top = v[p].most(top);
-    top = wave_max_u32(QuantPiece<DT>::most32(top));
-    if constexpr (TPR > WAVE) {
-        if (tid % WAVE == 0) part[tid / WAVE] = top;
-        __syncthreads();
-#pragma unroll
-        for (uint32_t i = 0; i < QUANT_T / WAVE; i++) top = part[i] > top ? part[i] : top;
-    }
-    const QuantScale s = quant_scale(top);
+    const QuantScale s = quant_scale(quant_top<TPR / WAVE>(QuantPiece<DT>::most32(top), part));
     if (tid == 0) scale[row] = s.scale;
     int8_t* qr = q + row * ldq;
 #pragma unroll
     for (uint32_t p = 0; p < PC; p++) {
         const uint32_t at = (p * TPR + tid) * 8;
-        if (at >= k) continue;
-        uint32_t r[8];
-        float far = 0.0f;
+        if (at < k) quant_write(v[p], s, qr + at, k - at);
+    }
+}
+
+// Rows too long to be held (over 32768): a workgroup each, every row read twice, the second time from a cache: 1024 x 65536 in
+// bf16 60 us (3.4 TB/s), 300 x 131071 in f32 72.
+template <uint32_t DT, uint32_t T, uint32_t PC>
+__global__ __launch_bounds__(T) void quantize_long_rows_kernel(const typename Elem<DT>::T* __restrict__ x, uint64_t ldx,
+                                                              uint32_t m, uint32_t k, int8_t* __restrict__ q, uint64_t ldq,
+                                                              float* __restrict__ scale) {
+    __shared__ uint32_t part[T / WAVE];
+    const uint32_t row = run_id(), tid = threadIdx.x;
+    if (row >= m) return;  // the whole workgroup
+    const auto* xr = x + row * ldx;
+    QuantPiece<DT> v[PC];
+    auto load = [&](uint32_t k0) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float t = v[p].get(i) * s.inv, u = t + QUANT_MAGIC;
-            r[i] = __float_as_uint(u);
-            far = __builtin_fmaxf(far, __builtin_fabsf(t - (u - QUANT_MAGIC)));
+        for (uint32_t p = 0; p < PC; p++) {
+            const uint32_t at = k0 + (p * T + tid) * 8;
+            v[p].load(xr + (at < k ? at : 0), at < k ? k - at : 0);
         }
-        if (far > QUANT_BORDER)
+    };
+    uint32_t top = 0;
+    for (uint32_t k0 = 0; k0 < k; k0 += PC * T * 8) {
+        load(k0);
 #pragma unroll
-            for (int i = 0; i < 8; i++) r[i] = (uint32_t)(int)quant_exact(v[p].get(i), s.top);
-        uint32_t w[2];
+        for (uint32_t p = 0; p < PC; p++) top = v[p].most(top);
+    }
+    const QuantScale s = quant_scale(quant_top<T / WAVE>(QuantPiece<DT>::most32(top), part));
+    if (tid == 0) scale[row] = s.scale;
+    int8_t* qr = q + row * ldq;
+    for (uint32_t k0 = 0; k0 < k; k0 += PC * T * 8) {
+        load(k0);
 #pragma unroll
-        for (int i = 0; i < 2; i++) {  // the low bytes of four words
-            const uint32_t lo = __builtin_amdgcn_perm(r[4 * i + 1], r[4 * i], 0x0c0c0400u);
-            const uint32_t hi = __builtin_amdgcn_perm(r[4 * i + 3], r[4 * i + 2], 0x04000c0cu);
-            w[i] = s.inv == 0.0f ? 0 : lo | hi;
-        }
-        if (at + 8 <= k) {
-            *reinterpret_cast<u32x2_any*>(qr + at) = u32x2_any{w[0], w[1]};
-        } else {
-#pragma unroll
-            for (uint32_t i = 0; i < 8; i++)
-                if (at + i < k) qr[at + i] = (int8_t)(w[i / 4] >> (8 * (i % 4)));
+        for (uint32_t p = 0; p < PC; p++) {
+            const uint32_t at = k0 + (p * T + tid) * 8;
+            if (at < k) quant_write(v[p], s, qr + at, k - at);
         }
     }
 }
@@ -183,9 +207,10 @@ void launch_quantize(const void* x, uint64_t ldx, uint32_t m, uint32_t k, int8_t
                      hipStream_t st) {
     typedef typename Elem<DT>::T T;
     const uint32_t per = k <= 2048 ? QUANT_T / WAVE : 1;  // rows of a workgroup: a wave each while they fit its registers
-    const geo::Grid2 g = geo::grid_run(((uint64_t)m + per - 1) / per, QUANT_T);
+    const uint32_t t = k <= 16384 ? QUANT_T : QUANT_LONG_T;
+    const geo::Grid2 g = geo::grid_run(((uint64_t)m + per - 1) / per, t);
     const dim3 grid(g.x, g.y);
-#define GO(TPR, PC) quantize_held_rows_kernel<DT, TPR, PC><<<grid, QUANT_T, 0, st>>>((const T*)x, ldx, m, k, q, ldq, scale)
+#define GO(TPR, PC) quantize_held_rows_kernel<DT, TPR, PC><<<grid, t, 0, st>>>((const T*)x, ldx, m, k, q, ldq, scale)
     if (k <= 512)
         GO(WAVE, 1);
     else if (k <= 1024)
@@ -198,8 +223,10 @@ void launch_quantize(const void* x, uint64_t ldx, uint32_t m, uint32_t k, int8_t
         GO(QUANT_T, 4);
     else if (k <= 16384)
         GO(QUANT_T, 8);
+    else if (k <= 32768)
+        GO(QUANT_LONG_T, 4);
     else
-        quantize_long_rows_kernel<DT><<<grid, QUANT_T, 0, st>>>((const T*)x, ldx, m, k, q, ldq, scale);
+        quantize_long_rows_kernel<DT, QUANT_LONG_T, 4><<<grid, t, 0, st>>>((const T*)x, ldx, m, k, q, ldq, scale);
 #undef GO
 }
 
