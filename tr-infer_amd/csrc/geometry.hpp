@@ -231,10 +231,11 @@ inline uint32_t plan_rows(uint32_t m, uint32_t slots, uint32_t E) {
     return avg <= 24 ? 32 : avg <= 48 ? 64 : 128;
 }
 // An expert's entries seldom need a second tile: its weights are then loaded past the caches' replacement order, so that
-// what does come again stays there (down's work rows, the entries' own).  Tiles below 128 rows: always; of 128: up to 64 entries
-// an expert on average for up, 128 for down.  us, without / with: up, 10 entries (10 of 512 x 512) 199 / 178, 4 (8 of 128 x 64)
-// 71 / 61, 62 (x 1000) 88 / 83, 80 (10 of 512 x 4096) 232 / 234, 125 (8 of 128 x 2000) 115 / 123, 250 (2 of 8 x 1000) 25 / 31; down,
-// 39 (10 of 512 x 2000) 189 / 178, 80 294 / 282, 125 135 / 132, 160 (10 of 512 x 8192) 543 / 548, 256 (4 of 64 x 4096) 262 / 282.
+// what does come again stays there (down's work rows, the entries' own).  Tiles below 128 rows: always; of 128: up to 64
+// entries an expert on average for up, 128 for down.  us, without / with: up, 10 entries (10 of 512 x 512) 199 / 178, 4 (8
+// of 128 x 64) 71 / 61, 62 (x 1000) 88 / 83, 80 (10 of 512 x 4096) 232 / 234, 125 (8 of 128 x 2000) 115 / 123, 250 (2 of 8
+// x 1000) 25 / 31; down, 39 (10 of 512 x 2000) 189 / 178, 80 294 / 282, 125 135 / 132, 160 (10 of 512 x 8192) 543 / 548, 256
+// (4 of 64 x 4096) 262 / 282.
 inline bool experts_once(uint32_t m, uint32_t slots, uint32_t E, uint32_t most) { return (uint64_t)m * slots / E <= most; }
 // The tiles address weight rows from their block's first, activation rows from the first of all, by 32 bits.
 inline bool i8_tile_addresses(uint64_t ldw, uint64_t ldq, uint64_t rows) {

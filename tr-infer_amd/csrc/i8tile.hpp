@@ -95,7 +95,8 @@ struct I8Tile {
         auto read_b = [&](uint32_t at, int kk, int h, int to) {
 #pragma unroll
             for (int j = 0; j < FH; j++)
-                if (!PART || h * FH + j < (int)live) b[to][j] = *reinterpret_cast<const i32x4*>(lds + at + (BN + wm + (h * FH + j) * 16) * BK + (la ^ (64 * kk)));
+                if (!PART || h * FH + j < (int)live)
+                    b[to][j] = *reinterpret_cast<const i32x4*>(lds + at + (BN + wm + (h * FH + j) * 16) * BK + (la ^ (64 * kk)));
         };
         // a phase's products, with the loads of a stage between them: all at once they would hold up every wave for as
         // long as the memory pipe takes to accept them

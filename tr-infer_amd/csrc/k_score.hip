@@ -138,9 +138,9 @@ constexpr uint32_t SC_CAND = 64 + 34;  // LDS entries a wave: candidates, then t
 // One row; false where 64 bits have to decide.  NJ: logits a lane holds.  Lanes are split evenly over the groups.  What the
 // policy asks for is in the template: with branches on it between a row's loads they wait for one another.
 template <int NJ, bool SOFT, bool BIAS, bool GROUPED>
-__device__ __forceinline__ bool score_row32(const float* __restrict__ lg, const float* __restrict__ bias, uint32_t E, const ScorePolicy& p,
-                            uint32_t lane, uint2* cand, uint32_t* __restrict__ ids, float* __restrict__ w,
-                            uint32_t* __restrict__ n_sel) {
+__device__ __forceinline__ bool score_row32(const float* __restrict__ lg, const float* __restrict__ bias, uint32_t E,
+                                            const ScorePolicy& p, uint32_t lane, uint2* cand, uint32_t* __restrict__ ids,
+                                            float* __restrict__ w, uint32_t* __restrict__ n_sel) {
     const float NONE = -__builtin_inff();
     const uint32_t gs = E / p.n_group, L = p.group_lanes, g = lane / L, r0 = lane % L;
     float v[NJ], key[NJ];
@@ -337,6 +337,8 @@ __device__ __forceinline__ bool score_row32(const float* __restrict__ lg, const 
     return true;
 }
 
+// 1 token x 256 (8 groups) 4.0 us and 2048 x 512 (softmax) 4.7: the chain of a row; 16384 x 256 (8 groups) 17.4 us, 1 TB/s:
+// some 540 vector instructions a row.  The weights' 64 bits are 1.5 us of those; every key in 64 bits took 62.
 template <int NJ, bool SOFT, bool BIAS, bool GROUPED>
 __global__ __launch_bounds__(SC_WAVES * WAVE) void route_scores_kernel(const float* __restrict__ logits,
                                                                        const float* __restrict__ bias, uint32_t m,
