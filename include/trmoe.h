@@ -276,7 +276,8 @@ typedef struct {
  * compared as if in 64 bits.  An expert whose logit (or key) is NaN or -inf is never chosen, and
  * adds nothing to the softmax's sum: a row chooses fewer than k, or none, where the others run out.
  * ids / w: [m][32], n_sel: [m]; slots n_sel .. k - 1 get id 0xffffffff and weight 0, later ones stay
- * as they were.  A softmax row with a logit of +inf has NaN scores: NaN weights, and with a bias no choice.  n_expert at most 1024. */
+ * as they were.  A softmax row with a logit of +inf has NaN scores: NaN weights, and with a bias no choice.
+ * n_expert at most 1024. */
 int trk_route_scores(const float *logits, const float *bias, uint32_t m, uint32_t n_expert,
                      const trk_score_policy *policy, uint32_t *ids, float *w, uint32_t *n_sel, void *stream);
 

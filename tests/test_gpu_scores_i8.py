@@ -469,6 +469,28 @@ def test_rows_far_apart(far):
         assert (np.abs(y - ref) <= 5.05 * R.EPS["f32"] * np.abs(ref) + 1.01 * R.round_rel(ref, "f32")).all()
 
 
+def test_experts_of_a_wider_plan():
+    """A plan of as many words that names experts which the stack does not hold: they are passed over."""
+    import torch
+    say("experts with a wider plan")
+    rng = np.random.default_rng(5)
+    m, slots, E, count, H, F = 10, 3, 64, 40, 96, 80
+    ids, w, n = routing(rng, m, E, slots, "plain")
+    assert (R.entries(ids, n, slots, E) & (ids[:, :slots] >= count)).any()
+    di, dw, dn = dev(ids), dev(w), dev(n)
+    wide, own = (trmoe.experts_plan(di, dn, slots, e) for e in (E, count))
+    assert wide.shape == own.shape
+    gate, up = (trmoe.I8Weights(padded(i8(rng, count, F, H)), dev(scales(rng, count, F, around=0.01))) for _ in range(2))
+    down = trmoe.I8Weights(padded(i8(rng, count, H, F)), dev(scales(rng, count, H, around=0.01)))
+    q, s, hq, hs = (dev(a) for a in (i8(rng, m, H), scales(rng, m), i8(rng, m * slots, F), scales(rng, m * slots)))
+    got = []
+    for plan in (own, wide):
+        h = torch.full((m * slots, F), 9.0, device="cuda")
+        trmoe.experts_up_i8(gate, up, q, s, di, dn, slots, plan=plan, out=h)
+        got.append((h, trmoe.experts_down_i8(down, hq, hs, di, dw, dn, slots, plan=plan)))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
 def test_experts_refuse():
     import torch
     say("experts refusals")

@@ -187,12 +187,12 @@ __global__ __launch_bounds__(DOWN_WAVES* WAVE) void experts_down_strip_kernel(I8
 
 // A tile's place: entries of one expert (the plan's tile) x a block of weight rows, the blocks of a tile next to one
 // another and each expert's tiles in turn on one XCD, whose L2 then holds the entries' rows and the expert's weights.
-template <typename Tile>
-__device__ __forceinline__ bool expert_tile(const Plan& P, uint32_t blocks, PlanTile& t, uint32_t& block) {
+// E: the stack's experts.  No plan made for it names others; of a plan made for more they are passed over, like ids.
+__device__ __forceinline__ bool expert_tile(const Plan& P, uint32_t E, uint32_t blocks, PlanTile& t, uint32_t& block) {
     uint32_t idx;
     if (!xcd_order_1d(*P.n_tiles * blocks, idx, run_id())) return false;
     t = P.tile[idx / blocks], block = idx % blocks;
-    return true;
+    return t.expert < E;
 }
 
 // gate and up: a tile's weight rows are BN / 2 rows of gate, then the same rows of up, and a wave has both of each.  ONCE:
@@ -205,8 +205,8 @@ __global__ __launch_bounds__(Tile::T) void experts_up_tile_kernel(I8Up a, Plan P
     static_assert(BR % (8 * Tile::NW) == 0 && Tile::WN % 32 == 0, "a load takes rows of one matrix");
     PlanTile pt;
     uint32_t block;
-    if (!expert_tile<Tile>(P, (a.gate.rows + BR - 1) / BR, pt, block)) return;  // the whole workgroup
-    const uint32_t r0 = block * BR, rl = a.gate.rows - r0 - 1;                  // the last row there is
+    if (!expert_tile(P, a.gate.count, (a.gate.rows + BR - 1) / BR, pt, block)) return;  // the whole workgroup
+    const uint32_t r0 = block * BR, rl = a.gate.rows - r0 - 1;                          // the last row there is
     Tile t;
     auto entry = [&](uint32_t i) { return P.ent[pt.row0 + (i < pt.rows ? i : pt.rows - 1)]; };
     const i32x4 bg = buffer_at(a.gate.ptr + pt.expert * a.gate.stride + r0 * a.gate.ld);
@@ -264,7 +264,7 @@ __global__ __launch_bounds__(Tile::T) void experts_down_tile_kernel(I8Down a, Pl
     __shared__ __attribute__((aligned(1024))) uint8_t lds[Tile::LDS];
     PlanTile pt;
     uint32_t block;
-    if (!expert_tile<Tile>(P, (a.down.rows + Tile::BN - 1) / Tile::BN, pt, block)) return;  // the whole workgroup
+    if (!expert_tile(P, a.down.count, (a.down.rows + Tile::BN - 1) / Tile::BN, pt, block)) return;  // the whole workgroup
     const uint32_t r0 = block * Tile::BN, rl = a.down.rows - r0 - 1;
     Tile t;
     auto entry = [&](uint32_t i) { return P.ent[pt.row0 + (i < pt.rows ? i : pt.rows - 1)]; };

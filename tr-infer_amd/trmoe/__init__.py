@@ -543,7 +543,8 @@ def gemv(wt, rows, k, fmt, item, count, kb, q, s, su, pair=False, y=None, ldy=No
 # ---- routing by scores, 8-bit products with a scale per token and per channel --------------------
 #
 # The kernels run on torch's current stream (or `stream`) of the current device; tensors elsewhere are
-# refused.  Outputs are allocated where none is given.
+# refused.  Outputs are allocated where none is given, on the current stream as torch does: a `stream` that is not
+# the current one has to wait for it before the call, as for whatever wrote the tensors given.
 
 _torch = None  # the module, its dtypes and its device lookup once a call has needed them
 _dt = None
