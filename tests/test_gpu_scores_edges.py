@@ -1,0 +1,44 @@
+"""Routing by scores at the ends of its types, on the GPU against the plain 64-bit form (tests/i8ref.py)."""
+from __future__ import annotations
+
+import i8ref as R
+import numpy as np
+import pytest
+
+import trmoe
+from test_gpu_scores_i8 import dev, host, say
+
+pytestmark = pytest.mark.gpu
+LOW = np.finfo(np.float32).min
+
+
+def check_route(lg, bias, score, rtol=2.0 ** -22, **kw):
+    """ids and n_sel equal, weights within rtol."""
+    kw = {**dict(n_group=1, topk_group=1, group_top=2, renorm=True, factor=1.0), **kw}
+    ids, w, n = trmoe.route_scores(dev(lg), bias=None if bias is None else dev(bias), score=score, **kw)
+    rid, rw, rn = R.route(lg, bias=bias, score=score, **kw)
+    assert np.array_equal(host(n), rn), (host(n), rn)
+    assert np.array_equal(host(ids)[:, :kw["k"]], rid)
+    np.testing.assert_allclose(host(w)[:, :kw["k"]], rw, rtol=rtol, atol=2.0 ** -149)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("E,groups,keep,k", [(16, 4, 2, 8), (256, 8, 4, 32), (256, 8, 8, 8), (1020, 17, 3, 32), (12, 6, 5, 9)])
+@pytest.mark.parametrize("low", [LOW, -2e38, "spread"])
+def test_groups_whose_sums_leave_the_type(score, E, groups, keep, k, low):
+    """Two keys of a group near the lowest number: their sum is below it, and the group is there all the same."""
+    say(f"route_scores group sums out of range {score} E={E} {groups}/{keep} {low}")
+    rng = np.random.default_rng(E + k)
+    lg = rng.standard_normal((12, E)).astype(np.float32)
+    gs = E // groups
+    bias = np.full(E, LOW, np.float32)
+    bias[:] = rng.choice(np.array([LOW, -3e38, -2.5e38, -1.8e38], np.float32), E) if low == "spread" else low
+    bias[:gs] = 0.0                       # one group as usual
+    lg[1, :gs] = -np.inf                  # and none
+    lg[2, gs:2 * gs] = -np.inf            # a group with nothing to choose
+    lg[3, 2 * gs + 1:3 * gs] = -np.inf    # with one
+    lg[4, gs:] = -np.inf
+    for top in (1, 2):
+        check_route(lg, bias, score, k=k, n_group=groups, topk_group=keep, group_top=top)
+    high = -bias
+    check_route(lg, high, score, k=k, n_group=groups, topk_group=keep)

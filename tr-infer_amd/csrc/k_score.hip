@@ -222,12 +222,14 @@ __device__ __forceinline__ bool score_row32(const float* __restrict__ lg, const 
         bool kept = rank < p.topk_group && worth > NONE;
         // the worst group kept and the best one dropped; a sum of two keys is off by twice a key and a rounding
         const uint32_t lo = ~wave_max_u32(kept ? ~fkey(worth) : 0u), hi = wave_max_u32(kept ? 0u : fkey(worth));
-        if (scored && hi && lo != 0xffffffffu) {
+        // a sum of two keys below the lowest number is -inf in 32 bits: its group is there, and its place open
+        const bool lost = sums && __ballot(g < p.n_group && a1 > NONE && !(worth > NONE));
+        if (scored && (lost || (hi && lo != 0xffffffffu))) {
             const float fl = fkey_inv(lo), fh = fkey_inv(hi);
             // of a sum: its keys' errors, their roundings and its own
             const float both = __builtin_fabsf(a1) + (a2 > NONE ? __builtin_fabsf(a2) : 0.0f);
             const float big = __uint_as_float(wave_max_u32(g < p.n_group && a1 > NONE ? __float_as_uint(both) : 0u));
-            if (!(fl - fh > 4.0f * tol + 0x1p-22f * big)) {
+            if (lost || !(fl - fh > 4.0f * tol + 0x1p-22f * big)) {
                 sum64();
                 double d1 = (double)NONE, d2 = (double)NONE;
 #pragma unroll
