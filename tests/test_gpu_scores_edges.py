@@ -42,3 +42,19 @@ def test_groups_whose_sums_leave_the_type(score, E, groups, keep, k, low):
         check_route(lg, bias, score, k=k, n_group=groups, topk_group=keep, group_top=top)
     high = -bias
     check_route(lg, high, score, k=k, n_group=groups, topk_group=keep)
+
+
+@pytest.mark.parametrize("E,k,groups,keep,bias", [(5, 5, 1, 1, False), (256, 8, 1, 1, False), (512, 10, 1, 1, True),
+                                                  (1024, 32, 32, 5, True), (160, 6, 8, 3, False)])
+def test_softmax_weights_left_as_they_are(E, k, groups, keep, bias):
+    """Not renormalised, a weight is exp(l - max) / sum in 64 bits, rounded once."""
+    say(f"route_scores softmax weights E={E} k={k} {groups}/{keep} bias={bias}")
+    rng = np.random.default_rng(E + k)
+    lg = (rng.standard_normal((400, E)) * rng.uniform(0.1, 6.0, (400, 1))).astype(np.float32)
+    lg[rng.random(lg.shape) < 0.05] = -np.inf
+    lg[7] = lg[7, 0] if np.isfinite(lg[7, 0]) else 0.25  # all alike
+    b = (rng.standard_normal(E) * 0.1).astype(np.float32) if bias else None
+    if bias:
+        b[::9] = -np.inf  # not to be chosen, but part of the sum
+    # half a step, and what 64-bit exponentials and their sum may differ by
+    check_route(lg, b, "softmax", rtol=1.001 * R.EPS["f32"], k=k, n_group=groups, topk_group=keep, renorm=False)
