@@ -639,7 +639,11 @@ class I8Weights:
 
 def quantize_weights(w, stream=None):
     """float [count][rows][k] or [rows][k] -> I8Weights: each row quantised as `quantize_rows` does."""
-    flat = w.reshape(-1, w.shape[-1])
+    if stream is None:
+        flat = w.reshape(-1, w.shape[-1])
+    else:
+        with (_torch or _late()).cuda.stream(stream):  # a copy, where the rows make no one matrix: made and given back there
+            flat = w.reshape(-1, w.shape[-1])
     q, s = quantize_rows(flat, stream=stream)
     q = q.as_strided((*w.shape[:-1], w.shape[-1]), (*[q.stride(0) * w.shape[-2]] * (w.dim() - 2), q.stride(0), 1))
     return I8Weights(q, s.view(w.shape[:-1]))
