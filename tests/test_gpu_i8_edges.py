@@ -2,6 +2,8 @@
 (tests/i8ref.py)."""
 from __future__ import annotations
 
+import i8ref as R
+import numpy as np
 import pytest
 
 import trmoe
@@ -29,3 +31,30 @@ def test_weights_of_a_wider_stack_on_a_stream():
         torch.cuda.synchronize()
         assert torch.equal(got.q, want.q) and torch.equal(got.scale, want.scale)
         del got, junk
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("k", [(1 << 32) - 5, (1 << 32) - (1 << 15)])
+def test_quantize_the_longest_rows(dtype, k):
+    """A row of nearly 2^32 values: places in it that 32 bits do not add up."""
+    import torch
+    say(f"quantize_rows {dtype} k={k}")
+    part = 1 << 28
+    # repeated at a length that divides no piece; the largest value far from both ends
+    base = torch.arange(part, device="cuda").remainder_(509).sub_(254).to(R.torch_dtype(dtype))
+    x = torch.empty((1, k), dtype=base.dtype, device="cuda")
+    for at in range(0, k, part):
+        x[0, at:at + part] = base[:k - at]
+    x[0, 3 * part + 17] = 508
+    q = torch.full((1, k + 16), 99, dtype=torch.int8, device="cuda")
+    s = torch.empty(1, device="cuda")
+    trmoe.quantize_rows(x, out=(q[:, :k], s))
+    assert s.item() == np.float32(508 / 127)
+    want = (base.double() / 4).round().to(torch.int8)  # 127 x / 508: whole quarters, ties to even
+    for at in range(0, k, part):
+        got = q[0, at:min(at + part, k)]
+        if at == 3 * part:
+            assert got[17] == 127
+            got[17] = want[17]
+        assert torch.equal(got, want[:got.numel()]), at
+    assert (q[0, k:] == 99).all()

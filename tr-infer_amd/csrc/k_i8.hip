@@ -175,30 +175,36 @@ __global__ __launch_bounds__(T) void quantize_long_rows_kernel(const typename El
     const uint32_t row = run_id(), tid = threadIdx.x;
     if (row >= m) return;  // the whole workgroup
     const auto* xr = x + row * ldx;
+    constexpr uint32_t STEP = PC * T * 8;
     QuantPiece<DT> v[PC];
-    auto load = [&](uint32_t k0) {
+    // the row from p on, `left` values of it: counted down, for sums of places near 2^32 do not fit 32 bits
+    auto load = [&](const typename Elem<DT>::T* p, uint32_t left) {
 #pragma unroll
-        for (uint32_t p = 0; p < PC; p++) {
-            const uint32_t at = k0 + (p * T + tid) * 8;
-            v[p].load(xr + (at < k ? at : 0), at < k ? k - at : 0);
+        for (uint32_t i = 0; i < PC; i++) {
+            const uint32_t at = (i * T + tid) * 8;
+            v[i].load(p + (at < left ? at : 0), at < left ? left - at : 0);
         }
     };
     uint32_t top = 0;
-    for (uint32_t k0 = 0; k0 < k; k0 += PC * T * 8) {
-        load(k0);
+    const auto* xp = xr;
+    for (uint32_t left = k;; left -= STEP, xp += STEP) {
+        load(xp, left);
 #pragma unroll
-        for (uint32_t p = 0; p < PC; p++) top = v[p].most(top);
+        for (uint32_t i = 0; i < PC; i++) top = v[i].most(top);
+        if (left <= STEP) break;
     }
     const QuantScale s = quant_scale(quant_top<T / WAVE>(QuantPiece<DT>::most32(top), part));
     if (tid == 0) scale[row] = s.scale;
-    int8_t* qr = q + row * ldq;
-    for (uint32_t k0 = 0; k0 < k; k0 += PC * T * 8) {
-        load(k0);
+    int8_t* qp = q + row * ldq;
+    xp = xr;
+    for (uint32_t left = k;; left -= STEP, xp += STEP, qp += STEP) {
+        load(xp, left);
 #pragma unroll
-        for (uint32_t p = 0; p < PC; p++) {
-            const uint32_t at = k0 + (p * T + tid) * 8;
-            if (at < k) quant_write(v[p], s, qr + at, k - at);
+        for (uint32_t i = 0; i < PC; i++) {
+            const uint32_t at = (i * T + tid) * 8;
+            if (at < left) quant_write(v[i], s, qp + at, left - at);
         }
+        if (left <= STEP) break;
     }
 }
 
