@@ -43,3 +43,50 @@ def test_weights_are_laid_out_on_the_stream_given(monkeypatch):
             trmoe.quantize_weights(Sliced(), stream=given)
         assert e.value.args == ([st] if given else [], given)
     assert not on
+
+
+def test_sizes_past_32_bits_are_refused():
+    """The C entry points take 32-bit sizes: a longer tensor would be cut to its size modulo 2^32."""
+    import torch
+
+    def meta(*shape, dtype=torch.int8):
+        return torch.empty(shape, dtype=dtype, device="meta")
+
+    far = (1 << 32) + 64
+    with pytest.raises(trmoe.TrkError, match="32 bits"):
+        trmoe.quantize_rows(meta(1, far, dtype=torch.bfloat16))
+    with pytest.raises(trmoe.TrkError, match="32 bits"):
+        trmoe.quantize_rows(meta(far, 16, dtype=torch.bfloat16))
+    for shape in ((1, far), (far, 16), (far, 2, 16)):
+        with pytest.raises(trmoe.TrkError, match="32 bits"):
+            trmoe.I8Weights(meta(*shape), meta(*shape[:-1], dtype=torch.float32))
+    with pytest.raises(trmoe.TrkError, match="32 bits"):
+        trmoe.route_scores(meta(far, 8, dtype=torch.float32), 2)
+
+    class W:  # a matrix [5][64]: only its sizes are looked at before the rows'
+        rows, k, count = 5, 64, 1
+    with pytest.raises(trmoe.TrkError, match="32 bits"):
+        trmoe.gemm_i8(W, meta(far, 64), meta(far, dtype=torch.float32))
+
+
+def test_numbers_past_32_bits_are_refused():
+    import torch
+    far = (1 << 32) + 2
+    lg = torch.zeros((2, 8))
+    for kw in (dict(k=far), dict(k=2, n_group=far), dict(k=2, topk_group=far - 1), dict(k=2, group_top=far), dict(k=-1)):
+        with pytest.raises(trmoe.TrkError, match="32 bits"):
+            trmoe.route_scores(lg, **kw)
+    ids, n = torch.zeros((9, 32), dtype=torch.int32), torch.zeros(9, dtype=torch.int32)
+    with pytest.raises(trmoe.TrkError, match="32 bits"):
+        trmoe.experts_plan(ids, n, far, 8)
+    with pytest.raises(trmoe.TrkError, match="32 bits"):
+        trmoe.experts_plan(ids, n, 2, far)
+    class W:
+        rows, k, count = 5, 64, 1
+    q, s = torch.zeros((2, 64), dtype=torch.int8), torch.ones(2)
+    for slots in (far, -1):
+        with pytest.raises(trmoe.TrkError, match="32 bits"):
+            trmoe.experts_up_i8(W, W, q, s, ids[:2], n[:2], slots)
+    for item in (1, far - 2, -1):
+        with pytest.raises(trmoe.TrkError, match="item"):
+            trmoe.gemm_i8(W, q, s, item=item)

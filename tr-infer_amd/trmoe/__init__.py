@@ -570,6 +570,13 @@ def _dtype(t):
     return d
 
 
+def _u32(*values):
+    """Sizes and counts as the C entry points take them; ctypes would cut what does not fit."""
+    for v in values:
+        if not 0 <= v < 1 << 32:
+            raise TrkError(f"{v} does not fit 32 bits")
+
+
 def _here(*tensors):
     """Every tensor given is on the current device."""
     dev = -1
@@ -589,6 +596,8 @@ def _rows(t, what, m=None, k=None):
     shape = t.shape
     if len(shape) != 2 or (m is not None and shape[0] != m) or (k is not None and shape[1] != k):
         raise TrkError(f"{what}: shape {tuple(shape)}, [{'m' if m is None else m}][{'k' if k is None else k}] is needed")
+    if (shape[0] | shape[1]) >> 32:
+        _u32(*shape)
     s = t.stride()
     if s[1] != 1 and shape[1] > 1:
         raise TrkError(f"{what}: the values of a row have to be contiguous")
@@ -621,6 +630,7 @@ class I8Weights:
         _vector(scale, "weight scales", torch.float32, *q.shape[:-1])
         if min(q.shape) == 0:
             raise TrkError(f"weights: empty shape {tuple(q.shape)}")
+        _u32(*q.shape)
         if q.shape[-1] > 1 and q.stride(-1) != 1:
             raise TrkError("weights: the values of a row have to be contiguous")
         _here(q, scale)
@@ -652,6 +662,7 @@ def quantize_weights(w, stream=None):
 @functools.lru_cache(maxsize=64)
 def _score_policy(*fields):
     """A trk_score_policy by reference: a program has few, and making one takes as long as a launch."""
+    _u32(*fields[:5])
     return C.byref(ScorePolicy(*fields))
 
 
@@ -662,10 +673,13 @@ def route_scores(logits, k, bias=None, score="sigmoid", n_group=1, topk_group=1,
     if logits.dim() != 2 or logits.dtype != torch.float32 or not logits.is_contiguous():
         raise TrkError(f"logits: contiguous float32 [m][E] is needed, not {logits.dtype} {tuple(logits.shape)}")
     m, E = logits.shape
+    if (m | E) >> 32:
+        _u32(m, E)
     if bias is not None:
         _vector(bias, "bias", torch.float32, E)
     if score not in SCORES:
         raise TrkError(f"score {score!r}: softmax or sigmoid")
+    p = _score_policy(k, SCORES[score], n_group, topk_group, group_top, int(renorm), factor)
     if out is None:
         ids = torch.empty((m, K_MAX), dtype=torch.int32, device=logits.device)
         w = logits.new_empty((m, K_MAX))
@@ -674,7 +688,6 @@ def route_scores(logits, k, bias=None, score="sigmoid", n_group=1, topk_group=1,
         ids, w, n = out
         _routing(ids, n, m, w)
     _here(logits, bias, ids, w, n)
-    p = _score_policy(k, SCORES[score], n_group, topk_group, group_top, int(renorm), factor)
     check(lib().trk_route_scores(logits.data_ptr(), _ptr(bias), m, E, p, ids.data_ptr(), w.data_ptr(),
                                  n.data_ptr(), _stream(stream)))
     return ids, w, n
@@ -727,6 +740,8 @@ def gemm_i8(w: I8Weights, q, scale, bias=None, dtype=None, out=None, accumulate=
     `out` says otherwise)."""
     torch = _torch or _late()
     m = q.shape[0]
+    if not 0 <= item < w.count:
+        raise TrkError(f"item {item} out of range")
     ldq = _i8_rows(q, scale, m, w.k)
     if bias is not None:
         _vector(bias, "bias", torch.float32, w.rows)
@@ -746,6 +761,7 @@ def gemm_i8(w: I8Weights, q, scale, bias=None, dtype=None, out=None, accumulate=
 @functools.lru_cache(maxsize=256)
 def _plan_words(m, slots, n_expert):
     n = C.c_uint64()
+    _u32(m, slots, n_expert)
     check(lib().trk_experts_plan_words(m, slots, n_expert, C.byref(n)))
     return n.value
 
@@ -754,6 +770,7 @@ def _plan_words(m, slots, n_expert):
 def _down_work(m, slots, n_expert, rows):
     """float32 values of trk_experts_down_i8's work."""
     n = C.c_uint64()
+    _u32(m, slots, n_expert, rows)
     check(lib().trk_experts_down_work_bytes(m, slots, n_expert, rows, C.byref(n)))
     return n.value // 4
 
@@ -766,14 +783,17 @@ def experts_plan(ids, n_sel, slots, n_expert, stream=None):
     _routing(ids, n_sel, m)
     if m <= EXPERTS_DIRECT_M:
         return None
+    words = _plan_words(m, slots, n_expert)
     _here(ids, n_sel)
-    plan = torch.empty(_plan_words(m, slots, n_expert), dtype=torch.int32, device=ids.device)
+    plan = torch.empty(words, dtype=torch.int32, device=ids.device)
     check(lib().trk_experts_plan(ids.data_ptr(), n_sel.data_ptr(), m, slots, n_expert, plan.data_ptr(), _stream(stream)))
     return plan
 
 
 def _check_plan(plan, m, slots, count):
     if m <= EXPERTS_DIRECT_M:
+        if slots >> 32:
+            _u32(slots)
         return
     if plan is None:
         raise TrkError(f"{m} tokens of {slots} slots need a plan (experts_plan)")
