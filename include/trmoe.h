@@ -285,7 +285,7 @@ int trk_route_scores(const float *logits, const float *bias, uint32_t m, uint32_
  * ptr + i * stride + r * ld, and stands for scale[i * rows + r] times them.  ptr, ld and (count > 1)
  * stride are multiples of 16; rows are read in 16-byte pieces, so the bytes behind a row's k-th up
  * to the next multiple of 16 have to be there (any value).  k at most 131071: every product
- * of two rows then fits its 32-bit sum. */
+ * of two rows then fits its 32-bit sum.  rows, and the tokens of trk_gemm_i8, at most 2^32 - 256. */
 typedef struct {
     const int8_t *ptr;
     const float *scale;

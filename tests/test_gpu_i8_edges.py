@@ -58,3 +58,32 @@ def test_quantize_the_longest_rows(dtype, k):
             got[17] = want[17]
         assert torch.equal(got, want[:got.numel()]), at
     assert (q[0, k:] == 99).all()
+
+
+@pytest.mark.parametrize("far", ["weight rows", "tokens"])
+def test_gemm_i8_of_the_most_rows(far):
+    """2^32 - 256 - 3 rows on one side (64 GB at k = 16), one on the other: the last tile's numbers still fit 32 bits."""
+    import torch
+    say(f"gemm_i8 most {far}")
+    n, k, part = (1 << 32) - 259, 16, 1 << 24
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    base = torch.randint(-127, 128, (part, k), dtype=torch.int8, device="cuda", generator=gen)
+    one = torch.randint(-127, 128, (1, k), dtype=torch.int8, device="cuda", generator=gen)
+    many = torch.empty((n, k), dtype=torch.int8, device="cuda")
+    scale = torch.ones(n, device="cuda")
+    for at in range(0, n, part):
+        many[at:at + part] = base[:n - at]
+        scale[at] = 2.0  # a mark at each part's head
+    unit = torch.ones(1, device="cuda")
+    if far == "tokens":
+        y = torch.empty((n, 1), dtype=torch.float16, device="cuda")
+        trmoe.gemm_i8(trmoe.I8Weights(one, unit), many, scale, out=y)
+    else:
+        y = torch.empty((1, n), dtype=torch.float16, device="cuda")
+        trmoe.gemm_i8(trmoe.I8Weights(many, scale), one, unit, out=y)
+    want = (base.double() @ one.double().t()).view(-1)  # whole numbers below 2^18
+    want[0] *= 2
+    want = want.half()
+    y = y.view(-1)
+    for at in range(0, n, part):
+        assert torch.equal(y[at:at + part], want[:n - at]), at

@@ -90,3 +90,29 @@ def test_numbers_past_32_bits_are_refused():
     for item in (1, far - 2, -1):
         with pytest.raises(trmoe.TrkError, match="item"):
             trmoe.gemm_i8(W, q, s, item=item)
+
+
+def test_rows_that_a_tile_cannot_number_are_refused():
+    """Weight rows or tokens within a tile of 2^32: the last tile's row numbers would wrap."""
+    import ctypes as C
+    L, P = trmoe.lib(), C.c_void_p(256)
+    most = (1 << 32) - 256
+
+    def mat(rows):
+        return C.byref(trmoe.I8Mat(256, 256, rows, 16, 1, 16, 0))
+
+    def gemm(rows, m):
+        return L.trk_gemm_i8(mat(rows), 0, P, 16, P, m, None, P, 0, 1 << 33, 0, None)
+
+    def up(rows, m, slots):
+        return L.trk_experts_up_i8(mat(rows), mat(rows), P, 16, P, m, P, P, slots, P, P, 1, 1 << 33, None)
+
+    for rows, m, word in ((most + 1, 1, "rows"), ((1 << 32) - 1, 0, "rows"), (5, most + 1, "m (4294967041)"),
+                          (5, (1 << 32) - 1, "m (4294967295)")):
+        assert gemm(rows, m) == -1 and word in L.trk_last_error().decode()
+    assert gemm(most, 0) == 0
+    for rows, slots, ok in ((most, 16, True), (most, 17, False), (1 << 31, 32, True), ((1 << 31) + 1, 32, False)):
+        assert up(rows, 0, slots) == (0 if ok else -1)
+        assert ok or "too large" in L.trk_last_error().decode()
+    assert L.trk_experts_down_i8(mat(most + 1), P, 16, P, 1, P, P, P, 1, None, None, P, 0, 1 << 33, 0, None) == -1
+    assert "rows" in L.trk_last_error().decode()

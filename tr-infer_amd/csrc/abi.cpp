@@ -914,6 +914,7 @@ static int check_elem_ptr(const void* p, uint32_t dt, const char* what) {
 }
 
 constexpr uint32_t I8_K_MAX = 131071;  // 2^14 k < 2^31: the sums of a row's products fit 32 bits
+constexpr uint32_t I8_ROWS_MAX = 0xffffff00u;  // weight rows, tokens: those of the last, ragged tile of 256 still have 32-bit numbers
 
 static int check_i8_rows(const void* q, uint64_t ldq, uint32_t k, const char* what) {
     if ((uintptr_t)q % 16 || ldq % 16) return fail(TRK_E_INVALID, "%s: pointer and row stride must be multiples of 16", what);
@@ -925,6 +926,7 @@ static int check_i8_mat(const trk_i8_mat* w, const char* what) {
     if (!w || !w->ptr || !w->scale) return fail(TRK_E_INVALID, "%s: null argument", what);
     if (w->rows == 0 || w->k == 0 || w->count == 0) return fail(TRK_E_INVALID, "%s: empty matrix", what);
     if (w->k > I8_K_MAX) return fail(TRK_E_INVALID, "%s: k (%u) above %u", what, w->k, I8_K_MAX);
+    if (w->rows > I8_ROWS_MAX) return fail(TRK_E_INVALID, "%s: rows (%u) above %u", what, w->rows, I8_ROWS_MAX);
     if (int rc = check_i8_rows(w->ptr, w->ld, w->k, what)) return rc;
     if (w->ld >> 40) return fail(TRK_E_INVALID, "%s: row stride %llu too large", what, (unsigned long long)w->ld);
     if (w->count > 1 && (w->stride % 16 || w->stride < (w->rows - 1ull) * w->ld + w->k))
@@ -958,6 +960,7 @@ extern "C" int trk_gemm_i8(const trk_i8_mat* w, uint32_t item, const int8_t* q, 
     if ((rc = check_dtype(dtype)) || (rc = check_elem_ptr(y, dtype, "y"))) return rc;
     if ((rc = check_i8_rows(q, ldq, w->k, "q"))) return rc;
     if (m > 1 && ldy < w->rows) return fail(TRK_E_INVALID, "ldy %llu below rows (%u)", (unsigned long long)ldy, w->rows);
+    if (m > I8_ROWS_MAX) return fail(TRK_E_INVALID, "m (%u) above %u", m, I8_ROWS_MAX);
     if (m == 0) return TRK_OK;
     if (!q || !scale || !y) return fail(TRK_E_INVALID, "null argument");
     const I8Mat M = i8_mat(*w);
@@ -1016,6 +1019,8 @@ extern "C" int trk_experts_up_i8(const trk_i8_mat* gate, const trk_i8_mat* up, c
     if ((rc = check_entries(m, slots, gate->count))) return rc;
     if ((rc = check_dtype(dtype)) || (rc = check_elem_ptr(h, dtype, "h"))) return rc;
     if ((rc = check_i8_rows(q, ldq, gate->k, "q"))) return rc;
+    if ((gate->rows + 15ull) / 16 * slots > 1ull << 32)  // workgroups of a token that takes its entries one by one
+        return fail(TRK_E_INVALID, "gate: rows * slots (%u * %u) too large", gate->rows, slots);
     if (ldh < gate->rows) return fail(TRK_E_INVALID, "ldh %llu below rows (%u)", (unsigned long long)ldh, gate->rows);
     if (m == 0) return TRK_OK;
     if (!q || !scale || !ids || !n_sel || !h) return fail(TRK_E_INVALID, "null argument");
