@@ -315,7 +315,9 @@ int trk_gemm_i8(const trk_i8_mat *w, uint32_t item, const int8_t *q, uint64_t ld
  *
  * plan: the entries sorted by expert, of trk_experts_plan_words words, made by trk_experts_plan for
  * the same ids, n_sel, m, slots and n_expert (= the stacks' count).  Up to TRK_EXPERTS_DIRECT_M tokens it has
- * 0 words: the products take their entries one by one, and no plan (NULL). */
+ * 0 words: the products take their entries one by one, and no plan (NULL).  A plan made for another m, slots
+ * or n_expert is not followed: every entry's row of h, and of y every token's that has one, are NaN.  (One made for
+ * more experts is where m * slots does not exceed the stacks' count; the experts beyond are passed over.) */
 #define TRK_EXPERTS_DIRECT_M 8
 int trk_experts_plan_words(uint32_t m, uint32_t slots, uint32_t n_expert, uint64_t *words);
 int trk_experts_plan(const uint32_t *ids, const uint32_t *n_sel, uint32_t m, uint32_t slots, uint32_t n_expert,

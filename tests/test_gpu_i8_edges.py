@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 import trmoe
-from test_gpu_scores_i8 import say
+from test_gpu_scores_i8 import dev, host, i8, padded, routing, say, scales
 
 pytestmark = pytest.mark.gpu
 
@@ -87,3 +87,46 @@ def test_gemm_i8_of_the_most_rows(far):
     y = y.view(-1)
     for at in range(0, n, part):
         assert torch.equal(y[at:at + part], want[:n - at]), at
+
+
+# (m, slots, E) of the call, of the plan: as many words, other entries or experts
+@pytest.mark.parametrize("call,made", [((199, 2, 64), (200, 2, 64)), ((200, 2, 64), (100, 4, 64)), ((10, 3, 64), (10, 3, 40)),
+                                       ((10, 3, 64), (15, 2, 64)), ((1200, 4, 80), (2400, 2, 80)), ((40, 2, 16), None)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_a_plan_of_another_call(call, made, dtype):
+    """A plan of as many words, made for other sizes, or none that was made: entries' rows of h, and of y the rows of tokens
+    that have any, are NaN; the rest stays."""
+    import torch
+    say(f"experts {call} with the plan of {made} {dtype}")
+    rng = np.random.default_rng(7)
+    m, slots, E = call
+    H, F = 96, 80
+    ids, w, n = routing(rng, m, E, slots, "elsewhere")
+    di, dw, dn = dev(ids), dev(w), dev(n)
+    own = trmoe.experts_plan(di, dn, slots, E)
+    if made:
+        mi, _, mn = routing(rng, made[0], made[2], made[1], "plain")
+        other = trmoe.experts_plan(dev(mi), dev(mn), made[1], made[2])
+    else:
+        other = torch.zeros_like(own)
+    assert other.shape == own.shape
+    gate, up = (trmoe.I8Weights(padded(i8(rng, E, F, H)), dev(scales(rng, E, F))) for _ in range(2))
+    down = trmoe.I8Weights(padded(i8(rng, E, H, F)), dev(scales(rng, E, H)))
+    q, s = dev(i8(rng, m, H)), dev(scales(rng, m))
+    hq, hs = dev(i8(rng, m * slots, F)), dev(scales(rng, m * slots))
+    live = R.entries(ids, n, slots, E)
+    has, live = live.any(1), live.reshape(-1)
+    assert has.any() and not has.all()
+    for plan in (other, own):
+        wide = torch.full((m * slots + 1, F + 3), 9.0, dtype=R.torch_dtype(dtype), device="cuda")
+        trmoe.experts_up_i8(gate, up, q, s, di, dn, slots, plan=plan, out=wide[:m * slots, :F])
+        h = host(wide)
+        assert (h[:-1][~live] == 9).all() and (h[-1] == 9).all() and (h[:, F:] == 9).all()
+        for acc in (False, True):
+            wide = torch.full((m + 1, H + 3), 9.0, dtype=R.torch_dtype(dtype), device="cuda")
+            trmoe.experts_down_i8(down, hq, hs, di, dw, dn, slots, plan=plan, out=wide[:m, :H], accumulate=acc)
+            y = host(wide)
+            assert (y[m] == 9).all() and (y[:, H:] == 9).all()
+            assert np.isnan(y[:m, :H][has]).all() if plan is other else np.isfinite(y[:m, :H]).all()
+            assert (y[:m, :H][~has] == (9 if acc else 0)).all()
+        assert np.isnan(h[:-1, :F][live]).all() if plan is other else not np.isnan(h).any()

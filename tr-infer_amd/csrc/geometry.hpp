@@ -250,7 +250,7 @@ inline ExpertsWidth experts_width(uint32_t rows, uint64_t tiles, bool wide) {
     const uint64_t wgs = (rows + 127) / 128 * tiles;
     return wgs < 512 ? X_NARROW : wide && wgs >= 1536 ? X_WIDE : X_128;
 }
-// The plan's words: {tiles, 3 unused}, ent [m * slots], (16-byte aligned) four words per tile, then the counts of each of
+// The plan's words: {tiles, m, slots, E}, ent [m * slots], (16-byte aligned) four words per tile, then the counts of each of
 // plan_workgroups' entries [workgroups][E].
 inline uint64_t plan_tiles(uint32_t m, uint32_t slots, uint32_t E, uint32_t rows) {  // no call has more
     const uint64_t n = (uint64_t)m * slots;

@@ -89,7 +89,7 @@ __global__ __launch_bounds__(PLAN_T) void experts_plan_kernel(const uint32_t* __
     if (blockIdx.x) return;
     for (uint32_t i = 0; i < tc; i++)
         P.tile[to + i] = PlanTile{tid, so + i * rows, c - i * rows < rows ? c - i * rows : rows, 0};
-    if (tid == PLAN_T - 1) *P.n_tiles = to + tc;
+    if (tid == PLAN_T - 1) *P.head = PlanHead{to + tc, m, slots, E};
 }
 
 // ============================================================================================
@@ -185,14 +185,34 @@ __global__ __launch_bounds__(DOWN_WAVES* WAVE) void experts_down_strip_kernel(I8
 // many entries: tiles of one expert's
 // ============================================================================================
 
+// Whether a plan is one for these sizes: its entries are then below m * slots, and its tiles fit the launch.  One made for more
+// experts is where each entry may have a tile of its own.  Nothing is read through another; what would be written is NaN.
+__device__ __forceinline__ bool plan_fits(const PlanHead& h, uint32_t m, uint32_t slots, uint32_t E) {
+    return h.m == m && h.slots == slots && (h.E == E || (h.E > E && h.E <= PLAN_T && m * slots <= E));
+}
+
 // A tile's place: entries of one expert (the plan's tile) x a block of weight rows, the blocks of a tile next to one
 // another and each expert's tiles in turn on one XCD, whose L2 then holds the entries' rows and the expert's weights.
 // E: the stack's experts.  No plan made for it names others; of a plan made for more they are passed over, like ids.
-__device__ __forceinline__ bool expert_tile(const Plan& P, uint32_t E, uint32_t blocks, PlanTile& t, uint32_t& block) {
+__device__ __forceinline__ bool expert_tile(const Plan& P, const PlanHead& h, uint32_t E, uint32_t blocks, PlanTile& t,
+                                            uint32_t& block) {
     uint32_t idx;
-    if (!xcd_order_1d(*P.n_tiles * blocks, idx, run_id())) return false;
+    if (!xcd_order_1d(h.n_tiles * blocks, idx, run_id())) return false;
     t = P.tile[idx / blocks], block = idx % blocks;
     return t.expert < E;
+}
+
+// NaN into every entry's row of y [m * slots][rows], the workgroups taking them in turn
+template <uint32_t DT, typename A>
+__device__ __forceinline__ void nan_rows(const A& a, uint32_t count, void* y, uint32_t rows, uint64_t ldy) {
+    typedef Elem<DT> O;
+    const uint32_t n = a.m * a.slots;
+    for (uint64_t i = run_id(); i < n; i += (uint64_t)gridDim.x * gridDim.y) {
+        const uint32_t t = (uint32_t)i / a.slots, j = (uint32_t)i % a.slots;
+        if (j >= a.n_sel[t] || a.ids[(size_t)t * K_MAX + j] >= count) continue;
+        for (uint64_t r = threadIdx.x; r < rows; r += blockDim.x)
+            reinterpret_cast<typename O::T*>(y)[i * ldy + r] = O::put(__builtin_nanf(""));
+    }
 }
 
 // gate and up: a tile's weight rows are BN / 2 rows of gate, then the same rows of up, and a wave has both of each.  ONCE:
@@ -205,8 +225,11 @@ __global__ __launch_bounds__(Tile::T) void experts_up_tile_kernel(I8Up a, Plan P
     static_assert(BR % (8 * Tile::NW) == 0 && Tile::WN % 32 == 0, "a load takes rows of one matrix");
     PlanTile pt;
     uint32_t block;
-    if (!expert_tile(P, a.gate.count, (a.gate.rows + BR - 1) / BR, pt, block)) return;  // the whole workgroup
-    const uint32_t r0 = block * BR, rl = a.gate.rows - r0 - 1;                          // the last row there is
+    const PlanHead head = *P.head;
+    if (!plan_fits(head, a.m, a.slots, a.gate.count))  // the whole workgroup, here and below
+        return nan_rows<DT>(a, a.gate.count, a.h, a.gate.rows, a.ldh);
+    if (!expert_tile(P, head, a.gate.count, (a.gate.rows + BR - 1) / BR, pt, block)) return;
+    const uint32_t r0 = block * BR, rl = a.gate.rows - r0 - 1;  // the last row there is
     Tile t;
     auto entry = [&](uint32_t i) { return P.ent[pt.row0 + (i < pt.rows ? i : pt.rows - 1)]; };
     const i32x4 bg = buffer_at(a.gate.ptr + pt.expert * a.gate.stride + r0 * a.gate.ld);
@@ -264,7 +287,10 @@ __global__ __launch_bounds__(Tile::T) void experts_down_tile_kernel(I8Down a, Pl
     __shared__ __attribute__((aligned(1024))) uint8_t lds[Tile::LDS];
     PlanTile pt;
     uint32_t block;
-    if (!expert_tile(P, a.down.count, (a.down.rows + Tile::BN - 1) / Tile::BN, pt, block)) return;  // the whole workgroup
+    const PlanHead head = *P.head;
+    if (!plan_fits(head, a.m, a.slots, a.down.count))  // the whole workgroup, here and below
+        return nan_rows<TRK_DT_F32>(a, a.down.count, a.work, a.down.rows, a.down.rows);
+    if (!expert_tile(P, head, a.down.count, (a.down.rows + Tile::BN - 1) / Tile::BN, pt, block)) return;
     const uint32_t r0 = block * Tile::BN, rl = a.down.rows - r0 - 1;
     Tile t;
     auto entry = [&](uint32_t i) { return P.ent[pt.row0 + (i < pt.rows ? i : pt.rows - 1)]; };
