@@ -130,3 +130,32 @@ def test_a_plan_of_another_call(call, made, dtype):
             assert np.isnan(y[:m, :H][has]).all() if plan is other else np.isfinite(y[:m, :H]).all()
             assert (y[:m, :H][~has] == (9 if acc else 0)).all()
         assert np.isnan(h[:-1, :F][live]).all() if plan is other else not np.isnan(h).any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("m", [1, 40])
+def test_silu_of_far_gates(m, dtype):
+    """Gates beyond the exponential's usual range: silu falls with it, down to the smallest numbers.  The exponential is
+    within 2^-22 as nearer to zero, two roundings follow: less than swiglu_tol counts."""
+    say(f"experts_up far gates m={m} {dtype}")
+    rng = np.random.default_rng(m)
+    G = np.concatenate([np.linspace(-130, -70, 241), [-1e3, -1e30, -300.0, 60.0, 200.0, 1e4, 0.0]])
+    F, H = G.size, 16
+    U = np.exp(rng.uniform(-10, 60 if dtype != "f16" else 5, F)) * rng.choice([-1, 1], F)
+    U[np.abs(G) > 150] = 0.5
+    q = np.zeros((m, H), np.int8)
+    q[:, 3] = 127
+    w = np.zeros((1, F, H), np.int8)
+    w[0, :, 3] = 127
+    gw, uw = w * np.where(G < 0, -1, 1).astype(np.int8)[None, :, None], w * np.where(U < 0, -1, 1).astype(np.int8)[None, :, None]
+    gs, us = ((np.abs(a) / 127 ** 2).astype(np.float32)[None] for a in (G, U))
+    s = np.ones(m, np.float32)
+    ids, n = np.zeros((m, 32), np.int32), np.ones(m, np.int32)
+    di, dn = dev(ids), dev(n)
+    gate, up = trmoe.I8Weights(dev(gw), dev(gs)), trmoe.I8Weights(dev(uw), dev(us))
+    got = host(trmoe.experts_up_i8(gate, up, dev(q), dev(s), di, dn, 1, plan=trmoe.experts_plan(di, dn, 1, 1),
+                                   dtype=R.torch_dtype(dtype))).astype(np.float64)
+    g, u = R.gemm(q, s, gw[0], gs[0]), R.gemm(q, s, uw[0], us[0])
+    with np.errstate(over="ignore"):
+        want, tol = R.swiglu(g, u), R.swiglu_tol(g, u, dtype)
+    assert (np.abs(got - want) <= tol).all(), np.argwhere(~(np.abs(got - want) <= tol))[:4]

@@ -271,10 +271,11 @@ __global__ __launch_bounds__(Tile::T) void experts_up_tile_kernel(I8Up a, Plan P
 #pragma unroll
         for (uint32_t i = 0; i < FR; i++) {
             const uint32_t r = r0 + wr + 16 * i + t.lane / 16 * 4;
-            float v[4];
+            float g[4], u[4], v[4];
 #pragma unroll
             for (int c = 0; c < 4; c++)
-                v[c] = swiglu(i8_scaled(t.acc[i][j][c], sx[j], sg[i][c]), i8_scaled(t.acc[FR + i][j][c], sx[j], su[i][c]));
+                g[c] = i8_scaled(t.acc[i][j][c], sx[j], sg[i][c]), u[c] = i8_scaled(t.acc[FR + i][j][c], sx[j], su[i][c]);
+            swiglu4(g, u, v);
             store4<DT>(h + r, v, r < a.gate.rows ? a.gate.rows - r : 0, a.vec);
         }
     }
