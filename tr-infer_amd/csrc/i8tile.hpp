@@ -13,16 +13,16 @@
 namespace trk {
 
 // 16 bytes a lane from base + off (per lane) to the 1024 bytes of LDS at `lds`; vmcnt counts it.  In asm, because the
-// compiler would hold every later LDS read until it has arrived; m0 is a register that it keeps nothing in.
+// compiler would hold every later LDS read until it has arrived.  m0 is named as overwritten: the compiler has uses for it too.
 // ONCE: nobody reads these bytes again, and they are the first that the caches drop.
 template <bool ONCE>
 __device__ __forceinline__ void lds_dma(i32x4 rsrc, uint32_t off, uint32_t lds) {
     if constexpr (ONCE)
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds" ::"s"(lds), "v"(off), "s"(rsrc)
-                     : "memory");
+                     : "memory", "m0");
     else
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc)
-                     : "memory");
+                     : "memory", "m0");
 }
 template <int N>
 __device__ __forceinline__ void wait_dma() {  // all but the last N, and this wave's LDS reads
