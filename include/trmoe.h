@@ -272,11 +272,13 @@ typedef struct {
 
 /* Per-row routing by scores.  Expert e's key is its score plus bias[e] (bias NULL: the order of the
  * logits); the k largest keys of the kept groups are chosen, in descending order, the lower index
- * first among equal ones, and weighted by their scores, without the bias.  Keys and group sums are
- * compared as if in 64 bits.  An expert whose logit (or key) is NaN or -inf is never chosen, and
- * adds nothing to the softmax's sum: a row chooses fewer than k, or none, where the others run out.
+ * first among equal ones, and weighted by their scores, without the bias.  Keys, group sums and
+ * weights are computed as if in 64 bits, the weights then rounded once.  An expert whose logit or
+ * key is NaN or -inf is never chosen: a row chooses fewer than k, or none, where the others run out.
+ * By its logit it adds nothing to the softmax's sum either; by its bias alone it does.
  * ids / w: [m][32], n_sel: [m]; slots n_sel .. k - 1 get id 0xffffffff and weight 0, later ones stay
- * as they were.  A softmax row with a logit of +inf has NaN scores: NaN weights, and with a bias no choice.
+ * as they were.  A softmax row with a logit of +inf has NaN scores: nothing is chosen where they enter
+ * the choice (a bias, or groups by the sum of two), else by the logits, with NaN weights.
  * n_expert at most 1024. */
 int trk_route_scores(const float *logits, const float *bias, uint32_t m, uint32_t n_expert,
                      const trk_score_policy *policy, uint32_t *ids, float *w, uint32_t *n_sel, void *stream);

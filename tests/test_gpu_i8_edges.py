@@ -159,3 +159,17 @@ def test_silu_of_far_gates(m, dtype):
     with np.errstate(over="ignore"):
         want, tol = R.swiglu(g, u), R.swiglu_tol(g, u, dtype)
     assert (np.abs(got - want) <= tol).all(), np.argwhere(~(np.abs(got - want) <= tol))[:4]
+
+
+@pytest.mark.parametrize("m", [1, 40])
+def test_silu_of_a_gate_out_of_range(m):
+    """A gate product below the lowest number: nothing is left of its silu."""
+    import torch
+    say(f"experts_up gate out of range m={m}")
+    one = torch.ones((1, 8, 16), dtype=torch.int8, device="cuda")
+    gate = trmoe.I8Weights(-one, torch.full((1, 8), 3e38, device="cuda"))
+    up = trmoe.I8Weights(one, torch.ones((1, 8), device="cuda"))
+    ids, n = torch.zeros((m, 32), dtype=torch.int32, device="cuda"), torch.ones(m, dtype=torch.int32, device="cuda")
+    h = trmoe.experts_up_i8(gate, up, one[0, :1].expand(m, 16).contiguous(), torch.ones(m, device="cuda"), ids, n, 1,
+                            plan=trmoe.experts_plan(ids, n, 1, 1))
+    assert (h == 0).all()

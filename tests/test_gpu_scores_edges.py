@@ -58,3 +58,40 @@ def test_softmax_weights_left_as_they_are(E, k, groups, keep, bias):
         b[::9] = -np.inf  # not to be chosen, but part of the sum
     # half a step, and what 64-bit exponentials and their sum may differ by
     check_route(lg, b, "softmax", rtol=1.001 * R.EPS["f32"], k=k, n_group=groups, topk_group=keep, renorm=False)
+
+
+def test_an_infinite_logit():
+    """A softmax row with a logit of +inf has NaN scores: nothing is chosen where they enter the choice, else NaN weights.  Its
+    sigmoid is 1."""
+    say("route_scores infinite logits")
+    E, k = 16, 3
+    lg = np.random.default_rng(4).standard_normal((3, E)).astype(np.float32)
+    lg[1, 9] = np.inf
+    lg[2, [2, 9]] = np.inf
+    bias = np.zeros(E, np.float32)
+    base = dict(k=k, n_group=1, topk_group=1, group_top=2, renorm=True, factor=1.0)
+    for kw, b, scored in ((base, None, False), (base, bias, True), ({**base, "n_group": 4, "topk_group": 2}, None, True),
+                          ({**base, "n_group": 4, "topk_group": 2, "group_top": 1}, None, False)):
+        ids, w, n = (host(t) for t in trmoe.route_scores(dev(lg), bias=None if b is None else dev(b), score="softmax", **kw))
+        assert n[0] == k and np.isfinite(w[0, :k]).all()
+        if scored:
+            assert (n[1:] == 0).all() and (ids[1:, :k] == -1).all() and (w[1:, :k] == 0).all()
+        else:
+            assert (n[1:] == k).all() and ids[1, 0] == 9 and ids[2, :2].tolist() == [2, 9] and np.isnan(w[1:, :k]).all()
+        check_route(lg, b, "sigmoid", **kw)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("bias", [False, True])
+def test_choices_that_hang_on_no_rounding(score, bias):
+    """Every logit moved by up to 1e-12 of itself, each by another amount: the plain form's choice stays, so the kernel's has to be
+    the same."""
+    say(f"route_scores settled {score} bias={bias}")
+    rng = np.random.default_rng(17 + bias)
+    lg = (rng.standard_normal((200, 256)) * 1.5).astype(np.float32)
+    lg[rng.random(lg.shape) < 0.05] = -np.inf
+    b = (rng.standard_normal(256) * 0.1).astype(np.float32) if bias else None
+    kw = dict(k=8, n_group=8, topk_group=4, group_top=2, renorm=True, factor=2.5)
+    moved = np.where(np.isfinite(lg), lg.astype(np.float64) * (1 + rng.uniform(-1e-12, 1e-12, lg.shape)), lg)
+    assert np.array_equal(R.route(lg, bias=b, score=score, **kw)[0], R.route(moved, bias=b, score=score, **kw)[0])
+    check_route(lg, b, score, **kw)

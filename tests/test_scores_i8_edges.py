@@ -116,3 +116,14 @@ def test_rows_that_a_tile_cannot_number_are_refused():
         assert ok or "too large" in L.trk_last_error().decode()
     assert L.trk_experts_down_i8(mat(most + 1), P, 16, P, 1, P, P, P, 1, None, None, P, 0, 1 << 33, 0, None) == -1
     assert "rows" in L.trk_last_error().decode()
+
+
+def test_plan_extents_by_its_entries(tmp_path):
+    import os
+    import subprocess
+    here = os.path.dirname(os.path.abspath(__file__))
+    exe = str(tmp_path / "i8_plan_check")
+    subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-Werror", os.path.join(here, "i8_plan_check.cpp"), "-o", exe],
+                   check=True)
+    r = subprocess.run([exe], capture_output=True, text=True)
+    assert r.returncode == 0 and r.stdout.startswith("ok"), r.stdout
