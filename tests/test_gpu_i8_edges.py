@@ -173,3 +173,29 @@ def test_silu_of_a_gate_out_of_range(m):
     h = trmoe.experts_up_i8(gate, up, one[0, :1].expand(m, 16).contiguous(), torch.ones(m, device="cuda"), ids, n, 1,
                             plan=trmoe.experts_plan(ids, n, 1, 1))
     assert (h == 0).all()
+
+
+def test_a_stream_of_another_device():
+    """Every call refuses it, and takes one of its own."""
+    import torch
+    from types import SimpleNamespace
+    say("streams of another device")
+    there = SimpleNamespace(cuda_stream=0, device_index=torch.cuda.current_device() + 1)
+    W = trmoe.quantize_weights(torch.randn((4, 32, 32), device="cuda"))
+    x = torch.randn((40, 32), device="cuda")
+    q, s = trmoe.quantize_rows(x)
+    ids, w, n = trmoe.route_scores(torch.randn((40, 4), device="cuda"), 2)
+    plan = trmoe.experts_plan(ids, n, 2, 4)
+    hq, hs = trmoe.quantize_rows(trmoe.experts_up_i8(W, W, q, s, ids, n, 2, plan=plan))
+    y, h = torch.full((40, 32), 9.0, device="cuda"), torch.full((80, 32), 9.0, device="cuda")
+    work = torch.empty(40 * 2 * 32, device="cuda")
+    for call in (lambda st: trmoe.quantize_rows(x, out=(hq[:40].clone(), s.clone()), stream=st),
+                 lambda st: trmoe.route_scores(x, 2, stream=st),
+                 lambda st: trmoe.gemm_i8(trmoe.I8Weights(W.q[0], W.scale[0]), q, s, out=y, stream=st),
+                 lambda st: trmoe.experts_plan(ids, n, 2, 4, stream=st),
+                 lambda st: trmoe.experts_up_i8(W, W, q, s, ids, n, 2, plan=plan, out=h, stream=st),
+                 lambda st: trmoe.experts_down_i8(W, hq, hs, ids, w, n, 2, plan=plan, out=y, work=work, stream=st)):
+        with pytest.raises(trmoe.TrkError, match="a stream of device"):
+            call(there)
+        call(torch.cuda.current_stream())
+    torch.cuda.synchronize()

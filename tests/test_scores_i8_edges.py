@@ -127,3 +127,12 @@ def test_plan_extents_by_its_entries(tmp_path):
                    check=True)
     r = subprocess.run([exe], capture_output=True, text=True)
     assert r.returncode == 0 and r.stdout.startswith("ok"), r.stdout
+
+
+def test_streams_of_other_devices_are_refused(monkeypatch):
+    from types import SimpleNamespace
+    trmoe._late()
+    monkeypatch.setattr(trmoe, "_device", lambda: 0)
+    assert trmoe._stream_here(SimpleNamespace(cuda_stream=5, device_index=0)) == 5
+    with pytest.raises(trmoe.TrkError, match="a stream of device 1"):
+        trmoe._stream_here(SimpleNamespace(cuda_stream=5, device_index=1))

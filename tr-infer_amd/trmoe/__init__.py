@@ -542,8 +542,8 @@ def gemv(wt, rows, k, fmt, item, count, kb, q, s, su, pair=False, y=None, ldy=No
 
 # ---- routing by scores, 8-bit products with a scale per token and per channel --------------------
 #
-# The kernels run on torch's current stream (or `stream`) of the current device; tensors elsewhere are
-# refused.  Outputs are allocated where none is given, on the current stream as torch does: a `stream` that is not
+# The kernels run on torch's current stream (or `stream`) of the current device; tensors and streams of
+# others are refused.  Outputs are allocated where none is given, on the current stream as torch does: a `stream` that is not
 # the current one has to wait for it before the call, as for whatever wrote the tensors given.
 
 _torch = None  # the module, its dtypes and its device lookup once a call has needed them
@@ -589,6 +589,13 @@ def _here(*tensors):
                 dev = _device()
             if at != dev:
                 raise TrkError(f"a tensor on device {at}: all have to be on the current device, {dev}")
+
+
+def _stream_here(stream):
+    """The hipStream_t of `stream`, which has to be one of the current device: work on another's would run there."""
+    if stream is not None and stream.device_index != _device():
+        raise TrkError(f"a stream of device {stream.device_index}: it has to be one of the current device, {_device()}")
+    return _stream(stream)
 
 
 def _rows(t, what, m=None, k=None):
@@ -689,7 +696,7 @@ def route_scores(logits, k, bias=None, score="sigmoid", n_group=1, topk_group=1,
         _routing(ids, n, m, w)
     _here(logits, bias, ids, w, n)
     check(lib().trk_route_scores(logits.data_ptr(), _ptr(bias), m, E, p, ids.data_ptr(), w.data_ptr(),
-                                 n.data_ptr(), _stream(stream)))
+                                 n.data_ptr(), _stream_here(stream)))
     return ids, w, n
 
 
@@ -714,7 +721,7 @@ def quantize_rows(x, out=None, stream=None):
         ldq = _i8_rows(q, scale, m, k, read=False)
     _here(x, q, scale)
     check(lib().trk_quantize_rows(x.data_ptr(), _dtype(x.dtype), ldx, m, k, q.data_ptr(), ldq, scale.data_ptr(),
-                                  _stream(stream)))
+                                  _stream_here(stream)))
     return q, scale
 
 
@@ -754,7 +761,7 @@ def gemm_i8(w: I8Weights, q, scale, bias=None, dtype=None, out=None, accumulate=
         ldy = _rows(out, "out", m, w.rows)
     _here(q, scale, bias, out, w.q)
     check(lib().trk_gemm_i8(w.ref, item, q.data_ptr(), ldq, scale.data_ptr(), m, _ptr(bias), out.data_ptr(),
-                            _dtype(out.dtype), ldy, int(accumulate), _stream(stream)))
+                            _dtype(out.dtype), ldy, int(accumulate), _stream_here(stream)))
     return out
 
 
@@ -786,7 +793,7 @@ def experts_plan(ids, n_sel, slots, n_expert, stream=None):
     words = _plan_words(m, slots, n_expert)
     _here(ids, n_sel)
     plan = torch.empty(words, dtype=torch.int32, device=ids.device)
-    check(lib().trk_experts_plan(ids.data_ptr(), n_sel.data_ptr(), m, slots, n_expert, plan.data_ptr(), _stream(stream)))
+    check(lib().trk_experts_plan(ids.data_ptr(), n_sel.data_ptr(), m, slots, n_expert, plan.data_ptr(), _stream_here(stream)))
     return plan
 
 
@@ -817,7 +824,7 @@ def experts_up_i8(gate: I8Weights, up: I8Weights, q, scale, ids, n_sel, slots, p
     _here(q, scale, ids, n_sel, plan, out, gate.q, up.q)
     check(lib().trk_experts_up_i8(gate.ref, up.ref, q.data_ptr(), ldq, scale.data_ptr(), m, ids.data_ptr(),
                                   n_sel.data_ptr(), slots, _ptr(plan), out.data_ptr(), _dtype(out.dtype), ldh,
-                                  _stream(stream)))
+                                  _stream_here(stream)))
     return out
 
 
@@ -848,7 +855,7 @@ def experts_down_i8(down: I8Weights, q, scale, ids, w, n_sel, slots, plan=None, 
     _here(q, scale, ids, w, n_sel, plan, work, out, down.q)
     check(lib().trk_experts_down_i8(down.ref, q.data_ptr(), ldq, scale.data_ptr(), m, ids.data_ptr(), w.data_ptr(),
                                     n_sel.data_ptr(), slots, _ptr(plan), _ptr(work), out.data_ptr(), _dtype(out.dtype),
-                                    ldy, int(accumulate), _stream(stream)))
+                                    ldy, int(accumulate), _stream_here(stream)))
     return out
 
 
