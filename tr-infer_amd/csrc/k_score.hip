@@ -220,16 +220,16 @@ __device__ __forceinline__ bool score_row32(const float* __restrict__ lg, const 
             rank += o > worth || (o == worth && i < g) ? 1u : 0u;
         }
         bool kept = rank < p.topk_group && worth > NONE;
-        // the worst group kept and the best one dropped; a sum of two keys is off by twice a key and a rounding
-        const uint32_t lo = ~wave_max_u32(kept ? ~fkey(worth) : 0u), hi = wave_max_u32(kept ? 0u : fkey(worth));
-        // a sum of two keys below the lowest number is -inf in 32 bits: its group is there, and its place open
-        const bool lost = sums && __ballot(g < p.n_group && a1 > NONE && !(worth > NONE));
-        if (scored && (lost || (hi && lo != 0xffffffffu))) {
+        // the worst group kept and the best one dropped; a sum of two keys is off by twice a key and a rounding, and -inf below
+        // the lowest number: its group (key 1) is there, and its place open
+        const uint32_t there = fkey(worth), drop = a1 > NONE && there == 0u ? 1u : there;
+        const uint32_t lo = ~wave_max_u32(kept ? ~there : 0u), hi = wave_max_u32(kept ? 0u : drop);
+        if (scored && hi) {
             const float fl = fkey_inv(lo), fh = fkey_inv(hi);
             // of a sum: its keys' errors, their roundings and its own
             const float both = __builtin_fabsf(a1) + (a2 > NONE ? __builtin_fabsf(a2) : 0.0f);
             const float big = __uint_as_float(wave_max_u32(g < p.n_group && a1 > NONE ? __float_as_uint(both) : 0u));
-            if (lost || !(fl - fh > 4.0f * tol + 0x1p-22f * big)) {
+            if (!(fl - fh > 4.0f * tol + 0x1p-22f * big)) {  // so too where one is no number, or none is kept
                 sum64();
                 double d1 = (double)NONE, d2 = (double)NONE;
 #pragma unroll
