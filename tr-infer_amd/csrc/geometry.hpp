@@ -188,7 +188,8 @@ inline uint64_t i8_tiles(uint64_t rows, uint64_t m, uint32_t bn, uint32_t bm) {
 // Strips have every wave's share of K in flight at once and win while each has a CU of its own; beyond it the weights come
 // faster through LDS.  us, strips / 64 x 32 tiles, k = 512 and 2560: [1024] x 16 rows (64 strips) 2.6 / 3.1 and 4.2 / 6.2,
 // [2560] x 16 (160) 2.7 / 3.1 and 4.8 / 6.4, [5000] x 1 (313) 2.6 / 3.0 and 5.4 / 6.5, x 16 3.1 / 3.1 and 7.1 / 6.5,
-// [12288] x 1 (768) 3.5 / 3.6 and 7.2 / 7.0, x 16 4.0 / 3.8 and 9.3 / 7.1.
+// [12288] x 1 (768) 3.5 / 3.6 and 7.2 / 7.0, x 16 4.0 / 3.8 and 9.3 / 7.1.  At long k, weights from memory: k = 8192 [2048] x 1
+// 9.4 / 18.6, x 16 12.3 / 18.9; k = 12288 [1024] x 1 12.2 / 25.9, [2560] x 1 13.1 / 25.1, x 16 17.6 / 25.6, [4096] x 16 19.6 / 26.9.
 inline bool i8_strips(uint32_t m, uint32_t rows) {
     const uint64_t wgs = i8_tiles(rows, m, 16, 16);
     return wgs <= 256 || (m <= 4 && wgs <= 512);
@@ -221,7 +222,9 @@ inline I8Form gemm_i8_form(uint32_t m, uint32_t rows, uint32_t k, uint64_t ldw, 
 // The int8 experts' products (k_i8x.hip): up to eight tokens each entry by itself, beyond it by a plan: entries sorted
 // by expert and cut into tiles of at most plan_rows entries of one expert.
 // us, up and down by themselves / planned (the plan included; H = 2048): 8 tokens of 10 in 512 experts of F = 512 52 / 58, of 8
-// in 128 of 768 60 / 67, of 2 in 8 of 1024 22 / 24; 16 tokens 90 / 89, 105 / 91 and 36 / 24.
+// in 128 of 768 60 / 67, of 2 in 8 of 1024 22 / 24; 16 tokens 90 / 89, 105 / 91 and 36 / 24.  By tokens alone: that is wrong for
+// many entries an expert, each of which reads its weights (a plan for each product, F = 1024): 8 tokens of 4 in 8 33 / 25, of 8 in
+// 8 57 / 26, of 8 in 16 62 / 33; right for few: 4 of 4 in 8 20 / 24, 2 of 8 in 8 21 / 25, 8 of 1 in 1 13 / 20.
 constexpr uint32_t DIRECT_M = 8;  // TRK_EXPERTS_DIRECT_M
 inline bool plan_used(uint32_t m) { return m > DIRECT_M; }
 // us, up at 32 / 64 / 128 rows: 2 entries an expert (4 of 16 x 100 tokens: 25) 7.1 / 7.3 / 8.1, 62 (8 of 128 x 1000) 110 / 94

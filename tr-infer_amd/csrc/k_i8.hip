@@ -243,7 +243,8 @@ void launch_quantize(const void* x, uint64_t ldx, uint32_t m, uint32_t k, int8_t
 constexpr uint32_t ST_WAVES = 4;  // 8 or 16 waves are as fast from one row of 2560 values to 16 of 10240
 
 // A workgroup takes 16 weight rows and up to 16 tokens: its waves share K and add their sums in LDS.  One trip to memory bounds
-// it: [2560] x 1 token at k = 2560 4.1 us, [1024] x 16 at k = 512 2.6.
+// it: [2560] x 1 token at k = 2560 4.2 us (3.6 where a cache holds the weights), at k = 12288 13.1 (10.4); [1024] x 16 at k = 512
+// 2.7.
 template <uint32_t DT>
 __global__ __launch_bounds__(ST_WAVES* WAVE) void gemm_i8_strip_kernel(I8Gemm g) {
     __shared__ int32_t part[ST_WAVES][16][16];  // [wave][token][weight row]
@@ -293,8 +294,8 @@ __device__ __forceinline__ void tile_place(uint32_t idx, uint32_t tn, uint32_t t
 }
 
 // Bound by the matrix cores where there are many rows (4096 x 12288 x 2560 126 us, 2050 TOP/s; 8192 cubed 433 us, 2540
-// TOP/s: busy two thirds of the cycles, and the clock gives way, at 1.9 GHz), by memory where there are few ([12288] x 1 at
-// k = 2560 7.0 us, 4.5 TB/s).  A workgroup per CU that goes on to its next tile, whose loads then fly while the last is
+// TOP/s: busy two thirds of the cycles, and the clock gives way, at 1.9 GHz), by their weights' way through the stages where there are few
+// ([12288] x 1 at k = 2560 6.1 us from a cache, 10.3 from memory, 3.1 TB/s).  A workgroup per CU that goes on to its next tile, whose loads then fly while the last is
 // written, was no faster (126.5 us, 436).
 template <typename Tile, uint32_t DT>
 __global__ __launch_bounds__(Tile::T) void gemm_i8_tile_kernel(I8Gemm g) {

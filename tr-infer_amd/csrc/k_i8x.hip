@@ -105,7 +105,7 @@ __device__ __forceinline__ const int8_t* strip_row(const I8Mat& w, uint32_t e, u
 }
 
 // A workgroup takes 16 rows of gate and up and one entry; its waves share K.  Two trips to memory, the ids' and the rows': one
-// token of 10 in 512 experts (H = 2048, F = 512; 21 MB) 7.2 us.
+// token of 10 in 512 experts (H = 2048, F = 512; 21 MB) 6.4 us where a cache holds the weights, 9.0 from memory.
 template <uint32_t DT>
 __global__ __launch_bounds__(ST_WAVES * WAVE) void experts_up_strip_kernel(I8Up a) {
     __shared__ int32_t part[2][ST_WAVES][16];  // [gate, up][wave][weight row]
@@ -138,8 +138,8 @@ __global__ __launch_bounds__(ST_WAVES * WAVE) void experts_up_strip_kernel(I8Up 
 
 // A workgroup takes 16 down rows and one token: a wave per slot (several where there are fewer slots than waves, sharing
 // K; in turn where there are more), then a thread per (slot, row) scales and weights, and a thread per row adds in slot
-// order.  Memory bounds it: four tokens of 10 in 512 (41 MB) 10 us.
-constexpr uint32_t DOWN_WAVES = 8;  // 12 and 16 are slower: four tokens of ten slots 11.3, 13.1 and 13.2 us
+// order.  Four tokens of 10 in 512 (41 MB) 9.4 us where a cache holds the weights, 11.7 from memory.
+constexpr uint32_t DOWN_WAVES = 8;  // 12 and 16 are slower where timed: four tokens of ten slots 11.3, 13.1 and 13.2 us
 
 template <uint32_t DT>
 __global__ __launch_bounds__(DOWN_WAVES* WAVE) void experts_down_strip_kernel(I8Down a) {
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(Tile::T) void experts_up_tile_kernel(I8Up a, Plan P
 }
 
 // down: the entries' weighted rows into work [m * slots][rows], in 32 bits, as they are then added.  ONCE: geo::experts_once.
-// Memory bounds it: 4096 tokens of 10 in 512 (H = 2048, F = 512) read 560 MB and write 336 in 225 us.
+// Memory bounds it: 4096 tokens of 10 in 512 (H = 2048, F = 512) read 560 MB and write 336 in some 225 us (239 under a trace).
 template <typename Tile, bool ONCE>
 __global__ __launch_bounds__(Tile::T) void experts_down_tile_kernel(I8Down a, Plan P) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[Tile::LDS];
