@@ -914,7 +914,7 @@ static int check_elem_ptr(const void* p, uint32_t dt, const char* what) {
 }
 
 constexpr uint32_t I8_K_MAX = 131071;  // 2^14 k < 2^31: the sums of a row's products fit 32 bits
-constexpr uint32_t I8_ROWS_MAX = 0xffffff00u;  // weight rows, tokens: those of the last, ragged tile of 256 still have 32-bit numbers
+constexpr uint32_t I8_ROWS_MAX = 0xffffff00u;  // weight rows, tokens: a ragged last tile of 256 is still numbered by 32 bits
 
 static int check_i8_rows(const void* q, uint64_t ldq, uint32_t k, const char* what) {
     if ((uintptr_t)q % 16 || ldq % 16) return fail(TRK_E_INVALID, "%s: pointer and row stride must be multiples of 16", what);

@@ -94,7 +94,7 @@ struct Elem<TRK_DT_F16> {
 
 // silu(g) u in 32 bits.  Below -80, where silu512's exponential is soon held (at 88.3) and silu would fall no further, it is
 // g e^g (1 + e^g is 1 there): e^g = 2^n e^r, and the power of two goes in last, so that the product rounds once where it
-// ends among the smallest numbers.  u may be 2^128, g e^r is below 2^9; below -400 nothing is left for any u.
+// ends among the smallest numbers.  u may be 2^128, g e^r is below 2^10; below -400 nothing is left for any u.
 __device__ __forceinline__ float swiglu_far(float g, float u) {
     g = __builtin_fmaxf(g, -400.0f);
     const float n = __builtin_rintf(g * 1.442695041f);

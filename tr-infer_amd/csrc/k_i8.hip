@@ -294,9 +294,9 @@ __device__ __forceinline__ void tile_place(uint32_t idx, uint32_t tn, uint32_t t
 }
 
 // Bound by the matrix cores where there are many rows (4096 x 12288 x 2560 126 us, 2050 TOP/s; 8192 cubed 433 us, 2540
-// TOP/s: busy two thirds of the cycles, and the clock gives way, at 1.9 GHz), by their weights' way through the stages where there are few
-// ([12288] x 1 at k = 2560 6.1 us from a cache, 10.3 from memory, 3.1 TB/s).  A workgroup per CU that goes on to its next tile, whose loads then fly while the last is
-// written, was no faster (126.5 us, 436).
+// TOP/s: busy two thirds of the cycles, and the clock gives way, at 1.9 GHz), by their weights' way through the stages
+// where there are few ([12288] x 1 at k = 2560 6.1 us from a cache, 10.3 from memory, 3.1 TB/s).  A workgroup per CU that
+// goes on to its next tile, whose loads then fly while the last is written, was no faster (126.5 us, 436).
 template <typename Tile, uint32_t DT>
 __global__ __launch_bounds__(Tile::T) void gemm_i8_tile_kernel(I8Gemm g) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[Tile::LDS];

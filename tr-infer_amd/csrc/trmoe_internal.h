@@ -291,7 +291,8 @@ struct Plan {
     PlanTile* tile;
 };
 __host__ __device__ inline Plan plan_at(uint32_t* p, uint32_t m, uint32_t slots) {
-    return Plan{reinterpret_cast<PlanHead*>(p), p + 4, reinterpret_cast<PlanTile*>(p + 4 + ((uint64_t)m * slots + 3) / 4 * 4)};  // geo::plan_tile_at
+    return Plan{reinterpret_cast<PlanHead*>(p), p + 4,
+                reinterpret_cast<PlanTile*>(p + 4 + ((uint64_t)m * slots + 3) / 4 * 4)};  // geo::plan_tile_at
 }
 hipError_t launch_quantize_rows(const void* x, uint32_t dt, uint64_t ldx, uint32_t m, uint32_t k, int8_t* q,
                                 uint64_t ldq, float* scale, hipStream_t st);
