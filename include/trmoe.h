@@ -340,6 +340,80 @@ int trk_experts_down_i8(const trk_i8_mat *down, const int8_t *q, uint64_t ldq, c
                         const uint32_t *plan, void *work, void *y, uint32_t dtype, uint64_t ldy, int accumulate,
                         void *stream);
 
+/* ---- microscaled 4-bit rows: their products, dense and for experts, and a whole layer ---- */
+/* No counterpart in the reference.  For layers whose experts or dense projections are 4-bit floating point with a
+ * power of two for each 32 neighbours of a row, multiplied with activation rows in the same form:
+ *
+ *   trk_route_scores -> trk_experts_plan -> trk_quantize_mx4 (x) -> trk_experts_up_mx4
+ *                    -> trk_quantize_mx4 (h) -> trk_experts_down_mx4
+ *
+ * or, for up to TRK_EXPERTS_DIRECT_M tokens and with activations that stay as they are, trk_moe_mx4.
+ *
+ * A row of k values is ceil(k / 32) blocks of 16 bytes, two values a byte, the first in the low four bits; the last block's
+ * values behind the k-th are zeros.  A value's four bits are a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6.  A block's scale is
+ * a byte s that stands for 2^(s - 127); with s = 255 (NaN) the block's values, and every product of the row, are NaN.
+ * Rows of values begin at multiples of 16 bytes, rows of scales at multiples of 4; scales are read in 4-byte pieces, so the bytes
+ * behind a row's last up to the next multiple of 4 have to be there (any value). */
+
+/* A stack of `count` 4-bit matrices [rows][k]: matrix i's row r has its values at ptr + i * stride + r * ld, its scales at
+ * scale + i * scale_stride + r * scale_ld (all in bytes; the strides count where count > 1).  k at most 2^30, rows, and the
+ * tokens of trk_gemm_mx4, at most 2^32 - 256. */
+typedef struct {
+    const uint8_t *ptr, *scale;
+    uint32_t rows, k, count;
+    uint64_t ld, stride;
+    uint64_t scale_ld, scale_stride;
+} trk_mx4_mat;
+
+/* Rows to 4-bit values: a block's scale is 2^e, e = floor(log2 max |x|) - 2, held to -127 from below; its values x / 2^e are
+ * rounded to the nearest of the sixteen, ties to the even one of two neighbours (0.25 to 0, 0.75 to 1, 1.25 to 1, 1.75 and
+ * 2.5 to 2, 3.5 and 5 to 4), magnitudes above 6 to 6, with x's sign.  A block of zeros gets scale byte 0; one with a NaN or an
+ * infinity gets 255, and zeros.  x: [m][k] of type `dtype`, rows ldx elements apart; whole blocks of q are written,
+ * and ceil(k / 32) scale bytes a row. */
+int trk_quantize_mx4(const void *x, uint32_t dtype, uint64_t ldx, uint32_t m, uint32_t k, uint8_t *q, uint64_t ldq,
+                     uint8_t *scale, uint64_t scale_ld, void *stream);
+
+/* What 4-bit rows stand for: y [m][k] of type `dtype`, rows ldy elements apart, rounded once. */
+int trk_dequantize_mx4(const uint8_t *q, uint64_t ldq, const uint8_t *scale, uint64_t scale_ld, uint32_t m, uint32_t k,
+                       void *y, uint32_t dtype, uint64_t ldy, void *stream);
+
+/* y[i][r] = sum_j q[i][j] w[r][j] (+ bias[r]) (+ y[i][r] with accumulate), for every row r of matrix `item`: products
+ * and a block's sum of them are exact, blocks are added in 32 bits, y's type is rounded to once.  y: rows ldy elements
+ * apart; bias: [rows] or NULL. */
+int trk_gemm_mx4(const trk_mx4_mat *w, uint32_t item, const uint8_t *q, uint64_t ldq, const uint8_t *scale,
+                 uint64_t scale_ld, uint32_t m, const float *bias, void *y, uint32_t dtype, uint64_t ldy, int accumulate,
+                 void *stream);
+
+/* trk_experts_up_i8 and trk_experts_down_i8 for 4-bit stacks and rows: entries, plan, h, y and work (of
+ * trk_experts_down_work_bytes) are theirs. */
+int trk_experts_up_mx4(const trk_mx4_mat *gate, const trk_mx4_mat *up, const uint8_t *q, uint64_t ldq,
+                       const uint8_t *scale, uint64_t scale_ld, uint32_t m, const uint32_t *ids, const uint32_t *n_sel,
+                       uint32_t slots, const uint32_t *plan, void *h, uint32_t dtype, uint64_t ldh, void *stream);
+int trk_experts_down_mx4(const trk_mx4_mat *down, const uint8_t *q, uint64_t ldq, const uint8_t *scale,
+                         uint64_t scale_ld, uint32_t m, const uint32_t *ids, const float *w, const uint32_t *n_sel,
+                         uint32_t slots, const uint32_t *plan, void *work, void *y, uint32_t dtype, uint64_t ldy,
+                         int accumulate, void *stream);
+
+/* A MoE layer on 4-bit experts.  The stacks hold n_expert routed experts, then n_shared (0..32) that every token takes:
+ * gate / up [n_expert + n_shared][F][H], down [n_expert + n_shared][H][F].  router: [n_expert][H], or NULL where each call
+ * brings its logits; bias: trk_route_scores', or NULL; shared_gate: [H], the shared experts are weighted with
+ * sigmoid(shared_gate . x), or NULL, with 1. */
+typedef struct {
+    const float *router, *bias, *shared_gate;
+    trk_mx4_mat gate, up, down;
+    uint32_t n_shared;
+} trk_moe_mx4_w;
+
+/* y[t] = sum_j w_j down_j (silu(gate_j x[t]) * up_j x[t]) over the experts that trk_route_scores chooses by the router's
+ * logits (rlog [m][n_expert] where it is given, else router . x in 32 bits), in that order, then the shared ones.  Up to
+ * TRK_EXPERTS_DIRECT_M tokens (more: TRK_E_CAPACITY).  Activations are not quantised: x, h and every sum are as 32 bits
+ * hold them, y is rounded to once.  A token with a NaN or an infinity in x gets NaN from each of its experts.
+ * x: rows ldx elements apart, of type xdtype; y: rows ldy apart, of type ydtype.  work: trk_moe_mx4_work_bytes of device memory,
+ * 16-byte aligned, of any content; calls that may overlap need one each.  k: the policy's. */
+int trk_moe_mx4_work_bytes(const trk_moe_mx4_w *w, uint32_t k, uint32_t m, uint64_t *bytes);
+int trk_moe_mx4(const trk_moe_mx4_w *w, const trk_score_policy *policy, const void *x, uint32_t xdtype, uint64_t ldx,
+                const float *rlog, uint32_t m, void *work, void *y, uint32_t ydtype, uint64_t ldy, void *stream);
+
 /* y = silu(g) * u (elem::swiglu_vec, elem.rs:173-175) over n floats. */
 int trk_swiglu(const float *g, const float *u, float *y, size_t n, void *stream);
 

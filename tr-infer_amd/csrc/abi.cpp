@@ -880,10 +880,7 @@ extern "C" int trk_gemv(const trk_mat* w, uint32_t item, uint32_t s0, uint32_t s
 
 // ---- routing by scores, 8-bit products with a scale per token and per channel ------------------------
 
-extern "C" int trk_route_scores(const float* logits, const float* bias, uint32_t m, uint32_t n_expert,
-                                const trk_score_policy* p, uint32_t* ids, float* w, uint32_t* n_sel, void* stream) {
-    if (!p) return fail(TRK_E_INVALID, "null argument");
-    if (n_expert == 0 || n_expert > 1024) return fail(TRK_E_INVALID, "n_expert (%u) must be in 1..1024", n_expert);
+static int check_score_policy(const trk_score_policy* p, uint32_t n_expert) {
     if (p->k < 1 || p->k > TRK_MOE_K_MAX || p->k > n_expert)
         return fail(TRK_E_POLICY, "score policy: k (%u) must be in 1..min(32, n_expert)", p->k);
     if (p->score != TRK_SCORE_SOFTMAX && p->score != TRK_SCORE_SIGMOID)
@@ -896,6 +893,14 @@ extern "C" int trk_route_scores(const float* logits, const float* bias, uint32_t
     if (p->group_top != 1 && p->group_top != 2)
         return fail(TRK_E_POLICY, "score policy: group_top (%u) must be 1 or 2", p->group_top);
     if (!std::isfinite(p->factor)) return fail(TRK_E_POLICY, "score policy: factor (%g) must be finite", (double)p->factor);
+    return TRK_OK;
+}
+
+extern "C" int trk_route_scores(const float* logits, const float* bias, uint32_t m, uint32_t n_expert,
+                                const trk_score_policy* p, uint32_t* ids, float* w, uint32_t* n_sel, void* stream) {
+    if (!p) return fail(TRK_E_INVALID, "null argument");
+    if (n_expert == 0 || n_expert > 1024) return fail(TRK_E_INVALID, "n_expert (%u) must be in 1..1024", n_expert);
+    if (int rc = check_score_policy(p, n_expert)) return rc;
     if (m == 0) return TRK_OK;
     if (!logits || !ids || !w || !n_sel) return fail(TRK_E_INVALID, "null argument");
     const ScorePolicy sp{p->k, p->score, p->n_group, p->topk_group, p->group_top, p->renorm, p->factor};
@@ -1057,6 +1062,220 @@ extern "C" int trk_experts_down_i8(const trk_i8_mat* down, const int8_t* q, uint
     const int vec = (uintptr_t)y % (dtype == TRK_DT_F32 ? 16 : 8) == 0 && (m == 1 || ldy % 4 == 0);
     const I8Down a{i8_mat(*down), q, ldq, scale, m, slots, ids, n_sel, w, (float*)work, y, dtype, ldy, accumulate, vec};
     HIP_TRY(launch_experts_down(a, plan, (hipStream_t)stream));
+    return TRK_OK;
+}
+
+// ---- microscaled 4-bit rows ---------------------------------------------------------------------------
+
+constexpr uint32_t MX4_K_MAX = 1u << 30;  // places in a row are counted by 32 bits
+constexpr uint32_t MX4_SHARED_MAX = 32;
+
+static uint32_t mx4_blocks(uint32_t k) { return k / 32 + (k % 32 ? 1u : 0u); }
+
+static int check_mx4_k(uint32_t k, const char* what) {
+    if (k == 0 || k > MX4_K_MAX) return fail(TRK_E_INVALID, "%s: k (%u) must be in 1..%u", what, k, MX4_K_MAX);
+    return TRK_OK;
+}
+
+// Rows of k values, `one` of them: the strides then say nothing.
+static int check_mx4_rows(const void* q, uint64_t ld, const void* s, uint64_t lds, uint32_t k, bool one, const char* what) {
+    const uint64_t nb = mx4_blocks(k);
+    if ((uintptr_t)q % 16 || (!one && ld % 16)) return fail(TRK_E_INVALID, "%s: pointer and row stride must be multiples of 16", what);
+    if ((uintptr_t)s % 4 || (!one && lds % 4))
+        return fail(TRK_E_INVALID, "%s: the scales' pointer and row stride must be multiples of 4", what);
+    if (!one && ld < 16 * nb)
+        return fail(TRK_E_INVALID, "%s: row stride %llu below %llu bytes", what, (unsigned long long)ld, (unsigned long long)(16 * nb));
+    if (!one && lds < nb)
+        return fail(TRK_E_INVALID, "%s: the scales' row stride %llu below %llu blocks", what, (unsigned long long)lds,
+                    (unsigned long long)nb);
+    return TRK_OK;
+}
+
+static int check_mx4_mat(const trk_mx4_mat* w, const char* what) {
+    if (!w || !w->ptr || !w->scale) return fail(TRK_E_INVALID, "%s: null argument", what);
+    if (w->rows == 0 || w->k == 0 || w->count == 0) return fail(TRK_E_INVALID, "%s: empty matrix", what);
+    if (int rc = check_mx4_k(w->k, what)) return rc;
+    if (w->rows > I8_ROWS_MAX) return fail(TRK_E_INVALID, "%s: rows (%u) above %u", what, w->rows, I8_ROWS_MAX);
+    if (int rc = check_mx4_rows(w->ptr, w->ld, w->scale, w->scale_ld, w->k, w->rows == 1, what)) return rc;
+    if ((w->ld | w->scale_ld) >> 40) return fail(TRK_E_INVALID, "%s: row stride too large", what);
+    const uint64_t nb = mx4_blocks(w->k);
+    if (w->count > 1 && (w->stride % 16 || w->stride < (w->rows - 1ull) * (w->rows > 1 ? w->ld : 0) + 16 * nb))
+        return fail(TRK_E_INVALID, "%s: stride %llu is no multiple of 16 that holds a matrix", what, (unsigned long long)w->stride);
+    if (w->count > 1 && (w->scale_stride % 4 || w->scale_stride < (w->rows - 1ull) * (w->rows > 1 ? w->scale_ld : 0) + nb))
+        return fail(TRK_E_INVALID, "%s: the scales' stride %llu is no multiple of 4 that holds a matrix's", what,
+                    (unsigned long long)w->scale_stride);
+    return TRK_OK;
+}
+
+static Mx4Mat mx4_mat(const trk_mx4_mat& w) {
+    const bool one = w.rows == 1, many = w.count > 1;
+    return Mx4Mat{w.ptr, w.scale, one ? 0 : w.ld, one ? 0 : w.scale_ld, many ? w.stride : 0, many ? w.scale_stride : 0, w.rows,
+                  mx4_blocks(w.k), w.count};
+}
+
+extern "C" int trk_quantize_mx4(const void* x, uint32_t dtype, uint64_t ldx, uint32_t m, uint32_t k, uint8_t* q, uint64_t ldq,
+                                uint8_t* scale, uint64_t scale_ld, void* stream) {
+    int rc = check_dtype(dtype);
+    if (rc || (rc = check_elem_ptr(x, dtype, "x"))) return rc;
+    if ((rc = check_mx4_k(k, "x")) || (rc = check_mx4_rows(q, ldq, scale, scale_ld, k, m <= 1, "q"))) return rc;
+    if (m > 1 && ldx < k) return fail(TRK_E_INVALID, "row stride below k (%u)", k);
+    if (m == 0) return TRK_OK;
+    if (!x || !q || !scale) return fail(TRK_E_INVALID, "null argument");
+    HIP_TRY(launch_rows_mx4(false, dtype, x, ldx, m, k, q, ldq, scale, scale_ld, nullptr, 0, (hipStream_t)stream));
+    return TRK_OK;
+}
+
+extern "C" int trk_dequantize_mx4(const uint8_t* q, uint64_t ldq, const uint8_t* scale, uint64_t scale_ld, uint32_t m, uint32_t k,
+                                  void* y, uint32_t dtype, uint64_t ldy, void* stream) {
+    int rc = check_dtype(dtype);
+    if (rc || (rc = check_elem_ptr(y, dtype, "y"))) return rc;
+    if ((rc = check_mx4_k(k, "y")) || (rc = check_mx4_rows(q, ldq, scale, scale_ld, k, m <= 1, "q"))) return rc;
+    if (m > 1 && ldy < k) return fail(TRK_E_INVALID, "row stride below k (%u)", k);
+    if (m == 0) return TRK_OK;
+    if (!q || !scale || !y) return fail(TRK_E_INVALID, "null argument");
+    HIP_TRY(launch_rows_mx4(true, dtype, nullptr, 0, m, k, const_cast<uint8_t*>(q), ldq, const_cast<uint8_t*>(scale), scale_ld, y,
+                            ldy, (hipStream_t)stream));
+    return TRK_OK;
+}
+
+extern "C" int trk_gemm_mx4(const trk_mx4_mat* w, uint32_t item, const uint8_t* q, uint64_t ldq, const uint8_t* scale,
+                            uint64_t scale_ld, uint32_t m, const float* bias, void* y, uint32_t dtype, uint64_t ldy, int accumulate,
+                            void* stream) {
+    int rc = check_mx4_mat(w, "w");
+    if (rc) return rc;
+    if (item >= w->count) return fail(TRK_E_INVALID, "item %u out of range", item);
+    if ((rc = check_dtype(dtype)) || (rc = check_elem_ptr(y, dtype, "y"))) return rc;
+    if ((rc = check_mx4_rows(q, ldq, scale, scale_ld, w->k, m <= 1, "q"))) return rc;
+    if (m > 1 && ldy < w->rows) return fail(TRK_E_INVALID, "ldy %llu below rows (%u)", (unsigned long long)ldy, w->rows);
+    if (m > I8_ROWS_MAX) return fail(TRK_E_INVALID, "m (%u) above %u", m, I8_ROWS_MAX);
+    if (m == 0) return TRK_OK;
+    if (!q || !scale || !y) return fail(TRK_E_INVALID, "null argument");
+    Mx4Mat M = mx4_mat(*w);
+    M.q += item * M.stride, M.s += item * M.sstride;
+    const int vec = (uintptr_t)y % (dtype == TRK_DT_F32 ? 16 : 8) == 0 && (m == 1 || ldy % 4 == 0);
+    const Mx4Gemm a{M, Mx4X{q, scale, m == 1 ? 0 : ldq, m == 1 ? 0 : scale_ld}, m, bias, y, dtype, ldy, accumulate, vec};
+    HIP_TRY(launch_gemm_mx4(a, (hipStream_t)stream));
+    return TRK_OK;
+}
+
+static int check_same_shape(const trk_mx4_mat* gate, const trk_mx4_mat* up) {
+    if (gate->rows != up->rows || gate->k != up->k || gate->count != up->count)
+        return fail(TRK_E_INVALID, "gate [%u][%u][%u] and up [%u][%u][%u] differ in shape", gate->count, gate->rows, gate->k,
+                    up->count, up->rows, up->k);
+    return TRK_OK;
+}
+
+extern "C" int trk_experts_up_mx4(const trk_mx4_mat* gate, const trk_mx4_mat* up, const uint8_t* q, uint64_t ldq,
+                                  const uint8_t* scale, uint64_t scale_ld, uint32_t m, const uint32_t* ids, const uint32_t* n_sel,
+                                  uint32_t slots, const uint32_t* plan, void* h, uint32_t dtype, uint64_t ldh, void* stream) {
+    int rc = check_mx4_mat(gate, "gate");
+    if (rc || (rc = check_mx4_mat(up, "up")) || (rc = check_same_shape(gate, up))) return rc;
+    if ((rc = check_entries(m, slots, gate->count))) return rc;
+    if ((rc = check_dtype(dtype)) || (rc = check_elem_ptr(h, dtype, "h"))) return rc;
+    if ((rc = check_mx4_rows(q, ldq, scale, scale_ld, gate->k, m <= 1, "q"))) return rc;
+    if ((gate->rows + 15ull) / 16 * slots > 1ull << 32)  // workgroups of a token that takes its entries one by one
+        return fail(TRK_E_INVALID, "gate: rows * slots (%u * %u) too large", gate->rows, slots);
+    if (ldh < gate->rows) return fail(TRK_E_INVALID, "ldh %llu below rows (%u)", (unsigned long long)ldh, gate->rows);
+    if (m == 0) return TRK_OK;
+    if (!q || !scale || !ids || !n_sel || !h) return fail(TRK_E_INVALID, "null argument");
+    if ((rc = check_plan(plan, m, slots, gate->count))) return rc;
+    const int vec = (uintptr_t)h % (dtype == TRK_DT_F32 ? 16 : 8) == 0 && ldh % 4 == 0;
+    const Mx4Up a{mx4_mat(*gate), mx4_mat(*up), Mx4X{q, scale, m == 1 ? 0 : ldq, m == 1 ? 0 : scale_ld}, m, slots, ids, n_sel, h,
+                  dtype, ldh, vec};
+    HIP_TRY(launch_experts_up_mx4(a, plan, (hipStream_t)stream));
+    return TRK_OK;
+}
+
+extern "C" int trk_experts_down_mx4(const trk_mx4_mat* down, const uint8_t* q, uint64_t ldq, const uint8_t* scale, uint64_t scale_ld,
+                                    uint32_t m, const uint32_t* ids, const float* w, const uint32_t* n_sel, uint32_t slots,
+                                    const uint32_t* plan, void* work, void* y, uint32_t dtype, uint64_t ldy, int accumulate,
+                                    void* stream) {
+    int rc = check_mx4_mat(down, "down");
+    if (rc) return rc;
+    if ((rc = check_entries(m, slots, down->count))) return rc;
+    if ((rc = check_dtype(dtype)) || (rc = check_elem_ptr(y, dtype, "y"))) return rc;
+    if ((rc = check_mx4_rows(q, ldq, scale, scale_ld, down->k, (uint64_t)m * slots <= 1, "q"))) return rc;
+    if (m > 1 && ldy < down->rows) return fail(TRK_E_INVALID, "ldy %llu below rows (%u)", (unsigned long long)ldy, down->rows);
+    if (m == 0) return TRK_OK;
+    if (!q || !scale || !ids || !w || !n_sel || !y) return fail(TRK_E_INVALID, "null argument");
+    if ((rc = check_plan(plan, m, slots, down->count))) return rc;
+    if (plan && (!work || (uintptr_t)work % 16))
+        return fail(TRK_E_INVALID, "work must be 16-byte aligned memory of trk_experts_down_work_bytes");
+    const int vec = (uintptr_t)y % (dtype == TRK_DT_F32 ? 16 : 8) == 0 && (m == 1 || ldy % 4 == 0);
+    const bool one = (uint64_t)m * slots == 1;
+    const Mx4Down a{mx4_mat(*down), Mx4X{q, scale, one ? 0 : ldq, one ? 0 : scale_ld}, m, slots, ids, n_sel, w, (float*)work, y,
+                    dtype, ldy, accumulate, vec};
+    HIP_TRY(launch_experts_down_mx4(a, plan, (hipStream_t)stream));
+    return TRK_OK;
+}
+
+// The layer's stacks, and where its work area's parts begin (16-byte aligned each).
+static int check_moe_mx4(const trk_moe_mx4_w* w, uint32_t k, uint32_t m) {
+    if (!w) return fail(TRK_E_INVALID, "null argument");
+    int rc = check_mx4_mat(&w->gate, "gate");
+    if (rc || (rc = check_mx4_mat(&w->up, "up")) || (rc = check_mx4_mat(&w->down, "down"))) return rc;
+    if ((rc = check_same_shape(&w->gate, &w->up))) return rc;
+    if (w->down.count != w->gate.count || w->down.rows != w->gate.k || w->down.k != w->gate.rows)
+        return fail(TRK_E_INVALID, "down [%u][%u][%u] does not go back from gate [%u][%u][%u]", w->down.count, w->down.rows,
+                    w->down.k, w->gate.count, w->gate.rows, w->gate.k);
+    if (w->n_shared > MX4_SHARED_MAX) return fail(TRK_E_INVALID, "n_shared (%u) above %u", w->n_shared, MX4_SHARED_MAX);
+    if (w->n_shared >= w->gate.count || w->gate.count - w->n_shared > 1024)
+        return fail(TRK_E_INVALID, "n_expert (%lld) must be in 1..1024", (long long)w->gate.count - w->n_shared);
+    if (k < 1 || k > TRK_MOE_K_MAX || k > w->gate.count - w->n_shared)
+        return fail(TRK_E_POLICY, "score policy: k (%u) must be in 1..min(32, n_expert)", k);
+    if (m > TRK_EXPERTS_DIRECT_M)
+        return fail(TRK_E_CAPACITY, "m (%u) above %u: trk_experts_up_mx4 and trk_experts_down_mx4 take more", m, TRK_EXPERTS_DIRECT_M);
+    return TRK_OK;
+}
+
+struct MoeMx4Work {
+    uint64_t logits, shlog, ids, w, n_sel, h, bytes;
+};
+static MoeMx4Work moe_mx4_work(const trk_moe_mx4_w& w, uint32_t k, uint32_t m) {
+    uint64_t at = 0;
+    auto take = [&](uint64_t words) {
+        const uint64_t a = at;
+        at += (4 * words + 15) / 16 * 16;
+        return a;
+    };
+    MoeMx4Work o;
+    o.logits = take((uint64_t)m * (w.gate.count - w.n_shared)), o.shlog = take(m);
+    o.ids = take((uint64_t)m * TRK_MOE_K_MAX), o.w = take((uint64_t)m * TRK_MOE_K_MAX), o.n_sel = take(m);
+    o.h = take((uint64_t)m * (k + w.n_shared) * w.gate.rows);
+    o.bytes = at;
+    return o;
+}
+
+extern "C" int trk_moe_mx4_work_bytes(const trk_moe_mx4_w* w, uint32_t k, uint32_t m, uint64_t* bytes) {
+    if (!bytes) return fail(TRK_E_INVALID, "null argument");
+    if (int rc = check_moe_mx4(w, k, m)) return rc;
+    *bytes = moe_mx4_work(*w, k, m).bytes;
+    return TRK_OK;
+}
+
+extern "C" int trk_moe_mx4(const trk_moe_mx4_w* w, const trk_score_policy* p, const void* x, uint32_t xdtype, uint64_t ldx,
+                           const float* rlog, uint32_t m, void* work, void* y, uint32_t ydtype, uint64_t ldy, void* stream) {
+    if (!p) return fail(TRK_E_INVALID, "null argument");
+    int rc = check_moe_mx4(w, p->k, m);
+    if (rc) return rc;
+    const uint32_t E = w->gate.count - w->n_shared, H = w->gate.k;
+    if ((rc = check_score_policy(p, E))) return rc;
+    if ((rc = check_dtype(xdtype)) || (rc = check_elem_ptr(x, xdtype, "x"))) return rc;
+    if ((rc = check_dtype(ydtype)) || (rc = check_elem_ptr(y, ydtype, "y"))) return rc;
+    if (m > 1 && (ldx < H || ldy < H)) return fail(TRK_E_INVALID, "row stride below hidden (%u)", H);
+    if (m == 0) return TRK_OK;
+    if (!x || !y || !work) return fail(TRK_E_INVALID, "null argument");
+    if ((uintptr_t)work % 16) return fail(TRK_E_INVALID, "work must be 16-byte aligned memory of trk_moe_mx4_work_bytes");
+    if (!rlog && !w->router) return fail(TRK_E_INVALID, "neither a router nor logits");
+    const MoeMx4Work o = moe_mx4_work(*w, p->k, m);
+    char* b = (char*)work;
+    float* wl = (float*)(b + o.logits);
+    const Mx4Layer a{rlog ? nullptr : w->router, w->n_shared ? w->shared_gate : nullptr, mx4_mat(w->gate), mx4_mat(w->up),
+                     mx4_mat(w->down), E, w->n_shared, H, m, p->k + w->n_shared, x, xdtype, ldx, rlog ? rlog : wl, wl,
+                     (float*)(b + o.shlog), (uint32_t*)(b + o.ids), (uint32_t*)(b + o.n_sel), (float*)(b + o.w), (float*)(b + o.h),
+                     y, ydtype, ldy};
+    const ScorePolicy sp{p->k, p->score, p->n_group, p->topk_group, p->group_top, p->renorm, p->factor};
+    HIP_TRY(launch_moe_mx4(a, w->bias, sp, (hipStream_t)stream));
     return TRK_OK;
 }
 

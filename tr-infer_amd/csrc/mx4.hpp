@@ -1,0 +1,87 @@
+// Microscaled 4-bit rows and their products: what the kernels share.
+//
+// A row is blocks of 32 values: 16 bytes, two values a byte, the first in the low half, and a scale byte s that stands for
+// 2^(s - 127) (255: NaN).  A value is a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6.  The matrix instructions take both as they
+// are: a lane's operand is one block of one row and its scale byte, and sum_32 a b 2^(sa + sb - 254) of the blocks goes into the 32-bit
+// sum.  Which of the instruction's k a block stands for does not matter as long as both operands agree, so a lane may hold any.
+//
+// Products of two 4-bit values have at most six bits, a block's sum of them eleven: only adding blocks rounds.
+#pragma once
+
+#include "i8.hpp"
+
+namespace trk {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr uint32_t MX_BLOCK = 32, MX_ONE = 127;  // values of a block; the scale byte of 1
+constexpr int MX_FP4 = 4;                        // the operands' format
+
+__host__ __device__ inline uint32_t mx_blocks(uint32_t k) { return k / MX_BLOCK + (k % MX_BLOCK ? 1u : 0u); }
+
+__device__ __forceinline__ i32x8 mx_operand(i32x4 v) { return i32x8{v[0], v[1], v[2], v[3], 0, 0, 0, 0}; }
+
+// C += A B: lane l holds a block of A's row l % 16 and of B's column l % 16, the four lane groups four blocks; rows 4 (l / 16)
+// .. + 3 of C's column l % 16.
+__device__ __forceinline__ f32x4 mfma_mx4(i32x4 a, uint32_t sa, i32x4 b, uint32_t sb, f32x4 c) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(a), mx_operand(b), c, MX_FP4, MX_FP4, 0, (int)sa, 0, (int)sb);
+}
+
+// 2^(s - 127), NaN for 255
+__device__ __forceinline__ float mx_scale(uint32_t s) {
+    return s == 255u ? __builtin_nanf("") : s ? __uint_as_float(s << 23) : 0x1p-127f;
+}
+
+// A lane's row of a stack of 4-bit matrices
+struct Mx4Row {
+    const uint8_t *q, *s;
+};
+
+// U groups of four blocks of NM matrices' rows and of an activation row, all requested before the first is needed.
+template <uint32_t U, uint32_t NM>
+__device__ __forceinline__ void mx4_pieces(const Mx4Row (&w)[NM], Mx4Row x, uint32_t at, uint32_t step, uint32_t g, f32x4 (&acc)[NM]) {
+    i32x4 wq[NM][U], xq[U];
+    uint32_t ws[NM][U], xs[U];
+#pragma unroll
+    for (uint32_t u = 0; u < U; u++) {
+        const uint64_t b = 4ull * (at + u * step) + g;
+        xq[u] = *reinterpret_cast<const i32x4*>(x.q + 16 * b);
+        xs[u] = x.s[b];
+#pragma unroll
+        for (uint32_t i = 0; i < NM; i++) wq[i][u] = *reinterpret_cast<const i32x4*>(w[i].q + 16 * b), ws[i][u] = w[i].s[b];
+    }
+    __builtin_amdgcn_sched_barrier(0);  // else some wait for others' registers
+#pragma unroll
+    for (uint32_t u = 0; u < U; u++)
+#pragma unroll
+        for (uint32_t i = 0; i < NM; i++) acc[i] = mfma_mx4(wq[i][u], ws[i][u], xq[u], xs[u], acc[i]);
+}
+
+// The sums of 16 weight rows of NM matrices and 16 activation rows over this wave's share of K (nb blocks a row): every `step`-th
+// four blocks from the first-th on.  w, x: this lane's row of each (row lane % 16).
+template <uint32_t NM>
+__device__ __forceinline__ void mx4_strip(const Mx4Row (&w)[NM], Mx4Row x, uint32_t nb, uint32_t first, uint32_t step, uint32_t lane,
+                                          f32x4 (&acc)[NM]) {
+#pragma unroll
+    for (uint32_t i = 0; i < NM; i++) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const uint32_t g = lane / 16, whole = nb / 4;
+    uint32_t n = first < whole ? (whole - first + step - 1) / step : 0, at = first;  // whole groups of this wave
+    for (; n >= 8; n -= 8, at += 8 * step) mx4_pieces<8, NM>(w, x, at, step, g, acc);
+    if (n & 4) mx4_pieces<4, NM>(w, x, at, step, g, acc), at += 4 * step;
+    if (n & 2) mx4_pieces<2, NM>(w, x, at, step, g, acc), at += 2 * step;
+    if (n & 1) mx4_pieces<1, NM>(w, x, at, step, g, acc);
+    if (nb % 4 && whole % step == first) {  // the row's end: lanes past it multiply zeros, by 1
+        const bool in = g < nb % 4;
+        const uint64_t b = in ? 4ull * whole + g : 0;
+        const i32x4 xl = *reinterpret_cast<const i32x4*>(x.q + 16 * b);
+        const uint32_t xs = in ? x.s[b] : MX_ONE;
+#pragma unroll
+        for (uint32_t i = 0; i < NM; i++) {
+            const i32x4 wl = *reinterpret_cast<const i32x4*>(w[i].q + 16 * b);
+            acc[i] = mfma_mx4(wl, in ? w[i].s[b] : MX_ONE, in ? xl : i32x4{0, 0, 0, 0}, xs, acc[i]);
+        }
+    }
+}
+
+}  // namespace trk

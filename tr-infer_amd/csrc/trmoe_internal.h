@@ -301,6 +301,69 @@ hipError_t launch_experts_plan(const uint32_t* ids, const uint32_t* n_sel, uint3
                                uint32_t* plan, hipStream_t st);
 hipError_t launch_experts_up(const I8Up& a, const uint32_t* plan, hipStream_t st);
 hipError_t launch_experts_down(const I8Down& a, const uint32_t* plan, hipStream_t st);
+// microscaled 4-bit rows and products (k_mx4.hip; the experts' k_mx4x.hip; the layer for a few tokens k_mx4l.hip)
+struct Mx4Mat {
+    const uint8_t *q, *s;
+    uint64_t ld, lds, stride, sstride;  // bytes from row to row and matrix to matrix, of the values and of the scales
+    uint32_t rows, nb, count;           // nb: blocks of a row
+};
+struct Mx4X {
+    const uint8_t *q, *s;
+    uint64_t ld, lds;
+};
+struct Mx4Gemm {
+    Mx4Mat w;  // the one matrix
+    Mx4X x;
+    uint32_t m;
+    const float* bias;
+    void* y;
+    uint32_t dt;
+    uint64_t ldy;
+    int accumulate, vec;  // vec: four neighbouring outputs lie on a boundary of four
+};
+struct Mx4Up {
+    Mx4Mat gate, up;
+    Mx4X x;
+    uint32_t m, slots;
+    const uint32_t *ids, *n_sel;
+    void* h;
+    uint32_t dt;
+    uint64_t ldh;
+    int vec;
+};
+struct Mx4Down {
+    Mx4Mat down;
+    Mx4X x;
+    uint32_t m, slots;
+    const uint32_t *ids, *n_sel;
+    const float* w;
+    float* work;
+    void* y;
+    uint32_t dt;
+    uint64_t ldy;
+    int accumulate, vec;
+};
+struct Mx4Layer {
+    const float *router, *shared_gate;  // either may be null
+    Mx4Mat gate, up, down;
+    uint32_t n_expert, n_shared, hidden, m, slots;  // slots: routed and shared
+    const void* x;
+    uint32_t xdt;
+    uint64_t ldx;
+    const float* logits;  // [m][n_expert]: the caller's, or what the router's launch writes
+    float *wlogits, *shlog;
+    uint32_t *ids, *n_sel;
+    float *w, *h;
+    void* y;
+    uint32_t ydt;
+    uint64_t ldy;
+};
+hipError_t launch_rows_mx4(bool back, uint32_t dt, const void* x, uint64_t ldx, uint32_t m, uint32_t k, uint8_t* q, uint64_t ldq,
+                           uint8_t* s, uint64_t lds, void* y, uint64_t ldy, hipStream_t st);
+hipError_t launch_gemm_mx4(const Mx4Gemm& a, hipStream_t st);
+hipError_t launch_experts_up_mx4(const Mx4Up& a, const uint32_t* plan, hipStream_t st);
+hipError_t launch_experts_down_mx4(const Mx4Down& a, const uint32_t* plan, hipStream_t st);
+hipError_t launch_moe_mx4(const Mx4Layer& a, const float* bias, const ScorePolicy& p, hipStream_t st);
 hipError_t launch_swiglu(const float* g, const float* u, float* y, size_t n, hipStream_t st);
 hipError_t launch_rmsnorm(const float* x, const float* w, float eps, uint32_t m, uint32_t n, float* y,
                           hipStream_t st);

@@ -63,6 +63,19 @@ class I8Mat(C.Structure):
                 ("count", C.c_uint32), ("ld", C.c_uint64), ("stride", C.c_uint64)]
 
 
+class Mx4Mat(C.Structure):
+    """trk_mx4_mat: a stack of 4-bit matrices with a power of two for each 32 values of a row."""
+    _fields_ = [("ptr", C.c_void_p), ("scale", C.c_void_p), ("rows", C.c_uint32), ("k", C.c_uint32),
+                ("count", C.c_uint32), ("ld", C.c_uint64), ("stride", C.c_uint64), ("scale_ld", C.c_uint64),
+                ("scale_stride", C.c_uint64)]
+
+
+class MoeMx4W(C.Structure):
+    """trk_moe_mx4_w: a MoE layer on 4-bit experts."""
+    _fields_ = [("router", C.c_void_p), ("bias", C.c_void_p), ("shared_gate", C.c_void_p), ("gate", Mx4Mat),
+                ("up", Mx4Mat), ("down", Mx4Mat), ("n_shared", C.c_uint32)]
+
+
 class Cfg(C.Structure):
     _fields_ = [("hidden", C.c_uint32), ("n_expert", C.c_uint32), ("n_ff", C.c_uint32),
                 ("n_expert_used", C.c_uint32), ("m_max", C.c_uint32), ("k_cap", C.c_uint32),
@@ -112,6 +125,15 @@ def lib() -> C.CDLL:
         L.trk_experts_down_work_bytes.argtypes = [u32, u32, u32, u32, C.POINTER(u64)]
         L.trk_experts_down_i8.argtypes = [C.POINTER(I8Mat), vp, u64, vp, u32, vp, vp, vp, u32, vp, vp, vp, u32, u64, i,
                                           vp]
+        L.trk_quantize_mx4.argtypes = [vp, u32, u64, u32, u32, vp, u64, vp, u64, vp]
+        L.trk_dequantize_mx4.argtypes = [vp, u64, vp, u64, u32, u32, vp, u32, u64, vp]
+        L.trk_gemm_mx4.argtypes = [C.POINTER(Mx4Mat), u32, vp, u64, vp, u64, u32, vp, vp, u32, u64, i, vp]
+        L.trk_experts_up_mx4.argtypes = [C.POINTER(Mx4Mat), C.POINTER(Mx4Mat), vp, u64, vp, u64, u32, vp, vp, u32, vp, vp,
+                                         u32, u64, vp]
+        L.trk_experts_down_mx4.argtypes = [C.POINTER(Mx4Mat), vp, u64, vp, u64, u32, vp, vp, vp, u32, vp, vp, vp, u32, u64,
+                                           i, vp]
+        L.trk_moe_mx4_work_bytes.argtypes = [C.POINTER(MoeMx4W), u32, u32, C.POINTER(u64)]
+        L.trk_moe_mx4.argtypes = [C.POINTER(MoeMx4W), C.POINTER(ScorePolicy), vp, u32, u64, vp, u32, vp, vp, u32, u64, vp]
         L.trk_swiglu.argtypes = [vp, vp, vp, sz, vp]
         L.trk_rmsnorm.argtypes = [vp, vp, f, u32, u32, vp, vp]
         L.trk_add_inplace.argtypes = [vp, vp, sz, vp]
@@ -856,6 +878,268 @@ def experts_down_i8(down: I8Weights, q, scale, ids, w, n_sel, slots, plan=None, 
     check(lib().trk_experts_down_i8(down.ref, q.data_ptr(), ldq, scale.data_ptr(), m, ids.data_ptr(), w.data_ptr(),
                                     n_sel.data_ptr(), slots, _ptr(plan), _ptr(work), out.data_ptr(), _dtype(out.dtype),
                                     ldy, int(accumulate), _stream_here(stream)))
+    return out
+
+
+# ---- microscaled 4-bit rows ----------------------------------------------------------------------
+#
+# Values uint8 [..][16 * blocks], two a byte, and scales uint8 [..][blocks], a block 32 values of a row: as the calls above in
+# all else.
+
+MX4_BLOCK = 32
+
+
+def _mx4_blocks(k):
+    return (k + MX4_BLOCK - 1) // MX4_BLOCK
+
+
+def _mx4_rows(q, scale, m, k, what):
+    """The strides between the rows of 4-bit values and of their scales, for [m][k]."""
+    torch = _torch or _late()
+    nb = _mx4_blocks(k)
+    if q.dtype != torch.uint8 or scale.dtype != torch.uint8:
+        raise TrkError(f"{what}: uint8 values and scales are needed, not {q.dtype} and {scale.dtype}")
+    if q.shape != (m, 16 * nb) or scale.shape != (m, nb):
+        raise TrkError(f"{what}: values [{m}][{16 * nb}] and scales [{m}][{nb}] are needed for k = {k}, not {tuple(q.shape)} "
+                       f"and {tuple(scale.shape)}")
+    (a, b), (c, d) = q.stride(), scale.stride()
+    if b != 1 or (d != 1 and nb > 1):
+        raise TrkError(f"{what}: the bytes of a row have to be contiguous")
+    if m <= 1:
+        a, c = 16 * nb, (nb + 3) // 4 * 4
+    if nb % 4 and m:
+        _whole_scales(scale, (m - 1) * c, nb, what)
+    return a, c
+
+
+def _whole_scales(scale, last, nb, what):
+    """The last row's last 4-byte piece lies inside the tensor's storage."""
+    if scale.storage_offset() + last + (nb + 3) // 4 * 4 > scale.untyped_storage().nbytes():
+        raise TrkError(f"{what}: scales are read in 4-byte pieces, and the storage ends inside the last one")
+
+
+class MX4Weights:
+    """A stack of 4-bit matrices (trk_mx4_mat): q uint8 [count][rows][16 * blocks] or [rows][16 * blocks], its rows and matrices
+    a multiple of 16 bytes apart, scale uint8 [count][rows][blocks] or [rows][blocks], a multiple of 4 (`quantize_weights_mx4`
+    makes them so); k: values of a row.  Keeps the tensors; copies nothing."""
+
+    def __init__(self, q, scale, k):
+        torch = _torch or _late()
+        nb = _mx4_blocks(k)
+        if q.dtype != torch.uint8 or scale.dtype != torch.uint8 or q.dim() not in (2, 3):
+            raise TrkError(f"weights: uint8 [count][rows][16 * blocks] or [rows][16 * blocks] and as many scales are needed, not "
+                           f"{q.dtype} {tuple(q.shape)} and {scale.dtype}")
+        if k < 1 or q.shape[-1] != 16 * nb or scale.shape != (*q.shape[:-1], nb):
+            raise TrkError(f"weights: values [..][{16 * nb}] and scales [..][{nb}] are needed for k = {k}, not {tuple(q.shape)} and "
+                           f"{tuple(scale.shape)}")
+        if min(q.shape) == 0:
+            raise TrkError(f"weights: empty shape {tuple(q.shape)}")
+        _u32(*q.shape, k)
+        if q.stride(-1) != 1 or (scale.stride(-1) != 1 and nb > 1):
+            raise TrkError("weights: the bytes of a row have to be contiguous")
+        _here(q, scale)
+        self.q, self.scale, self.k = q, scale, k
+        self.count = q.shape[0] if q.dim() == 3 else 1
+        self.rows = q.shape[-2]
+        many = self.count > 1
+        ld, sld = (q.stride(-2), scale.stride(-2)) if self.rows > 1 else (16 * nb, (nb + 3) // 4 * 4)
+        stride, sstride = (q.stride(0), scale.stride(0)) if many else (0, 0)
+        if nb % 4:
+            _whole_scales(scale, sstride * (self.count - 1) + sld * (self.rows - 1), nb, "weights")
+        self.mat = Mx4Mat(q.data_ptr(), scale.data_ptr(), self.rows, k, self.count, ld, stride, sld, sstride)
+        self.ref = C.byref(self.mat)
+        self.device = q.get_device()
+
+
+def _mx4_empty(torch, m, k, device):
+    """4-bit rows and scales [m][blocks], the scales' rows a multiple of 4 bytes apart."""
+    nb = _mx4_blocks(k)
+    q = torch.empty((m, 16 * nb), dtype=torch.uint8, device=device)
+    if nb % 4 == 0:
+        return q, q.new_empty((m, nb))
+    return q, q.new_empty((m, (nb + 3) // 4 * 4))[:, :nb]
+
+
+def quantize_mx4(x, out=None, stream=None):
+    """trk_quantize_mx4: x [m][k] -> (q uint8 [m][16 * blocks], scale uint8 [m][blocks])."""
+    torch = _torch or _late()
+    ldx = _rows(x, "x")
+    m, k = x.shape
+    q, scale = _mx4_empty(torch, m, k, x.device) if out is None else out
+    ldq, lds = _mx4_rows(q, scale, m, k, "q")
+    _here(x, q, scale)
+    check(lib().trk_quantize_mx4(x.data_ptr(), _dtype(x.dtype), ldx, m, k, q.data_ptr(), ldq, scale.data_ptr(), lds,
+                                 _stream_here(stream)))
+    return q, scale
+
+
+def dequantize_mx4(q, scale, k, dtype=None, out=None, stream=None):
+    """trk_dequantize_mx4: 4-bit rows of k values -> [m][k] (float32 unless `dtype` or `out` says otherwise)."""
+    torch = _torch or _late()
+    m = q.shape[0]
+    _u32(m, k)
+    ldq, lds = _mx4_rows(q, scale, m, k, "q")
+    if out is None:
+        out = torch.empty((m, k), dtype=dtype or torch.float32, device=q.device)
+    ldy = _rows(out, "out", m, k)
+    _here(q, scale, out)
+    check(lib().trk_dequantize_mx4(q.data_ptr(), ldq, scale.data_ptr(), lds, m, k, out.data_ptr(), _dtype(out.dtype), ldy,
+                                   _stream_here(stream)))
+    return out
+
+
+def quantize_weights_mx4(w, stream=None):
+    """float [count][rows][k] or [rows][k] -> MX4Weights: each row quantised as `quantize_mx4` does."""
+    if stream is None:
+        flat = w.reshape(-1, w.shape[-1])
+    else:
+        with (_torch or _late()).cuda.stream(stream):  # a copy, where the rows make no one matrix: made and given back there
+            flat = w.reshape(-1, w.shape[-1])
+    q, s = quantize_mx4(flat, stream=stream)
+    lead = w.shape[:-1]
+
+    def shaped(t):
+        return t.as_strided((*lead, t.shape[1]), (*[t.stride(0) * lead[-1]] * (len(lead) - 1), t.stride(0), 1))
+    return MX4Weights(shaped(q), shaped(s), w.shape[-1])
+
+
+def gemm_mx4(w: MX4Weights, q, scale, bias=None, dtype=None, out=None, accumulate=False, item=0, stream=None):
+    """trk_gemm_mx4: 4-bit rows [m] times matrix `item` of w -> [m][rows] (float32 unless `dtype` or `out` says otherwise)."""
+    torch = _torch or _late()
+    m = q.shape[0]
+    if not 0 <= item < w.count:
+        raise TrkError(f"item {item} out of range")
+    _u32(m)
+    ldq, lds = _mx4_rows(q, scale, m, w.k, "q")
+    if bias is not None:
+        _vector(bias, "bias", torch.float32, w.rows)
+    if out is None:
+        if accumulate:
+            raise TrkError("accumulate needs the output that is added to")
+        out = torch.empty((m, w.rows), dtype=dtype or torch.float32, device=q.device)
+        ldy = w.rows
+    else:
+        ldy = _rows(out, "out", m, w.rows)
+    _here(q, scale, bias, out, w.q)
+    check(lib().trk_gemm_mx4(w.ref, item, q.data_ptr(), ldq, scale.data_ptr(), lds, m, _ptr(bias), out.data_ptr(),
+                             _dtype(out.dtype), ldy, int(accumulate), _stream_here(stream)))
+    return out
+
+
+def experts_up_mx4(gate: MX4Weights, up: MX4Weights, q, scale, ids, n_sel, slots, plan=None, dtype=None, out=None, stream=None):
+    """trk_experts_up_mx4: 4-bit rows [m] through each token's experts -> h [m * slots][F]; rows that are no entry's are not
+    written."""
+    torch = _torch or _late()
+    m = q.shape[0]
+    ldq, lds = _mx4_rows(q, scale, m, gate.k, "q")
+    _routing(ids, n_sel, m)
+    _check_plan(plan, m, slots, gate.count)
+    if out is None:
+        out = torch.empty((m * slots, gate.rows), dtype=dtype or torch.float32, device=q.device)
+        ldh = gate.rows
+    else:
+        ldh = _rows(out, "out", m * slots, gate.rows)
+    _here(q, scale, ids, n_sel, plan, out, gate.q, up.q)
+    check(lib().trk_experts_up_mx4(gate.ref, up.ref, q.data_ptr(), ldq, scale.data_ptr(), lds, m, ids.data_ptr(),
+                                   n_sel.data_ptr(), slots, _ptr(plan), out.data_ptr(), _dtype(out.dtype), ldh,
+                                   _stream_here(stream)))
+    return out
+
+
+def experts_down_mx4(down: MX4Weights, q, scale, ids, w, n_sel, slots, plan=None, dtype=None, out=None, work=None,
+                     accumulate=False, stream=None):
+    """trk_experts_down_mx4: 4-bit rows [m * slots] through the experts' down rows, weighted with w and summed per token ->
+    [m][H].  work: at least trk_experts_down_work_bytes as a float32 tensor, allocated where it is not given."""
+    torch = _torch or _late()
+    m = ids.shape[0]
+    ldq, lds = _mx4_rows(q, scale, m * slots, down.k, "q")
+    _routing(ids, n_sel, m, w)
+    _check_plan(plan, m, slots, down.count)
+    if out is None:
+        if accumulate:
+            raise TrkError("accumulate needs the output that is added to")
+        out = torch.empty((m, down.rows), dtype=dtype or torch.float32, device=q.device)
+        ldy = down.rows
+    else:
+        ldy = _rows(out, "out", m, down.rows)
+    need = _down_work(m, slots, down.count, down.rows) if m > EXPERTS_DIRECT_M else 0
+    work = _work_of(torch, work, need, q.device, stream)
+    _here(q, scale, ids, w, n_sel, plan, work, out, down.q)
+    check(lib().trk_experts_down_mx4(down.ref, q.data_ptr(), ldq, scale.data_ptr(), lds, m, ids.data_ptr(), w.data_ptr(),
+                                     n_sel.data_ptr(), slots, _ptr(plan), _ptr(work), out.data_ptr(), _dtype(out.dtype), ldy,
+                                     int(accumulate), _stream_here(stream)))
+    return out
+
+
+def _work_of(torch, work, need, device, stream):
+    """`work` checked, or memory of `need` float32 values for this call."""
+    if work is None:
+        if need:
+            work = torch.empty(need, dtype=torch.float32, device=device)
+            if stream is not None:
+                work.record_stream(stream)  # given back on return, while that stream still works on it
+    elif work.dtype != torch.float32 or not work.is_contiguous() or work.numel() < need:
+        raise TrkError(f"work: {need} contiguous float32 values are needed")
+    return work
+
+
+class MX4Layer:
+    """A MoE layer on 4-bit experts (trk_moe_mx4_w): gate / up / down MX4Weights of the routed experts, then n_shared that every
+    token takes; router float32 [E][H] (None where each call brings its logits), bias float32 [E] of the choice, shared_gate
+    float32 [H].  Keeps the tensors; copies nothing."""
+
+    def __init__(self, gate: MX4Weights, up: MX4Weights, down: MX4Weights, router=None, bias=None, n_shared=0, shared_gate=None):
+        torch = _torch or _late()
+        if not 0 <= n_shared < gate.count:
+            raise TrkError(f"n_shared ({n_shared}) must leave routed experts of {gate.count}")
+        self.n_expert, self.hidden = gate.count - n_shared, gate.k
+        for t, what, shape in ((router, "router", (self.n_expert, self.hidden)), (bias, "bias", (self.n_expert,)),
+                               (shared_gate, "shared_gate", (self.hidden,))):
+            if t is not None:
+                _vector(t, what, torch.float32, *shape)
+        _here(router, bias, shared_gate, gate.q, up.q, down.q)
+        self.gate, self.up, self.down, self.n_shared = gate, up, down, n_shared
+        self.router, self.bias, self.shared_gate = router, bias, shared_gate
+        self.w = MoeMx4W(_ptr(router), _ptr(bias), _ptr(shared_gate), gate.mat, up.mat, down.mat, n_shared)
+        self.ref = C.byref(self.w)
+        self._work = {}
+
+    def work_values(self, k, m):
+        """float32 values of trk_moe_mx4's work."""
+        n = self._work.get((k, m))
+        if n is None:
+            n = C.c_uint64()
+            _u32(k, m)
+            check(lib().trk_moe_mx4_work_bytes(self.ref, k, m, C.byref(n)))
+            n = self._work[k, m] = n.value // 4
+        return n
+
+
+def moe_mx4(layer: MX4Layer, x, k, rlog=None, score="sigmoid", n_group=1, topk_group=1, group_top=2, renorm=True, factor=1.0,
+            dtype=None, out=None, work=None, stream=None):
+    """trk_moe_mx4: x [m][H] of up to EXPERTS_DIRECT_M tokens through the layer, k experts a token chosen as `route_scores` does
+    -> [m][H] (x's type unless `dtype` or `out` says otherwise).  rlog: float32 [m][E], the router's logits.  work: at least
+    layer.work_values(k, m) float32 values, allocated where it is not given."""
+    torch = _torch or _late()
+    H = layer.hidden
+    ldx = _rows(x, "x", k=H)
+    m = x.shape[0]
+    if rlog is not None:
+        _vector(rlog, "rlog", torch.float32, m, layer.n_expert)
+    elif layer.router is None:
+        raise TrkError("the layer has no router: rlog is needed")
+    if score not in SCORES:
+        raise TrkError(f"score {score!r}: softmax or sigmoid")
+    p = _score_policy(k, SCORES[score], n_group, topk_group, group_top, int(renorm), factor)
+    if out is None:
+        out = torch.empty((m, H), dtype=dtype or x.dtype, device=x.device)
+        ldy = H
+    else:
+        ldy = _rows(out, "out", m, H)
+    work = _work_of(torch, work, layer.work_values(k, m), x.device, stream)
+    _here(x, rlog, work, out, layer.gate.q)
+    check(lib().trk_moe_mx4(layer.ref, p, x.data_ptr(), _dtype(x.dtype), ldx, _ptr(rlog), m, _ptr(work), out.data_ptr(),
+                            _dtype(out.dtype), ldy, _stream_here(stream)))
     return out
 
 
