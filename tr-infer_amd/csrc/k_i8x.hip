@@ -1,5 +1,6 @@
 // The int8 products of each token with its experts (trk_experts_plan, trk_experts_up_i8, trk_experts_down_i8).
 #include "i8tile.hpp"
+#include "plan.hpp"
 
 namespace trk {
 
@@ -8,8 +9,6 @@ namespace {
 // ============================================================================================
 // the plan: entries sorted by expert
 // ============================================================================================
-
-constexpr uint32_t PLAN_T = 1024;  // threads, and the most experts
 
 // The expert of entry i, ~0 for a slot that is none.
 __device__ __forceinline__ uint32_t entry_expert(const uint32_t* __restrict__ ids, const uint32_t* __restrict__ n_sel,
@@ -184,36 +183,6 @@ __global__ __launch_bounds__(DOWN_WAVES* WAVE) void experts_down_strip_kernel(I8
 // ============================================================================================
 // many entries: tiles of one expert's
 // ============================================================================================
-
-// Whether a plan is one for these sizes: its entries are then below m * slots, and its tiles fit the launch.  One made for more
-// experts is where each entry may have a tile of its own.  Nothing is read through another; what would be written is NaN.
-__device__ __forceinline__ bool plan_fits(const PlanHead& h, uint32_t m, uint32_t slots, uint32_t E) {
-    return h.m == m && h.slots == slots && (h.E == E || (h.E > E && h.E <= PLAN_T && m * slots <= E));
-}
-
-// A tile's place: entries of one expert (the plan's tile) x a block of weight rows, the blocks of a tile next to one
-// another and each expert's tiles in turn on one XCD, whose L2 then holds the entries' rows and the expert's weights.
-// E: the stack's experts.  No plan made for it names others; of a plan made for more they are passed over, like ids.
-__device__ __forceinline__ bool expert_tile(const Plan& P, const PlanHead& h, uint32_t E, uint32_t blocks, PlanTile& t,
-                                            uint32_t& block) {
-    uint32_t idx;
-    if (!xcd_order_1d(h.n_tiles * blocks, idx, run_id())) return false;
-    t = P.tile[idx / blocks], block = idx % blocks;
-    return t.expert < E;
-}
-
-// NaN into every entry's row of y [m * slots][rows], the workgroups taking them in turn
-template <uint32_t DT, typename A>
-__device__ __forceinline__ void nan_rows(const A& a, uint32_t count, void* y, uint32_t rows, uint64_t ldy) {
-    typedef Elem<DT> O;
-    const uint32_t n = a.m * a.slots;
-    for (uint64_t i = run_id(); i < n; i += (uint64_t)gridDim.x * gridDim.y) {
-        const uint32_t t = (uint32_t)i / a.slots, j = (uint32_t)i % a.slots;
-        if (j >= a.n_sel[t] || a.ids[(size_t)t * K_MAX + j] >= count) continue;
-        for (uint64_t r = threadIdx.x; r < rows; r += blockDim.x)
-            reinterpret_cast<typename O::T*>(y)[i * ldy + r] = O::put(__builtin_nanf(""));
-    }
-}
 
 // gate and up: a tile's weight rows are BN / 2 rows of gate, then the same rows of up, and a wave has both of each.  ONCE:
 // geo::experts_once.  2000 tokens of 8 in 128 (H = 2048, F = 768; 432 MB, 101 G operations) 115 us; 4096 of 10 in 512 (F = 512;
@@ -516,7 +485,10 @@ hipError_t launch_experts_down(const I8Down& a, const uint32_t* plan, hipStream_
         narrow ? launch_down_tile<I8Tile<64, 128, 32, 64, 3>, false>(a, P, tiles, st)
                : launch_down_tile<I8Tile<128, 128, 64, 64, 2>, false>(a, P, tiles, st);
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    return e != hipSuccess ? e : launch_experts_combine(a, st);
+}
+
+hipError_t launch_experts_combine(const I8Down& a, hipStream_t st) {
     const uint32_t q = (a.down.rows + 3) / 4, per = q < 256 ? 256 / q : 1;
     const dim3 g = run_of((uint64_t)((q + 255) / 256) * ((a.m + per - 1) / per), 256);
     if (a.dt == TRK_DT_F32)

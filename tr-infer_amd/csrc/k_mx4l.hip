@@ -161,6 +161,7 @@ __global__ __launch_bounds__(LU_WAVES* WAVE) void layer_up_kernel(Mx4Layer a) {
             u = parts.mul(i * LU_WAVES + wv, lane, uq[i].q, uq[i].s, u);
         }
     }
+    mx_here(g), mx_here(u);
     if (lane % 16 < P) {
         *reinterpret_cast<f32x4*>(&part[0][wv][lane % 16][lane / 16 * 4]) = g;
         *reinterpret_cast<f32x4*>(&part[1][wv][lane % 16][lane / 16 * 4]) = u;
@@ -217,6 +218,7 @@ __global__ __launch_bounds__(LD_WAVES* WAVE) void layer_down_kernel(Mx4Layer a) 
                 acc = parts.mul(i, lane, wq[i].q, wq[i].s, acc);
             }
         }
+        mx_here(acc);
         if (lane % 16 < P) *reinterpret_cast<f32x4*>(&part[j][lane % 16][lane / 16 * 4]) = acc;
     }
     __syncthreads();

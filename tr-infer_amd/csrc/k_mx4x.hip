@@ -1,5 +1,6 @@
 // The microscaled 4-bit products of each token with its experts (trk_experts_up_mx4, trk_experts_down_mx4).
-#include "mx4.hpp"
+#include "mx4tile.hpp"
+#include "plan.hpp"
 
 namespace trk {
 
@@ -93,6 +94,130 @@ __global__ __launch_bounds__(DOWN_WAVES* WAVE) void experts_down_mx4_strip_kerne
     *y = O::put(a.accumulate ? O::get(*y) + v : v);
 }
 
+// ============================================================================================
+// many entries: tiles of one expert's
+// ============================================================================================
+
+// What a tile loads: for its BN weight rows, the first `split` of one matrix and the rest of another (or the same), and for its
+// activation rows, `row(i)` of all.
+struct Mx4Side {
+    i32x4 q, s;
+    uint32_t ld, lds;
+};
+__device__ __forceinline__ Mx4Side mx4_side(const Mx4Mat& w, uint32_t e, uint64_t r0) {
+    return Mx4Side{buffer_at((const int8_t*)w.q + e * w.stride + r0 * w.ld), buffer_at((const int8_t*)w.s + e * w.sstride + r0 * w.lds),
+                   (uint32_t)w.ld, (uint32_t)w.lds};
+}
+template <typename Tile, bool ONCE, typename Row>
+__device__ __forceinline__ void mx4_expert_run(Tile& t, uint8_t* lds, const Mx4Side& w0, const Mx4Side& w1, uint32_t split, uint32_t last,
+                                               const Mx4X& x, Row&& row, uint32_t nb, uint32_t live, uint32_t a0, uint32_t astep) {
+    i32x4 rw[Tile::NA], rs[Tile::NS];
+    uint32_t wo[Tile::NA], xo[Tile::NB], so[Tile::NS];
+    const i32x4 bx = buffer_at((const int8_t*)x.q), bxs = buffer_at((const int8_t*)x.s);
+#pragma unroll
+    for (int i = 0; i < Tile::NB; i++) xo[i] = row(t.load_row(i)) * (uint32_t)x.ld;
+#pragma unroll
+    for (int i = 0; i < Tile::NA; i++) {
+        const bool two = (i * Tile::NW + t.wv) * 8 >= split;
+        const uint32_t r = t.load_row(i) - (two ? split : 0), rc = r < last ? r : last;
+        rw[i] = two ? w1.q : w0.q, wo[i] = rc * (two ? w1.ld : w0.ld);
+    }
+#pragma unroll
+    for (int i = 0; i < Tile::NS; i++) {
+        const uint32_t p = t.scale_piece(i) * 32, n = t.lane / 2;
+        const bool mine = p >= Tile::BN, two = !mine && p >= split;
+        if (mine) {
+            rs[i] = bxs, so[i] = row(p - Tile::BN + n) * (uint32_t)x.lds;
+        } else {
+            const uint32_t r = p - (two ? split : 0) + n, rc = r < last ? r : last;
+            rs[i] = two ? w1.s : w0.s, so[i] = rc * (two ? w1.lds : w0.lds);
+        }
+    }
+    t.template run<true, ONCE>(lds, rw, wo, bx, xo, rs, so, nb, live, a0, astep);
+}
+
+// gate and up: a tile's weight rows are BN / 2 rows of gate, then the same rows of up.  A wave's 32 rows of a matrix instruction are
+// 16 of each, so that a lane has both sums of its rows.  ONCE: geo::experts_once.
+template <typename Tile, uint32_t DT, bool ONCE>
+__global__ __launch_bounds__(Tile::T) void experts_up_mx4_tile_kernel(Mx4Up a, Plan P) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[Tile::LDS];
+    constexpr uint32_t BR = Tile::BN / 2;
+    static_assert(BR % 32 == 0, "a load takes rows of one matrix");
+    PlanTile pt;
+    uint32_t block;
+    const PlanHead head = *P.head;
+    if (!plan_fits(head, a.m, a.slots, a.gate.count))  // the whole workgroup, here and below
+        return nan_rows<DT>(a, a.gate.count, a.h, a.gate.rows, a.ldh);
+    if (!expert_tile(P, head, a.gate.count, (a.gate.rows + BR - 1) / BR, pt, block)) return;
+    const uint32_t r0 = block * BR;
+    Tile t;
+    auto entry = [&](uint32_t i) { return P.ent[pt.row0 + (i < pt.rows ? i : pt.rows - 1)]; };
+    const uint32_t wr = t.wn / 2, c = t.lane % 32;  // this wave's first row of both
+    uint32_t en[Tile::FM];
+#pragma unroll
+    for (int j = 0; j < Tile::FM; j++) en[j] = entry(t.wm + 32 * j + c);
+    const uint32_t live = t.wm < pt.rows ? (pt.rows - t.wm + 31) / 32 : 0;
+    mx4_expert_run<Tile, ONCE>(t, lds, mx4_side(a.gate, pt.expert, r0), mx4_side(a.up, pt.expert, r0), BR, a.gate.rows - r0 - 1, a.x,
+                               [&](uint32_t i) { return entry(i) / a.slots; }, a.gate.nb, live, wr + (c < 16 ? c : BR + c - 16), 16);
+    typedef Elem<DT> O;
+#pragma unroll
+    for (int j = 0; j < Tile::FM; j++) {
+        if (t.wm + 32 * j + c >= pt.rows) continue;
+        typename O::T* h = reinterpret_cast<typename O::T*>(a.h) + en[j] * a.ldh;
+#pragma unroll
+        for (int i = 0; i < Tile::FN; i++)
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                const uint32_t r = r0 + wr + 16 * i + 8 * q + 4 * (t.lane / 32);
+                float g[4], u[4], v[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) g[e] = t.acc[i][j][4 * q + e], u[e] = t.acc[i][j][8 + 4 * q + e];
+                swiglu4(g, u, v);
+                store4<DT>(h + r, v, r < a.gate.rows ? a.gate.rows - r : 0, a.vec);
+            }
+    }
+}
+
+// down: the entries' weighted rows into work [m * slots][rows], in 32 bits, as they are then added.  ONCE: geo::experts_once.
+template <typename Tile, bool ONCE>
+__global__ __launch_bounds__(Tile::T) void experts_down_mx4_tile_kernel(Mx4Down a, Plan P) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[Tile::LDS];
+    PlanTile pt;
+    uint32_t block;
+    const PlanHead head = *P.head;
+    if (!plan_fits(head, a.m, a.slots, a.down.count))  // the whole workgroup, here and below
+        return nan_rows<TRK_DT_F32>(a, a.down.count, a.work, a.down.rows, a.down.rows);
+    if (!expert_tile(P, head, a.down.count, (a.down.rows + Tile::BN - 1) / Tile::BN, pt, block)) return;
+    const uint32_t r0 = block * Tile::BN;
+    Tile t;
+    auto entry = [&](uint32_t i) { return P.ent[pt.row0 + (i < pt.rows ? i : pt.rows - 1)]; };
+    const uint32_t c = t.lane % 32;
+    uint32_t en[Tile::FM];
+    float w[Tile::FM];
+#pragma unroll
+    for (int j = 0; j < Tile::FM; j++) en[j] = entry(t.wm + 32 * j + c);
+#pragma unroll
+    for (int j = 0; j < Tile::FM; j++) w[j] = a.w[(size_t)(en[j] / a.slots) * K_MAX + en[j] % a.slots];
+    const uint32_t live = t.wm < pt.rows ? (pt.rows - t.wm + 31) / 32 : 0;
+    const Mx4Side ws = mx4_side(a.down, pt.expert, r0);
+    mx4_expert_run<Tile, ONCE>(t, lds, ws, ws, Tile::BN, a.down.rows - r0 - 1, a.x, entry, a.down.nb, live, t.wn + c, 32);
+#pragma unroll
+    for (int j = 0; j < Tile::FM; j++) {
+        if (t.wm + 32 * j + c >= pt.rows) continue;
+        float* y = a.work + (uint64_t)en[j] * a.down.rows;
+#pragma unroll
+        for (int i = 0; i < Tile::FN; i++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const uint32_t r = r0 + t.wn + 32 * i + 8 * q + 4 * (t.lane / 32);
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = t.acc[i][j][4 * q + e] * w[j];
+                store4<TRK_DT_F32>(y + r, v, r < a.down.rows ? a.down.rows - r : 0, a.down.rows % 4 == 0);
+            }
+    }
+}
+
 dim3 run_of(uint64_t wgs, uint32_t threads) {
     const geo::Grid2 g = geo::grid_run(wgs, threads);
     return dim3(g.x, g.y);
@@ -139,16 +264,91 @@ void launch_down_strip(Mx4Down a, hipStream_t st) {
     }
 }
 
+template <typename Tile, bool ONCE = true>
+void launch_up_tile(const Mx4Up& a, const Plan& P, uint64_t tiles, hipStream_t st) {
+    const dim3 g = run_of((a.gate.rows + Tile::BN / 2 - 1) / (Tile::BN / 2) * tiles, Tile::T);
+    if (a.dt == TRK_DT_F32)
+        experts_up_mx4_tile_kernel<Tile, TRK_DT_F32, ONCE><<<g, Tile::T, 0, st>>>(a, P);
+    else if (a.dt == TRK_DT_BF16)
+        experts_up_mx4_tile_kernel<Tile, TRK_DT_BF16, ONCE><<<g, Tile::T, 0, st>>>(a, P);
+    else
+        experts_up_mx4_tile_kernel<Tile, TRK_DT_F16, ONCE><<<g, Tile::T, 0, st>>>(a, P);
+}
+
+template <bool ONCE>
+void launch_up_128(const Mx4Up& a, const Plan& P, uint64_t tiles, geo::ExpertsWidth w, hipStream_t st) {
+    if (w == geo::X_NARROW)
+        launch_up_tile<Mx4Tile<64, 128, 32, 64, 3>, ONCE>(a, P, tiles, st);
+    else
+        w == geo::X_WIDE ? launch_up_tile<Mx4Tile<256, 128, 64, 64, 3>, ONCE>(a, P, tiles, st)
+                         : launch_up_tile<Mx4Tile<128, 128, 64, 64, 2>, ONCE>(a, P, tiles, st);
+}
+
+template <typename Tile, bool ONCE = true>
+void launch_down_tile(const Mx4Down& a, const Plan& P, uint64_t tiles, hipStream_t st) {
+    const dim3 g = run_of((a.down.rows + Tile::BN - 1) / Tile::BN * tiles, Tile::T);
+    experts_down_mx4_tile_kernel<Tile, ONCE><<<g, Tile::T, 0, st>>>(a, P);
+}
+
+// The tiles address values and scales by 32 bits, weight rows from their block's first, activation rows from the first of all.
+bool tile_addresses(const Mx4Mat& w, const Mx4X& x, uint64_t rows) {
+    return geo::i8_tile_addresses(w.ld, x.ld, rows) && geo::i8_tile_addresses(w.lds, x.lds, rows);
+}
+
 }  // namespace
 
 hipError_t launch_experts_up_mx4(const Mx4Up& a, const uint32_t* plan, hipStream_t st) {
-    launch_up_strip(a, st);
+    const uint32_t E = a.gate.count;
+    if (!plan || !tile_addresses(a.gate, a.x, a.m) || !tile_addresses(a.up, a.x, a.m)) {
+        launch_up_strip(a, st);
+        return hipGetLastError();
+    }
+    const uint32_t rows = geo::plan_rows(a.m, a.slots, E);
+    const Plan P = plan_at(const_cast<uint32_t*>(plan), a.m, a.slots);
+    const uint64_t tiles = geo::plan_tiles(a.m, a.slots, E, rows);
+    const geo::ExpertsWidth w = geo::experts_width(2 * a.gate.rows, tiles, rows == 128);
+    if (rows == 32)
+        w == geo::X_NARROW ? launch_up_tile<Mx4Tile<64, 32, 32, 32, 4>>(a, P, tiles, st)
+                           : launch_up_tile<Mx4Tile<128, 32, 32, 32, 3>>(a, P, tiles, st);
+    else if (rows == 64)
+        w == geo::X_NARROW ? launch_up_tile<Mx4Tile<64, 64, 32, 32, 4>>(a, P, tiles, st)
+                           : launch_up_tile<Mx4Tile<128, 64, 64, 32, 3>>(a, P, tiles, st);
+    else if (geo::experts_once(a.m, a.slots, E, 64))
+        launch_up_128<true>(a, P, tiles, w, st);
+    else
+        launch_up_128<false>(a, P, tiles, w, st);
     return hipGetLastError();
 }
 
 hipError_t launch_experts_down_mx4(const Mx4Down& a, const uint32_t* plan, hipStream_t st) {
-    launch_down_strip(a, st);
-    return hipGetLastError();
+    const uint32_t E = a.down.count;
+    if (!plan || !tile_addresses(a.down, a.x, (uint64_t)a.m * a.slots)) {
+        launch_down_strip(a, st);
+        return hipGetLastError();
+    }
+    const uint32_t rows = geo::plan_rows(a.m, a.slots, E);
+    const Plan P = plan_at(const_cast<uint32_t*>(plan), a.m, a.slots);
+    const uint64_t tiles = geo::plan_tiles(a.m, a.slots, E, rows);
+    const bool narrow = geo::experts_width(a.down.rows, tiles, false) == geo::X_NARROW;
+    if (rows == 32)
+        narrow ? launch_down_tile<Mx4Tile<64, 32, 32, 32, 4>>(a, P, tiles, st)
+               : launch_down_tile<Mx4Tile<128, 32, 32, 32, 3>>(a, P, tiles, st);
+    else if (rows == 64)
+        narrow ? launch_down_tile<Mx4Tile<64, 64, 32, 32, 4>>(a, P, tiles, st)
+               : launch_down_tile<Mx4Tile<128, 64, 64, 32, 3>>(a, P, tiles, st);
+    else if (geo::experts_once(a.m, a.slots, E, 128))
+        narrow ? launch_down_tile<Mx4Tile<64, 128, 32, 64, 3>>(a, P, tiles, st)
+               : launch_down_tile<Mx4Tile<128, 128, 64, 64, 2>>(a, P, tiles, st);
+    else
+        narrow ? launch_down_tile<Mx4Tile<64, 128, 32, 64, 3>, false>(a, P, tiles, st)
+               : launch_down_tile<Mx4Tile<128, 128, 64, 64, 2>, false>(a, P, tiles, st);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    I8Down c{};
+    c.down.rows = a.down.rows, c.down.count = a.down.count;
+    c.m = a.m, c.slots = a.slots, c.ids = a.ids, c.n_sel = a.n_sel, c.work = a.work;
+    c.y = a.y, c.dt = a.dt, c.ldy = a.ldy, c.accumulate = a.accumulate, c.vec = a.vec;
+    return launch_experts_combine(c, st);
 }
 
 }  // namespace trk

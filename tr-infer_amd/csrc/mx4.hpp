@@ -28,6 +28,10 @@ __device__ __forceinline__ f32x4 mfma_mx4(i32x4 a, uint32_t sa, i32x4 b, uint32_
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(a), mx_operand(b), c, MX_FP4, MX_FP4, 0, (int)sa, 0, (int)sb);
 }
 
+// The sum is made here, by the whole wave: sunk into a branch that lanes part at, the instructions' operands would be made in the
+// lanes that take it alone.
+__device__ __forceinline__ void mx_here(f32x4& c) { asm volatile("" : "+v"(c)); }
+
 // 2^(s - 127), NaN for 255
 __device__ __forceinline__ float mx_scale(uint32_t s) {
     return s == 255u ? __builtin_nanf("") : s ? __uint_as_float(s << 23) : 0x1p-127f;
@@ -82,6 +86,8 @@ __device__ __forceinline__ void mx4_strip(const Mx4Row (&w)[NM], Mx4Row x, uint3
             acc[i] = mfma_mx4(wl, in ? w[i].s[b] : MX_ONE, in ? xl : i32x4{0, 0, 0, 0}, xs, acc[i]);
         }
     }
+#pragma unroll
+    for (uint32_t i = 0; i < NM; i++) mx_here(acc[i]);
 }
 
 }  // namespace trk

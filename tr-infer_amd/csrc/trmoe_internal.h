@@ -301,6 +301,8 @@ hipError_t launch_experts_plan(const uint32_t* ids, const uint32_t* n_sel, uint3
                                uint32_t* plan, hipStream_t st);
 hipError_t launch_experts_up(const I8Up& a, const uint32_t* plan, hipStream_t st);
 hipError_t launch_experts_down(const I8Down& a, const uint32_t* plan, hipStream_t st);
+// y from work: of `a`, the stack's rows and count, and what follows the plan
+hipError_t launch_experts_combine(const I8Down& a, hipStream_t st);
 // microscaled 4-bit rows and products (k_mx4.hip; the experts' k_mx4x.hip; the layer for a few tokens k_mx4l.hip)
 struct Mx4Mat {
     const uint8_t *q, *s;
