@@ -1,5 +1,5 @@
 // Rows to microscaled 4-bit values and back (trk_quantize_mx4, trk_dequantize_mx4), and their dense product (trk_gemm_mx4).
-#include "mx4tile.hpp"
+#include "mx4gemm.hpp"
 #include "rows.hpp"
 
 namespace trk {
@@ -200,81 +200,6 @@ void launch_strip(const Mx4Gemm& a, hipStream_t st) {
         gemm_mx4_strip_kernel<TRK_DT_F16><<<grid, ST_WAVES * WAVE, 0, st>>>(a);
 }
 
-// The tiles' place in the launch: panels of eight weight tiles, activation tiles after one another inside each, so that
-// the tiles that run at once on an XCD (a contiguous run of them) share rows of both in its L2.
-__device__ __forceinline__ void tile_place(uint32_t idx, uint32_t tn, uint32_t tm, uint32_t& n, uint32_t& m) {
-    const uint32_t panel = idx / (8 * tm), left = tn - panel * 8, w = left < 8 ? left : 8, rem = idx - panel * 8 * tm;
-    n = panel * 8 + rem % w, m = rem / w;
-}
-
-template <typename Tile, uint32_t DT>
-__global__ __launch_bounds__(Tile::T) void gemm_mx4_tile_kernel(Mx4Gemm g) {
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[Tile::LDS];
-    const uint32_t tn = (g.w.rows + Tile::BN - 1) / Tile::BN, tm = (g.m + Tile::BM - 1) / Tile::BM;
-    uint32_t idx, n, m;
-    if (!xcd_order_1d(tn * tm, idx, run_id())) return;  // the whole workgroup
-    tile_place(idx, tn, tm, n, m);
-    const uint32_t r0 = n * Tile::BN, t0 = m * Tile::BM, rl = g.w.rows - r0 - 1, tl = g.m - t0 - 1;  // the last rows there are
-    Tile t;
-    i32x4 rw[Tile::NA], rs[Tile::NS];
-    uint32_t wo[Tile::NA], xo[Tile::NB], so[Tile::NS];
-    const i32x4 bw = buffer_at((const int8_t*)g.w.q + r0 * g.w.ld), bx = buffer_at((const int8_t*)g.x.q + t0 * g.x.ld);
-    const i32x4 bws = buffer_at((const int8_t*)g.w.s + r0 * g.w.lds), bxs = buffer_at((const int8_t*)g.x.s + t0 * g.x.lds);
-#pragma unroll
-    for (int i = 0; i < Tile::NA; i++) {
-        const uint32_t r = t.load_row(i);
-        rw[i] = bw, wo[i] = (r < rl ? r : rl) * (uint32_t)g.w.ld;
-    }
-#pragma unroll
-    for (int i = 0; i < Tile::NB; i++) {
-        const uint32_t r = t.load_row(i);
-        xo[i] = (r < tl ? r : tl) * (uint32_t)g.x.ld;
-    }
-#pragma unroll
-    for (int i = 0; i < Tile::NS; i++) {
-        const uint32_t p = t.scale_piece(i);
-        const bool w = p < Tile::BN / 32;
-        const uint32_t r = (w ? p : p - Tile::BN / 32) * 32 + t.lane / 2, l = w ? rl : tl;
-        rs[i] = w ? bws : bxs;
-        so[i] = (r < l ? r : l) * (uint32_t)(w ? g.w.lds : g.x.lds);
-    }
-    t.template run<false, false>(lds, rw, wo, bx, xo, rs, so, g.w.nb, 0, t.wn + t.lane % 32, 32);
-    typedef Elem<DT> O;
-#pragma unroll
-    for (int j = 0; j < Tile::FM; j++) {
-        const uint32_t row = t0 + t.wm + 32 * j + t.lane % 32;
-        if (row >= g.m) continue;
-        typename O::T* y = reinterpret_cast<typename O::T*>(g.y) + row * g.ldy;
-#pragma unroll
-        for (int i = 0; i < Tile::FN; i++)
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const uint32_t r = r0 + t.wn + 32 * i + 8 * q + 4 * (t.lane / 32), left = r < g.w.rows ? g.w.rows - r : 0;
-                float v[4];
-#pragma unroll
-                for (uint32_t c = 0; c < 4; c++) {
-                    v[c] = t.acc[i][j][4 * q + c];
-                    if (g.bias && c < left) v[c] += g.bias[r + c];
-                    if (g.accumulate && c < left) v[c] += O::get(y[r + c]);
-                }
-                store4<DT>(y + r, v, left, g.vec);
-            }
-    }
-}
-
-template <typename Tile>
-void launch_tile(const Mx4Gemm& a, hipStream_t st) {
-    const uint64_t wgs = (uint64_t)((a.w.rows + Tile::BN - 1) / Tile::BN) * (((uint64_t)a.m + Tile::BM - 1) / Tile::BM);
-    const geo::Grid2 g = geo::grid_run(wgs, Tile::T);
-    const dim3 grid(g.x, g.y);
-    if (a.dt == TRK_DT_F32)
-        gemm_mx4_tile_kernel<Tile, TRK_DT_F32><<<grid, Tile::T, 0, st>>>(a);
-    else if (a.dt == TRK_DT_BF16)
-        gemm_mx4_tile_kernel<Tile, TRK_DT_BF16><<<grid, Tile::T, 0, st>>>(a);
-    else
-        gemm_mx4_tile_kernel<Tile, TRK_DT_F16><<<grid, Tile::T, 0, st>>>(a);
-}
-
 }  // namespace
 
 hipError_t launch_rows_mx4(bool back, uint32_t dt, const void* x, uint64_t ldx, uint32_t m, uint32_t k, uint8_t* q, uint64_t ldq,
@@ -291,12 +216,13 @@ hipError_t launch_rows_mx4(bool back, uint32_t dt, const void* x, uint64_t ldx, 
 hipError_t launch_gemm_mx4(const Mx4Gemm& a, hipStream_t st) {
     static const int form = getenv("MX4_FORM") ? atoi(getenv("MX4_FORM")) : 0;  // PROBE
     switch (form) {
-    case 1: launch_tile<Mx4Tile<64, 32, 32, 32, 4>>(a, st); break;
-    case 2: launch_tile<Mx4Tile<64, 64, 32, 32, 4>>(a, st); break;
-    case 3: launch_tile<Mx4Tile<128, 128, 64, 64, 2>>(a, st); break;
-    case 4: launch_tile<Mx4Tile<256, 256, 64, 128, 2>>(a, st); break;
-    case 5: launch_tile<Mx4Tile<128, 64, 64, 32, 3>>(a, st); break;
-    case 6: launch_tile<Mx4Tile<256, 128, 64, 64, 3>>(a, st); break;
+    case 1: launch_mx4_tile<Mx4Tile<64, 32, 32, 32, 4>>(a, st); break;
+    case 2: launch_mx4_tile<Mx4Tile<64, 64, 32, 32, 4>>(a, st); break;
+    case 3: launch_mx4_tile<Mx4Tile<128, 128, 64, 64, 2>>(a, st); break;
+    case 4: launch_mx4_tile<Mx4Tile<256, 256, 64, 128, 2, 8>>(a, st); break;
+    case 5: launch_mx4_tile<Mx4Tile<128, 64, 64, 32, 3>>(a, st); break;
+    case 6: launch_mx4_tile<Mx4Tile<256, 128, 64, 64, 3>>(a, st); break;
+    case 7: launch_gemm_mx4_wide(a, st); break;
     default: launch_strip(a, st);
     }
     return hipGetLastError();

@@ -124,7 +124,7 @@ __device__ __forceinline__ void mx4_expert_run(Tile& t, uint8_t* lds, const Mx4S
     }
 #pragma unroll
     for (int i = 0; i < Tile::NS; i++) {
-        const uint32_t p = t.scale_piece(i) * 32, n = t.lane / 2;
+        const uint32_t p = t.scale_load(i) * Tile::SR, n = t.lane / Tile::SW;
         const bool mine = p >= Tile::BN, two = !mine && p >= split;
         if (mine) {
             rs[i] = bxs, so[i] = row(p - Tile::BN + n) * (uint32_t)x.lds;
@@ -133,7 +133,7 @@ __device__ __forceinline__ void mx4_expert_run(Tile& t, uint8_t* lds, const Mx4S
             rs[i] = two ? w1.s : w0.s, so[i] = rc * (two ? w1.lds : w0.lds);
         }
     }
-    t.template run<true, ONCE>(lds, rw, wo, bx, xo, rs, so, nb, live, a0, astep);
+    t.template run<true, ONCE>(lds, rw, wo, bx, xo, [&](int i, i32x4& r, uint32_t& o) { r = rs[i], o = so[i]; }, nb, live, a0, astep);
 }
 
 // gate and up: a tile's weight rows are BN / 2 rows of gate, then the same rows of up.  A wave's 32 rows of a matrix instruction are
@@ -160,21 +160,27 @@ __global__ __launch_bounds__(Tile::T) void experts_up_mx4_tile_kernel(Mx4Up a, P
     mx4_expert_run<Tile, ONCE>(t, lds, mx4_side(a.gate, pt.expert, r0), mx4_side(a.up, pt.expert, r0), BR, a.gate.rows - r0 - 1, a.x,
                                [&](uint32_t i) { return entry(i) / a.slots; }, a.gate.nb, live, wr + (c < 16 ? c : BR + c - 16), 16);
     typedef Elem<DT> O;
+    constexpr int CW = Tile::WN / 2;
+    const uint32_t r = r0 + wr + t.lane % (CW / 4) * 4, left = r < a.gate.rows ? a.gate.rows - r : 0;
 #pragma unroll
     for (int j = 0; j < Tile::FM; j++) {
-        if (t.wm + 32 * j + c >= pt.rows) continue;
-        typename O::T* h = reinterpret_cast<typename O::T*>(a.h) + en[j] * a.ldh;
+        if (j >= (int)live) break;  // the wave as a whole
+        float v[CW / 8][4];
 #pragma unroll
         for (int i = 0; i < Tile::FN; i++)
 #pragma unroll
             for (int q = 0; q < 2; q++) {
-                const uint32_t r = r0 + wr + 16 * i + 8 * q + 4 * (t.lane / 32);
-                float g[4], u[4], v[4];
+                float g[4], u[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) g[e] = t.acc[i][j][4 * q + e], u[e] = t.acc[i][j][8 + 4 * q + e];
-                swiglu4(g, u, v);
-                store4<DT>(h + r, v, r < a.gate.rows ? a.gate.rows - r : 0, a.vec);
+                swiglu4(g, u, v[2 * i + q]);
             }
+        t.template turn<CW>(lds, v, [&](uint32_t tr, uint32_t, f32x4 x) {
+            const uint32_t e = __shfl(en[j], tr);
+            if (t.wm + 32 * j + tr >= pt.rows || left == 0) return;
+            const float o[4] = {x[0], x[1], x[2], x[3]};
+            store4<DT>(reinterpret_cast<typename O::T*>(a.h) + e * a.ldh + r, o, left, a.vec);
+        });
     }
 }
 
@@ -201,20 +207,21 @@ __global__ __launch_bounds__(Tile::T) void experts_down_mx4_tile_kernel(Mx4Down 
     const uint32_t live = t.wm < pt.rows ? (pt.rows - t.wm + 31) / 32 : 0;
     const Mx4Side ws = mx4_side(a.down, pt.expert, r0);
     mx4_expert_run<Tile, ONCE>(t, lds, ws, ws, Tile::BN, a.down.rows - r0 - 1, a.x, entry, a.down.nb, live, t.wn + c, 32);
+    const uint32_t r = r0 + t.wn + t.lane % (Tile::WN / 4) * 4, left = r < a.down.rows ? a.down.rows - r : 0;
 #pragma unroll
     for (int j = 0; j < Tile::FM; j++) {
-        if (t.wm + 32 * j + c >= pt.rows) continue;
-        float* y = a.work + (uint64_t)en[j] * a.down.rows;
+        if (j >= (int)live) break;  // the wave as a whole
+        float v[Tile::WN / 8][4];
 #pragma unroll
         for (int i = 0; i < Tile::FN; i++)
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const uint32_t r = r0 + t.wn + 32 * i + 8 * q + 4 * (t.lane / 32);
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = t.acc[i][j][4 * q + e] * w[j];
-                store4<TRK_DT_F32>(y + r, v, r < a.down.rows ? a.down.rows - r : 0, a.down.rows % 4 == 0);
-            }
+            for (int q = 0; q < 16; q++) v[4 * i + q / 4][q % 4] = t.acc[i][j][q] * w[j];
+        t.template turn<Tile::WN>(lds, v, [&](uint32_t tr, uint32_t, f32x4 x) {
+            const uint32_t e = __shfl(en[j], tr);
+            if (t.wm + 32 * j + tr >= pt.rows || left == 0) return;
+            const float o[4] = {x[0], x[1], x[2], x[3]};
+            store4<TRK_DT_F32>(a.work + (uint64_t)e * a.down.rows + r, o, left, a.down.rows % 4 == 0);
+        });
     }
 }
 

@@ -1,13 +1,14 @@
 // One BN x BM tile of a microscaled 4-bit product on the matrix cores: BN weight rows times BM activation rows over all of K.
 //
-// K goes by in stages of eight blocks (128 bytes and 8 scale bytes a row), NST of them in LDS at once.  Both arrive there by LDS
-// DMA, no register between: 16 bytes a lane of the values (a wave's instruction brings eight rows), 4 of the scales (32 rows).
-// A row's eight blocks lie permuted (block c of row r in slot c ^ (r & 7)), so that lanes that read one block of eight rows
-// meet no bank twice.  Waves hold WN x WM of the tile as 32 x 32 sums.  A matrix instruction takes two blocks of each row, one
-// from either half of the stage (4 h + s for the lanes' half h at step s): a lane then has its four steps' scales in one word,
-// which the instruction picks its byte from.  Each step's fragments are read during the step before.  At the last step of a
-// stage every wave has its fragments in registers: one barrier there hands the stage's LDS to the rows NST stages on
-// and opens the next stage.
+// K goes by in stages of eight blocks (128 bytes a row), NST of them in LDS at once, and their scales by GS stages (8 GS bytes a
+// row), for a row's eight bytes of one stage are a cache line's trip by themselves.  Both arrive by LDS DMA, no register between: 16
+// bytes a lane of the values (a wave's instruction brings eight rows), 4 of the scales (32 / GS rows).  A row's blocks lie permuted
+// (block c of row r in slot c ^ (r & 7) ^ (r >> 3 & 1)), and its words of scales, so that neither read meets a bank twice.  Waves hold WN x
+// WM of the tile as 32 x 32 sums.  A matrix instruction takes two blocks of each row, one from either half of the stage (4 h + s for
+// the lanes' half h at step s): a lane then has its four steps' scales in one word, which the instruction picks its byte from.
+// Each step's fragments are read during the step before.  At the last step of a stage every wave has its fragments in
+// registers: one barrier there hands the stage's LDS to the rows NST stages on and opens the next stage.  The scales' LDS is
+// handed on one stage before their last (that stage's are read before the barrier), which leaves the next ones a stage to arrive.
 #pragma once
 
 #include "i8tile.hpp"
@@ -28,14 +29,16 @@ __device__ __forceinline__ void lds_dma4(i32x4 rsrc, uint32_t off, uint32_t lds)
                  : "memory", "m0");
 }
 
-template <int BN_, int BM_, int WN_, int WM_, int NST_>
+// ACC: the sums live in accumulator registers (a file built for those), which leaves the others to a wave tile of 128 x 128.
+template <int BN_, int BM_, int WN_, int WM_, int NST_, int GS_ = 4, bool ACC = false>
 struct Mx4Tile {
-    static constexpr int BN = BN_, BM = BM_, WN = WN_, WM = WM_, NST = NST_, BK = 128, BS = 8;  // a stage's bytes of a row
+    static constexpr int BN = BN_, BM = BM_, WN = WN_, WM = WM_, NST = NST_, GS = GS_, BK = 128;  // BK: a stage's bytes of a row
     static constexpr int NW = BN / WN * (BM / WM), T = NW * WAVE;
     static constexpr int FN = WN / 32, FM = WM / 32;
-    static constexpr int NA = BN / 8 / NW, NB = BM / 8 / NW, NSC = (BN + BM) / 32, NS = (NSC + NW - 1) / NW;  // a wave's loads of a stage
-    static constexpr int NL = NA + NB + NS;
-    static constexpr int SCALES = (BN + BM) * BK, STAGE = SCALES + (BN + BM) * BS, LDS = STAGE * NST;
+    static constexpr int NA = BN / 8 / NW, NB = BM / 8 / NW, NL = NA + NB;  // a wave's loads of a stage
+    static constexpr int SW = 2 * GS, SR = WAVE / SW;                           // words of scales a row and group, rows a load
+    static constexpr int NSC = (BN + BM) / SR, NS = (NSC + NW - 1) / NW;        // loads of a group's scales, a wave's
+    static constexpr int STAGE = (BN + BM) * BK, SCALES = STAGE * NST, LDS = SCALES + (BN + BM) * SW * 4;
     static_assert(BN % (8 * NW) == 0 && BM % (8 * NW) == 0 && BN % 32 == 0 && BM % 32 == 0 && LDS <= 160 * 1024, "tile");
 
     f32x16 acc[FN][FM];
@@ -53,41 +56,47 @@ struct Mx4Tile {
     }
     // the tile row that this lane loads of its wave's i-th piece of weights (activations: the same with NB)
     __device__ __forceinline__ uint32_t load_row(int i) const { return (i * NW + wv) * 8 + lane / 8; }
-    // its wave's i-th piece of scales, 32 rows, the weights' before the activations' (the last may be taken by several waves)
-    __device__ __forceinline__ uint32_t scale_piece(int i) const {
+    // of its wave's i-th load of scales (the last may be taken by several waves)
+    __device__ __forceinline__ uint32_t scale_load(int i) const {
         const uint32_t n = i * NW + wv;
         return n < NSC ? n : NSC - 1;
     }
+    __device__ __forceinline__ uint32_t scale_row(int i) const { return scale_load(i) * SR + lane / SW; }
 
-    // rw[i], wo[i]: buffer and this lane's row offset for its i-th eight weight rows; rx, xo: the activations'.  rs[i], so[i]: its
-    // i-th scales', lanes 2 n and 2 n + 1 a row's.
-    // a0: the LDS row of this lane's weight row of the wave's first 32 (a place in eight as lane % 8 has); the i-th's: a0 + i * astep.
+    // rw[i], wo[i]: buffer and this lane's row offset for its i-th eight weight rows; rx, xo: the activations'.  scales(i, rs, so) gives the
+    // buffer and this lane's row offset for its i-th scales.
+    // a0: the LDS row of this lane's weight row of the wave's first 32 (its place in sixteen is the lane's); the i-th's: a0 + i * astep.
     // live: this wave's 32-row groups of activations that hold any (PART: the others' products are left out).
     // ONCE: the weight rows are this workgroup's alone.
-    template <bool PART, bool ONCE>
+    template <bool PART, bool ONCE, typename Scales>
     __device__ __forceinline__ void run(uint8_t* lds, const i32x4 (&rw)[NA], const uint32_t (&wo)[NA], i32x4 rx,
-                                        const uint32_t (&xo)[NB], const i32x4 (&rs)[NS], const uint32_t (&so)[NS], uint32_t nb,
-                                        uint32_t live, uint32_t a0, uint32_t astep) {
+                                        const uint32_t (&xo)[NB], Scales&& scales, uint32_t nb, uint32_t live, uint32_t a0, uint32_t astep) {
         const uint32_t l0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
         const uint32_t S = (nb + 7) / 8, bytes = 16 * nb, words = (nb + 3) / 4 * 4;
-        const uint32_t piece = 16 * (lane % 8 ^ lane / 8);  // where in a row this lane loads
-        uint32_t sat[NS];
-#pragma unroll
-        for (int i = 0; i < NS; i++) sat[i] = SCALES + scale_piece(i) * 256;
+        static_assert(NW % 2 == 0, "a wave's eight rows are all even ones of their sixteen, or all odd");
+        const uint32_t piece = 16 * (lane % 8 ^ lane / 8 ^ wv % 2);  // where in a row this lane loads
         // the n-th of a wave's loads of stage s; past the row's end anything, it multiplies zeros by 1
         auto load1 = [&](uint32_t s, uint32_t at, int n) {
-            const uint32_t o = s * BK + piece, oc = o < bytes ? o : 0, q = s * BS + 4 * (lane % 2), qc = q < words ? q : 0;
+            const uint32_t o = s * BK + piece, oc = o < bytes ? o : 0;
             if (n < NA)
                 lds_dma<ONCE>(rw[n < NA ? n : 0], wo[n < NA ? n : 0] + oc, at + (n * NW + wv) * 1024);
-            else if (n < NA + NB)
-                lds_dma<false>(rx, xo[n < NA + NB ? n - NA : 0] + oc, at + (n * NW + wv) * 1024);  // the activations' rows follow the weights'
             else
-                lds_dma4(rs[n - NA - NB], so[n - NA - NB] + qc, at + sat[n - NA - NB]);
+                lds_dma<false>(rx, xo[n < NA ? 0 : n - NA] + oc, at + (n * NW + wv) * 1024);  // the activations' rows follow the weights'
         };
-        auto load_at = [&](uint32_t s) { return l0 + s % NST * STAGE; };
+        // the scales of GS stages from s on
+        auto load_scales = [&](uint32_t s) {
+#pragma unroll
+            for (int i = 0; i < NS; i++) {
+                const uint32_t n = scale_load(i), q = 8 * s + 4 * (lane % SW ^ 2 * (n % GS));
+                i32x4 rs;
+                uint32_t so;
+                scales(i, rs, so);
+                lds_dma4(rs, so + (q < words ? q : 0), l0 + SCALES + n * 256);
+            }
+        };
         i32x4 a[2][FN], b[2][FM];
         uint32_t sa[2][FN], sb[2][FM];
-        const uint32_t row = lane % 32, half = lane / 32, slot = 16 * (4 * half ^ row % 8), b0 = BN + wm + row;
+        const uint32_t row = lane % 32, half = lane / 32, slot = 16 * (4 * half ^ row % 8 ^ row / 8 % 2), b0 = BN + wm + row;
         auto read = [&](uint32_t at, int s, int to) {
 #pragma unroll
             for (int i = 0; i < FN; i++) a[to][i] = *reinterpret_cast<const i32x4*>(lds + at + (a0 + i * astep) * BK + (slot ^ (16 * s)));
@@ -96,40 +105,52 @@ struct Mx4Tile {
                 if (!PART || j < (int)live)
                     b[to][j] = *reinterpret_cast<const i32x4*>(lds + at + (b0 + j * 32) * BK + (slot ^ (16 * s)));
         };
-        auto read_scales = [&](uint32_t at, int to) {
+        auto read_scales = [&](uint32_t s, int to) {
+            auto word = [&](uint32_t r) {  // row r's of this lane's half
+                return *reinterpret_cast<const uint32_t*>(lds + SCALES + r * (4 * SW) + 4 * ((2 * (s % GS) + half) ^ (2 * (r / SR % GS))));
+            };
 #pragma unroll
-            for (int i = 0; i < FN; i++)
-                sa[to][i] = *reinterpret_cast<const uint32_t*>(lds + at + SCALES + (a0 + i * astep) * BS + 4 * half);
+            for (int i = 0; i < FN; i++) sa[to][i] = word(a0 + i * astep);
 #pragma unroll
             for (int j = 0; j < FM; j++)
-                if (!PART || j < (int)live)
-                    sb[to][j] = *reinterpret_cast<const uint32_t*>(lds + at + SCALES + (b0 + j * 32) * BS + 4 * half);
+                if (!PART || j < (int)live) sb[to][j] = word(b0 + j * 32);
         };
         // a step's products, with the loads of a stage between them
-        auto mul = [&](auto step, int from, int sc, bool loads, uint32_t s, uint32_t at) {
+        auto mul = [&](auto step, int from, auto loads, uint32_t s, uint32_t at) {
             constexpr int ST = decltype(step)::value;
 #pragma unroll
             for (int j = 0; j < FM; j++) {
                 if (!PART || j < (int)live) {
 #pragma unroll
                     for (int i = 0; i < FN; i++)
-                        acc[i][j] = mfma_mx4_32<ST>(a[from][i], sa[sc][i], b[from][j], sb[sc][j], acc[i][j]);
+                        acc[i][j] = mfma_mx4_32<ST>(a[from][i], sa[0][i], b[from][j], sb[0][j], acc[i][j]);
                     // the products stay where they are: on their side of the barrier, and before any branch that lanes part at
                     // (their operands would be made in the lanes that take it alone)
 #pragma unroll
-                    for (int i = 0; i < FN; i++) asm volatile("" : "+v"(acc[i][j]));
+                    for (int i = 0; i < FN; i++) {
+                        if constexpr (ACC)
+                            asm volatile("" : "+a"(acc[i][j]));
+                        else
+                            asm volatile("" : "+v"(acc[i][j]));
+                    }
                 }
-                if (loads)
+                if constexpr (decltype(loads)::value)
 #pragma unroll
                     for (int n = j * NL / FM; n < (j + 1) * NL / FM; n++) load1(s, at, n);
             }
             __builtin_amdgcn_sched_barrier(0);
         };
+        constexpr std::integral_constant<int, 0> S0{};
+        constexpr std::integral_constant<int, 1> S1{};
+        constexpr std::integral_constant<int, 2> S2{};
+        constexpr std::integral_constant<int, 3> S3{};
+        constexpr std::false_type NO{};
+        load_scales(0);
 #pragma unroll
         for (uint32_t s = 0; s < NST; s++)
             if (s < S)
 #pragma unroll
-                for (int n = 0; n < NL; n++) load1(s, load_at(s), n);
+                for (int n = 0; n < NL; n++) load1(s, l0 + s * STAGE, n);
         if (S >= NST)
             wait_dma<(NST - 1) * NL>();
         else
@@ -138,28 +159,40 @@ struct Mx4Tile {
         read(0, 0, 0);
         read_scales(0, 0);
         uint32_t cur = 0;
-        for (uint32_t s = 0; s + 1 < S; s++) {
-            const uint32_t nxt = cur + STAGE == LDS ? 0 : cur + STAGE;
+        // a stage that is not the last; `loads`: the stage NST on comes in its place
+        auto stage = [&](uint32_t s, auto loads) {
+            const uint32_t nxt = cur + STAGE == SCALES ? 0 : cur + STAGE;
+            const bool group = (s + 1) % GS == 0;  // the next stage begins one
             read(cur, 1, 1);
-            mul(std::integral_constant<int, 0>{}, 0, 0, false, 0, 0);
+            mul(S0, 0, NO, 0, 0);
             read(cur, 2, 0);
-            mul(std::integral_constant<int, 1>{}, 1, 0, false, 0, 0);
+            mul(S1, 1, NO, 0, 0);
             read(cur, 3, 1);
-            mul(std::integral_constant<int, 2>{}, 0, 0, false, 0, 0);
-            if (s + NST <= S)
-                wait_dma<(NST - 2) * NL>();
-            else
+            if (!group) read_scales(s + 1, 1);
+            mul(S2, 0, NO, 0, 0);
+            // the next stage's rows are there; before a group its scales, which no more than one stage's loads follow
+            if (!(decltype(loads)::value || s + NST <= S))
                 wait_dma<0>();
+            else if (NST > 3 && group)
+                wait_dma<NL>();
+            else
+                wait_dma<(NST - 2) * NL>();
             wg_barrier();
             read(nxt, 0, 0);
-            read_scales(nxt, 1);
-            mul(std::integral_constant<int, 3>{}, 1, 0, s + NST < S, s + NST, load_at(s + NST));
+            if (group)
+                read_scales(s + 1, 1);
+            else if ((s + 2) % GS == 0 && s + 2 < S)
+                load_scales(s + 2);
+            mul(S3, 1, loads, s + NST, l0 + cur);
 #pragma unroll
             for (int i = 0; i < FN; i++) sa[0][i] = sa[1][i];
 #pragma unroll
             for (int j = 0; j < FM; j++) sb[0][j] = sb[1][j];
             cur = nxt;
-        }
+        };
+        uint32_t s = 0;
+        for (; s + NST < S; s++) stage(s, std::true_type{});
+        for (; s + 1 < S; s++) stage(s, NO);
         // the last stage: past the row's end zeros, by 1
         const uint32_t first = 8 * (S - 1) + 4 * half, in = first < nb ? (nb - first < 4 ? nb - first : 4u) : 0u;
         const uint32_t keep = in >= 4 ? 0xffffffffu : (1u << (8 * in)) - 1u, one = MX_ONE * 0x01010101u & ~keep;
@@ -174,15 +207,37 @@ struct Mx4Tile {
         };
         read(cur, 1, 1);
         cut(0, 0);
-        mul(std::integral_constant<int, 0>{}, 0, 0, false, 0, 0);
+        mul(S0, 0, NO, 0, 0);
         read(cur, 2, 0);
         cut(1, 1);
-        mul(std::integral_constant<int, 1>{}, 1, 0, false, 0, 0);
+        mul(S1, 1, NO, 0, 0);
         read(cur, 3, 1);
         cut(2, 0);
-        mul(std::integral_constant<int, 2>{}, 0, 0, false, 0, 0);
+        mul(S2, 0, NO, 0, 0);
         cut(3, 1);
-        mul(std::integral_constant<int, 3>{}, 1, 0, false, 0, 0);
+        mul(S3, 1, NO, 0, 0);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        wg_barrier();  // the stages' LDS is the outputs' from here on
+    }
+
+    // A wave's outputs of 32 activation rows by CW weight rows, turned in its part of LDS so that what lies next to another in
+    // memory is written together: lane l has row l % 32, v[g] its columns 8 g + 4 (l / 32) .. + 3; out(r, c, x) is given four columns of
+    // a row, neighbouring lanes neighbouring ones.
+    template <int CW, typename Out>
+    __device__ __forceinline__ void turn(uint8_t* lds, const float (&v)[CW / 8][4], Out&& out) const {
+        constexpr uint32_t PITCH = CW * 4 + 16, LPR = CW / 4;
+        static_assert(NW * 32 * PITCH <= LDS, "the outputs' LDS");
+        uint8_t* buf = lds + wv * (32 * PITCH);
+        wave_sync();  // the turn before has been read
+#pragma unroll
+        for (int g = 0; g < CW / 8; g++)
+            *reinterpret_cast<f32x4*>(buf + lane % 32 * PITCH + 32 * g + 16 * (lane / 32)) = f32x4{v[g][0], v[g][1], v[g][2], v[g][3]};
+        wave_sync();
+#pragma unroll
+        for (uint32_t n = 0; n < 32 * LPR / WAVE; n++) {
+            const uint32_t r = (n * WAVE + lane) / LPR, c = lane % LPR * 4;
+            out(r, c, *reinterpret_cast<const f32x4*>(buf + r * PITCH + 4 * c));
+        }
     }
 };
 
