@@ -1229,19 +1229,21 @@ static int check_moe_mx4(const trk_moe_mx4_w* w, uint32_t k, uint32_t m) {
 }
 
 struct MoeMx4Work {
-    uint64_t logits, shlog, ids, w, n_sel, h, bytes;
+    uint64_t logits, shlog, ids, w, n_sel, x, h, bytes;
 };
 static MoeMx4Work moe_mx4_work(const trk_moe_mx4_w& w, uint32_t k, uint32_t m) {
     uint64_t at = 0;
-    auto take = [&](uint64_t words) {
+    auto bytes = [&](uint64_t n) {
         const uint64_t a = at;
-        at += (4 * words + 15) / 16 * 16;
+        at += (n + 15) / 16 * 16;
         return a;
     };
+    auto take = [&](uint64_t words) { return bytes(4 * words); };
     MoeMx4Work o;
     o.logits = take((uint64_t)m * (w.gate.count - w.n_shared)), o.shlog = take(m);
     o.ids = take((uint64_t)m * TRK_MOE_K_MAX), o.w = take((uint64_t)m * TRK_MOE_K_MAX), o.n_sel = take(m);
-    o.h = take((uint64_t)m * (k + w.n_shared) * w.gate.rows);
+    o.x = bytes(m * mx4_parts_bytes(mx4_blocks(w.gate.k)));
+    o.h = bytes((uint64_t)m * (k + w.n_shared) * mx4_parts_bytes(mx4_blocks(w.gate.rows)));
     o.bytes = at;
     return o;
 }
@@ -1272,8 +1274,8 @@ extern "C" int trk_moe_mx4(const trk_moe_mx4_w* w, const trk_score_policy* p, co
     float* wl = (float*)(b + o.logits);
     const Mx4Layer a{rlog ? nullptr : w->router, w->n_shared ? w->shared_gate : nullptr, mx4_mat(w->gate), mx4_mat(w->up),
                      mx4_mat(w->down), E, w->n_shared, H, m, p->k + w->n_shared, x, xdtype, ldx, rlog ? rlog : wl, wl,
-                     (float*)(b + o.shlog), (uint32_t*)(b + o.ids), (uint32_t*)(b + o.n_sel), (float*)(b + o.w), (float*)(b + o.h),
-                     y, ydtype, ldy};
+                     (float*)(b + o.shlog), (uint32_t*)(b + o.ids), (uint32_t*)(b + o.n_sel), (float*)(b + o.w), (uint8_t*)(b + o.x),
+                     (uint8_t*)(b + o.h), y, ydtype, ldy};
     const ScorePolicy sp{p->k, p->score, p->n_group, p->topk_group, p->group_top, p->renorm, p->factor};
     HIP_TRY(launch_moe_mx4(a, w->bias, sp, (hipStream_t)stream));
     return TRK_OK;

@@ -42,49 +42,72 @@ struct Mx4Row {
     const uint8_t *q, *s;
 };
 
-// U groups of four blocks of NM matrices' rows and of an activation row, all requested before the first is needed.
+typedef uint32_t u32x4_s __attribute__((ext_vector_type(4), aligned(4)));  // sixteen scale bytes
+
+// A unit of a row: sixteen blocks as four matrix instructions take them, lane group g the block 4 u + g of instruction u.  The
+// scales come in one load (one byte a lane is a load as slow each); the lane's byte of word u is its group's.
+constexpr uint32_t MX_UNIT = 16;
+struct Mx4Unit {
+    i32x4 q[4];
+    u32x4_s s;
+    __device__ __forceinline__ void load(const Mx4Row& w, uint32_t unit, uint32_t g) {
+        const uint64_t b = (uint64_t)MX_UNIT * unit;
+        s = *reinterpret_cast<const u32x4_s*>(w.s + b);
+#pragma unroll
+        for (int u = 0; u < 4; u++) q[u] = *reinterpret_cast<const i32x4*>(w.q + 16 * (b + 4 * u + g));
+    }
+    __device__ __forceinline__ uint32_t scale(int u, uint32_t g) const { return s[u] >> (8 * g); }
+};
+// A lane's block of four, past the row's end its first and the scale 1 (what it meets is zero)
+struct Mx4Block {
+    i32x4 q;
+    uint32_t s;
+    __device__ __forceinline__ void load(const Mx4Row& w, uint32_t b, uint32_t nb) {
+        const uint64_t bc = b < nb ? b : 0;
+        q = *reinterpret_cast<const i32x4*>(w.q + 16 * bc);
+        s = b < nb ? w.s[bc] : MX_ONE;
+    }
+};
+
+// U units of NM matrices' rows and of an activation row, all requested before the first is needed.
 template <uint32_t U, uint32_t NM>
-__device__ __forceinline__ void mx4_pieces(const Mx4Row (&w)[NM], Mx4Row x, uint32_t at, uint32_t step, uint32_t g, f32x4 (&acc)[NM]) {
-    i32x4 wq[NM][U], xq[U];
-    uint32_t ws[NM][U], xs[U];
+__device__ __forceinline__ void mx4_units(const Mx4Row (&w)[NM], const Mx4Row& x, uint32_t at, uint32_t step, uint32_t g,
+                                          f32x4 (&acc)[NM]) {
+    Mx4Unit wu[NM][U], xu[U];
 #pragma unroll
-    for (uint32_t u = 0; u < U; u++) {
-        const uint64_t b = 4ull * (at + u * step) + g;
-        xq[u] = *reinterpret_cast<const i32x4*>(x.q + 16 * b);
-        xs[u] = x.s[b];
+    for (uint32_t v = 0; v < U; v++) {
+        xu[v].load(x, at + v * step, g);
 #pragma unroll
-        for (uint32_t i = 0; i < NM; i++) wq[i][u] = *reinterpret_cast<const i32x4*>(w[i].q + 16 * b), ws[i][u] = w[i].s[b];
+        for (uint32_t i = 0; i < NM; i++) wu[i][v].load(w[i], at + v * step, g);
     }
     __builtin_amdgcn_sched_barrier(0);  // else some wait for others' registers
 #pragma unroll
-    for (uint32_t u = 0; u < U; u++)
+    for (uint32_t v = 0; v < U; v++)
 #pragma unroll
-        for (uint32_t i = 0; i < NM; i++) acc[i] = mfma_mx4(wq[i][u], ws[i][u], xq[u], xs[u], acc[i]);
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (uint32_t i = 0; i < NM; i++) acc[i] = mfma_mx4(wu[i][v].q[u], wu[i][v].scale(u, g), xu[v].q[u], xu[v].scale(u, g), acc[i]);
 }
 
 // The sums of 16 weight rows of NM matrices and 16 activation rows over this wave's share of K (nb blocks a row): every `step`-th
-// four blocks from the first-th on.  w, x: this lane's row of each (row lane % 16).
+// unit from the first-th on, and of what is left every `step`-th four blocks.  w, x: this lane's row of each (row lane % 16).
 template <uint32_t NM>
-__device__ __forceinline__ void mx4_strip(const Mx4Row (&w)[NM], Mx4Row x, uint32_t nb, uint32_t first, uint32_t step, uint32_t lane,
-                                          f32x4 (&acc)[NM]) {
+__device__ __forceinline__ void mx4_strip(const Mx4Row (&w)[NM], const Mx4Row& x, uint32_t nb, uint32_t first, uint32_t step,
+                                          uint32_t lane, f32x4 (&acc)[NM]) {
 #pragma unroll
     for (uint32_t i = 0; i < NM; i++) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const uint32_t g = lane / 16, whole = nb / 4;
-    uint32_t n = first < whole ? (whole - first + step - 1) / step : 0, at = first;  // whole groups of this wave
-    for (; n >= 8; n -= 8, at += 8 * step) mx4_pieces<8, NM>(w, x, at, step, g, acc);
-    if (n & 4) mx4_pieces<4, NM>(w, x, at, step, g, acc), at += 4 * step;
-    if (n & 2) mx4_pieces<2, NM>(w, x, at, step, g, acc), at += 2 * step;
-    if (n & 1) mx4_pieces<1, NM>(w, x, at, step, g, acc);
-    if (nb % 4 && whole % step == first) {  // the row's end: lanes past it multiply zeros, by 1
-        const bool in = g < nb % 4;
-        const uint64_t b = in ? 4ull * whole + g : 0;
-        const i32x4 xl = *reinterpret_cast<const i32x4*>(x.q + 16 * b);
-        const uint32_t xs = in ? x.s[b] : MX_ONE;
+    const uint32_t g = lane / 16, units = nb / MX_UNIT;
+    uint32_t n = first < units ? (units - first + step - 1) / step : 0, at = first;  // this wave's units
+    for (; n >= 2; n -= 2, at += 2 * step) mx4_units<2, NM>(w, x, at, step, g, acc);
+    if (n) mx4_units<1, NM>(w, x, at, step, g, acc);
+    for (uint32_t q = MX_UNIT / 4 * units + first; 4 * q < nb; q += step) {
+        Mx4Block wl[NM], xl;
+        xl.load(x, 4 * q + g, nb);
+        if (4 * q + g >= nb) xl.q = i32x4{0, 0, 0, 0};
 #pragma unroll
-        for (uint32_t i = 0; i < NM; i++) {
-            const i32x4 wl = *reinterpret_cast<const i32x4*>(w[i].q + 16 * b);
-            acc[i] = mfma_mx4(wl, in ? w[i].s[b] : MX_ONE, in ? xl : i32x4{0, 0, 0, 0}, xs, acc[i]);
-        }
+        for (uint32_t i = 0; i < NM; i++) wl[i].load(w[i], 4 * q + g, nb);
+#pragma unroll
+        for (uint32_t i = 0; i < NM; i++) acc[i] = mfma_mx4(wl[i].q, wl[i].s, xl.q, xl.s, acc[i]);
     }
 #pragma unroll
     for (uint32_t i = 0; i < NM; i++) mx_here(acc[i]);

@@ -355,7 +355,8 @@ struct Mx4Layer {
     const float* logits;  // [m][n_expert]: the caller's, or what the router's launch writes
     float *wlogits, *shlog;
     uint32_t *ids, *n_sel;
-    float *w, *h;
+    float* w;
+    uint8_t *xparts, *hparts;  // rows in parts (mx4_parts_bytes): of the tokens, of h [m * slots]
     void* y;
     uint32_t ydt;
     uint64_t ldy;
@@ -366,6 +367,7 @@ hipError_t launch_gemm_mx4(const Mx4Gemm& a, hipStream_t st);
 void launch_gemm_mx4_wide(const Mx4Gemm& a, hipStream_t st);  // k_mx4w.hip
 hipError_t launch_experts_up_mx4(const Mx4Up& a, const uint32_t* plan, hipStream_t st);
 hipError_t launch_experts_down_mx4(const Mx4Down& a, const uint32_t* plan, hipStream_t st);
+uint64_t mx4_parts_bytes(uint32_t blocks);
 hipError_t launch_moe_mx4(const Mx4Layer& a, const float* bias, const ScorePolicy& p, hipStream_t st);
 hipError_t launch_swiglu(const float* g, const float* u, float* y, size_t n, hipStream_t st);
 hipError_t launch_rmsnorm(const float* x, const float* w, float eps, uint32_t m, uint32_t n, float* y,
