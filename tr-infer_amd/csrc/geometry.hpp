@@ -273,6 +273,16 @@ inline uint64_t plan_words(uint32_t m, uint32_t slots, uint32_t E) {
     return plan_counts_at(m, slots, E) + (wgs > 1 ? (uint64_t)wgs * E : 0);
 }
 
+// trk_moe_mx4 (k_mx4l.hip): the choice by a launch of its own, or by each workgroup of the gate and up launch (`wgs` of them: 32
+// rows of an entry each).  us a layer, inside / apart, bf16 x, one shared expert: H = 2048, F = 512, 10 of 512: 1 token (176
+// workgroups) 18.8 / 20.4, 2 23.2 / 25.4, 4 (704) 32.8 / 34.7, 8 (1408) 52.9 / 50.7; 8 of 256, F = 768, 8 tokens (1728) 62.3 / 57.5;
+// 2 of 8, F = 1024, 8 (768) 22.9 / 24.9; 8 of 8 (2304) 50.0 / 46.0.
+inline bool layer_routes_apart(uint64_t wgs) { return wgs > 1024; }
+// Waves of its down launch (`wgs` workgroups: 16 rows of a token each), a slot at a time each.  us a layer, 4 / 12: the same
+// layers' 1 token (128 workgroups) 19.8 / 18.7, 2 24.4 / 23.1, 4 (512) 32.8 / 31.4, 8 (1024) 46.8 / 47.5; F = 768, 8 53.2 / 53.6;
+// few slots: 2 of 8, 8 21.1 / 23.0.
+inline uint32_t layer_down_waves(uint64_t wgs, uint32_t slots) { return slots <= 4 || wgs > 512 ? 4 : 12; }
+
 // Every invariant a call of m rows with kcap selections per token relies on; returns nullptr when
 // they hold, else what failed.  tq: the experts are TQ strips (k_tq.hip), not GGUF superblocks.
 inline const char* check_call(const Caps& c, uint32_t m, uint32_t kcap, bool tq = false) {

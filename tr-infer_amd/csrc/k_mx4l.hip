@@ -77,13 +77,16 @@ __device__ __forceinline__ void part_unit(const Mx4Row (&w)[NM], const uint8_t* 
         mul(std::integral_constant<int, 0>{}), mul(std::integral_constant<int, 1>{});
         mul(std::integral_constant<int, 2>{}), mul(std::integral_constant<int, 3>{});
     } else {
+        const uint32_t q0 = unit * (MX_UNIT / 4);
         Mx4Block wl[NM][4];
 #pragma unroll
         for (uint32_t u = 0; u < 4; u++)
+            if (4 * (q0 + u) < nb)  // the wave as a whole
 #pragma unroll
-            for (uint32_t i = 0; i < NM; i++) wl[i][u].load(w[i], unit * MX_UNIT + 4 * u + g, nb);
+                for (uint32_t i = 0; i < NM; i++) wl[i][u].load(w[i], q0 + u, g, nb);
         auto mul = [&](auto U) {
             constexpr int u = decltype(U)::value;
+            if (4 * (q0 + u) >= nb) return;
 #pragma unroll
             for (uint32_t i = 0; i < NM; i++) acc[i] = mfma_part<u>(wl[i][u].q, wl[i][u].s, xu, acc[i]);
         };
@@ -183,35 +186,61 @@ __global__ __launch_bounds__(LG_WAVES* WAVE) void layer_logits_kernel(Mx4Layer a
 
 constexpr uint32_t LU_WAVES = 4;
 
-// A workgroup takes 32 rows (a block of h) of gate and up and one entry; its waves share K.  Its first wave chooses the token's
-// experts, as route_scores_kernel does (a launch for it would take longer); the entry 0 of a token, first rows, leaves them
-// for the next launch.
+// Slot j of a token: its j-th expert, then the shared ones; none where the router chose fewer.
+__device__ __forceinline__ bool layer_slot(const Mx4Layer& a, uint32_t t, uint32_t j, uint32_t& e) {
+    const uint32_t k = a.slots - a.n_shared;
+    e = j < k ? a.ids[t * K_MAX + j] : a.n_expert + j - k;
+    return j >= k || j < a.n_sel[t];
+}
+
+// A wave's choice of its workgroup's token, as route_scores_kernel makes it; the workgroup of a token's first rows and entry
+// leaves it for the next launch.
 template <int NJ, bool SOFT, bool BIAS, bool GROUPED>
-__global__ __launch_bounds__(LU_WAVES* WAVE) void layer_up_kernel(Mx4Layer a, const float* __restrict__ bias, ScorePolicy p) {
-    extern __shared__ double keys[];  // [n_expert]
-    __shared__ uint2 cand[SC_CAND];
-    __shared__ uint32_t ids[K_MAX], n_sel;
-    __shared__ float wts[K_MAX];
-    __shared__ float part[2][LU_WAVES][MX_PARTS][32];  // [gate, up][wave][part][weight row]
-    const uint32_t strips = (a.gate.rows + 31) / 32, id = run_id(), r0 = id % strips * 32, en = id / strips;
-    const uint32_t t = en / a.slots, j = en % a.slots, k = a.slots - a.n_shared;
-    if (t >= a.m) return;  // the whole workgroup, here and below
-    const uint32_t wv = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, nb = a.gate.nb;
-    uint32_t e = a.n_expert + j - k;
-    if (j < k) {
-        if (wv == 0) {
+struct LayerChoice {
+    static constexpr bool HERE = true;
+    uint2 cand[SC_CAND];
+    uint32_t ids[K_MAX], n_sel;
+    float w[K_MAX];
+    __device__ __forceinline__ bool slot(const Mx4Layer& a, const float* __restrict__ bias, const ScorePolicy& p, uint32_t t, uint32_t j,
+                                         bool first, double* keys, uint32_t& e) {
+        const uint32_t k = a.slots - a.n_shared, lane = threadIdx.x % WAVE;
+        e = a.n_expert + j - k;
+        if (j >= k) return true;
+        if (threadIdx.x < WAVE) {
             const float* lg = a.logits + (uint64_t)t * a.n_expert;
-            if (!score_row32<NJ, SOFT, BIAS, GROUPED>(lg, bias, a.n_expert, p, lane, cand, ids, wts, &n_sel))
-                score_row(lg, bias, a.n_expert, p, lane, keys, ids, wts, &n_sel);
+            if (!score_row32<NJ, SOFT, BIAS, GROUPED>(lg, bias, a.n_expert, p, lane, cand, ids, w, &n_sel))
+                score_row(lg, bias, a.n_expert, p, lane, keys, ids, w, &n_sel);
         }
         __syncthreads();
-        if (r0 == 0 && j == 0) {
-            if (threadIdx.x < k) a.ids[t * K_MAX + threadIdx.x] = ids[threadIdx.x], a.w[t * K_MAX + threadIdx.x] = wts[threadIdx.x];
+        if (first && j == 0) {
+            if (threadIdx.x < k) a.ids[t * K_MAX + threadIdx.x] = ids[threadIdx.x], a.w[t * K_MAX + threadIdx.x] = w[threadIdx.x];
             if (threadIdx.x == 0) a.n_sel[t] = n_sel;
         }
-        if (j >= n_sel) return;
         e = __builtin_amdgcn_readfirstlane(ids[j]);
+        return j < n_sel;
     }
+};
+struct LayerChosen {  // by a launch before
+    static constexpr bool HERE = false;
+    __device__ __forceinline__ bool slot(const Mx4Layer& a, const float*, const ScorePolicy&, uint32_t t, uint32_t j, bool, double*,
+                                         uint32_t& e) {
+        return layer_slot(a, t, j, e);
+    }
+};
+
+// A workgroup takes 32 rows (a block of h) of gate and up and one entry; its waves share K.  (Eight waves, four for each half of
+// the rows, hold fewer registers and are slower: 8 tokens of 8 in 256, H = 2048, F = 768 57 us a layer against 53.)
+template <typename Choice>
+__global__ __launch_bounds__(LU_WAVES* WAVE) void layer_up_kernel(Mx4Layer a, const float* __restrict__ bias, ScorePolicy p) {
+    extern __shared__ double keys[];  // [n_expert]
+    __shared__ Choice choice;
+    __shared__ float part[2][LU_WAVES][MX_PARTS][32];  // [gate, up][wave][part][weight row]
+    const uint32_t strips = (a.gate.rows + 31) / 32, id = run_id(), r0 = id % strips * 32, en = id / strips;
+    const uint32_t t = en / a.slots, j = en % a.slots;
+    if (t >= a.m) return;  // the whole workgroup, here and below
+    const uint32_t wv = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, nb = a.gate.nb;
+    uint32_t e;
+    if (!choice.slot(a, bias, p, t, j, r0 == 0, keys, e)) return;
     const uint8_t* x = a.xparts + t * parts_bytes(nb);
     const Mx4Row w[4] = {layer_row(a.gate, e, r0, lane), layer_row(a.gate, e, r0 + 16, lane), layer_row(a.up, e, r0, lane),
                          layer_row(a.up, e, r0 + 16, lane)};
@@ -260,20 +289,11 @@ __global__ __launch_bounds__(LU_WAVES* WAVE) void layer_up_kernel(Mx4Layer a, co
 
 // ---- down, and the sum -------------------------------------------------------------------------------
 
-constexpr uint32_t LD_SLOTS = 64;  // most slots
-
-// Slot j of a token: its j-th expert, then the shared ones; none where the router chose fewer.
-__device__ __forceinline__ bool layer_slot(const Mx4Layer& a, uint32_t t, uint32_t j, uint32_t& e) {
-    const uint32_t k = a.slots - a.n_shared;
-    e = j < k ? a.ids[t * K_MAX + j] : a.n_expert + j - k;
-    return j >= k || j < a.n_sel[t];
-}
-
 // A workgroup takes 16 down rows and one token: a wave per slot, in turn where there are more.  Then a thread per (slot, row)
 // weights, and a thread per row adds in slot order.
 template <uint32_t DT, uint32_t WAVES>
 __global__ __launch_bounds__(WAVES* WAVE) void layer_down_kernel(Mx4Layer a) {
-    __shared__ float part[LD_SLOTS][MX_PARTS][16];
+    extern __shared__ float part[][MX_PARTS][16];  // [slots]
     const uint32_t strips = (a.down.rows + 15) / 16, id = run_id(), r0 = id % strips * 16, t = id / strips;
     if (t >= a.m) return;  // the whole workgroup
     const uint32_t wv = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, nb = a.down.nb;
@@ -324,7 +344,7 @@ template <int NJ>
 void launch_up(const Mx4Layer& a, const float* bias, const ScorePolicy& p, hipStream_t st) {
     const dim3 grid = run_of((uint64_t)((a.gate.rows + 31) / 32) * a.m * a.slots, LU_WAVES * WAVE);
     const size_t lds = a.n_expert * sizeof(double);
-#define GO(S, B, G) layer_up_kernel<NJ, S, B, G><<<grid, LU_WAVES * WAVE, lds, st>>>(a, bias, p)
+#define GO(S, B, G) layer_up_kernel<LayerChoice<NJ, S, B, G>><<<grid, LU_WAVES * WAVE, lds, st>>>(a, bias, p)
     const bool b = bias, g = p.n_group > 1;
     if (p.score == TRK_SCORE_SOFTMAX)
         b ? (g ? GO(true, true, true) : GO(true, true, false)) : (g ? GO(true, false, true) : GO(true, false, false));
@@ -335,10 +355,11 @@ void launch_up(const Mx4Layer& a, const float* bias, const ScorePolicy& p, hipSt
 template <uint32_t DT>
 void launch_down(const Mx4Layer& a, hipStream_t st) {
     const uint64_t wgs = (uint64_t)((a.down.rows + 15) / 16) * a.m;
-    if (a.slots <= 8)
-        layer_down_kernel<DT, 8><<<run_of(wgs, 8 * WAVE), 8 * WAVE, 0, st>>>(a);
+    const size_t lds = a.slots * MX_PARTS * 16 * sizeof(float);  // 64 slots at most: 36 KB
+    if (geo::layer_down_waves(wgs, a.slots) == 4)
+        layer_down_kernel<DT, 4><<<run_of(wgs, 4 * WAVE), 4 * WAVE, lds, st>>>(a);
     else
-        layer_down_kernel<DT, 16><<<run_of(wgs, 16 * WAVE), 16 * WAVE, 0, st>>>(a);
+        layer_down_kernel<DT, 12><<<run_of(wgs, 12 * WAVE), 12 * WAVE, lds, st>>>(a);
 }
 
 }  // namespace
@@ -351,6 +372,16 @@ hipError_t launch_moe_mx4(const Mx4Layer& a, const float* bias, const ScorePolic
                            : launch_before<TRK_DT_F16>(a, st);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
+    const uint64_t wgs = (uint64_t)((a.gate.rows + 31) / 32) * a.m * a.slots;
+    if (geo::layer_routes_apart(wgs)) {
+        if ((e = launch_route_scores(a.logits, bias, a.m, a.n_expert, policy, a.ids, a.w, a.n_sel, st)) != hipSuccess) return e;
+        layer_up_kernel<LayerChosen><<<run_of(wgs, LU_WAVES * WAVE), LU_WAVES * WAVE, 0, st>>>(a, bias, policy);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+        a.ydt == TRK_DT_F32    ? launch_down<TRK_DT_F32>(a, st)
+        : a.ydt == TRK_DT_BF16 ? launch_down<TRK_DT_BF16>(a, st)
+                               : launch_down<TRK_DT_F16>(a, st);
+        return hipGetLastError();
+    }
     ScorePolicy p = policy;
     const uint32_t nj = score_lanes(p, a.n_expert);
     if (nj <= 2)

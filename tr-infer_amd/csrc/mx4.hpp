@@ -58,14 +58,16 @@ struct Mx4Unit {
     }
     __device__ __forceinline__ uint32_t scale(int u, uint32_t g) const { return s[u] >> (8 * g); }
 };
-// A lane's block of four, past the row's end its first and the scale 1 (what it meets is zero)
+// A lane's block of the four from 4 q on (one at least is there), past the row's end the first and the scale 1: what it meets is zero
 struct Mx4Block {
     i32x4 q;
     uint32_t s;
-    __device__ __forceinline__ void load(const Mx4Row& w, uint32_t b, uint32_t nb) {
-        const uint64_t bc = b < nb ? b : 0;
-        q = *reinterpret_cast<const i32x4*>(w.q + 16 * bc);
-        s = b < nb ? w.s[bc] : MX_ONE;
+    __device__ __forceinline__ void load(const Mx4Row& w, uint32_t at, uint32_t g, uint32_t nb) {
+        const uint64_t b = 4ull * at;
+        const bool in = b + g < nb;
+        q = *reinterpret_cast<const i32x4*>(w.q + 16 * (b + (in ? g : 0)));
+        const uint32_t word = *reinterpret_cast<const uint32_t*>(w.s + b);
+        s = in ? word >> (8 * g) : MX_ONE;
     }
 };
 
@@ -102,10 +104,10 @@ __device__ __forceinline__ void mx4_strip(const Mx4Row (&w)[NM], const Mx4Row& x
     if (n) mx4_units<1, NM>(w, x, at, step, g, acc);
     for (uint32_t q = MX_UNIT / 4 * units + first; 4 * q < nb; q += step) {
         Mx4Block wl[NM], xl;
-        xl.load(x, 4 * q + g, nb);
+        xl.load(x, q, g, nb);
         if (4 * q + g >= nb) xl.q = i32x4{0, 0, 0, 0};
 #pragma unroll
-        for (uint32_t i = 0; i < NM; i++) wl[i].load(w[i], 4 * q + g, nb);
+        for (uint32_t i = 0; i < NM; i++) wl[i].load(w[i], q, g, nb);
 #pragma unroll
         for (uint32_t i = 0; i < NM; i++) acc[i] = mfma_mx4(wl[i].q, wl[i].s, xl.q, xl.s, acc[i]);
     }
