@@ -60,10 +60,15 @@ __global__ __launch_bounds__(Tile::T) void gemm_mx4_tile_kernel(Mx4Gemm g) {
     };
     t.template run<false, false>(lds, rw, wo, bx, xo, scales, g.w.nb, 0, t.wn + t.lane % 32, 32);
     typedef Elem<DT> O;
-    const uint32_t col = t.lane % (Tile::WN / 4) * 4, r = r0 + t.wn + col, left = r < g.w.rows ? g.w.rows - r : 0;
-    float bias[4];
+    const uint32_t r = r0 + t.wn + t.lane % (Tile::WN / 4) * 4, left = r < g.w.rows ? g.w.rows - r : 0;
+    const bool inside = g.vec && !g.accumulate && r0 + Tile::BN <= g.w.rows && t0 + Tile::BM <= g.m;  // the workgroup as a whole
+    f32x4 bias{0.0f, 0.0f, 0.0f, 0.0f};
+    if (g.bias) {
 #pragma unroll
-    for (uint32_t c = 0; c < 4; c++) bias[c] = g.bias && c < left ? g.bias[r + c] : 0.0f;
+        for (uint32_t c = 0; c < 4; c++) bias[c] = g.bias[c < left ? r + c : g.w.rows - 1];
+        asm volatile("" : "+v"(bias));  // here, or every store is waited for before the next
+    }
+    typename O::T* y0 = reinterpret_cast<typename O::T*>(g.y) + (uint64_t)(t0 + t.wm) * g.ldy + r;
 #pragma unroll
     for (int j = 0; j < Tile::FM; j++) {
         float v[Tile::WN / 8][4];
@@ -71,16 +76,20 @@ __global__ __launch_bounds__(Tile::T) void gemm_mx4_tile_kernel(Mx4Gemm g) {
         for (int i = 0; i < Tile::FN; i++)
 #pragma unroll
             for (int q = 0; q < 16; q++) v[4 * i + q / 4][q % 4] = t.acc[i][j][q];
-        t.template turn<Tile::WN>(lds, v, [&](uint32_t tr, uint32_t, f32x4 x) {
-            const uint32_t row = t0 + t.wm + 32 * j + tr;
-            if (row >= g.m || left == 0) return;
-            typename O::T* y = reinterpret_cast<typename O::T*>(g.y) + row * g.ldy + r;
-            float o[4];
+        if (inside)
+            t.template turn<Tile::WN>(lds, v, [&](uint32_t tr, uint32_t, f32x4 x) {
+                store4_whole<DT>(y0 + (32 * j + tr) * g.ldy, g.bias ? x + bias : x);
+            });
+        else
+            t.template turn<Tile::WN>(lds, v, [&](uint32_t tr, uint32_t, f32x4 x) {
+                if (t0 + t.wm + 32 * j + tr >= g.m || left == 0) return;
+                typename O::T* y = y0 + (32 * j + tr) * g.ldy;
+                float o[4];
 #pragma unroll
-            for (uint32_t c = 0; c < 4; c++) o[c] = g.bias ? x[c] + bias[c] : x[c];
-            if (g.accumulate) load_add4<DT>(y, o, left, g.vec);
-            store4<DT>(y, o, left, g.vec);
-        });
+                for (uint32_t c = 0; c < 4; c++) o[c] = g.bias ? x[c] + bias[c] : x[c];
+                if (g.accumulate) load_add4<DT>(y, o, left, g.vec);
+                store4<DT>(y, o, left, g.vec);
+            });
     }
 }
 

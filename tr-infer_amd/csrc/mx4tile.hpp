@@ -29,6 +29,21 @@ __device__ __forceinline__ void lds_dma4(i32x4 rsrc, uint32_t off, uint32_t lds)
                  : "memory", "m0");
 }
 
+// Four neighbouring values of a row of type DT, all there, on a boundary of four
+template <uint32_t DT>
+__device__ __forceinline__ void store4_whole(typename Elem<DT>::T* y, f32x4 v) {
+    if constexpr (DT == TRK_DT_F32) {
+        *reinterpret_cast<f32x4*>(y) = v;
+    } else {
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        typedef typename std::conditional<DT == TRK_DT_BF16, __bf16, _Float16>::type E;
+        typedef E e16x2 __attribute__((ext_vector_type(2)));
+        const uint32_t lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v[0], v[1]}), e16x2));
+        const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v[2], v[3]}), e16x2));
+        *reinterpret_cast<uint2*>(y) = make_uint2(lo, hi);
+    }
+}
+
 // ACC: the sums live in accumulator registers (a file built for those), which leaves the others to a wave tile of 128 x 128.
 template <int BN_, int BM_, int WN_, int WM_, int NST_, int GS_ = 4, bool ACC = false>
 struct Mx4Tile {
@@ -233,11 +248,12 @@ struct Mx4Tile {
         for (int g = 0; g < CW / 8; g++)
             *reinterpret_cast<f32x4*>(buf + lane % 32 * PITCH + 32 * g + 16 * (lane / 32)) = f32x4{v[g][0], v[g][1], v[g][2], v[g][3]};
         wave_sync();
+        f32x4 x[32 * LPR / WAVE];  // all of them before the first goes on
 #pragma unroll
-        for (uint32_t n = 0; n < 32 * LPR / WAVE; n++) {
-            const uint32_t r = (n * WAVE + lane) / LPR, c = lane % LPR * 4;
-            out(r, c, *reinterpret_cast<const f32x4*>(buf + r * PITCH + 4 * c));
-        }
+        for (uint32_t n = 0; n < 32 * LPR / WAVE; n++)
+            x[n] = *reinterpret_cast<const f32x4*>(buf + (n * WAVE + lane) / LPR * PITCH + lane % LPR * 16);
+#pragma unroll
+        for (uint32_t n = 0; n < 32 * LPR / WAVE; n++) out((n * WAVE + lane) / LPR, lane % LPR * 4, x[n]);
     }
 };
 
