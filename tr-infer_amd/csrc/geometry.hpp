@@ -273,6 +273,37 @@ inline uint64_t plan_words(uint32_t m, uint32_t slots, uint32_t E) {
     return plan_counts_at(m, slots, E) + (wgs > 1 ? (uint64_t)wgs * E : 0);
 }
 
+// trk_gemm_mx4 (k_mx4.hip): the int8 product's forms for 4-bit rows of nb blocks.  A form's time in ns, S stages of eight blocks,
+// fitted to 129 sizes; what it chooses there is 1.4 % slower than the best of each (us, strips / 64 x 32 / 64 x 64 / 128 x 128 /
+// 256 x 256): k = 512: [512] x 400 3.2 / 3.5 / 3.6 / 5.0 / 11, [5003] x 33 3.2 / 3.9 / 4.0 / 5.8 / 9.9, [12288] x 400 30 / 11.8 / 10.3 / 8.2 / 12.7,
+// x 4096 - / 81 / 67 / 38 / 33; k = 2560: [12288] x 1 4.3 / 5.7 / 5.7 / 9.2 / 19, x 64 16.5 / 7.1 / 6.0 / 10.6 / 20, x 800 - / 40 / 34 / 25 / 27,
+// x 4096 - / 190 / 151 / 89 / 85; k = 8192: [2560] x 33 10.8 / 11.8 / 12.1 / 22 / 46, x 800 - / 29 / 28 / 27 / 49, [12288] x 800 - / 100 / 81 / 64 / 62.
+inline uint64_t mx4_form_ns(I8Form f, uint32_t m, uint32_t rows, uint64_t S) {
+    if (f == I8_STRIP) {
+        const uint64_t n = i8_tiles(rows, m, 16, 16);  // one to four tokens' rows come from a cache
+        return 2200 + 60 * S + (m <= 4 ? n * 70 * S : n * (200 + 110 * S)) / 256;
+    }
+    auto per_cu = [&](uint32_t bn, uint32_t bm) { return (i8_tiles(rows, m, bn, bm) + 255) / 256; };
+    if (f == I8_TILE_32) {
+        const uint64_t n = i8_tiles(rows, m, 64, 32);
+        return 2900 + 270 * S + (n > 256 ? n - 256 : 0) * (550 + 142 * S) / 256;
+    }
+    if (f == I8_TILE_64) return 2900 + 272 * S + (per_cu(64, 64) - 1) * (900 + 219 * S);
+    if (f == I8_TILE_128) {  // two resident on a CU
+        const uint64_t n = per_cu(128, 128);
+        return 1500 + n / 2 * (4000 + 1050 * S) + n % 2 * (3300 + 560 * S);
+    }
+    return per_cu(256, 256) * (8500 + 1800 * S);
+}
+inline I8Form gemm_mx4_form(uint32_t m, uint32_t rows, uint32_t nb, uint64_t ldw, uint64_t ldx, uint64_t sldw, uint64_t sldx) {
+    // the tiles address their rows by 32-bit offsets from the first
+    if ((ldw | ldx | sldw | sldx) >= 1u << 23) return I8_STRIP;
+    I8Form best = I8_STRIP;
+    for (I8Form f : {I8_TILE_32, I8_TILE_64, I8_TILE_128, I8_TILE_256})
+        if (mx4_form_ns(f, m, rows, (nb + 7ull) / 8) < mx4_form_ns(best, m, rows, (nb + 7ull) / 8)) best = f;
+    return best;
+}
+
 // trk_moe_mx4 (k_mx4l.hip): the choice by a launch of its own, or by each workgroup of the gate and up launch (`wgs` of them: 32
 // rows of an entry each).  us a layer, inside / apart, bf16 x, one shared expert: H = 2048, F = 512, 10 of 512: 1 token (176
 // workgroups) 18.8 / 20.4, 2 23.2 / 25.4, 4 (704) 32.8 / 34.7, 8 (1408) 52.9 / 50.7; 8 of 256, F = 768, 8 tokens (1728) 62.3 / 57.5;

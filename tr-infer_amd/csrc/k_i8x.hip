@@ -327,8 +327,9 @@ __global__ __launch_bounds__(256) void experts_combine_kernel(I8Down a) {
             on[j] = j0 + j < n && a.ids[(size_t)t * K_MAX + jc] < a.down.count;
             if (j0 + j >= n) continue;  // a row of no entry is read (anything) and not added: no load waits for another
             const float* f = s + (uint64_t)jc * w;
-            if (w % 4 == 0) {
-                const f32x4 x = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(f));
+            if (r + 4 <= w) {
+                typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+                const f32x4_any x = __builtin_nontemporal_load(reinterpret_cast<const f32x4_any*>(f));
 #pragma unroll
                 for (uint32_t c = 0; c < 4; c++) p[j][c] = x[c];
             } else {

@@ -1,5 +1,5 @@
 // Rows to microscaled 4-bit values and back (trk_quantize_mx4, trk_dequantize_mx4), and their dense product (trk_gemm_mx4).
-#include "mx4gemm.hpp"
+#include "mx4tile.hpp"
 #include "rows.hpp"
 
 namespace trk {
@@ -200,6 +200,105 @@ void launch_strip(const Mx4Gemm& a, hipStream_t st) {
         gemm_mx4_strip_kernel<TRK_DT_F16><<<grid, ST_WAVES * WAVE, 0, st>>>(a);
 }
 
+// v += the four neighbouring values of a row at any address, `left` of them there
+template <uint32_t DT>
+__device__ __forceinline__ f32x4 load_add4(const typename Elem<DT>::T* y, f32x4 v, uint32_t left) {
+    typedef uint16_t u16x4_h __attribute__((ext_vector_type(4), aligned(2)));
+    typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+    if (left >= 4) {
+        typename std::conditional<DT == TRK_DT_F32, f32x4_any, u16x4_h>::type o;
+        o = *reinterpret_cast<const decltype(o)*>(y);
+#pragma unroll
+        for (uint32_t c = 0; c < 4; c++) v[c] += Elem<DT>::get(o[c]);
+        return v;
+    }
+#pragma unroll
+    for (uint32_t c = 0; c < 4; c++)
+        if (c < left) v[c] += Elem<DT>::get(y[c]);
+    return v;
+}
+
+// The tiles' place in the launch: panels of eight weight tiles, activation tiles after one another inside each, so that
+// the tiles that run at once on an XCD (a contiguous run of them) share rows of both in its L2.
+__device__ __forceinline__ void tile_place(uint32_t idx, uint32_t tn, uint32_t tm, uint32_t& n, uint32_t& m) {
+    const uint32_t panel = idx / (8 * tm), left = tn - panel * 8, w = left < 8 ? left : 8, rem = idx - panel * 8 * tm;
+    n = panel * 8 + rem % w, m = rem / w;
+}
+
+template <typename Tile, uint32_t DT>
+__global__ __launch_bounds__(Tile::T) void gemm_mx4_tile_kernel(Mx4Gemm g) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[Tile::LDS];
+    const uint32_t tn = (g.w.rows + Tile::BN - 1) / Tile::BN, tm = (g.m + Tile::BM - 1) / Tile::BM;
+    uint32_t idx, n, m;
+    if (!xcd_order_1d(tn * tm, idx, run_id())) return;  // the whole workgroup
+    tile_place(idx, tn, tm, n, m);
+    const uint32_t r0 = n * Tile::BN, t0 = m * Tile::BM, rl = g.w.rows - r0 - 1, tl = g.m - t0 - 1;  // the last rows there are
+    Tile t;
+    i32x4 rw[Tile::NA];
+    uint32_t wo[Tile::NA], xo[Tile::NB];
+    const i32x4 bw = buffer_at((const int8_t*)g.w.q + r0 * g.w.ld), bx = buffer_at((const int8_t*)g.x.q + t0 * g.x.ld);
+    const i32x4 bws = buffer_at((const int8_t*)g.w.s + r0 * g.w.lds), bxs = buffer_at((const int8_t*)g.x.s + t0 * g.x.lds);
+#pragma unroll
+    for (int i = 0; i < Tile::NA; i++) {
+        const uint32_t r = t.load_row(i);
+        rw[i] = bw, wo[i] = (r < rl ? r : rl) * (uint32_t)g.w.ld;
+    }
+#pragma unroll
+    for (int i = 0; i < Tile::NB; i++) {
+        const uint32_t r = t.load_row(i);
+        xo[i] = (r < tl ? r : tl) * (uint32_t)g.x.ld;
+    }
+    auto scales = [&](int i, i32x4& rs, uint32_t& so) {
+        const bool w = t.scale_load(i) < Tile::BN / Tile::SR;
+        const uint32_t r = t.scale_row(i) - (w ? 0 : Tile::BN), l = w ? rl : tl;
+        rs = w ? bws : bxs, so = (r < l ? r : l) * (uint32_t)(w ? g.w.lds : g.x.lds);
+    };
+    t.template run<false, false>(lds, rw, wo, bx, xo, scales, g.w.nb, 0, t.wn + t.lane % 32, 32);
+    typedef Elem<DT> O;
+    const uint32_t r = r0 + t.wn + t.lane % (Tile::WN / 4) * 4, left = r < g.w.rows ? g.w.rows - r : 0;
+    const bool inside = !g.accumulate && r0 + Tile::BN <= g.w.rows && t0 + Tile::BM <= g.m;  // the workgroup as a whole
+    f32x4 bias{0.0f, 0.0f, 0.0f, 0.0f};
+    if (g.bias) {
+#pragma unroll
+        for (uint32_t c = 0; c < 4; c++) bias[c] = g.bias[c < left ? r + c : g.w.rows - 1];
+        asm volatile("" : "+v"(bias));  // here, or every store is waited for before the next
+    }
+    typename O::T* y0 = reinterpret_cast<typename O::T*>(g.y) + (uint64_t)(t0 + t.wm) * g.ldy + r;
+#pragma unroll
+    for (int j = 0; j < Tile::FM; j++) {
+        float v[Tile::WN / 8][4];
+#pragma unroll
+        for (int i = 0; i < Tile::FN; i++)
+#pragma unroll
+            for (int q = 0; q < 16; q++) v[4 * i + q / 4][q % 4] = t.acc[i][j][q];
+        if (inside)
+            t.template turn<Tile::WN>(lds, v, [&](uint32_t tr, uint32_t, f32x4 x) {
+                store4_any<DT>(y0 + (32 * j + tr) * g.ldy, g.bias ? x + bias : x, 4);
+            });
+        else
+            t.template turn<Tile::WN>(lds, v, [&](uint32_t tr, uint32_t, f32x4 x) {
+                if (t0 + t.wm + 32 * j + tr >= g.m || left == 0) return;
+                typename O::T* y = y0 + (32 * j + tr) * g.ldy;
+                if (g.bias) x += bias;
+                if (g.accumulate) x = load_add4<DT>(y, x, left);
+                store4_any<DT>(y, x, left);
+            });
+    }
+}
+
+template <typename Tile>
+void launch_tile(const Mx4Gemm& a, hipStream_t st) {
+    const uint64_t wgs = (uint64_t)((a.w.rows + Tile::BN - 1) / Tile::BN) * (((uint64_t)a.m + Tile::BM - 1) / Tile::BM);
+    const geo::Grid2 g = geo::grid_run(wgs, Tile::T);
+    const dim3 grid(g.x, g.y);
+    if (a.dt == TRK_DT_F32)
+        gemm_mx4_tile_kernel<Tile, TRK_DT_F32><<<grid, Tile::T, 0, st>>>(a);
+    else if (a.dt == TRK_DT_BF16)
+        gemm_mx4_tile_kernel<Tile, TRK_DT_BF16><<<grid, Tile::T, 0, st>>>(a);
+    else
+        gemm_mx4_tile_kernel<Tile, TRK_DT_F16><<<grid, Tile::T, 0, st>>>(a);
+}
+
 }  // namespace
 
 hipError_t launch_rows_mx4(bool back, uint32_t dt, const void* x, uint64_t ldx, uint32_t m, uint32_t k, uint8_t* q, uint64_t ldq,
@@ -214,15 +313,11 @@ hipError_t launch_rows_mx4(bool back, uint32_t dt, const void* x, uint64_t ldx, 
 }
 
 hipError_t launch_gemm_mx4(const Mx4Gemm& a, hipStream_t st) {
-    static const int form = getenv("MX4_FORM") ? atoi(getenv("MX4_FORM")) : 0;  // PROBE
-    switch (form) {
-    case 1: launch_mx4_tile<Mx4Tile<64, 32, 32, 32, 4>>(a, st); break;
-    case 2: launch_mx4_tile<Mx4Tile<64, 64, 32, 32, 4>>(a, st); break;
-    case 3: launch_mx4_tile<Mx4Tile<128, 128, 64, 64, 2>>(a, st); break;
-    case 4: launch_mx4_tile<Mx4Tile<256, 256, 64, 128, 2, 8>>(a, st); break;
-    case 5: launch_mx4_tile<Mx4Tile<128, 64, 64, 32, 3>>(a, st); break;
-    case 6: launch_mx4_tile<Mx4Tile<256, 128, 64, 64, 3>>(a, st); break;
-    case 7: launch_gemm_mx4_wide(a, st); break;
+    switch (geo::gemm_mx4_form(a.m, a.w.rows, a.w.nb, a.w.ld, a.x.ld, a.w.lds, a.x.lds)) {
+    case geo::I8_TILE_256: launch_tile<Mx4Tile<256, 256, 64, 128, 2, 8>>(a, st); break;
+    case geo::I8_TILE_128: launch_tile<Mx4Tile<128, 128, 64, 64, 2>>(a, st); break;
+    case geo::I8_TILE_64: launch_tile<Mx4Tile<64, 64, 32, 32, 4>>(a, st); break;
+    case geo::I8_TILE_32: launch_tile<Mx4Tile<64, 32, 32, 32, 4>>(a, st); break;
     default: launch_strip(a, st);
     }
     return hipGetLastError();

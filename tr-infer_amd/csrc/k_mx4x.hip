@@ -162,7 +162,7 @@ __global__ __launch_bounds__(Tile::T) void experts_up_mx4_tile_kernel(Mx4Up a, P
     typedef Elem<DT> O;
     constexpr int CW = Tile::WN / 2;
     const uint32_t r = r0 + wr + t.lane % (CW / 4) * 4, left = r < a.gate.rows ? a.gate.rows - r : 0;
-    const bool whole = a.vec && r0 + BR <= a.gate.rows;  // the workgroup as a whole
+    const bool whole = r0 + BR <= a.gate.rows;  // the workgroup as a whole
 #pragma unroll
     for (int j = 0; j < Tile::FM; j++) {
         if (j >= (int)live) break;  // the wave as a whole
@@ -180,8 +180,7 @@ __global__ __launch_bounds__(Tile::T) void experts_up_mx4_tile_kernel(Mx4Up a, P
             const uint32_t e = __shfl(en[j], tr);
             if (t.wm + 32 * j + tr >= pt.rows || left == 0) return;
             typename O::T* h = reinterpret_cast<typename O::T*>(a.h) + e * a.ldh + r;
-            const float o[4] = {x[0], x[1], x[2], x[3]};
-            whole ? store4_whole<DT>(h, x) : store4<DT>(h, o, left, a.vec);
+            store4_any<DT>(h, x, whole ? 4 : left);
         });
     }
 }
@@ -210,7 +209,7 @@ __global__ __launch_bounds__(Tile::T) void experts_down_mx4_tile_kernel(Mx4Down 
     const Mx4Side ws = mx4_side(a.down, pt.expert, r0);
     mx4_expert_run<Tile, ONCE>(t, lds, ws, ws, Tile::BN, a.down.rows - r0 - 1, a.x, entry, a.down.nb, live, t.wn + c, 32);
     const uint32_t r = r0 + t.wn + t.lane % (Tile::WN / 4) * 4, left = r < a.down.rows ? a.down.rows - r : 0;
-    const bool whole = a.down.rows % 4 == 0 && r0 + Tile::BN <= a.down.rows;  // the workgroup as a whole
+    const bool whole = r0 + Tile::BN <= a.down.rows;  // the workgroup as a whole
 #pragma unroll
     for (int j = 0; j < Tile::FM; j++) {
         if (j >= (int)live) break;  // the wave as a whole
@@ -223,8 +222,7 @@ __global__ __launch_bounds__(Tile::T) void experts_down_mx4_tile_kernel(Mx4Down 
             const uint32_t e = __shfl(en[j], tr);
             if (t.wm + 32 * j + tr >= pt.rows || left == 0) return;
             float* y = a.work + (uint64_t)e * a.down.rows + r;
-            const float o[4] = {x[0], x[1], x[2], x[3]};
-            whole ? store4_whole<TRK_DT_F32>(y, x) : store4<TRK_DT_F32>(y, o, left, false);
+            store4_any<TRK_DT_F32>(y, x, whole ? 4 : left);
         });
     }
 }

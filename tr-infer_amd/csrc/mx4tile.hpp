@@ -29,23 +29,30 @@ __device__ __forceinline__ void lds_dma4(i32x4 rsrc, uint32_t off, uint32_t lds)
                  : "memory", "m0");
 }
 
-// Four neighbouring values of a row of type DT, all there, on a boundary of four
+// Four neighbouring values of a row of type DT at any address, `left` of them there
 template <uint32_t DT>
-__device__ __forceinline__ void store4_whole(typename Elem<DT>::T* y, f32x4 v) {
-    if constexpr (DT == TRK_DT_F32) {
-        *reinterpret_cast<f32x4*>(y) = v;
-    } else {
-        typedef float f32x2 __attribute__((ext_vector_type(2)));
-        typedef typename std::conditional<DT == TRK_DT_BF16, __bf16, _Float16>::type E;
-        typedef E e16x2 __attribute__((ext_vector_type(2)));
-        const uint32_t lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v[0], v[1]}), e16x2));
-        const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v[2], v[3]}), e16x2));
-        *reinterpret_cast<uint2*>(y) = make_uint2(lo, hi);
+__device__ __forceinline__ void store4_any(typename Elem<DT>::T* y, f32x4 v, uint32_t left) {
+    if (left >= 4) {
+        if constexpr (DT == TRK_DT_F32) {
+            typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+            *reinterpret_cast<f32x4_any*>(y) = v;
+        } else {
+            typedef float f32x2 __attribute__((ext_vector_type(2)));
+            typedef uint32_t u32x2_h __attribute__((ext_vector_type(2), aligned(2)));
+            typedef typename std::conditional<DT == TRK_DT_BF16, __bf16, _Float16>::type E;
+            typedef E e16x2 __attribute__((ext_vector_type(2)));
+            *reinterpret_cast<u32x2_h*>(y) =
+                u32x2_h{__builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v[0], v[1]}), e16x2)),
+                        __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v[2], v[3]}), e16x2))};
+        }
+        return;
     }
+#pragma unroll
+    for (uint32_t c = 0; c < 4; c++)
+        if (c < left) y[c] = Elem<DT>::put(v[c]);
 }
 
-// ACC: the sums live in accumulator registers (a file built for those), which leaves the others to a wave tile of 128 x 128.
-template <int BN_, int BM_, int WN_, int WM_, int NST_, int GS_ = 4, bool ACC = false>
+template <int BN_, int BM_, int WN_, int WM_, int NST_, int GS_ = 4>
 struct Mx4Tile {
     static constexpr int BN = BN_, BM = BM_, WN = WN_, WM = WM_, NST = NST_, GS = GS_, BK = 128;  // BK: a stage's bytes of a row
     static constexpr int NW = BN / WN * (BM / WM), T = NW * WAVE;
@@ -142,12 +149,7 @@ struct Mx4Tile {
                     // the products stay where they are: on their side of the barrier, and before any branch that lanes part at
                     // (their operands would be made in the lanes that take it alone)
 #pragma unroll
-                    for (int i = 0; i < FN; i++) {
-                        if constexpr (ACC)
-                            asm volatile("" : "+a"(acc[i][j]));
-                        else
-                            asm volatile("" : "+v"(acc[i][j]));
-                    }
+                    for (int i = 0; i < FN; i++) asm volatile("" : "+v"(acc[i][j]));
                 }
                 if constexpr (decltype(loads)::value)
 #pragma unroll

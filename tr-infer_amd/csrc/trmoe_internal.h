@@ -364,7 +364,6 @@ struct Mx4Layer {
 hipError_t launch_rows_mx4(bool back, uint32_t dt, const void* x, uint64_t ldx, uint32_t m, uint32_t k, uint8_t* q, uint64_t ldq,
                            uint8_t* s, uint64_t lds, void* y, uint64_t ldy, hipStream_t st);
 hipError_t launch_gemm_mx4(const Mx4Gemm& a, hipStream_t st);
-void launch_gemm_mx4_wide(const Mx4Gemm& a, hipStream_t st);  // k_mx4w.hip
 hipError_t launch_experts_up_mx4(const Mx4Up& a, const uint32_t* plan, hipStream_t st);
 hipError_t launch_experts_down_mx4(const Mx4Down& a, const uint32_t* plan, hipStream_t st);
 uint64_t mx4_parts_bytes(uint32_t blocks);
