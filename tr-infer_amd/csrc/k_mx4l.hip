@@ -197,7 +197,6 @@ __device__ __forceinline__ bool layer_slot(const Mx4Layer& a, uint32_t t, uint32
 // leaves it for the next launch.
 template <int NJ, bool SOFT, bool BIAS, bool GROUPED>
 struct LayerChoice {
-    static constexpr bool HERE = true;
     uint2 cand[SC_CAND];
     uint32_t ids[K_MAX], n_sel;
     float w[K_MAX];
@@ -221,7 +220,6 @@ struct LayerChoice {
     }
 };
 struct LayerChosen {  // by a launch before
-    static constexpr bool HERE = false;
     __device__ __forceinline__ bool slot(const Mx4Layer& a, const float*, const ScorePolicy&, uint32_t t, uint32_t j, bool, double*,
                                          uint32_t& e) {
         return layer_slot(a, t, j, e);

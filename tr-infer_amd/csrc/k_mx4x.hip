@@ -284,15 +284,6 @@ void launch_up_tile(const Mx4Up& a, const Plan& P, uint64_t tiles, hipStream_t s
         experts_up_mx4_tile_kernel<Tile, TRK_DT_F16, ONCE><<<g, Tile::T, 0, st>>>(a, P);
 }
 
-template <bool ONCE>
-void launch_up_128(const Mx4Up& a, const Plan& P, uint64_t tiles, geo::ExpertsWidth w, hipStream_t st) {
-    if (w == geo::X_NARROW)
-        launch_up_tile<Mx4Tile<64, 128, 32, 64, 3>, ONCE>(a, P, tiles, st);
-    else
-        w == geo::X_WIDE ? launch_up_tile<Mx4Tile<256, 128, 64, 64, 3>, ONCE>(a, P, tiles, st)
-                         : launch_up_tile<Mx4Tile<128, 128, 64, 64, 2>, ONCE>(a, P, tiles, st);
-}
-
 template <typename Tile, bool ONCE = true>
 void launch_down_tile(const Mx4Down& a, const Plan& P, uint64_t tiles, hipStream_t st) {
     const dim3 g = run_of((a.down.rows + Tile::BN - 1) / Tile::BN * tiles, Tile::T);
@@ -315,17 +306,22 @@ hipError_t launch_experts_up_mx4(const Mx4Up& a, const uint32_t* plan, hipStream
     const uint32_t rows = geo::plan_rows(a.m, a.slots, E);
     const Plan P = plan_at(const_cast<uint32_t*>(plan), a.m, a.slots);
     const uint64_t tiles = geo::plan_tiles(a.m, a.slots, E, rows);
-    const geo::ExpertsWidth w = geo::experts_width(2 * a.gate.rows, tiles, rows == 128);
+    const bool narrow = geo::experts_width(2 * a.gate.rows, tiles, false) == geo::X_NARROW;
+    // us at 128 entries a tile, four waves of 64 x 64 / eight of 32 x 64, two workgroups on a CU either way / 256 x 128 by eight of 64 x
+    // 64: 2000 tokens of 8 in 128 (H = 2048, F = 768) 89.7 / 87.4 / 92.4, 400 of 8 in 64 (1024, 512) - / 18.1 / 20.3, 3000 of 2 in 8 (2048, 1024)
+    // 39.7 / 37.9 / 40.4, 4096 of 10 in 512 (2048, 512) 177 / 175 / 182
     if (rows == 32)
-        w == geo::X_NARROW ? launch_up_tile<Mx4Tile<64, 32, 32, 32, 4>>(a, P, tiles, st)
-                           : launch_up_tile<Mx4Tile<128, 32, 32, 32, 3>>(a, P, tiles, st);
+        narrow ? launch_up_tile<Mx4Tile<64, 32, 32, 32, 4>>(a, P, tiles, st)
+               : launch_up_tile<Mx4Tile<128, 32, 32, 32, 3>>(a, P, tiles, st);
     else if (rows == 64)
-        w == geo::X_NARROW ? launch_up_tile<Mx4Tile<64, 64, 32, 32, 4>>(a, P, tiles, st)
-                           : launch_up_tile<Mx4Tile<128, 64, 64, 32, 3>>(a, P, tiles, st);
+        narrow ? launch_up_tile<Mx4Tile<64, 64, 32, 32, 4>>(a, P, tiles, st)
+               : launch_up_tile<Mx4Tile<128, 64, 64, 32, 3>>(a, P, tiles, st);
     else if (geo::experts_once(a.m, a.slots, E, 64))
-        launch_up_128<true>(a, P, tiles, w, st);
+        narrow ? launch_up_tile<Mx4Tile<64, 128, 32, 64, 3>>(a, P, tiles, st)
+               : launch_up_tile<Mx4Tile<128, 128, 32, 64, 2>>(a, P, tiles, st);
     else
-        launch_up_128<false>(a, P, tiles, w, st);
+        narrow ? launch_up_tile<Mx4Tile<64, 128, 32, 64, 3>, false>(a, P, tiles, st)
+               : launch_up_tile<Mx4Tile<128, 128, 32, 64, 2>, false>(a, P, tiles, st);
     return hipGetLastError();
 }
 
@@ -339,12 +335,14 @@ hipError_t launch_experts_down_mx4(const Mx4Down& a, const uint32_t* plan, hipSt
     const Plan P = plan_at(const_cast<uint32_t*>(plan), a.m, a.slots);
     const uint64_t tiles = geo::plan_tiles(a.m, a.slots, E, rows);
     const bool narrow = geo::experts_width(a.down.rows, tiles, false) == geo::X_NARROW;
+    // An expert's rows are short: more workgroups on a CU are worth more than a third stage.  us, three stages / two: 512 tokens of 10 in
+    // 512 (H = 2048, F = 512) 97 / 83, 150 of 6 in 60 (1100, 347) 18.8 / 17.2, 300 of 8 in 128 (2048, 768) 42.3 / 41.2; 2000 of 10 in 512 144 / 133.
     if (rows == 32)
         narrow ? launch_down_tile<Mx4Tile<64, 32, 32, 32, 4>>(a, P, tiles, st)
-               : launch_down_tile<Mx4Tile<128, 32, 32, 32, 3>>(a, P, tiles, st);
+               : launch_down_tile<Mx4Tile<128, 32, 32, 32, 2>>(a, P, tiles, st);
     else if (rows == 64)
         narrow ? launch_down_tile<Mx4Tile<64, 64, 32, 32, 4>>(a, P, tiles, st)
-               : launch_down_tile<Mx4Tile<128, 64, 64, 32, 3>>(a, P, tiles, st);
+               : launch_down_tile<Mx4Tile<128, 64, 32, 32, 2>>(a, P, tiles, st);
     else if (geo::experts_once(a.m, a.slots, E, 128))
         narrow ? launch_down_tile<Mx4Tile<64, 128, 32, 64, 3>>(a, P, tiles, st)
                : launch_down_tile<Mx4Tile<128, 128, 64, 64, 2>>(a, P, tiles, st);

@@ -951,23 +951,24 @@ class MX4Weights:
         self.device = q.get_device()
 
 
-def _mx4_empty(torch, m, k, device):
-    """4-bit rows and scales [m][blocks], the scales' rows a multiple of 4 bytes apart."""
-    nb = _mx4_blocks(k)
-    q = torch.empty((m, 16 * nb), dtype=torch.uint8, device=device)
-    if nb % 4 == 0:
-        return q, q.new_empty((m, nb))
-    return q, q.new_empty((m, (nb + 3) // 4 * 4))[:, :nb]
-
-
 def quantize_mx4(x, out=None, stream=None):
-    """trk_quantize_mx4: x [m][k] -> (q uint8 [m][16 * blocks], scale uint8 [m][blocks])."""
+    """trk_quantize_mx4: x [m][k] -> (q uint8 [m][16 * blocks], scale uint8 [m][blocks]); the scales' rows of a new pair are a
+    multiple of 4 bytes apart."""
     torch = _torch or _late()
     ldx = _rows(x, "x")
     m, k = x.shape
-    q, scale = _mx4_empty(torch, m, k, x.device) if out is None else out
-    ldq, lds = _mx4_rows(q, scale, m, k, "q")
-    _here(x, q, scale)
+    if out is None:
+        nb = (k + 31) // 32
+        ldq, lds = 16 * nb, (nb + 3) // 4 * 4
+        q = torch.empty((m, ldq), dtype=torch.uint8, device=x.device)
+        scale = q.new_empty((m, lds))
+        if lds != nb:
+            scale = scale[:, :nb]
+        _here(x)
+    else:
+        q, scale = out
+        ldq, lds = _mx4_rows(q, scale, m, k, "q")
+        _here(x, q, scale)
     check(lib().trk_quantize_mx4(x.data_ptr(), _dtype(x.dtype), ldx, m, k, q.data_ptr(), ldq, scale.data_ptr(), lds,
                                  _stream_here(stream)))
     return q, scale
@@ -977,11 +978,14 @@ def dequantize_mx4(q, scale, k, dtype=None, out=None, stream=None):
     """trk_dequantize_mx4: 4-bit rows of k values -> [m][k] (float32 unless `dtype` or `out` says otherwise)."""
     torch = _torch or _late()
     m = q.shape[0]
-    _u32(m, k)
+    if (m | k) >> 32 or k < 0:
+        _u32(m, k)
     ldq, lds = _mx4_rows(q, scale, m, k, "q")
     if out is None:
         out = torch.empty((m, k), dtype=dtype or torch.float32, device=q.device)
-    ldy = _rows(out, "out", m, k)
+        ldy = k
+    else:
+        ldy = _rows(out, "out", m, k)
     _here(q, scale, out)
     check(lib().trk_dequantize_mx4(q.data_ptr(), ldq, scale.data_ptr(), lds, m, k, out.data_ptr(), _dtype(out.dtype), ldy,
                                    _stream_here(stream)))
