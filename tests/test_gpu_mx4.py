@@ -141,6 +141,28 @@ def test_gemm(m, rows, k, dtype):
     within(host(y), want if bias is None else want + bias, tol)
 
 
+@pytest.mark.parametrize("m,rows,k,bias,acc", [(4000, 4000, 2100, False, False), (4096, 4096, 2080, True, False), (4001, 4003, 300, True, True)])
+def test_gemm_large(m, rows, k, bias, acc):
+    """Tiles of 256 x 256, whole and ragged: several groups of scales, a bias, an output that is added to."""
+    import torch
+    say(f"gemm_mx4 large {m} x {rows} x {k}")
+    rng = np.random.default_rng(3)
+    (q, s), (wq, ws) = rows4(rng, m, k), rows4(rng, rows, k)
+    W, xs = trmoe.MX4Weights(*apart(wq, ws), k), apart(q, s)
+    b = rng.standard_normal(rows).astype(np.float32) if bias else None
+    old = torch.randn((m, rows), device="cuda") if acc else None
+    y = trmoe.gemm_mx4(W, *xs, bias=None if b is None else dev(b), out=None if old is None else old.clone(), accumulate=acc)
+    x, w = dev(R.values(q, s, k)), dev(R.values(wq, ws, k))  # in 64 bits on the GPU
+    want, mag = x @ w.T, x.abs() @ w.abs().T
+    tol = (R.blocks(k) + 8) * R.STEP * mag + 2 ** -23 * want.abs()
+    if bias:
+        want, tol = want + dev(b).double(), tol + 2 ** -23 * (want.abs() + dev(b).abs())
+    if acc:
+        want, tol = want + old.double(), tol + 2 ** -23 * (want.abs() + old.abs())
+    far = ((y.double() - want).abs() / (tol + 1e-30)).max().item()
+    assert far <= 1, far
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("m,rows,k", [(3, 50, 70), (200, 300, 160)])
 def test_gemm_accumulates_and_takes_an_item(dtype, m, rows, k):
@@ -284,6 +306,95 @@ def test_experts_down(m, E, slots, F, H, kind, dtype):
     assert (want[n == 0] == 0).all() and (host(before)[n == 0] == 0).all()
 
 
+# m, E, slots, k, rows (of gate and up, or of down): every shape of tile, several stages and groups of scales
+MANY = [(300, 200, 4, 1100, 272, "even"), (500, 64, 4, 640, 400, "ragged"), (1000, 64, 4, 2100, 390, "even"),
+        (2000, 16, 4, 416, 512, "one"), (60, 20, 2, 2100, 96, "foreign"), (120, 12, 4, 1300, 130, "even"), (900, 8, 2, 1600, 80, "even")]
+
+
+@pytest.mark.parametrize("m,E,slots,k,rows,kind", MANY)
+def test_experts_of_many_entries(m, E, slots, k, rows, kind):
+    import torch
+    say(f"experts mx4 many m={m} E={E} slots={slots} k={k} rows={rows} {kind}")
+    rng = np.random.default_rng(m + E)
+    (gq, gs), (uq, us) = rows4(rng, E, rows, k, spread=k ** -0.5), rows4(rng, E, rows, k, spread=k ** -0.5)
+    (xq, xs), (hq, hs) = rows4(rng, m, k), rows4(rng, m * slots, k)
+    ids, w, n = routing(rng, m, E, slots, kind)
+    idt, nt, wt = dev(ids), dev(n), dev(w)
+    plan = trmoe.experts_plan(idt, nt, slots, E)
+    G, U = trmoe.MX4Weights(*apart(gq, gs), k), trmoe.MX4Weights(*apart(uq, us), k)
+    h = torch.full((m * slots, rows), 9.0, device="cuda")
+    trmoe.experts_up_mx4(G, U, *apart(xq, xs), idt, nt, slots, plan=plan, out=h)
+    y = host(trmoe.experts_down_mx4(G, *apart(hq, hs), idt, wt, nt, slots, plan=plan))
+    x, x2, gate, up = R.values(xq, xs, k), R.values(hq, hs, k), R.values(gq, gs, k), R.values(uq, us, k)
+    there, got = i8ref.entries(ids, n, slots, E), host(h)
+    assert (got[~there.reshape(-1)] == 9).all()
+    want, tol, mag = np.zeros((m, rows)), np.zeros((m, rows)), np.zeros((m, rows))
+    for e in range(E):
+        t, j = np.nonzero(there & (ids[:, :slots] == e))
+        if not t.size:
+            continue
+        g, u = x[t] @ gate[e].T, x[t] @ up[e].T
+        within(got[t * slots + j], R.silu(g) * u, R.swiglu_tol(g, u, R.sum_tol(x[t], gate[e]), R.sum_tol(x[t], up[e]), "f32"))
+        share, rows_ = w[t, j].astype(np.float64)[:, None], x2[t * slots + j]
+        v = rows_ @ gate[e].T * share
+        np.add.at(want, t, v), np.add.at(mag, t, np.abs(v)), np.add.at(tol, t, R.sum_tol(rows_, gate[e]) * share)
+    tol = tol + (slots + 2) * i8ref.EPS["f32"] * mag
+    within(y, want, tol + 1.01 * i8ref.round_rel(mag + tol, "f32"))
+
+
+@pytest.mark.parametrize("call", ["up", "down"])
+@pytest.mark.parametrize("made", [(100, 2, 8), (90, 3, 8), (100, 3, 9)])
+def test_a_plan_of_another_call(call, made):
+    """A plan made for another m, slots or number of experts, of as many words or more, is not followed: what it would write is
+    NaN, and nothing else is written."""
+    import torch
+    say(f"experts mx4 {call} with a plan of {made}")
+    rng = np.random.default_rng(5)
+    m, slots, E, k, rows = 100, 3, 8, 96, 64
+    ids, w, n = routing(rng, m, E, slots, "ragged")
+    idt, nt, wt = dev(ids), dev(n), dev(w)
+    oids, _, on = routing(rng, made[0], made[2], made[1], "even")
+    words = trmoe._plan_words(m, slots, E)
+    plan = torch.zeros(words + 4096, dtype=torch.int32, device="cuda")
+    other = trmoe.experts_plan(dev(oids), dev(on), made[1], made[2])
+    plan[:other.numel()] = other[:plan.numel()]
+    plan = plan[:words].contiguous()
+    G = trmoe.MX4Weights(*apart(*rows4(rng, E, rows, k)), k)
+    there = i8ref.entries(ids, n, slots, E)
+    if call == "up":
+        h = torch.full((m * slots, rows), 9.0, device="cuda")
+        trmoe.experts_up_mx4(G, G, *apart(*rows4(rng, m, k)), idt, nt, slots, plan=plan, out=h)
+        got = host(h)
+        assert np.isnan(got[there.reshape(-1)]).all() and (got[~there.reshape(-1)] == 9).all()
+    else:
+        y = host(trmoe.experts_down_mx4(G, *apart(*rows4(rng, m * slots, k)), idt, wt, nt, slots, plan=plan))
+        assert np.isnan(y[there.any(1)]).all() and (y[~there.any(1)] == 0).all()
+
+
+def test_rows_far_apart():
+    """Rows whose tiles' 32-bit offsets would not hold them go entry by entry, tile by strip."""
+    import torch
+    say("mx4 rows far apart")
+    rng = np.random.default_rng(6)
+    m, E, slots, k, rows = 40, 3, 2, 96, 40
+    (wq, ws), (xq, xs) = rows4(rng, E, rows, k), rows4(rng, m, k)
+    ids, w, n = routing(rng, m, E, slots, "even")
+    plan = trmoe.experts_plan(dev(ids), dev(n), slots, E)
+    near = trmoe.MX4Weights(dev(wq), apart(wq, ws, 0)[1], k)
+    far = torch.zeros((E, rows, 1 << 23), dtype=torch.uint8, device="cuda")[:, :, :48]
+    far.copy_(dev(wq))
+    F = trmoe.MX4Weights(far, near.scale, k)
+    sx = torch.zeros((m, 1 << 23), dtype=torch.uint8, device="cuda")[:, :3]
+    sx.copy_(dev(xs))
+    x, xn = (dev(xq), sx), (dev(xq), apart(xq, xs, 0)[1])
+    for W, rowsx in ((F, xn), (near, x), (F, x)):
+        assert torch.equal(trmoe.gemm_mx4(W, *rowsx, item=1), trmoe.gemm_mx4(near, *xn, item=1))
+        a = trmoe.experts_up_mx4(W, near, *rowsx, dev(ids), dev(n), slots, plan=plan)
+        b = trmoe.experts_up_mx4(near, near, *xn, dev(ids), dev(n), slots, plan=plan)
+        tol = 1e-5 * b.abs().max()
+        assert (a - b).abs().max() <= tol
+
+
 # ---- the layer ---------------------------------------------------------------------------------------
 
 def layer_of(rng, E, H, F, n_shared=0, gated=False, bias=False, router=True):
@@ -337,6 +448,24 @@ def test_layer(m, E, k, H, F, shared, gated, bias, score, groups, keep, xt, yt):
     # the logits given: the same experts
     y2 = trmoe.moe_mx4(L, xd, rlog=dev(logits.astype(np.float32)), score=score, dtype=torch.float32, **kw)
     within(host(y2), want, R.layer(x, w["gate"], w["up"], w["down"], ids, share, "f32")[1] + tol)
+
+
+@pytest.mark.parametrize("m,E,k,H,F,shared", [(8, 40, 8, 512, 600, 1), (8, 16, 2, 1030, 1100, 0), (5, 300, 12, 640, 200, 2)])
+def test_layer_of_many_entries(m, E, k, H, F, shared):
+    """The choice by a launch of its own, several units of K, slots in turn."""
+    say(f"moe_mx4 many m={m} E={E} k={k} H={H} F={F} shared={shared}")
+    rng = np.random.default_rng(m + E + k)
+    L, w, _, _, _ = layer_of(rng, E, H, F, shared, router=False)
+    x = rng.standard_normal((m, H)).astype(np.float32) * np.exp2(rng.integers(-20, 20, (m, H // 2 + 1)).repeat(2, 1)[:, :H]).astype(np.float32)
+    x = x / np.abs(x).max() * 4  # values far below their block's largest
+    logits = (rng.permutation(m * E).reshape(m, E) / (m * E)).astype(np.float32)
+    kw = dict(k=k, n_group=1, topk_group=1, group_top=2, renorm=False, factor=1.0)
+    rid, rw, rn = i8ref.route(logits, bias=None, score="sigmoid", **kw)
+    ids = np.concatenate((rid, np.tile(np.arange(E, E + shared), (m, 1))), 1)
+    share = np.concatenate((rw, np.ones((m, shared))), 1)
+    y = host(trmoe.moe_mx4(L, dev(x), rlog=dev(logits), score="sigmoid", **kw))
+    want, tol = R.layer(x.astype(np.float64), w["gate"], w["up"], w["down"], ids, share, "f32")
+    within(y, want, tol)
 
 
 def test_layer_rows_that_choose_nothing():

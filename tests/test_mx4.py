@@ -109,7 +109,9 @@ def moe(w=None, p=None, x=P, xdt=0, ldx=100, rlog=None, m=3, work=P, y=P, ydt=0,
 @pytest.mark.parametrize("kw,rc,word", [
     (dict(w=layer_w(up=mat(rows=63))), -1, "differ"), (dict(w=layer_w(down=mat())), -1, "go back"),
     (dict(w=layer_w(gate=mat(ptr=8))), -1, "multiples"), (dict(w=layer_w(n_shared=4)), -1, "n_expert"),
-    (dict(w=layer_w(n_shared=33)), -1, "n_shared"), (dict(w=layer_w(router=0)), -1, "router"), (dict(m=9), -3, "m (9)"),
+    (dict(w=layer_w(n_shared=33)), -1, "n_shared"),
+    (dict(w=layer_w(gate=mat(rows=(1 << 24) + 1, count=1), up=mat(rows=(1 << 24) + 1, count=1),
+                    down=mat(rows=100, k=(1 << 24) + 1, ld=1 << 23 | 16, scale_ld=1 << 20, count=1)), p=policy(k=1)), -1, "at most"), (dict(w=layer_w(router=0)), -1, "router"), (dict(m=9), -3, "m (9)"),
     (dict(p=policy(k=5)), -2, "k (5)"), (dict(p=policy(k=0)), -2, "k (0)"), (dict(w=layer_w(n_shared=3)), -2, "k (2)"),
     (dict(p=policy(n_group=3)), -2, "n_group"), (dict(p=policy(factor=float("nan"))), -2, "factor"),
     (dict(xdt=3), -1, "element type"), (dict(ydt=3), -1, "element type"), (dict(ldx=99), -1, "stride"), (dict(ldy=99), -1, "stride"),
@@ -162,6 +164,18 @@ def test_python_calls_refuse():
         trmoe.dequantize_mx4(q, torch.zeros((3, 2), dtype=torch.uint8), 64)
     with pytest.raises(trmoe.TrkError, match="32 bits"):
         trmoe.dequantize_mx4(q, s, 1 << 32)
+
+
+def test_forms_on_the_host(tmp_path):
+    """The rules that choose a form, at sizes where the forms were timed."""
+    import os
+    import subprocess
+    here = os.path.dirname(os.path.abspath(__file__))
+    exe = str(tmp_path / "mx4_rules_check")
+    subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-Werror", os.path.join(here, "mx4_rules_check.cpp"), "-o", exe],
+                   check=True)
+    out = subprocess.run([exe], check=True, capture_output=True, text=True).stdout
+    assert out.startswith("ok"), out
 
 
 def test_the_plain_form_rounds_as_it_says():

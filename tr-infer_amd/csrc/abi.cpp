@@ -1068,7 +1068,7 @@ extern "C" int trk_experts_down_i8(const trk_i8_mat* down, const int8_t* q, uint
 // ---- microscaled 4-bit rows ---------------------------------------------------------------------------
 
 constexpr uint32_t MX4_K_MAX = 1u << 30;  // places in a row are counted by 32 bits
-constexpr uint32_t MX4_SHARED_MAX = 32;
+constexpr uint32_t MX4_SHARED_MAX = 32, MX4_LAYER_MAX = 1u << 24;  // the layer's workgroups are numbered by 32 bits
 
 static uint32_t mx4_blocks(uint32_t k) { return k / 32 + (k % 32 ? 1u : 0u); }
 
@@ -1223,6 +1223,8 @@ static int check_moe_mx4(const trk_moe_mx4_w* w, uint32_t k, uint32_t m) {
         return fail(TRK_E_INVALID, "n_expert (%lld) must be in 1..1024", (long long)w->gate.count - w->n_shared);
     if (k < 1 || k > TRK_MOE_K_MAX || k > w->gate.count - w->n_shared)
         return fail(TRK_E_POLICY, "score policy: k (%u) must be in 1..min(32, n_expert)", k);
+    if (w->gate.k > MX4_LAYER_MAX || w->gate.rows > MX4_LAYER_MAX)
+        return fail(TRK_E_INVALID, "hidden (%u) and width (%u) must be at most %u", w->gate.k, w->gate.rows, MX4_LAYER_MAX);
     if (m > TRK_EXPERTS_DIRECT_M)
         return fail(TRK_E_CAPACITY, "m (%u) above %u: trk_experts_up_mx4 and trk_experts_down_mx4 take more", m, TRK_EXPERTS_DIRECT_M);
     return TRK_OK;
