@@ -108,33 +108,40 @@ __device__ __forceinline__ Mx4Side mx4_side(const Mx4Mat& w, uint32_t e, uint64_
     return Mx4Side{buffer_at((const int8_t*)w.q + e * w.stride + r0 * w.ld), buffer_at((const int8_t*)w.s + e * w.sstride + r0 * w.lds),
                    (uint32_t)w.ld, (uint32_t)w.lds};
 }
-template <typename Tile, bool ONCE, typename Row>
-__device__ __forceinline__ void mx4_expert_run(Tile& t, uint8_t* lds, const Mx4Side& w0, const Mx4Side& w1, uint32_t split, uint32_t last,
-                                               const Mx4X& x, Row&& row, uint32_t nb, uint32_t live, uint32_t a0, uint32_t astep) {
-    i32x4 rw[Tile::NA], rs[Tile::NS];
+template <typename Tile>
+struct Mx4Loads {
+    i32x4 rw[Tile::NA], rs[Tile::NS], rx;
     uint32_t wo[Tile::NA], xo[Tile::NB], so[Tile::NS];
-    const i32x4 bx = buffer_at((const int8_t*)x.q), bxs = buffer_at((const int8_t*)x.s);
+    template <typename Row>
+    __device__ __forceinline__ Mx4Loads(const Tile& t, const Mx4Side& w0, const Mx4Side& w1, uint32_t split, uint32_t last, const Mx4X& x,
+                                        Row&& row) {
+        rx = buffer_at((const int8_t*)x.q);
+        const i32x4 rxs = buffer_at((const int8_t*)x.s);
 #pragma unroll
-    for (int i = 0; i < Tile::NB; i++) xo[i] = row(t.load_row(i)) * (uint32_t)x.ld;
+        for (int i = 0; i < Tile::NB; i++) xo[i] = row(t.load_row(i)) * (uint32_t)x.ld;
 #pragma unroll
-    for (int i = 0; i < Tile::NA; i++) {
-        const bool two = (i * Tile::NW + t.wv) * 8 >= split;
-        const uint32_t r = t.load_row(i) - (two ? split : 0), rc = r < last ? r : last;
-        rw[i] = two ? w1.q : w0.q, wo[i] = rc * (two ? w1.ld : w0.ld);
-    }
+        for (int i = 0; i < Tile::NA; i++) {
+            const bool two = (i * Tile::NW + t.wv) * 8 >= split;
+            const uint32_t r = t.load_row(i) - (two ? split : 0), rc = r < last ? r : last;
+            rw[i] = two ? w1.q : w0.q, wo[i] = rc * (two ? w1.ld : w0.ld);
+        }
 #pragma unroll
-    for (int i = 0; i < Tile::NS; i++) {
-        const uint32_t p = t.scale_load(i) * Tile::SR, n = t.lane / Tile::SW;
-        const bool mine = p >= Tile::BN, two = !mine && p >= split;
-        if (mine) {
-            rs[i] = bxs, so[i] = row(p - Tile::BN + n) * (uint32_t)x.lds;
-        } else {
-            const uint32_t r = p - (two ? split : 0) + n, rc = r < last ? r : last;
-            rs[i] = two ? w1.s : w0.s, so[i] = rc * (two ? w1.lds : w0.lds);
+        for (int i = 0; i < Tile::NS; i++) {
+            const uint32_t p = t.scale_load(i) * Tile::SR, n = t.lane / Tile::SW;
+            const bool mine = p >= Tile::BN, two = !mine && p >= split;
+            if (mine) {
+                rs[i] = rxs, so[i] = row(p - Tile::BN + n) * (uint32_t)x.lds;
+            } else {
+                const uint32_t r = p - (two ? split : 0) + n, rc = r < last ? r : last;
+                rs[i] = two ? w1.s : w0.s, so[i] = rc * (two ? w1.lds : w0.lds);
+            }
         }
     }
-    t.template run<true, ONCE>(lds, rw, wo, bx, xo, [&](int i, i32x4& r, uint32_t& o) { r = rs[i], o = so[i]; }, nb, live, a0, astep);
-}
+    template <bool ONCE>
+    __device__ __forceinline__ void run(Tile& t, uint8_t* lds, uint32_t nb, uint32_t live, uint32_t a0, uint32_t astep) const {
+        t.template run<true, ONCE>(lds, rw, wo, rx, xo, [&](int i, i32x4& r, uint32_t& o) { r = rs[i], o = so[i]; }, nb, live, a0, astep);
+    }
+};
 
 // gate and up: a tile's weight rows are BN / 2 rows of gate, then the same rows of up.  A wave's 32 rows of a matrix instruction are
 // 16 of each, so that a lane has both sums of its rows.  ONCE: geo::experts_once.
@@ -157,8 +164,9 @@ __global__ __launch_bounds__(Tile::T) void experts_up_mx4_tile_kernel(Mx4Up a, P
 #pragma unroll
     for (int j = 0; j < Tile::FM; j++) en[j] = entry(t.wm + 32 * j + c);
     const uint32_t live = t.wm < pt.rows ? (pt.rows - t.wm + 31) / 32 : 0;
-    mx4_expert_run<Tile, ONCE>(t, lds, mx4_side(a.gate, pt.expert, r0), mx4_side(a.up, pt.expert, r0), BR, a.gate.rows - r0 - 1, a.x,
-                               [&](uint32_t i) { return entry(i) / a.slots; }, a.gate.nb, live, wr + (c < 16 ? c : BR + c - 16), 16);
+    const Mx4Loads<Tile> at(t, mx4_side(a.gate, pt.expert, r0), mx4_side(a.up, pt.expert, r0), BR, a.gate.rows - r0 - 1, a.x,
+                            [&](uint32_t i) { return entry(i) / a.slots; });
+    at.template run<ONCE>(t, lds, a.gate.nb, live, wr + (c < 16 ? c : BR + c - 16), 16);
     typedef Elem<DT> O;
     constexpr int CW = Tile::WN / 2;
     const uint32_t r = r0 + wr + t.lane % (CW / 4) * 4, left = r < a.gate.rows ? a.gate.rows - r : 0;
@@ -203,11 +211,13 @@ __global__ __launch_bounds__(Tile::T) void experts_down_mx4_tile_kernel(Mx4Down 
     float w[Tile::FM];
 #pragma unroll
     for (int j = 0; j < Tile::FM; j++) en[j] = entry(t.wm + 32 * j + c);
-#pragma unroll
-    for (int j = 0; j < Tile::FM; j++) w[j] = a.w[(size_t)(en[j] / a.slots) * K_MAX + en[j] % a.slots];
     const uint32_t live = t.wm < pt.rows ? (pt.rows - t.wm + 31) / 32 : 0;
     const Mx4Side ws = mx4_side(a.down, pt.expert, r0);
-    mx4_expert_run<Tile, ONCE>(t, lds, ws, ws, Tile::BN, a.down.rows - r0 - 1, a.x, entry, a.down.nb, live, t.wn + c, 32);
+    const Mx4Loads<Tile> at(t, ws, ws, Tile::BN, a.down.rows - r0 - 1, a.x, entry);
+    // the entries' weights are asked for after the tile's own addresses: its first loads then wait for one trip to memory less
+#pragma unroll
+    for (int j = 0; j < Tile::FM; j++) w[j] = a.w[(size_t)(en[j] / a.slots) * K_MAX + en[j] % a.slots];
+    at.template run<ONCE>(t, lds, a.down.nb, live, t.wn + c, 32);
     const uint32_t r = r0 + t.wn + t.lane % (Tile::WN / 4) * 4, left = r < a.down.rows ? a.down.rows - r : 0;
     const bool whole = r0 + Tile::BN <= a.down.rows;  // the workgroup as a whole
 #pragma unroll
