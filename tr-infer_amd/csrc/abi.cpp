@@ -1152,8 +1152,7 @@ extern "C" int trk_gemm_mx4(const trk_mx4_mat* w, uint32_t item, const uint8_t* 
     if (!q || !scale || !y) return fail(TRK_E_INVALID, "null argument");
     Mx4Mat M = mx4_mat(*w);
     M.q += item * M.stride, M.s += item * M.sstride;
-    const int vec = (uintptr_t)y % (dtype == TRK_DT_F32 ? 16 : 8) == 0 && (m == 1 || ldy % 4 == 0);
-    const Mx4Gemm a{M, Mx4X{q, scale, m == 1 ? 0 : ldq, m == 1 ? 0 : scale_ld}, m, bias, y, dtype, ldy, accumulate, vec};
+    const Mx4Gemm a{M, Mx4X{q, scale, m == 1 ? 0 : ldq, m == 1 ? 0 : scale_ld}, m, bias, y, dtype, ldy, accumulate};
     HIP_TRY(launch_gemm_mx4(a, (hipStream_t)stream));
     return TRK_OK;
 }
@@ -1179,9 +1178,8 @@ extern "C" int trk_experts_up_mx4(const trk_mx4_mat* gate, const trk_mx4_mat* up
     if (m == 0) return TRK_OK;
     if (!q || !scale || !ids || !n_sel || !h) return fail(TRK_E_INVALID, "null argument");
     if ((rc = check_plan(plan, m, slots, gate->count))) return rc;
-    const int vec = (uintptr_t)h % (dtype == TRK_DT_F32 ? 16 : 8) == 0 && ldh % 4 == 0;
     const Mx4Up a{mx4_mat(*gate), mx4_mat(*up), Mx4X{q, scale, m == 1 ? 0 : ldq, m == 1 ? 0 : scale_ld}, m, slots, ids, n_sel, h,
-                  dtype, ldh, vec};
+                  dtype, ldh};
     HIP_TRY(launch_experts_up_mx4(a, plan, (hipStream_t)stream));
     return TRK_OK;
 }

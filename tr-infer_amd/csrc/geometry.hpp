@@ -274,10 +274,10 @@ inline uint64_t plan_words(uint32_t m, uint32_t slots, uint32_t E) {
 }
 
 // trk_gemm_mx4 (k_mx4.hip): the int8 product's forms for 4-bit rows of nb blocks.  A form's time in ns, S stages of eight blocks,
-// fitted to 129 sizes; what it chooses there is 1.4 % slower than the best of each (us, strips / 64 x 32 / 64 x 64 / 128 x 128 /
-// 256 x 256): k = 512: [512] x 400 3.2 / 3.5 / 3.6 / 5.0 / 11, [5003] x 33 3.2 / 3.9 / 4.0 / 5.8 / 9.9, [12288] x 400 30 / 11.8 / 10.3 / 8.2 / 12.7,
-// x 4096 - / 81 / 67 / 38 / 33; k = 2560: [12288] x 1 4.3 / 5.7 / 5.7 / 9.2 / 19, x 64 16.5 / 7.1 / 6.0 / 10.6 / 20, x 800 - / 40 / 34 / 25 / 27,
-// x 4096 - / 190 / 151 / 89 / 85; k = 8192: [2560] x 33 10.8 / 11.8 / 12.1 / 22 / 46, x 800 - / 29 / 28 / 27 / 49, [12288] x 800 - / 100 / 81 / 64 / 62.
+// fitted to 129 sizes; what it chooses there is 0.8 % slower than the best of each (us, strips / 64 x 32 / 64 x 64 / 128 x 128 /
+// 256 x 256): k = 512: [512] x 400 3.2 / 3.5 / 3.6 / 4.4 / 10, [5003] x 33 3.2 / 3.9 / 3.8 / 4.6 / 9.2, [12288] x 400 30 / 11.8 / 10.0 / 7.5 / 12,
+// x 4096 - / 81 / 66 / 36 / 34; k = 2560: [12288] x 1 4.3 / 5.7 / 6.0 / 8.2 / 20, x 64 16.5 / 7.1 / 6.0 / 8.5 / 20, x 800 - / 40 / 34 / 23 / 27,
+// x 4096 - / 190 / 152 / 87 / 81; k = 8192: [2560] x 33 10.8 / 11.8 / 12.0 / 17.5 / 45, x 800 - / 29 / 28 / 25 / 49, [12288] x 800 - / 100 / 79 / 63 / 61.
 inline uint64_t mx4_form_ns(I8Form f, uint32_t m, uint32_t rows, uint64_t S) {
     if (f == I8_STRIP) {
         const uint64_t n = i8_tiles(rows, m, 16, 16);  // one to four tokens' rows come from a cache
@@ -291,9 +291,9 @@ inline uint64_t mx4_form_ns(I8Form f, uint32_t m, uint32_t rows, uint64_t S) {
     if (f == I8_TILE_64) return 2900 + 272 * S + (per_cu(64, 64) - 1) * (900 + 219 * S);
     if (f == I8_TILE_128) {  // two resident on a CU
         const uint64_t n = per_cu(128, 128);
-        return 1500 + n / 2 * (4000 + 1050 * S) + n % 2 * (3300 + 560 * S);
+        return 1200 + n / 2 * (4050 + 830 * S) + n % 2 * (2650 + 490 * S);
     }
-    return per_cu(256, 256) * (8500 + 1800 * S);
+    return per_cu(256, 256) * (8050 + 1310 * S);
 }
 inline I8Form gemm_mx4_form(uint32_t m, uint32_t rows, uint32_t nb, uint64_t ldw, uint64_t ldx, uint64_t sldw, uint64_t sldx) {
     // the tiles address their rows by 32-bit offsets from the first

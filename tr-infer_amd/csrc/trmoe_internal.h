@@ -321,7 +321,7 @@ struct Mx4Gemm {
     void* y;
     uint32_t dt;
     uint64_t ldy;
-    int accumulate, vec;  // vec: four neighbouring outputs lie on a boundary of four
+    int accumulate;
 };
 struct Mx4Up {
     Mx4Mat gate, up;
@@ -331,7 +331,6 @@ struct Mx4Up {
     void* h;
     uint32_t dt;
     uint64_t ldh;
-    int vec;
 };
 struct Mx4Down {
     Mx4Mat down;
@@ -343,7 +342,7 @@ struct Mx4Down {
     void* y;
     uint32_t dt;
     uint64_t ldy;
-    int accumulate, vec;
+    int accumulate, vec;  // vec: as I8Down's
 };
 struct Mx4Layer {
     const float *router, *shared_gate;  // either may be null
