@@ -35,6 +35,8 @@ __device__ __forceinline__ void mx_next(MxPlace& p, uint32_t P, uint32_t rows, u
 
 // Four lanes hold a block, 8 values each; its largest magnitude by two DPP steps, its exponent from that one's bits, and the
 // conversion instruction, which rounds to nearest even and holds magnitudes at 6, divides by the scale exactly (a power of two).
+// One read, one write; a thread's four pieces are all requested before the first is needed.  8192 x 4096 bf16 15.9 us, 5.3 TB/s (the
+// reads alone would be 11); 4 x 2048 f32 2.6: the trip to memory and back.
 template <uint32_t DT>
 __global__ __launch_bounds__(MQ_T) void quantize_mx4_kernel(const typename Elem<DT>::T* __restrict__ x, uint64_t ldx, uint32_t m,
                                                            uint32_t k, uint32_t P, uint32_t step_rows, uint32_t step_pieces,
@@ -97,6 +99,8 @@ __device__ __forceinline__ void mx_store(typename Elem<DT>::T* y, const float (&
         if (i < n) y[i] = Elem<DT>::put(v[i]);
 }
 
+// The same pieces back; the conversion instruction multiplies by the scale, exactly.  8192 x 4096 to bf16 14.6 us, 5.8 TB/s, most
+// of it the writes.
 template <uint32_t DT>
 __global__ __launch_bounds__(MQ_T) void dequantize_mx4_kernel(const uint8_t* __restrict__ q, uint64_t ldq,
                                                              const uint8_t* __restrict__ s, uint64_t lds, uint32_t m, uint32_t k,
@@ -160,7 +164,9 @@ void launch_rows(bool back, const void* x, uint64_t ldx, uint32_t m, uint32_t k,
 
 constexpr uint32_t ST_WAVES = 4;
 
-// A workgroup takes 16 weight rows and up to 16 tokens: its waves share K and add their sums in LDS.
+// A workgroup takes 16 weight rows and up to 16 tokens: its waves share K and add their sums in LDS.  For few rows and short K, where the
+// trips to memory are all there is: two units of both rows a wave are requested at once.  [12288] x 1 row at k = 2560 4.3 us (3.9
+// TB/s, the weights in the last cache), [512] x 1 at k = 512 2.3.
 template <uint32_t DT>
 __global__ __launch_bounds__(ST_WAVES* WAVE) void gemm_mx4_strip_kernel(Mx4Gemm g) {
     __shared__ float part[ST_WAVES][16][16];  // [wave][token][weight row]
@@ -225,6 +231,10 @@ __device__ __forceinline__ void tile_place(uint32_t idx, uint32_t tn, uint32_t t
     n = panel * 8 + rem % w, m = rem / w;
 }
 
+// 4096 x 12288 x 2560 to bf16 81 us, 3.2 PFLOP/s; 8192 cubed 299, 3.7 (from registers alone the instruction reached 6.6 on random
+// bits, 8.9 on constants).  What bounds it is the clock that random bits leave (1.6 GHz; 8192 cubed of zeros takes 208 us) with the matrix
+// cores busy half of it, the rest the stages' loads: tiles of 256 x 256 halve the rows' traffic against 128 x 128, at one workgroup a
+// CU.  Where whole tiles do not fill the CUs smaller ones do (geo::gemm_mx4_form).
 template <typename Tile, uint32_t DT>
 __global__ __launch_bounds__(Tile::T) void gemm_mx4_tile_kernel(Mx4Gemm g) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[Tile::LDS];

@@ -141,7 +141,8 @@ __device__ __forceinline__ void put_parts(uint8_t* row, uint32_t piece, const fl
     }
 }
 
-// A wave per row of the router and token, then (workgroups from `logits` on) a thread per piece of a token's row.
+// A wave per row of the router and token, then (workgroups from `logits` on) a thread per piece of a token's row: the two need
+// only x, and share a launch.  512 + 1 rows of 2048, 1 token 4.6 us, 8 tokens of 256 + 0 4.8: the trip to memory and the wave's sum.
 template <uint32_t DT>
 __global__ __launch_bounds__(LG_WAVES* WAVE) void layer_logits_kernel(Mx4Layer a, uint32_t rows, uint32_t logits) {
     const uint32_t lane = threadIdx.x % WAVE;
@@ -226,8 +227,10 @@ struct LayerChosen {  // by a launch before
     }
 };
 
-// A workgroup takes 32 rows (a block of h) of gate and up and one entry; its waves share K.  (Eight waves, four for each half of
-// the rows, hold fewer registers and are slower: 8 tokens of 8 in 256, H = 2048, F = 768 57 us a layer against 53.)
+// A workgroup takes 32 rows (a block of h) of gate and up and one entry; its waves share K, a unit of all rows at once each.  With the
+// choice inside (some 3 us of it, which every workgroup makes for itself and no launch waits for) 1 token of 10 in 512 and a shared one
+// (H = 2048, F = 512) 9.4 us; chosen before, 8 tokens of 8 in 256 and one (F = 768) 22.2, 5.4 TB/s counting each entry's weights.
+// (Eight waves, four for each half of the rows, hold fewer registers and are slower: that layer 57 us against 53.)
 template <typename Choice>
 __global__ __launch_bounds__(LU_WAVES* WAVE) void layer_up_kernel(Mx4Layer a, const float* __restrict__ bias, ScorePolicy p) {
     extern __shared__ double keys[];  // [n_expert]
@@ -288,7 +291,8 @@ __global__ __launch_bounds__(LU_WAVES* WAVE) void layer_up_kernel(Mx4Layer a, co
 // ---- down, and the sum -------------------------------------------------------------------------------
 
 // A workgroup takes 16 down rows and one token: a wave per slot, in turn where there are more.  Then a thread per (slot, row)
-// weights, and a thread per row adds in slot order.
+// weights, and a thread per row adds in slot order.  1 token of 11 slots (H = 2048, F = 512) 5.4 us, 8 tokens of 9 (F = 768) 16.  (The next
+// slot's loads before this one's sum: 8 tokens 46.4 -> 45.7 us a layer, but 4 tokens 31.4 -> 32.8 and 1 token 18.8 -> 19.1.)
 template <uint32_t DT, uint32_t WAVES>
 __global__ __launch_bounds__(WAVES* WAVE) void layer_down_kernel(Mx4Layer a) {
     extern __shared__ float part[][MX_PARTS][16];  // [slots]
