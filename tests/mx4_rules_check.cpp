@@ -33,7 +33,7 @@ int main() {
         if (bad(gemm_mx4_form(4096, 12288, 80, ld[0], ld[1], ld[2], ld[3]) == I8_STRIP, "far rows", i, 0, 0)) return 1;
     }
     if (bad(!layer_routes_apart(704) && layer_routes_apart(1408), "routes", 0, 0, 0)) return 1;
-    if (bad(layer_down_waves(128, 11) == 12 && layer_down_waves(1024, 11) == 4 && layer_down_waves(128, 2) == 4, "waves", 0, 0, 0))
+    if (bad(layer_down_waves(128, 11) == 12 && layer_down_waves(1024, 11) == 8 && layer_down_waves(1024, 64) == 4 && layer_down_waves(128, 2) == 4, "waves", 0, 0, 0))
         return 1;
     printf("ok %llu\n", checks);
     return 0;

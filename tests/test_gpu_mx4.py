@@ -450,7 +450,8 @@ def test_layer(m, E, k, H, F, shared, gated, bias, score, groups, keep, xt, yt):
     within(host(y2), want, R.layer(x, w["gate"], w["up"], w["down"], ids, share, "f32")[1] + tol)
 
 
-@pytest.mark.parametrize("m,E,k,H,F,shared", [(8, 40, 8, 512, 600, 1), (8, 16, 2, 1030, 1100, 0), (5, 300, 12, 640, 200, 2)])
+@pytest.mark.parametrize("m,E,k,H,F,shared", [(8, 40, 8, 512, 600, 1), (8, 16, 2, 1030, 1100, 0), (5, 300, 12, 640, 200, 2),
+                                                (8, 30, 6, 1041, 70, 1), (7, 9, 5, 1200, 1100, 0), (8, 36, 32, 1039, 33, 21)])
 def test_layer_of_many_entries(m, E, k, H, F, shared):
     """The choice by a launch of its own, several units of K, slots in turn."""
     say(f"moe_mx4 many m={m} E={E} k={k} H={H} F={F} shared={shared}")
@@ -491,6 +492,58 @@ def test_layer_rows_that_choose_nothing():
         assert np.isnan(y[4]).all()
         with pytest.raises(trmoe.TrkError, match="rlog"):
             trmoe.moe_mx4(L, dev(x), score="softmax", **kw)
+
+
+def test_layer_poison_in_the_weights():
+    """A scale byte of 255 in one expert's down row is that row's NaN, in its gate row all of its output's, for the tokens that
+    choose it; rows and scales behind the stack's last are not looked at."""
+    say("moe_mx4 poisoned weights")
+    rng = np.random.default_rng(13)
+    m, E, k, H, F = 6, 12, 3, 200, 70
+    x, logits = rng.standard_normal((m, H)).astype(np.float32), rng.permutation(m * E).reshape(m, E).astype(np.float32) / (m * E)
+    kw = dict(k=k, rlog=dev(logits), score="sigmoid")
+    L, _, _, _, _ = layer_of(rng, E, H, F, router=False)
+    clean = host(trmoe.moe_mx4(L, dev(x), **kw))
+    e = int(np.argmax(logits[2]))
+    chosen = np.array([e in np.argsort(-logits[t])[:k] for t in range(m)])
+    assert chosen.any() and not chosen.all() and np.isfinite(clean).all()
+    L.down.scale[e, 37, 2] = 255
+    y = host(trmoe.moe_mx4(L, dev(x), **kw))
+    assert np.isnan(y[chosen, 37]).all() and np.isnan(y).sum() == chosen.sum()
+    assert np.array_equal(np.delete(y, 37, 1), np.delete(clean, 37, 1))
+    L.gate.scale[e, 69, 6] = 255
+    y = host(trmoe.moe_mx4(L, dev(x), **kw))
+    assert np.isnan(y[chosen]).all() and np.array_equal(y[~chosen], clean[~chosen])
+
+
+@pytest.mark.parametrize("m", [3, 8])
+def test_work_of_any_content(m):
+    """Memory that is given is used whatever it holds, and refused where it is too small; x may be the output."""
+    import torch
+    say(f"mx4 calls on given work, m={m}")
+    rng = np.random.default_rng(14)
+    E, k, H, F = 20, 5, 1100, 300
+    L, _, _, _, _ = layer_of(rng, E, H, F, n_shared=1, gated=True)
+    x = dev(rng.standard_normal((m, H)).astype(np.float32))
+    want = trmoe.moe_mx4(L, x, k)
+    n = L.work_values(k, m)
+    for fill in (float("nan"), 1e38, 0.0):
+        work = torch.full((n,), fill, device="cuda")
+        assert torch.equal(trmoe.moe_mx4(L, x, k, work=work), want)
+        assert torch.equal(trmoe.moe_mx4(L, x, k, work=work), want)
+    for small in (work[:-1], work.double(), torch.empty((n, 2), device="cuda")[:, 0]):
+        with pytest.raises(trmoe.TrkError, match="work"):
+            trmoe.moe_mx4(L, x, k, work=small)
+    assert torch.equal(trmoe.moe_mx4(L, x, k, out=x, work=work), want)
+    big = dev(rng.standard_normal((40, H)).astype(np.float32))
+    ids, w, ns = trmoe.route_scores((big @ L.router.T).contiguous(), k)
+    plan = trmoe.experts_plan(ids, ns, k, E + 1)
+    hq, hs = trmoe.quantize_mx4(trmoe.experts_up_mx4(L.gate, L.up, *trmoe.quantize_mx4(big), ids, ns, k, plan=plan))
+    y = trmoe.experts_down_mx4(L.down, hq, hs, ids, w, ns, k, plan=plan)
+    work = torch.full((40 * k * H,), float("nan"), device="cuda")
+    assert torch.equal(trmoe.experts_down_mx4(L.down, hq, hs, ids, w, ns, k, plan=plan, work=work), y)
+    with pytest.raises(trmoe.TrkError, match="work"):
+        trmoe.experts_down_mx4(L.down, hq, hs, ids, w, ns, k, plan=plan, work=work[:-4])
 
 
 # ---- together ----------------------------------------------------------------------------------------
@@ -639,3 +692,54 @@ def test_empty_batches():
     assert trmoe.moe_mx4(L, x, 2).shape == (0, 64)
     with pytest.raises(trmoe.TrkError, match="above 8"):
         trmoe.moe_mx4(L, torch.zeros((9, 64), device="cuda"), 2)
+
+
+def test_a_stream_of_another_device():
+    """Every call refuses it, and takes one of its own."""
+    import torch
+    from types import SimpleNamespace
+    say("mx4 calls: streams of another device")
+    there = SimpleNamespace(cuda_stream=0, device_index=torch.cuda.current_device() + 1)
+    W = trmoe.quantize_weights_mx4(torch.randn((4, 32, 32), device="cuda"))
+    x = torch.randn((40, 32), device="cuda")
+    q, s = trmoe.quantize_mx4(x)
+    ids, w, n = trmoe.route_scores(torch.randn((40, 4), device="cuda"), 2)
+    plan = trmoe.experts_plan(ids, n, 2, 4)
+    hq, hs = trmoe.quantize_mx4(trmoe.experts_up_mx4(W, W, q, s, ids, n, 2, plan=plan))
+    L = trmoe.MX4Layer(W, W, W, router=torch.randn((4, 32), device="cuda"))
+    y, h = torch.full((40, 32), 9.0, device="cuda"), torch.full((80, 32), 9.0, device="cuda")
+    work, few = torch.empty(40 * 2 * 32, device="cuda"), torch.empty(L.work_values(2, 8), device="cuda")
+    one = trmoe.MX4Weights(W.q[0], W.scale[0], 32)
+    for call in (lambda st: trmoe.quantize_mx4(x, out=(q.clone(), torch.empty((40, 4), dtype=torch.uint8, device="cuda")[:, :1]), stream=st),
+                 lambda st: trmoe.dequantize_mx4(q, s, 32, out=y, stream=st),
+                 lambda st: trmoe.gemm_mx4(one, q, s, out=y, stream=st),
+                 lambda st: trmoe.experts_up_mx4(W, W, q, s, ids, n, 2, plan=plan, out=h, stream=st),
+                 lambda st: trmoe.experts_down_mx4(W, hq, hs, ids, w, n, 2, plan=plan, out=y, work=work, stream=st),
+                 lambda st: trmoe.moe_mx4(L, x[:8], 2, out=y[:8], work=few, stream=st)):
+        with pytest.raises(trmoe.TrkError, match="a stream of device"):
+            call(there)
+        call(torch.cuda.current_stream())
+    torch.cuda.synchronize()
+
+
+def test_the_layer_captured_with_a_launch_for_the_choice():
+    import torch
+    say("moe_mx4 captured, the choice apart")
+    rng = np.random.default_rng(15)
+    m, E, k, H, F = 8, 24, 6, 1100, 700
+    L, _, _, _, _ = layer_of(rng, E, H, F, n_shared=1)
+    x = dev(rng.standard_normal((m, H)).astype(np.float32))
+    work = torch.empty(L.work_values(k, m), device="cuda")
+    trmoe.moe_mx4(L, x, k, work=work)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = trmoe.moe_mx4(L, x, k, work=work)
+        y2 = trmoe.moe_mx4(L, y, k, work=work)  # one after another on the same work
+    for _ in range(3):
+        x.copy_(dev(rng.standard_normal((m, H)).astype(np.float32)))
+        g.replay()
+        torch.cuda.synchronize()
+        a, b = y.clone(), y2.clone()
+        assert torch.equal(trmoe.moe_mx4(L, x, k), a) and torch.equal(trmoe.moe_mx4(L, a, k), b)
+        torch.cuda.synchronize()

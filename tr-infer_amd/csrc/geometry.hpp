@@ -309,10 +309,14 @@ inline I8Form gemm_mx4_form(uint32_t m, uint32_t rows, uint32_t nb, uint64_t ldw
 // workgroups) 18.8 / 20.4, 2 23.2 / 25.4, 4 (704) 32.8 / 34.7, 8 (1408) 52.9 / 50.7; 8 of 256, F = 768, 8 tokens (1728) 62.3 / 57.5;
 // 2 of 8, F = 1024, 8 (768) 22.9 / 24.9; 8 of 8 (2304) 50.0 / 46.0.
 inline bool layer_routes_apart(uint64_t wgs) { return wgs > 1024; }
-// Waves of its down launch (`wgs` workgroups: 16 rows of a token each), a slot at a time each.  us a layer, 4 / 12: the same
-// layers' 1 token (128 workgroups) 19.8 / 18.7, 2 24.4 / 23.1, 4 (512) 32.8 / 31.4, 8 (1024) 46.8 / 47.5; F = 768, 8 53.2 / 53.6;
-// few slots: 2 of 8, 8 21.1 / 23.0.
-inline uint32_t layer_down_waves(uint64_t wgs, uint32_t slots) { return slots <= 4 || wgs > 512 ? 4 : 12; }
+// Waves of a workgroup of its down launch, a slot at a time each: 4 or 12 of 16 rows of a token (`wgs` such workgroups), 8 of 32.  us a
+// layer, 4 / 8 / 12: the same layers' 1 token (128 workgroups) 19.8 / 20.3 / 18.7, 2 24.4 / 26.2 / 23.1, 4 (512) 32.8 / 31.6 / 31.4, 8
+// (1024) 46.5 / 45.7 / 47.5; F = 768, 8 52.6 / 51.5 / 53.6; 8 of 8, 8 45.8 / 43.9 / -; few slots: 2 of 8, 8 21.0 / 21.0 / 23.0, 2 of 10
+// 13.7 / 14.1 / -.  The eight hold 32 slots' sums in LDS.
+inline uint32_t layer_down_waves(uint64_t wgs, uint32_t slots) {
+    if (slots <= 4) return 4;
+    return wgs <= 512 ? 12 : slots <= 32 ? 8 : 4;
+}
 
 // Every invariant a call of m rows with kcap selections per token relies on; returns nullptr when
 // they hold, else what failed.  tq: the experts are TQ strips (k_tq.hip), not GGUF superblocks.

@@ -290,28 +290,36 @@ __global__ __launch_bounds__(LU_WAVES* WAVE) void layer_up_kernel(Mx4Layer a, co
 
 // ---- down, and the sum -------------------------------------------------------------------------------
 
-// A workgroup takes 16 down rows and one token: a wave per slot, in turn where there are more.  Then a thread per (slot, row)
-// weights, and a thread per row adds in slot order.  1 token of 11 slots (H = 2048, F = 512) 5.4 us, 8 tokens of 9 (F = 768) 16.  (The next
-// slot's loads before this one's sum: 8 tokens 46.4 -> 45.7 us a layer, but 4 tokens 31.4 -> 32.8 and 1 token 18.8 -> 19.1.)
-template <uint32_t DT, uint32_t WAVES>
+// A workgroup takes 16 NR down rows and one token: a wave per slot, in turn where there are more (geo::layer_down_waves).  Then a
+// thread per (slot, row) weights, and a thread per row adds in slot order.  Every workgroup reads its token's h, which is as long in
+// parts as 12 rows of weights: more rows a workgroup read less of it.  1 token of 11 slots (H = 2048, F = 512) 5.4 us, 8 tokens of 9 (F =
+// 768) 15.  (The next slot's loads before this one's sum: 8 tokens 46.4 -> 45.7 us a layer, but 4 tokens 31.4 -> 32.8, 1 token 18.8 -> 19.1.)
+template <uint32_t DT, uint32_t WAVES, uint32_t NR>
 __global__ __launch_bounds__(WAVES* WAVE) void layer_down_kernel(Mx4Layer a) {
-    extern __shared__ float part[][MX_PARTS][16];  // [slots]
-    const uint32_t strips = (a.down.rows + 15) / 16, id = run_id(), r0 = id % strips * 16, t = id / strips;
+    constexpr uint32_t ROWS = 16 * NR;
+    extern __shared__ float lds[];
+    float(*part)[MX_PARTS][ROWS] = reinterpret_cast<float(*)[MX_PARTS][ROWS]>(lds);  // [slots]
+    const uint32_t strips = (a.down.rows + ROWS - 1) / ROWS, id = run_id(), r0 = id % strips * ROWS, t = id / strips;
     if (t >= a.m) return;  // the whole workgroup
     const uint32_t wv = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, nb = a.down.nb;
     for (uint32_t j = wv; j < a.slots; j += WAVES) {
         uint32_t e;
         if (!layer_slot(a, t, j, e)) continue;
-        const Mx4Row w = layer_row(a.down, e, r0, lane);
+        Mx4Row w[NR];
+        f32x4 acc[NR];
+#pragma unroll
+        for (uint32_t i = 0; i < NR; i++) w[i] = layer_row(a.down, e, r0 + 16 * i, lane), acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         const uint8_t* h = a.hparts + ((uint64_t)t * a.slots + j) * parts_bytes(nb);
-        f32x4 acc[1] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
-        for (uint32_t n = 0; n < mx_units(nb); n++) part_unit<1>({w}, h, n, nb, lane, acc);
-        mx_here(acc[0]);
-        if (lane % 16 < MX_PARTS) *reinterpret_cast<f32x4*>(&part[j][lane % 16][lane / 16 * 4]) = acc[0];
+        for (uint32_t n = 0; n < mx_units(nb); n++) part_unit<NR>(w, h, n, nb, lane, acc);
+#pragma unroll
+        for (uint32_t i = 0; i < NR; i++) mx_here(acc[i]);
+        if (lane % 16 < MX_PARTS)
+#pragma unroll
+            for (uint32_t i = 0; i < NR; i++) *reinterpret_cast<f32x4*>(&part[j][lane % 16][16 * i + lane / 16 * 4]) = acc[i];
     }
     __syncthreads();
-    const uint32_t ri = threadIdx.x % 16, r = r0 + ri, k = a.slots - a.n_shared;
-    for (uint32_t j = threadIdx.x / 16; j < a.slots; j += WAVES * WAVE / 16) {
+    const uint32_t ri = threadIdx.x % ROWS, r = r0 + ri, k = a.slots - a.n_shared;
+    for (uint32_t j = threadIdx.x / ROWS; j < a.slots; j += WAVES * WAVE / ROWS) {
         uint32_t e;
         float v = 0.0f;
         if (layer_slot(a, t, j, e)) {
@@ -323,7 +331,7 @@ __global__ __launch_bounds__(WAVES* WAVE) void layer_down_kernel(Mx4Layer a) {
         part[j][0][ri] = v;  // its own
     }
     __syncthreads();
-    if (threadIdx.x >= 16 || r >= a.down.rows) return;
+    if (threadIdx.x >= ROWS || r >= a.down.rows) return;
     float v = 0.0f;
 #pragma unroll 8
     for (uint32_t j = 0; j < a.slots; j++) v += part[j][0][ri];
@@ -358,10 +366,15 @@ template <uint32_t DT>
 void launch_down(const Mx4Layer& a, hipStream_t st) {
     const uint64_t wgs = (uint64_t)((a.down.rows + 15) / 16) * a.m;
     const size_t lds = a.slots * MX_PARTS * 16 * sizeof(float);  // 64 slots at most: 36 KB
-    if (geo::layer_down_waves(wgs, a.slots) == 4)
-        layer_down_kernel<DT, 4><<<run_of(wgs, 4 * WAVE), 4 * WAVE, lds, st>>>(a);
-    else
-        layer_down_kernel<DT, 12><<<run_of(wgs, 12 * WAVE), 12 * WAVE, lds, st>>>(a);
+    switch (geo::layer_down_waves(wgs, a.slots)) {
+    case 4: layer_down_kernel<DT, 4, 1><<<run_of(wgs, 4 * WAVE), 4 * WAVE, lds, st>>>(a); break;
+    case 8: {  // at most 32 slots
+        const uint64_t wgs2 = (uint64_t)((a.down.rows + 31) / 32) * a.m;
+        layer_down_kernel<DT, 8, 2><<<run_of(wgs2, 8 * WAVE), 8 * WAVE, 2 * lds, st>>>(a);
+        break;
+    }
+    default: layer_down_kernel<DT, 12, 1><<<run_of(wgs, 12 * WAVE), 12 * WAVE, lds, st>>>(a);
+    }
 }
 
 }  // namespace
