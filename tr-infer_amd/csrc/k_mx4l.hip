@@ -292,8 +292,8 @@ __global__ __launch_bounds__(LU_WAVES* WAVE) void layer_up_kernel(Mx4Layer a, co
 
 // A workgroup takes 16 NR down rows and one token: a wave per slot, in turn where there are more (geo::layer_down_waves).  Then a
 // thread per (slot, row) weights, and a thread per row adds in slot order.  Every workgroup reads its token's h, which is as long in
-// parts as 12 rows of weights: more rows a workgroup read less of it.  1 token of 11 slots (H = 2048, F = 512) 5.4 us, 8 tokens of 9 (F =
-// 768) 15.  (The next slot's loads before this one's sum: 8 tokens 46.4 -> 45.7 us a layer, but 4 tokens 31.4 -> 32.8, 1 token 18.8 -> 19.1.)
+// parts as 12 rows of weights: more rows a workgroup read less of it.  1 token of 11 slots (H = 2048, F = 512) 5.3 us, 8 tokens of 9 (F =
+// 768) 14.4, 4.2 TB/s counting each entry's weights.  (The next slot's loads before this one's sum: 8 tokens 46.4 -> 45.7 us a layer, but 4 tokens 31.4 -> 32.8, 1 token 18.8 -> 19.1.)
 template <uint32_t DT, uint32_t WAVES, uint32_t NR>
 __global__ __launch_bounds__(WAVES* WAVE) void layer_down_kernel(Mx4Layer a) {
     constexpr uint32_t ROWS = 16 * NR;
