@@ -147,8 +147,9 @@ struct Mx4Loads {
 
 // gate and up: a tile's weight rows are BN / 2 rows of gate, then the same rows of up.  A wave's 32 rows of a matrix instruction are
 // 16 of each, so that a lane has both sums of its rows and SwiGLU is the epilogue.  ONCE: geo::experts_once.  2000 tokens of 8 in 128
-// (H = 2048, F = 768) 78 us: 1.3 PFLOP/s, 2.7 TB/s of weights.  A stage takes some 1.9 us, the latency of its loads with
-// two workgroups a CU and one stage each on its way; the matrix cores wait.
+// (H = 2048, F = 768) 78 us: 1.3 PFLOP/s, 2.7 TB/s of weights.  What bounds it is the latency of the weights' loads, two workgroups
+// a CU with one to two stages each on their way (all loads from a few lines: 52), and beside it LDS: a stage of both workgroups reads and
+// writes 1 us of it.  Without its matrix instructions it takes 75.
 template <typename Tile, uint32_t DT, bool ONCE>
 __global__ __launch_bounds__(Tile::T) void experts_up_mx4_tile_kernel(Mx4Up a, Plan P) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[Tile::LDS];
