@@ -317,6 +317,15 @@ __global__ __launch_bounds__(WAVES* WAVE) void layer_down_kernel(Mx4Layer a) {
 #pragma unroll
             for (uint32_t i = 0; i < NR; i++) *reinterpret_cast<f32x4*>(&part[j][lane % 16][16 * i + lane / 16 * 4]) = acc[i];
     }
+    // A NaN or an infinity in x reaches y by any product.  Where there is none (its logits are then NaN as a rule, and nothing is
+    // chosen) the token's scales say it.
+    bool poison = false;
+    if (!a.n_shared && a.n_sel[t] == 0) {  // the workgroup as a whole
+        const uint8_t* x = a.xparts + t * parts_bytes(a.gate.nb);
+        for (uint32_t b = threadIdx.x; b < a.gate.nb; b += WAVES * WAVE)
+            poison |= x[(uint64_t)(b / MX_UNIT) * PU_BYTES + part_scale_at(b, 0)] == 255;
+        poison = __syncthreads_or(poison);
+    }
     __syncthreads();
     const uint32_t ri = threadIdx.x % ROWS, r = r0 + ri, k = a.slots - a.n_shared;
     for (uint32_t j = threadIdx.x / ROWS; j < a.slots; j += WAVES * WAVE / ROWS) {
@@ -336,7 +345,7 @@ __global__ __launch_bounds__(WAVES* WAVE) void layer_down_kernel(Mx4Layer a) {
 #pragma unroll 8
     for (uint32_t j = 0; j < a.slots; j++) v += part[j][0][ri];
     typedef Elem<DT> O;
-    reinterpret_cast<typename O::T*>(a.y)[t * a.ldy + r] = O::put(v);
+    reinterpret_cast<typename O::T*>(a.y)[t * a.ldy + r] = O::put(poison ? __builtin_nanf("") : v);
 }
 
 dim3 run_of(uint64_t wgs, uint32_t threads) {
