@@ -407,8 +407,9 @@ typedef struct {
 /* y[t] = sum_j w_j down_j (silu(gate_j x[t]) * up_j x[t]) over the experts that trk_route_scores chooses by the router's
  * logits (rlog [m][n_expert] where it is given, else router . x in 32 bits), in that order, then the shared ones.  Up to
  * TRK_EXPERTS_DIRECT_M tokens (more: TRK_E_CAPACITY), hidden size and width up to 2^24.  Activations are not quantised: x, h
- * and every sum are as 32 bits hold them (a value to 2^-26 of the largest of its 32, and to 2^-129), y is rounded to once.  A
- * token with a NaN or an infinity in x gets a row of NaN, also where no expert is chosen; an expert whose h has either gives NaN.
+ * and every sum are as 32 bits hold them (a value to 2^-26 of the largest of its 32, and to 2^-129; a sum whose terms'
+ * magnitudes add up to half of 2^128 or more may overflow), y is rounded to once.  A token with a NaN or an infinity in x
+ * gets a row of NaN, also where no expert is chosen; an expert whose h has either gives NaN.
  * x: rows ldx elements apart, of type xdtype; y: rows ldy apart, of type ydtype.  work: trk_moe_mx4_work_bytes of device memory,
  * 16-byte aligned, of any content; calls that may overlap need one each.  k: the policy's. */
 int trk_moe_mx4_work_bytes(const trk_moe_mx4_w *w, uint32_t k, uint32_t m, uint64_t *bytes);

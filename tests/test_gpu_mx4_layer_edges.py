@@ -1,12 +1,13 @@
-"""The layer on 4-bit experts where its activations are no numbers."""
+"""The layer on 4-bit experts where its activations are no numbers or nearly too large."""
 from __future__ import annotations
 
 import i8ref
+import mx4ref as R
 import numpy as np
 import pytest
 
 import trmoe
-from test_gpu_mx4 import dev, host, layer_of, say
+from test_gpu_mx4 import apart, dev, host, layer_of, rows4, say, within
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +54,57 @@ def test_a_poisoned_token_that_chooses_nothing(m, F):
     nan = np.isin(np.arange(m), (1, 3, 4))
     assert np.isnan(y[nan]).all() and np.isfinite(y[~nan]).all()
     assert (y[[0, 2]] == 0).all() and (y[5:] != 0).any(1).all()
+
+
+@pytest.mark.parametrize("xt", ["f32", "bf16"])
+@pytest.mark.parametrize("m,F", CHOICES)
+def test_values_near_the_largest(m, F, xt):
+    """x up to the largest number, with weights so small that every sum is an ordinary one."""
+    import torch
+    say(f"moe_mx4 x near the largest m={m} F={F} {xt}")
+    rng = np.random.default_rng(m + F)
+    E, k, H = 6, 4, 200
+    w = {"gate": rows4(rng, E, F, H, spread=2.0 ** -123), "up": rows4(rng, E, F, H, spread=2.0 ** -123),
+         "down": rows4(rng, E, H, F, spread=0.1)}
+    L = trmoe.MX4Layer(*[trmoe.MX4Weights(*apart(*w[i]), K) for i, K in (("gate", H), ("up", H), ("down", F))])
+    x = (rng.uniform(2.9e38, 3.38e38, (m, H)) * rng.choice([-1, 0, 0, 0, 1], (m, H))).astype(np.float32)
+    x[0, :32] = 3.38e38
+    x[1, 64:96] = np.linspace(2.95e38, 3.01e38, 32)  # about the first part's border, 3.5 2^126
+    xd = dev(x).to(i8ref.torch_dtype(xt))
+    assert xd.isfinite().all()
+    logits = (rng.permutation(m * E).reshape(m, E) / (m * E)).astype(np.float32)
+    kw = dict(k=k, n_group=1, topk_group=1, group_top=2, renorm=True, factor=1.0)
+    rid, rw, _ = i8ref.route(logits, bias=None, score="sigmoid", **kw)
+    v = {i: R.values(*w[i], K) for i, K in (("gate", H), ("up", H), ("down", F))}
+    want, tol = R.layer(host(xd).astype(np.float64), v["gate"], v["up"], v["down"], rid, rw, "f32")
+    within(host(trmoe.moe_mx4(L, xd, rlog=dev(logits), score="sigmoid", dtype=torch.float32, **kw)), want, tol)
+
+
+@pytest.mark.parametrize("m,F", CHOICES)
+def test_activations_near_the_largest(m, F):
+    """The same of h: silu(4) 2^126 is 3.34e38."""
+    say(f"moe_mx4 h near the largest m={m} F={F}")
+    rng = np.random.default_rng(m + F)
+    E, k, H = 6, 4, 64
+    one, flat = np.searchsorted(R.VALUES[:8], [1.0, 4.0]), {}
+    for i, code, scale in (("gate", one[1], 127), ("up", one[0], 127 + 126)):
+        c = np.zeros((E, F, H), np.uint8)
+        c[:, :, 0] = code + (8 * rng.integers(0, 2, (E, F)) if i == "up" else 0)
+        s = np.full((E, F, 2), 127, np.uint8)
+        s[:, :, 0] = scale
+        c[:, ::3, 0] = np.searchsorted(R.VALUES[:8], 1.0)  # every third row smaller by its gate or up
+        if i == "up":
+            c[:, ::3, 0] = np.searchsorted(R.VALUES[:8], 0.5)
+        flat[i] = R.pack(c), s
+    flat["down"] = rows4(rng, E, H, F, spread=2.0 ** -122)
+    L = trmoe.MX4Layer(*[trmoe.MX4Weights(*apart(*flat[i]), K) for i, K in (("gate", H), ("up", H), ("down", F))])
+    x = np.zeros((m, H), np.float32)
+    x[:, 0], x[:, 40] = 1.0, np.arange(m)  # the second value meets zeros
+    logits = (rng.permutation(m * E).reshape(m, E) / (m * E)).astype(np.float32)
+    kw = dict(k=k, n_group=1, topk_group=1, group_top=2, renorm=True, factor=1.0)
+    rid, rw, _ = i8ref.route(logits, bias=None, score="sigmoid", **kw)
+    v = {i: R.values(*flat[i], K) for i, K in (("gate", H), ("up", H), ("down", F))}
+    h = R.silu(v["gate"][0, :, 0]) * v["up"][0, :, 0]
+    assert 3.3e38 < np.abs(h).max() < 3.4e38
+    want, tol = R.layer(x.astype(np.float64), v["gate"], v["up"], v["down"], rid, rw, "f32")
+    within(host(trmoe.moe_mx4(L, dev(x), rlog=dev(logits), score="sigmoid", **kw)), want, tol)

@@ -29,15 +29,22 @@ __host__ __device__ inline uint64_t parts_bytes(uint32_t nb) { return (uint64_t)
 __device__ __forceinline__ uint32_t part_at(uint32_t b, uint32_t p) { return b / 4 % 4 * PU_GROUP + p * 64 + b % 4 * 16; }
 __device__ __forceinline__ uint32_t part_scale_at(uint32_t b, uint32_t p) { return PU_VALUES + b % 4 * 64 + p * 4 + b / 4 % 4; }
 
-// A block's scales from its largest magnitude's bits: the largest magnitude lies in [2, 4) of the first.
+// A block's scales from its largest magnitude's bits: the largest magnitude lies in [2, 4) of the first.  Where that is 2^126 a
+// first part that rounds up to 4 of it is 2^128, which 32 bits do not hold: such a block's values are split by their halves,
+// with halved scales (what a half among the smallest numbers loses is far below the last part).
 struct MxScales {
     bool poison;  // the block's products are NaN
+    uint32_t half;
     int e;
-    __device__ __forceinline__ explicit MxScales(uint32_t top) : poison(top >= 0x7f800000u), e((int)(top >> 23) - 1) {}
+    __device__ __forceinline__ explicit MxScales(uint32_t top)
+        : poison(top >= 0x7f800000u), half(top >= 0x7f000000u && !poison), e((int)(top >> 23) - 1) {}
     __device__ __forceinline__ uint32_t byte(uint32_t p) const {
         const int ep = e - (int)(MX_STEP * p);
         return ep > 0 ? (uint32_t)ep : 0u;
     }
+    // what is split, and part p's scale for it
+    __device__ __forceinline__ float start(float x) const { return poison ? 0.0f : x * (half ? 0.5f : 1.0f); }
+    __device__ __forceinline__ float scale(uint32_t p) const { return mx_scale(byte(p) - half); }
 };
 
 // This lane's part of a unit (parts beyond the last: the first, whose sums nobody reads).
@@ -118,12 +125,11 @@ __device__ __forceinline__ void put_parts(uint8_t* row, uint32_t piece, const fl
     const MxScales sc(top);
     float r[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) r[i] = sc.poison ? 0.0f : x[i];
+    for (int i = 0; i < 8; i++) r[i] = sc.start(x[i]);
     uint8_t* b = row + (uint64_t)(piece / 64) * PU_BYTES;
 #pragma unroll
     for (uint32_t p = 0; p < MX_PARTS; p++) {
-        const uint32_t byte = sc.byte(p);
-        const float f = mx_scale(byte);
+        const float f = sc.scale(p);
         uint32_t w = 0;
         w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, r[0], r[1], f, 0);
         w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, r[2], r[3], f, 1);
@@ -137,7 +143,7 @@ __device__ __forceinline__ void put_parts(uint8_t* row, uint32_t piece, const fl
             less(6, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, f, 3));
         }
         *reinterpret_cast<uint32_t*>(b + part_at(piece / 4, p) + piece % 4 * 4) = w;
-        if (piece % 4 == 0) b[part_scale_at(piece / 4, p)] = sc.poison ? 255 : (uint8_t)byte;
+        if (piece % 4 == 0) b[part_scale_at(piece / 4, p)] = sc.poison ? 255 : (uint8_t)sc.byte(p);
     }
 }
 
@@ -268,17 +274,16 @@ __global__ __launch_bounds__(LU_WAVES* WAVE) void layer_up_kernel(Mx4Layer a, co
     const uint32_t b = r0 / 32, nf = (a.gate.rows + 31) / 32;
     if (r0 + lane % 32 >= a.gate.rows) h = 0.0f;
     const MxScales sc(row32_allreduce(__float_as_uint(h) & 0x7fffffffu, [](uint32_t c, uint32_t d) { return c > d ? c : d; }));
-    float r = sc.poison ? 0.0f : h;
+    float r = sc.start(h);
     uint8_t* hp = a.hparts + en * parts_bytes(nf) + (uint64_t)(b / MX_UNIT) * PU_BYTES;
 #pragma unroll
     for (uint32_t q = 0; q < MX_PARTS; q++) {
-        const uint32_t byte = sc.byte(q);
-        const float f = mx_scale(byte);
+        const float f = sc.scale(q);
         const uint32_t v = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, r, r, f, 0);
         r -= __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v, f, 0)[0];
         const uint32_t next = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, false);  // lane ^ 1
         if (lane < 32 && lane % 2 == 0) hp[part_at(b, q) + lane / 2] = (uint8_t)((v & 15u) | (next & 15u) << 4);
-        if (lane == 0) hp[part_scale_at(b, q)] = sc.poison ? 255 : (uint8_t)byte;
+        if (lane == 0) hp[part_scale_at(b, q)] = sc.poison ? 255 : (uint8_t)sc.byte(q);
     }
     // past the row's last block zeros, up to its unit's end
     if (b + 1 == nf)
