@@ -1,4 +1,4 @@
-"""The layer on 4-bit experts where its activations are no numbers or nearly too large."""
+"""The layer on 4-bit experts where its activations are no numbers or nearly too large, and where its choice takes 64 bits."""
 from __future__ import annotations
 
 import i8ref
@@ -108,3 +108,68 @@ def test_activations_near_the_largest(m, F):
     assert 3.3e38 < np.abs(h).max() < 3.4e38
     want, tol = R.layer(x.astype(np.float64), v["gate"], v["up"], v["down"], rid, rw, "f32")
     within(host(trmoe.moe_mx4(L, dev(x), rlog=dev(logits), score="sigmoid", **kw)), want, tol)
+
+
+# ---- the choice in 64 bits ---------------------------------------------------------------------------
+
+def alike(rng, m, E, kind):
+    """Logits that 32 bits do not decide: all alike, alike but for a few, in runs of a hundred."""
+    l = np.full((m, E), 0.25, np.float32)
+    if kind == "few":
+        l[:, ::37] = 0.5
+        l[m - 1, 5] = -np.inf
+    if kind == "runs":
+        l = (np.arange(E) // 100)[None, :].repeat(m, 0).astype(np.float32) / 8
+    return l
+
+
+@pytest.mark.parametrize("E,k,score,bias,groups,keep,renorm", [
+    (300, 5, "sigmoid", False, 1, 1, True), (300, 5, "softmax", False, 1, 1, False), (300, 32, "softmax", True, 1, 1, True),
+    (1024, 7, "sigmoid", True, 4, 2, True), (1024, 4, "softmax", False, 2, 1, True), (256, 8, "sigmoid", True, 8, 4, False)])
+@pytest.mark.parametrize("kind", ["all", "few", "runs"])
+@pytest.mark.parametrize("m,F", [(2, 40), (8, 1100)])
+def test_a_choice_among_equals(m, F, kind, E, k, score, bias, groups, keep, renorm):
+    """More than 64 candidates: every key in 64 bits, the lower index first.  By route_scores' choice of the same logits."""
+    import torch
+    say(f"moe_mx4 equal logits m={m} F={F} {kind} E={E} k={k} {score} bias={bias} groups={groups}")
+    rng = np.random.default_rng(E + k)
+    H = 32
+    if F > 100 and E > 256:
+        E //= 4  # fewer experts where they are wide: 75 and more stay in question
+    L, w, _, b, _ = layer_of(rng, E, H, F, bias=bias, router=False)
+    if bias:
+        L.bias.fill_(0.125)
+    x = rng.standard_normal((m, H)).astype(np.float32)
+    logits = alike(rng, m, E, kind)
+    kw = dict(score=score, n_group=groups, topk_group=keep, renorm=renorm, factor=1.5)
+    ids, wt, n = trmoe.route_scores(dev(logits), k, bias=L.bias, **kw)
+    want_ids, _, want_n = i8ref.route(logits, k, None if b is None else np.full(E, 0.125), score, groups, keep, 2, renorm, 1.5)
+    assert np.array_equal(host(n), want_n) and np.array_equal(host(ids)[:, :k], want_ids)
+    y = host(trmoe.moe_mx4(L, dev(x), k, rlog=dev(logits), **kw))
+    want, tol = R.layer(x.astype(np.float64), w["gate"], w["up"], w["down"], host(ids)[:, :k], host(wt)[:, :k].astype(np.float64), "f32")
+    within(y, want, tol)
+    assert torch.equal(trmoe.moe_mx4(L, dev(x), k, rlog=dev(logits), **kw), dev(y))
+
+
+@pytest.mark.parametrize("m,F", CHOICES)
+def test_a_logit_of_infinity(m, F):
+    """Under softmax it makes the row's scores NaN: chosen by the logits without a bias, with NaN weights; with one nothing is
+    chosen.  Under sigmoid it is the largest."""
+    say(f"moe_mx4 infinite logits m={m} F={F}")
+    rng = np.random.default_rng(m + F)
+    E, k, H = 20, 4, 96
+    x, logits = rng.standard_normal((m, H)).astype(np.float32), rng.standard_normal((m, E)).astype(np.float32)
+    logits[2, 7] = np.inf
+    for bias in (False, True):
+        L, w, _, b, _ = layer_of(rng, E, H, F, bias=bias, router=False)
+        for score in ("softmax", "sigmoid"):
+            ids, wt, n = trmoe.route_scores(dev(logits), k, bias=L.bias, score=score)
+            y = host(trmoe.moe_mx4(L, dev(x), k, rlog=dev(logits), score=score))
+            ids, wt, n = host(ids)[:, :k], host(wt)[:, :k].astype(np.float64), host(n)
+            rows = np.arange(m)
+            if score == "softmax":
+                assert n[2] == (0 if bias else k)
+                assert (y[2] == 0).all() if bias else np.isnan(y[2]).all()
+                rows = np.delete(rows, 2)
+            want, tol = R.layer(x[rows].astype(np.float64), w["gate"], w["up"], w["down"], ids[rows], wt[rows], "f32")
+            within(y[rows], want, tol)
