@@ -347,7 +347,10 @@ int trk_experts_down_i8(const trk_i8_mat *down, const int8_t *q, uint64_t ldq, c
  *   trk_route_scores -> trk_experts_plan -> trk_quantize_mx4 (x) -> trk_experts_up_mx4
  *                    -> trk_quantize_mx4 (h) -> trk_experts_down_mx4
  *
- * or, for up to TRK_EXPERTS_DIRECT_M tokens and with activations that stay as they are, trk_moe_mx4.
+ * or, for up to TRK_EXPERTS_DIRECT_M tokens and with activations that stay as they are, trk_moe_mx4.  The two differ by the
+ * rounding of x and h to 4 bits: a program that goes from one to the other with the size of its batch gets other results.
+ * Experts are SwiGLU without biases or clamps.  Shared experts go through the calls above as further entries of every token:
+ * their ids and weights behind the chosen ones, n_sel and slots by as many more.
  *
  * A row of k values is ceil(k / 32) blocks of 16 bytes, two values a byte, the first in the low four bits; the last block's
  * values behind the k-th are zeros.  A value's four bits are a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6.  A block's scale is
@@ -385,7 +388,7 @@ int trk_gemm_mx4(const trk_mx4_mat *w, uint32_t item, const uint8_t *q, uint64_t
                  void *stream);
 
 /* trk_experts_up_i8 and trk_experts_down_i8 for 4-bit stacks and rows: entries, plan, h, y and work (of
- * trk_experts_down_work_bytes) are theirs. */
+ * trk_experts_down_work_bytes) are theirs.  Up takes rows and slots of which (rows / 16 rounded up) * slots is at most 2^32. */
 int trk_experts_up_mx4(const trk_mx4_mat *gate, const trk_mx4_mat *up, const uint8_t *q, uint64_t ldq,
                        const uint8_t *scale, uint64_t scale_ld, uint32_t m, const uint32_t *ids, const uint32_t *n_sel,
                        uint32_t slots, const uint32_t *plan, void *h, uint32_t dtype, uint64_t ldh, void *stream);

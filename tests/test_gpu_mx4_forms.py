@@ -229,3 +229,46 @@ def test_experts_of_rows_far_apart(call, what):
     tol = tol + (slots + 2) * i8ref.EPS["f32"] * mag
     assert (np.abs(y - want) <= tol + 1.01 * i8ref.round_rel(mag + tol, "f32")).all()
     assert (y[~there.any(1)] == 0).all()
+
+
+# ---- shared experts --------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("m", [5, 200])
+def test_shared_experts_as_further_entries(m):
+    """A shared expert behind each token's chosen ones, also where those are fewer than k: the same up and down calls."""
+    import torch
+    say(f"mx4 calls with shared experts as entries, m={m}")
+    rng = np.random.default_rng(m)
+    E, k, H, F = 12, 3, 320, 200
+    w = {"gate": rows4(rng, E + 1, F, H, spread=H ** -0.5), "up": rows4(rng, E + 1, F, H, spread=H ** -0.5), "down": rows4(rng, E + 1, H, F)}
+    size = {"gate": H, "up": H, "down": F}
+    gate, up, down = [trmoe.MX4Weights(*apart(*w[i]), size[i]) for i in w]
+    v = {i: R.values(*w[i], size[i]) for i in w}
+    x = dev(rng.standard_normal((m, H)).astype(np.float32))
+    logits = dev(rng.standard_normal((m, E)).astype(np.float32))
+    logits[0], logits[1, 2:] = -np.inf, -np.inf  # none and two of them
+    share = dev(rng.uniform(0.1, 0.9, (m, 1)).astype(np.float32))
+    ids, wt, n = trmoe.route_scores(logits, k, score="softmax")
+    at = n.long()[:, None]
+    ids.scatter_(1, at, E), wt.scatter_(1, at, share), n.add_(1)
+    assert host(n)[:2].tolist() == [1, 3] and (host(n)[2:] == k + 1).all()
+    plan = trmoe.experts_plan(ids, n, k + 1, E + 1)
+    q, s = trmoe.quantize_mx4(x)
+    h = torch.zeros((m * (k + 1), F), device="cuda")
+    trmoe.experts_up_mx4(gate, up, q, s, ids, n, k + 1, plan=plan, out=h)
+    hq, hs = trmoe.quantize_mx4(h)
+    y = host(trmoe.experts_down_mx4(down, hq, hs, ids, wt, n, k + 1, plan=plan))
+    x64, h64 = R.values(host(q), host(s), H), R.values(host(hq), host(hs), F)
+    ids, wt, n, h = host(ids), host(wt).astype(np.float64), host(n), host(h)
+    for t in range(m):
+        want, tol, mag = np.zeros(H), np.zeros(H), np.zeros(H)
+        for j in range(n[t]):
+            e, xt, ht = ids[t, j], x64[t:t + 1], h64[t * (k + 1) + j][None]
+            assert (e == E) == (j == n[t] - 1)
+            g, u = xt @ v["gate"][e].T, xt @ v["up"][e].T
+            off = R.swiglu_tol(g, u, R.sum_tol(xt, v["gate"][e]), R.sum_tol(xt, v["up"][e]), "f32")
+            assert (np.abs(h[t * (k + 1) + j] - R.silu(g) * u) <= off).all()
+            a = (ht @ v["down"][e].T)[0] * wt[t, j]
+            want, mag, tol = want + a, mag + np.abs(a), tol + R.sum_tol(ht, v["down"][e])[0] * wt[t, j]
+        tol = tol + (k + 3) * i8ref.EPS["f32"] * mag
+        assert (np.abs(y[t] - want) <= tol + 1.01 * i8ref.round_rel(mag + tol, "f32")).all()

@@ -233,8 +233,11 @@ __device__ __forceinline__ void tile_place(uint32_t idx, uint32_t tn, uint32_t t
 
 // 4096 x 12288 x 2560 to bf16 81 us, 3.2 PFLOP/s; 8192 cubed 299, 3.7 (from registers alone the instruction reached 6.6 on random
 // bits, 8.9 on constants).  What bounds it is the clock that random bits leave (1.6 GHz; 8192 cubed of zeros takes 208 us) with the matrix
-// cores busy half of it, the rest the stages' loads: tiles of 256 x 256 halve the rows' traffic against 128 x 128, at one workgroup a
-// CU.  Where whole tiles do not fill the CUs smaller ones do (geo::gemm_mx4_form).
+// cores busy half of it, and beside them LDS: a stage of 256 x 256 reads 192 KB of fragments and writes 64, 2048 clocks, as many as
+// its products take at the nominal rate.  And the scales: sixteen loads a wave for eight stages, whose row offsets do not fit beside
+// the sums (256 registers, 68 bytes of scratch a lane): seven of them wait for an offset from scratch, and with it for all that
+// is on its way, eight for a stride's scalar load.  Tiles of 256 x 256 halve the rows' traffic against 128 x 128, at one workgroup
+// a CU.  Where whole tiles do not fill the CUs smaller ones do (geo::gemm_mx4_form).
 template <typename Tile, uint32_t DT>
 __global__ __launch_bounds__(Tile::T) void gemm_mx4_tile_kernel(Mx4Gemm g) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[Tile::LDS];

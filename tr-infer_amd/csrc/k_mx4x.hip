@@ -101,7 +101,8 @@ __global__ __launch_bounds__(DOWN_WAVES* WAVE) void experts_down_mx4_strip_kerne
 // ============================================================================================
 
 // What a tile loads: for its BN weight rows, the first `split` of one matrix and the rest of another (or the same), and for its
-// activation rows, `row(i)` of all.
+// activation rows, `row(i)` of all.  Before a tile's first load lie its plan's head and place, the entries of its activation rows'
+// values, then those of their scales: a trip to memory each.
 struct Mx4Side {
     i32x4 q, s;
     uint32_t ld, lds;

@@ -58,7 +58,9 @@ struct Mx4Unit {
     }
     __device__ __forceinline__ uint32_t scale(int u, uint32_t g) const { return s[u] >> (8 * g); }
 };
-// A lane's block of the four from 4 q on (one at least is there), past the row's end the first and the scale 1: what it meets is zero
+// A lane's block of the four from 4 q on (one at least is there), past the row's end the first and the scale 1: what it meets is zero.
+// (The compiler has the scale's load in the lanes' choice and waits for it there: a row's end that is no whole unit costs a trip to
+// memory for each four blocks and matrix.)
 struct Mx4Block {
     i32x4 q;
     uint32_t s;
