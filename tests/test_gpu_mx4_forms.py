@@ -160,6 +160,36 @@ def test_down_of_each_form(form, dtype):
     assert torch.equal(again.isnan(), hit) and torch.equal(again[~hit], y[~hit])
 
 
+@pytest.mark.parametrize("H", [1, 2, 3, 4, 5, 6, 7, 1021, 1022, 1023, 1026])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_down_of_any_number_of_columns(bits, H):
+    """The sum over a token's entries, four columns at a time, in slot order: as numpy adds the same 32-bit rows."""
+    import torch
+    say(f"experts_down bits={bits} H={H}")
+    rng = np.random.default_rng(H)
+    m, E, slots, k = 30, 6, 5, 64
+    ids, wt, n = routing(rng, m, E, slots, "ragged")
+    idt, nt, wd = dev(ids), dev(n), dev(wt)
+    plan = trmoe.experts_plan(idt, nt, slots, E)
+    x, w = [dev(rng.standard_normal(s).astype(np.float32)) for s in ((m * slots, k), (E, H, k))]
+    if bits == 4:
+        q, W, down = trmoe.quantize_mx4(x), trmoe.quantize_weights_mx4(w), trmoe.experts_down_mx4
+    else:
+        q, W, down = trmoe.quantize_rows(x), trmoe.quantize_weights(w), trmoe.experts_down_i8
+    work = torch.full((m * slots * H + 64,), float("nan"), device="cuda")
+    old = torch.randn((m, H + 3), device="cuda")
+    y = old.clone()
+    down(W, *q, idt, wd, nt, slots, plan=plan, out=y[:, 1:1 + H], work=work, accumulate=True)
+    rows = host(work)[:m * slots * H].reshape(m, slots, H)  # the entries' weighted rows
+    there = i8ref.entries(ids, n, slots, E)
+    assert np.isfinite(rows[there]).all() and (np.abs(rows[there]).max(1) > 0).all() and work[m * slots * H:].isnan().all()
+    want = np.zeros((m, H), np.float32)
+    for j in range(slots):
+        want = np.where(there[:, j:j + 1], want + rows[:, j], want)
+    assert np.array_equal(host(y)[:, 1:1 + H], want + host(old)[:, 1:1 + H])
+    assert torch.equal(y[:, 0], old[:, 0]) and torch.equal(y[:, 1 + H:], old[:, 1 + H:])
+
+
 # ---- rows too far apart for the tiles' 32-bit offsets ---------------------------------------------------
 
 def far_rows(t, ld):
